@@ -752,6 +752,85 @@ SGH_API int sgh_pool_bwd_f16(const sgh_pool_geom *g, const uint16_t *dy, const u
 SGH_API int sgh_pool_bwd_bf16(const sgh_pool_geom *g, const uint16_t *dy, const uint16_t *x,
                               const uint16_t *y, uint16_t *dx, void *stream);
 
+/* =====================================================================================
+ * The two ends of a token model (no counterpart in this reference version): the table of token
+ * vectors in front of its dense layers, and the loss over the vocabulary behind them.  fp32, and
+ * 16-bit tensors with fp32 arithmetic and one rounding at the store.
+ * ===================================================================================== */
+/* y[t] = scale * W[ids[t]]: rows of W [vocab, dim] by id, y [tokens, dim].  An id equal to padding_idx (any
+ * number; -1 where there is no padding) gives a row of zeros, and so does one outside [0, vocab), which is also counted
+ * (sgh_embedding_index_errors).  dim up to 2^24, tokens and vocab up to 2^31 - 1; rows need no alignment.  y must not overlap
+ * W or ids. */
+SGH_API int sgh_embedding_fwd_f32(const int32_t *ids, const float *W, float *y, size_t tokens, size_t vocab, size_t dim,
+                                  float scale, int padding_idx, void *stream);
+SGH_API int sgh_embedding_fwd_f16(const int32_t *ids, const uint16_t *W, uint16_t *y, size_t tokens, size_t vocab, size_t dim,
+                                  float scale, int padding_idx, void *stream);
+SGH_API int sgh_embedding_fwd_bf16(const int32_t *ids, const uint16_t *W, uint16_t *y, size_t tokens, size_t vocab, size_t dim,
+                                   float scale, int padding_idx, void *stream);
+/* The gradient of W: dW[v] = add[v] + scale * (sum over t with ids[t] = v of dy[t]), every row written; tokens that the
+ * forward pass gave zeros for take part in nothing.  add: NULL, a tensor of W's size, or dW itself (rows without a token then
+ * stay as they are) -- the gradient that a matrix got elsewhere, as the weights of the output layer for one.  A row's tokens are
+ * summed in fp32 in an order that follows from the ids alone: the same bits every time.  dW must not overlap dy, ids or a
+ * part of add.  workspace: sgh_embedding_bwd_workspace_bytes (0 for few tokens, NULL is then taken). */
+SGH_API size_t sgh_embedding_bwd_workspace_bytes(size_t tokens, size_t vocab, size_t dim);
+SGH_API int sgh_embedding_bwd_f32(const int32_t *ids, const float *dy, const float *add, float *dW, size_t tokens,
+                                  size_t vocab, size_t dim, float scale, int padding_idx, void *workspace,
+                                  size_t ws_bytes, void *stream);
+SGH_API int sgh_embedding_bwd_f16(const int32_t *ids, const uint16_t *dy, const uint16_t *add, uint16_t *dW, size_t tokens,
+                                  size_t vocab, size_t dim, float scale, int padding_idx, void *workspace,
+                                  size_t ws_bytes, void *stream);
+SGH_API int sgh_embedding_bwd_bf16(const int32_t *ids, const uint16_t *dy, const uint16_t *add, uint16_t *dW, size_t tokens,
+                                   size_t vocab, size_t dim, float scale, int padding_idx, void *workspace,
+                                   size_t ws_bytes, void *stream);
+/* Number of ids outside the table that were not padding, in both directions, since the last call (synchronises the stream). */
+SGH_API int sgh_embedding_index_errors(void *stream, int *count);
+
+/* Distillation from a teacher's top logits, beside or instead of labels.  Row n of x [batch, dim] are the student's logits;
+ * top [batch, k] names columns (-1: no entry, lists may differ in length) and teacher [batch, k] their logits in the
+ * teacher; labels [batch] (-1: none) may be NULL, so may weights [batch] (fp32, all 1).  With p the softmax of
+ * teacher / temperature over a row's entries, q and r those of x / temperature and x over all columns:
+ *   loss[n] = weights[n] * (soft * temperature^2 * sum_k p_k (log p_k - log q[top_k]) - hard * log r[label])
+ *   dx[n][j] = scale * weights[n] * (soft * temperature * (q_j - sum of p_k with top_k = j) + hard * (r_j - [j = label]))
+ * A term without its list, its label or its factor (0) is left out; a row with no term, or of weight 0, has loss and gradient 0 and
+ * its logits are not looked at.  An entry of logit -inf is none.  A column may be listed twice: its shares add up.  Entries and labels
+ * below -1 or not below dim are treated as -1 and counted (sgh_distill_index_errors; the gradient alone does not count again).
+ * k = 0 (top and teacher NULL) is a cross entropy that stores no probabilities.  x -inf has probability 0; a row of nothing else,
+ * or with a NaN or +inf, has NaN results.  temperature > 0 and finite; k up to SGH_DISTILL_MAX_TOP (SGH_ELIMIT beyond).
+ *   _fwd      loss and stats [batch, 3] = the row's maximum m, sum exp((x - m) / temperature), sum exp(x - m): what the gradient
+ *             needs of the forward pass; 0 where no term asks for it
+ *   _bwd      dx from the stats of the same arguments; dx may be x itself
+ *   _fwd_bwd  both in one call, the logits' row still at hand for the gradient; dx may be x itself */
+#define SGH_DISTILL_MAX_TOP 1024
+SGH_API int sgh_distill_fwd_f32(const float *x, const int32_t *top, const float *teacher, const int32_t *labels,
+                               const float *weights, size_t batch, size_t dim, size_t k, float temperature, float soft,
+                               float hard, float *loss, float *stats, void *stream);
+SGH_API int sgh_distill_bwd_f32(const float *x, const float *stats, const int32_t *top, const float *teacher,
+                               const int32_t *labels, const float *weights, size_t batch, size_t dim, size_t k,
+                               float temperature, float soft, float hard, float scale, float *dx, void *stream);
+SGH_API int sgh_distill_fwd_bwd_f32(const float *x, const int32_t *top, const float *teacher, const int32_t *labels,
+                                   const float *weights, size_t batch, size_t dim, size_t k, float temperature,
+                                   float soft, float hard, float scale, float *loss, float *dx, void *stream);
+SGH_API int sgh_distill_fwd_f16(const uint16_t *x, const int32_t *top, const float *teacher, const int32_t *labels,
+                               const float *weights, size_t batch, size_t dim, size_t k, float temperature, float soft,
+                               float hard, float *loss, float *stats, void *stream);
+SGH_API int sgh_distill_bwd_f16(const uint16_t *x, const float *stats, const int32_t *top, const float *teacher,
+                               const int32_t *labels, const float *weights, size_t batch, size_t dim, size_t k,
+                               float temperature, float soft, float hard, float scale, uint16_t *dx, void *stream);
+SGH_API int sgh_distill_fwd_bwd_f16(const uint16_t *x, const int32_t *top, const float *teacher, const int32_t *labels,
+                                   const float *weights, size_t batch, size_t dim, size_t k, float temperature,
+                                   float soft, float hard, float scale, float *loss, uint16_t *dx, void *stream);
+SGH_API int sgh_distill_fwd_bf16(const uint16_t *x, const int32_t *top, const float *teacher, const int32_t *labels,
+                               const float *weights, size_t batch, size_t dim, size_t k, float temperature, float soft,
+                               float hard, float *loss, float *stats, void *stream);
+SGH_API int sgh_distill_bwd_bf16(const uint16_t *x, const float *stats, const int32_t *top, const float *teacher,
+                               const int32_t *labels, const float *weights, size_t batch, size_t dim, size_t k,
+                               float temperature, float soft, float hard, float scale, uint16_t *dx, void *stream);
+SGH_API int sgh_distill_fwd_bwd_bf16(const uint16_t *x, const int32_t *top, const float *teacher, const int32_t *labels,
+                                   const float *weights, size_t batch, size_t dim, size_t k, float temperature,
+                                   float soft, float hard, float scale, float *loss, uint16_t *dx, void *stream);
+/* Number of list entries and labels outside the columns that the forward pass has met since the last call (synchronises the stream). */
+SGH_API int sgh_distill_index_errors(void *stream, int *count);
+
 #ifdef __cplusplus
 }
 #endif

@@ -765,6 +765,134 @@ def AddRow(v, m):
     check(_L().sgh_add_row_f32(v.ptr, m.ptr, m.shape(0), m.shape(1), m.device().stream), "sgh_add_row_f32")
 
 
+# ------------------------------------------------------------------------------------ token models
+
+def _plain(what, device, *tensors):
+    """Dense tensors of one device (None: left out)."""
+    for t in tensors:
+        if t is not None and (t._transposed or t._dev is not device):
+            raise SingaHipError("%s: tensors of one device that are not transposed are expected" % what)
+
+
+def _embedding_dims(what, ids, W, *like_rows):
+    if ids._dtype != kInt:
+        raise SingaHipError("%s: the ids must be int32" % what)
+    if len(W._shape) != 2:
+        raise SingaHipError("%s: the table is a matrix, got %s" % (what, W.shape()))
+    _plain(what, W._dev, ids, W, *like_rows)
+
+
+def EmbeddingForward(ids, W, scale=1.0, padding_idx=-1):
+    """``scale * W[ids]``: a row of the table `W` [vocab, dim] for every id, shape ``ids.shape + (dim,)``.  Ids equal to `padding_idx`
+    give zeros; so do ids outside the table, which ``IndexErrors`` counts."""
+    _embedding_dims("EmbeddingForward", ids, W)
+    fn, name = _fn("embedding_fwd", W)
+    vocab, dim = W._shape
+    y = _empty(Tensor, ids._shape + (dim,), W._dev, W._dtype)
+    check(fn(ids.ptr, W.ptr, y.ptr, ids.Size(), vocab, dim, scale, padding_idx, W._dev.stream), name)
+    return y
+
+
+def EmbeddingBackwardW(dy, ids, W, scale=1.0, padding_idx=-1, add=None, out=None):
+    """The gradient of `W` in ``EmbeddingForward(ids, W, scale, padding_idx)``: for every row the sum of `dy` over its tokens, times
+    `scale`, on top of `add` if given (the gradient that the matrix got elsewhere, as the output layer's weights for one).  `out`: the
+    tensor that receives it; it may be `add` itself, whose rows without a token then stay as they are.  `W` gives the shape."""
+    _embedding_dims("EmbeddingBackwardW", ids, W, dy, add, out)
+    if dy._dtype != W._dtype or dy._shape != ids._shape + W._shape[1:]:
+        raise SingaHipError("EmbeddingBackwardW: dy does not match the ids and the table: %s" % dy.shape())
+    for t in (add, out):
+        if t is not None and (t._dtype != W._dtype or t._shape != W._shape):
+            raise SingaHipError("EmbeddingBackwardW: a gradient of the table's shape and type is expected, got %s" % t.shape())
+    fn, name = _fn("embedding_bwd", W)
+    vocab, dim = W._shape
+    tokens, dev = ids.Size(), W._dev
+    dW = _like(W) if out is None else out
+    need = _L().sgh_embedding_bwd_workspace_bytes(tokens, vocab, dim)
+    # (a block of the pool for this call: calls that are recorded or run side by side share none)
+    ws = _empty(Tensor, (need // 4,), dev, kFloat32) if need else None
+    check(fn(ids.ptr, dy.ptr, add.ptr if add is not None else None, dW.ptr, tokens, vocab, dim, scale, padding_idx,
+             ws.ptr if need else None, need, dev.stream), name)
+    return dW
+
+
+def IndexErrors(device):
+    """How many ids, list entries and labels outside their range ``EmbeddingForward``, ``EmbeddingBackwardW`` and the distillation's
+    forward pass have met since the last call."""
+    total = 0
+    for name in ("sgh_embedding_index_errors", "sgh_distill_index_errors"):
+        n = C.c_int()
+        check(getattr(_L(), name)(device.stream, C.byref(n)), name)
+        total += n.value
+    return total
+
+
+def _distill_args(what, x, top, teacher, labels, weights):
+    if len(x._shape) != 2:
+        raise SingaHipError("%s: a matrix of logits is expected, got %s" % (what, x.shape()))
+    batch, dim = x._shape
+    _plain(what, x._dev, x, top, teacher, labels, weights)
+    k = 0
+    if (top is None) != (teacher is None):
+        raise SingaHipError("%s: a list has ids and the teacher's logits" % what)
+    if top is not None:
+        if top._dtype != kInt or teacher._dtype != kFloat32:
+            raise SingaHipError("%s: the list's ids are int32, the teacher's logits float32" % what)
+        if len(top._shape) != 2 or top._shape[0] != batch or teacher._shape != top._shape:
+            raise SingaHipError("%s: the lists do not match: %s, %s" % (what, top.shape(), teacher.shape()))
+        k = top._shape[1]
+    if labels is not None and (labels._dtype != kInt or labels.Size() != batch):
+        raise SingaHipError("%s: an int32 label for every row is expected" % what)
+    if weights is not None and (weights._dtype != kFloat32 or weights.Size() != batch):
+        raise SingaHipError("%s: a float32 weight for every row is expected" % what)
+    return (top.ptr if k else None, teacher.ptr if k else None, labels.ptr if labels is not None else None,
+            weights.ptr if weights is not None else None, batch, dim, k)
+
+
+def DistillationFwd(x, top, teacher, labels=None, weights=None, temperature=1.0, soft=1.0, hard=0.0):
+    """(loss, stats): for every row of the student's logits `x` [batch, dim] the divergence from a teacher known by its top logits,
+    ``soft * temperature^2 * KL(p || q)`` with p the softmax of `teacher` [batch, k] (float32) / temperature over the columns `top`
+    [batch, k] (int32, -1: no entry) and q that of ``x / temperature``, plus ``hard`` times the cross entropy of `labels` [batch] (int32,
+    -1: none), times `weights` [batch].  `top` and `teacher` may be None (labels alone).  `stats` [batch, 3] is what
+    ``DistillationBwd`` needs.  Entries and labels out of range are left out and counted (``IndexErrors``)."""
+    args = _distill_args("DistillationFwd", x, top, teacher, labels, weights)
+    fn, name = _fn("distill_fwd", x)
+    batch = x._shape[0]
+    loss, stats = _empty(Tensor, (batch,), x._dev, kFloat32), _empty(Tensor, (batch, 3), x._dev, kFloat32)
+    check(fn(x.ptr, *args, temperature, soft, hard, loss.ptr, stats.ptr, x._dev.stream), name)
+    return loss, stats
+
+
+def _distill_out(what, x, out):
+    if out is None:
+        return _like(x)
+    _plain(what, x._dev, out)
+    if out._dtype != x._dtype or out._shape != x._shape:
+        raise SingaHipError("%s: a gradient of the logits' shape and type is expected, got %s" % (what, out.shape()))
+    return out
+
+
+def DistillationBwd(x, stats, top, teacher, labels=None, weights=None, temperature=1.0, soft=1.0, hard=0.0, scale=1.0, out=None):
+    """The gradient of ``scale * sum(loss)`` by `x`, from the statistics of ``DistillationFwd`` on the same arguments.  `out`: the tensor
+    that receives it; it may be `x` itself."""
+    args = _distill_args("DistillationBwd", x, top, teacher, labels, weights)
+    _plain("DistillationBwd", x._dev, stats)
+    if stats._dtype != kFloat32 or stats._shape != (x._shape[0], 3):
+        raise SingaHipError("DistillationBwd: the statistics do not match: %s" % stats.shape())
+    fn, name = _fn("distill_bwd", x)
+    dx = _distill_out("DistillationBwd", x, out)
+    check(fn(x.ptr, stats.ptr, *args, temperature, soft, hard, scale, dx.ptr, x._dev.stream), name)
+    return dx
+
+
+def DistillationFwdBwd(x, top, teacher, labels=None, weights=None, temperature=1.0, soft=1.0, hard=0.0, scale=1.0, out=None):
+    """(loss of ``DistillationFwd``, gradient of ``DistillationBwd``) in one call."""
+    args = _distill_args("DistillationFwdBwd", x, top, teacher, labels, weights)
+    fn, name = _fn("distill_fwd_bwd", x)
+    loss, dx = _empty(Tensor, x._shape[:1], x._dev, kFloat32), _distill_out("DistillationFwdBwd", x, out)
+    check(fn(x.ptr, *args, temperature, soft, hard, scale, loss.ptr, dx.ptr, x._dev.stream), name)
+    return loss, dx
+
+
 # ------------------------------------------------------------------------------------ operations
 
 # A handle's geometry goes to the library by address.  The address is asked for at every call: a copied or unpickled handle,
