@@ -21,10 +21,9 @@ __device__ int g_index_errors = 0;
 struct RowLanes {
   int epl, lanes, slices;
 };
-template <class S>
-RowLanes row_lanes(size_t dim) {
+RowLanes row_lanes(size_t dim, int vec) {   // vec: elements of 16 bytes
   RowLanes r;
-  r.epl = dim < size_t(S::VEC) ? 1 : S::VEC;
+  r.epl = dim < size_t(vec) ? 1 : vec;
   const size_t vecs = (dim + r.epl - 1) / r.epl;
   r.lanes = 1;
   while (r.lanes < SGH_WAVE && size_t(r.lanes) < vecs) r.lanes *= 2;
@@ -97,20 +96,75 @@ int embed_fwd(const int32_t *ids, const typename S::elem *W, typename S::elem *y
   hipStream_t s = sgh_stream_of(stream);
   sgh_note_write(y, tokens * dim * e);
   sgh_prof_kernel_scope prof("embedding_fwd/k_embed_fwd", double(tokens) * (4 + 2.0 * dim * e), s);
-  const RowLanes r = row_lanes<S>(dim);
+  const RowLanes r = row_lanes(dim, S::VEC);
   if (r.epl == 1) return launch_fwd<S, 1, 1>(ids, W, y, tokens, vocab, dim, scale, pad, r, s);
   return launch_fwd<S, S::VEC, 4>(ids, W, y, tokens, vocab, dim, scale, pad, r, s);
 }
 
-// ------------------------------------------------------------------------------------ the order of the tokens
+// ------------------------------------------------------------------------------------ the gradient
 
-// Stable sort of (id, place) by id: passes of at most 9 bits from the lowest.  A pass counts the digits of each workgroup's stretch of
-// tokens, turns the counts into the place of every stretch's first token with a digit, and moves the tokens there.
-constexpr int kDigitBits = 9, kBins = 1 << kDigitBits;
-constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / SGH_WAVE;
-constexpr int kItems = 4;                              // tokens of a thread at a time
-constexpr int kStretch = kSortThreads * kItems;
-constexpr int kMostStretches = 64;                     // workgroups of a pass: each reads all their counts
+// A token in the sorted list: its id (`vocab` where it takes part in nothing) and its place
+struct alignas(8) Token {
+  unsigned key, place;
+};
+
+// A call's tensors and how they are cut
+template <class T>
+struct Bwd {
+  const int32_t *ids;
+  const T *dy, *add;
+  T *dW;
+  const Token *sorted;
+  unsigned *tail;                  // of every tile: the first of the sums that its last row is to be joined from, if any
+  float *partial;                  // [tiles][2][pitch]: sums of a row's tokens that hold whole tiles: a tile's head or all of it, its tail
+  size_t pitch;
+  size_t dim, vocab;
+  unsigned tokens, tile;           // sorted tokens that a wavefront goes through
+  float scale;
+  int pad, lanes, slices;
+};
+
+// Stores one vector of a row: acc * scale on top of `add`.  `moved`: the row's last vector, moved back to end with the row; its first
+// elements are the vector's before it, which may be stored already where `add` is the result itself.
+template <class S, int EPL>
+__device__ __forceinline__ void store_row(const Bwd<typename S::elem> &a, size_t row, size_t at, size_t vec, float *acc) {
+  typename S::elem *out = a.dW + row * a.dim + at;
+  const typename S::elem *add = a.add ? a.add + row * a.dim + at : nullptr;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) acc[j] *= a.scale;
+  if (at != vec * EPL) {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j)
+      if (at + j >= vec * EPL) S::st(out + j, add ? S::ld(add + j) + acc[j] : acc[j]);
+  } else {
+    if (add) {
+      float g[EPL];
+      sgh_load_any<S, EPL>(add, g);
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) acc[j] += g[j];
+    }
+    sgh_store_any<S, EPL>(out, acc);
+  }
+}
+
+// Sum of rows place[from .. to) of dy, ascending, on top of acc
+template <class S, int EPL>
+__device__ __forceinline__ void add_tokens(const typename S::elem *dy, size_t dim, size_t at, const unsigned *place, unsigned from,
+                                           unsigned to, float *acc) {
+  constexpr int U = 8;
+  for (unsigned i = from; i < to; i += U) {
+    float v[U][EPL];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u < to) sgh_load_any<S, EPL>(dy + size_t(place[i + u]) * dim + at, v[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u < to) {
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) acc[j] += v[u][j];
+      }
+  }
+}
 
 // LDS as the wavefront's lanes left it, before and after
 __device__ __forceinline__ void wave_sync() {
@@ -119,292 +173,106 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-__device__ __forceinline__ unsigned key_of(int id, unsigned vocab, int pad) {
-  return id < 0 || unsigned(id) >= vocab || id == pad ? vocab : unsigned(id);
-}
-
-__global__ __launch_bounds__(kSortThreads) void k_embed_count(const int32_t *__restrict__ ids, const unsigned *__restrict__ keys,
-                                                              unsigned tokens, unsigned vocab, int pad, int shift, int bins,
-                                                              unsigned per_block, unsigned *__restrict__ counts) {
-  __shared__ unsigned h[kBins];
-  for (int d = threadIdx.x; d < bins; d += kSortThreads) h[d] = 0;
-  __syncthreads();
-  const size_t from = size_t(blockIdx.x) * per_block, to = from + per_block < tokens ? from + per_block : tokens;
-  for (size_t i = from + threadIdx.x; i < to; i += kSortThreads) {
-    unsigned k;
-    if (ids) {
-      const int id = ids[i];
-      k = key_of(id, vocab, pad);
-      if (k == vocab && id != pad) atomicAdd(&g_index_errors, 1);
-    } else {
-      k = keys[i];
-    }
-    atomicAdd(&h[(k >> shift) & (bins - 1)], 1u);
-  }
-  __syncthreads();
-  for (int d = threadIdx.x; d < bins; d += kSortThreads) counts[size_t(blockIdx.x) * bins + d] = h[d];
-}
-
-__global__ __launch_bounds__(kSortThreads) void k_embed_move(const int32_t *__restrict__ ids, const unsigned *__restrict__ keys,
-                                                             const unsigned *__restrict__ places, unsigned tokens, unsigned vocab,
-                                                             int pad, int shift, int bins, unsigned per_block,
-                                                             const unsigned *__restrict__ counts, unsigned *__restrict__ keys_out,
-                                                             unsigned *__restrict__ places_out) {
-  __shared__ unsigned next[kBins];               // where the next token with a digit goes
-  __shared__ unsigned in_wave[kSortWaves][kBins];
-  __shared__ unsigned sums[kSortWaves];
-  const int tid = threadIdx.x, lane = tid & (SGH_WAVE - 1), wave = tid >> 6;
-  // all tokens with a lower digit, then this digit's of the stretches in front
-  {
-    unsigned all = 0, before = 0;
-    if (tid < bins)
-      for (unsigned b = 0; b < gridDim.x; ++b) {
-        const unsigned c = counts[size_t(b) * bins + tid];
-        all += c;
-        if (b < blockIdx.x) before += c;
-      }
-    unsigned upto = all;
-#pragma unroll
-    for (int o = 1; o < SGH_WAVE; o <<= 1) {
-      const unsigned u = __shfl_up(upto, o, SGH_WAVE);
-      if (lane >= o) upto += u;
-    }
-    if (lane == SGH_WAVE - 1) sums[wave] = upto;
-    __syncthreads();
-    unsigned lower = 0;
-    for (int w = 0; w < wave; ++w) lower += sums[w];
-    if (tid < bins) next[tid] = lower + upto - all + before;
-  }
-  const size_t from = size_t(blockIdx.x) * per_block, to = from + per_block < tokens ? from + per_block : tokens;
-  for (size_t base = from; base < to; base += kStretch) {
-    for (int i = tid; i < kSortWaves * bins; i += kSortThreads) in_wave[i / bins][i % bins] = 0;
-    __syncthreads();
-    unsigned key[kItems], place[kItems], rank[kItems];
-#pragma unroll
-    for (int u = 0; u < kItems; ++u) {
-      const size_t i = base + size_t(wave) * (SGH_WAVE * kItems) + u * SGH_WAVE + lane;
-      const bool there = i < to;
-      key[u] = there ? (ids ? key_of(ids[i], vocab, pad) : keys[i]) : 0;
-      place[u] = there ? (ids ? unsigned(i) : places[i]) : 0xffffffffu;
-    }
-#pragma unroll
-    for (int u = 0; u < kItems; ++u) {
-      const bool there = place[u] != 0xffffffffu;
-      const unsigned digit = (key[u] >> shift) & (bins - 1);
-      unsigned long long same = __ballot(there);   // lanes with this digit
-#pragma unroll
-      for (int b = 0; b < kDigitBits; ++b) {
-        const bool bit = (digit >> b) & 1;
-        const unsigned long long set = __ballot(bit);
-        same &= bit ? set : ~set;
-      }
-      const int ahead = __popcll(same & ((1ull << lane) - 1));
-      const unsigned old = in_wave[wave][digit];
-      rank[u] = old + ahead;
-      wave_sync();   // (every lane has read the count before one of them writes it)
-      if (there && ahead == 0) in_wave[wave][digit] = old + __popcll(same);
-      wave_sync();
-    }
-    __syncthreads();
-    if (tid < bins) {
-      unsigned at = next[tid];
-      for (int w = 0; w < kSortWaves; ++w) {
-        const unsigned c = in_wave[w][tid];
-        in_wave[w][tid] = at;
-        at += c;
-      }
-      next[tid] = at;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < kItems; ++u)
-      if (place[u] != 0xffffffffu) {
-        const unsigned to_ = in_wave[wave][(key[u] >> shift) & (bins - 1)] + rank[u];
-        keys_out[to_] = key[u];
-        places_out[to_] = place[u];
-      }
-    __syncthreads();
-  }
-}
-
-// ------------------------------------------------------------------------------------ the gradient
-
-// Rows of the gradient that take part in a call, and where their tokens are found
-template <class T>
-struct Rows {
-  const T *dy, *add;
-  T *dW;
-  const unsigned *keys, *places;   // sorted
-  const int32_t *ids;              // few tokens: as they came
-  float *partial;                  // sums of whole tiles of one row, [tiles][dim]
-  size_t dim, vocab;
-  unsigned tokens, tile;           // tokens of a tile, a power of two
-  float scale;
-  int pad, lanes, slices, rows;    // rows: of a workgroup
-};
-
-// Sum of rows place[from .. to) of dy, ascending, on top of acc
-template <class S, int EPL>
-__device__ __forceinline__ void add_tokens(const typename S::elem *dy, size_t dim, size_t at, const unsigned *place, unsigned from,
-                                           unsigned to, float *acc) {
-  constexpr int U = 8;
-  unsigned i = from;
-  for (; i + U <= to; i += U) {
-    float v[U][EPL];
-#pragma unroll
-    for (int u = 0; u < U; ++u) sgh_load_any<S, EPL>(dy + size_t(place[i + u]) * dim + at, v[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int j = 0; j < EPL; ++j) acc[j] += v[u][j];
-  }
-  for (; i < to; ++i) {
-    float v[EPL];
-    sgh_load_any<S, EPL>(dy + size_t(place[i]) * dim + at, v);
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) acc[j] += v[j];
-  }
-}
-
-// Tiles of `tile` sorted tokens that are all of one row: their sums, so that a row with many tokens is not one wavefront's work
-template <class S, int EPL>
-__global__ __launch_bounds__(kBlock) void k_embed_tiles(Rows<typename S::elem> a) {
-  const unsigned first = blockIdx.x * a.tile, last = first + a.tile - 1;   // (only whole tiles are launched)
-  const unsigned key = a.keys[first];
-  if (key >= a.vocab || a.keys[last] != key) return;
+// Inclusive sum over the lanes in front
+__device__ __forceinline__ unsigned wave_upto(unsigned v) {
   const int lane = threadIdx.x & (SGH_WAVE - 1);
-  const size_t vecs = (a.dim + EPL - 1) / EPL;
-  for (size_t sl = blockIdx.y * kWaves + (threadIdx.x >> 6); sl < size_t(a.slices); sl += gridDim.y * kWaves) {
-    const size_t vec = sl * SGH_WAVE + lane;
-    if (vec >= vecs) continue;
-    const size_t at = vec * EPL + EPL > a.dim ? a.dim - EPL : vec * EPL;
-    float acc[EPL];
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) acc[j] = 0.f;
-    add_tokens<S, EPL>(a.dy, a.dim, at, a.places, first, last + 1, acc);
-    float *out = a.partial + size_t(blockIdx.x) * a.dim + at;
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) out[j] = acc[j];
+  for (int o = 1; o < SGH_WAVE; o <<= 1) {
+    const unsigned u = __shfl_up(v, o, SGH_WAVE);
+    if (lane >= o) v += u;
   }
+  return v;
 }
 
-// First of the sorted keys that is not below x, by a wavefront: 64 probes a step
-__device__ __forceinline__ unsigned lower_bound(const unsigned *keys, unsigned n, unsigned x) {
-  unsigned lo = 0, hi = n;
-  const unsigned lane = threadIdx.x & (SGH_WAVE - 1);
-  while (lo < hi) {
-    const unsigned step = (hi - lo + SGH_WAVE - 1) / SGH_WAVE;
-    const size_t probe = size_t(lo) + size_t(lane + 1) * step - 1;   // the last of each of 64 stretches
-    const bool below = probe < hi && keys[probe] < x;
-    const unsigned whole = unsigned(__popcll(__ballot(below)));
-    const size_t start = size_t(lo) + size_t(whole) * step, stop = start + step - 1;
-    lo = start < hi ? unsigned(start) : hi;
-    hi = stop < hi ? unsigned(stop) : hi;
-  }
-  return lo;
+// How many of the lanes in `mask` are in front of this one
+__device__ __forceinline__ int lanes_below(unsigned long long mask) {
+  return __builtin_amdgcn_mbcnt_hi(unsigned(mask >> 32), __builtin_amdgcn_mbcnt_lo(unsigned(mask), 0));
 }
 
-constexpr int kMostRows = 256;        // of a workgroup
-constexpr unsigned kScanTokens = 1024;   // up to here a workgroup looks through the ids itself
+// Lanes of the wavefront (those with `there`) whose value agrees with this lane's in its low BITS bits
+template <int BITS>
+__device__ __forceinline__ unsigned long long same_lanes(unsigned v, bool there) {
+  const unsigned long long all = __ballot(there);
+  unsigned lo = unsigned(all), hi = unsigned(all >> 32);
+#pragma unroll
+  for (int b = 0; b < BITS; ++b) {
+    const unsigned mine = unsigned(int(v << (31 - b)) >> 31);   // all ones where the bit is set
+    const unsigned long long set = __ballot(int(mine) < 0);
+    lo &= ~(unsigned(set) ^ mine);
+    hi &= ~(unsigned(set >> 32) ^ mine);
+  }
+  return (static_cast<unsigned long long>(hi) << 32) | lo;
+}
 
-// Workgroup: a few consecutive rows of the gradient.  It finds their tokens -- in the sorted list, or (SCAN) among all ids -- and every
-// wavefront sums and stores rows, or slices of them; rows without a token become zero, or `add`.
-template <class S, int EPL, bool SCAN>
-__global__ __launch_bounds__(kBlock) void k_embed_rows(Rows<typename S::elem> a) {
-  typedef typename S::elem T;
+// ------------------------------------------------------------------------------------ few tokens
+
+constexpr int kMostRows = 256;           // rows of a workgroup
+constexpr unsigned kScanTokens = 1024;
+
+// Up to kScanTokens tokens, in one launch: a workgroup has a few consecutive rows, looks through all ids for theirs, sorts those in LDS and
+// sums and stores its rows, or slices of them; rows without a token become zero, or `add`.
+template <class S, int EPL>
+__global__ __launch_bounds__(kBlock) void k_embed_rows(Bwd<typename S::elem> a, int rows_each) {
   __shared__ unsigned begin[kMostRows], end[kMostRows];
-  __shared__ unsigned found[SCAN ? kScanTokens : 2];   // SCAN: places of the rows' tokens, by row; else the bounds of the rows' tokens
-  __shared__ unsigned listed[SCAN ? kScanTokens : 1];  // (row, place) in the order of the places
+  __shared__ unsigned found[kScanTokens];    // places of the rows' tokens, by row
+  __shared__ unsigned listed[kScanTokens];   // (row, place) in the order of the places
   __shared__ unsigned sums[kWaves];
   const int tid = threadIdx.x, lane = tid & (SGH_WAVE - 1), wave = tid >> 6;
-  const size_t row0 = size_t(blockIdx.x) * a.rows;
-  const int rows = a.vocab - row0 < size_t(a.rows) ? int(a.vocab - row0) : a.rows;
+  const size_t row0 = size_t(blockIdx.x) * rows_each;
+  const int rows = a.vocab - row0 < size_t(rows_each) ? int(a.vocab - row0) : rows_each;
   for (int r = tid; r < rows; r += kBlock) begin[r] = end[r] = 0;
-  if constexpr (SCAN) {
-    constexpr int P = kScanTokens / kBlock;   // a thread's tokens are neighbours: one prefix sum keeps the order
-    unsigned mine[P], n = 0;
+  constexpr int P = kScanTokens / kBlock;   // a thread's tokens are neighbours: one prefix sum keeps the order
+  unsigned mine[P], n = 0;
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      const unsigned t = tid * P + p;
-      mine[p] = 0xffffffffu;
-      if (t < a.tokens) {
-        const int id = a.ids[t];
-        if (id != a.pad && (id < 0 || size_t(id) >= a.vocab)) {
-          if (blockIdx.x == 0 && blockIdx.y == 0) atomicAdd(&g_index_errors, 1);
-        } else if (id != a.pad && size_t(id) >= row0 && size_t(id) < row0 + rows) {
-          mine[p] = unsigned(size_t(id) - row0);
-          ++n;
-        }
+  for (int p = 0; p < P; ++p) {
+    const unsigned t = tid * P + p;
+    mine[p] = 0xffffffffu;
+    if (t < a.tokens) {
+      const int id = a.ids[t];
+      if (id != a.pad && (id < 0 || size_t(id) >= a.vocab)) {
+        if (blockIdx.x == 0 && blockIdx.y == 0) atomicAdd(&g_index_errors, 1);
+      } else if (id != a.pad && size_t(id) >= row0 && size_t(id) < row0 + rows) {
+        mine[p] = unsigned(size_t(id) - row0);
+        ++n;
       }
     }
-    unsigned upto = n;
-#pragma unroll
-    for (int o = 1; o < SGH_WAVE; o <<= 1) {
-      const unsigned u = __shfl_up(upto, o, SGH_WAVE);
-      if (lane >= o) upto += u;
-    }
-    if (lane == SGH_WAVE - 1) sums[wave] = upto;
-    __syncthreads();
-    unsigned at = upto - n, total = 0;
-    for (int w = 0; w < kWaves; ++w) {
-      if (w < wave) at += sums[w];
-      total += sums[w];
-    }
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-      if (mine[p] != 0xffffffffu) {
-        listed[at++] = (mine[p] << 16) | unsigned(tid * P + p);
-        atomicAdd(&end[mine[p]], 1u);
-      }
-    __syncthreads();
-    if (wave == 0) {   // a stable counting sort by row: end[] holds the counts
-      unsigned carry = 0;
-      for (int r = lane; r - lane < rows; r += SGH_WAVE) {
-        const unsigned c = r < rows ? end[r] : 0;
-        unsigned up = c;
-#pragma unroll
-        for (int o = 1; o < SGH_WAVE; o <<= 1) {
-          const unsigned u = __shfl_up(up, o, SGH_WAVE);
-          if (lane >= o) up += u;
-        }
-        if (r < rows) begin[r] = end[r] = carry + up - c;
-        carry += __shfl(up, SGH_WAVE - 1, SGH_WAVE);
-      }
-      wave_sync();
-      for (unsigned i = lane; i - lane < total; i += SGH_WAVE) {
-        const bool there = i < total;
-        const unsigned e = there ? listed[i] : 0, r = e >> 16;
-        unsigned long long same = __ballot(there);
-#pragma unroll
-        for (int b = 0; b < 8; ++b) {
-          const bool bit = (r >> b) & 1;
-          const unsigned long long set = __ballot(bit);
-          same &= bit ? set : ~set;
-        }
-        const int ahead = __popcll(same & ((1ull << lane) - 1));
-        const unsigned old = there ? end[r] : 0;
-        wave_sync();
-        if (there) found[old + ahead] = e & 0xffffu;
-        if (there && ahead == 0) end[r] = old + __popcll(same);
-        wave_sync();
-      }
-    }
-    __syncthreads();
-  } else {
-    if (wave < 2) {
-      const unsigned b = a.tokens ? lower_bound(a.keys, a.tokens, unsigned(row0 + (wave ? rows : 0))) : 0;
-      if (lane == 0) found[wave] = b;
-    }
-    __syncthreads();
-    const unsigned lo = found[0], hi = found[1];
-    for (unsigned i = lo + tid; i < hi; i += kBlock) {
-      const unsigned k = a.keys[i], r = unsigned(k - row0);
-      if (i == lo || a.keys[i - 1] != k) begin[r] = i;
-      if (i + 1 == hi || a.keys[i + 1] != k) end[r] = i + 1;
-    }
-    __syncthreads();
   }
-  const unsigned *place = SCAN ? found : a.places;
+  const unsigned upto = wave_upto(n);
+  if (lane == SGH_WAVE - 1) sums[wave] = upto;
+  __syncthreads();
+  unsigned slot = upto - n, total = 0;
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) slot += sums[w];
+    total += sums[w];
+  }
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+    if (mine[p] != 0xffffffffu) {
+      listed[slot++] = (mine[p] << 16) | unsigned(tid * P + p);
+      atomicAdd(&end[mine[p]], 1u);
+    }
+  __syncthreads();
+  if (wave == 0) {   // a stable counting sort by row: end[] holds the counts
+    unsigned carry = 0;
+    for (int r = lane; r - lane < rows; r += SGH_WAVE) {
+      const unsigned c = r < rows ? end[r] : 0, up = wave_upto(c);
+      if (r < rows) begin[r] = end[r] = carry + up - c;
+      carry += __shfl(up, SGH_WAVE - 1, SGH_WAVE);
+    }
+    wave_sync();
+    for (unsigned i = lane; i - lane < total; i += SGH_WAVE) {
+      const bool there = i < total;
+      const unsigned e = there ? listed[i] : 0, r = e >> 16;
+      const unsigned long long same = same_lanes<8>(r, there);
+      const int ahead = lanes_below(same);
+      const unsigned old = there ? end[r] : 0;
+      wave_sync();
+      if (there) found[old + ahead] = e & 0xffffu;
+      if (there && ahead == 0) end[r] = old + __popcll(same);
+      wave_sync();
+    }
+  }
+  __syncthreads();
   const size_t vecs = (a.dim + EPL - 1) / EPL;
   const int per_wave = SGH_WAVE / a.lanes, groups = (rows + per_wave - 1) / per_wave;
   for (size_t unit = size_t(blockIdx.y) * kWaves + wave; unit < size_t(groups) * a.slices; unit += size_t(gridDim.y) * kWaves) {
@@ -412,65 +280,480 @@ __global__ __launch_bounds__(kBlock) void k_embed_rows(Rows<typename S::elem> a)
     const size_t vec = (unit - size_t(group) * a.slices) * SGH_WAVE + (lane & (a.lanes - 1));
     const int r = group * per_wave + lane / a.lanes;
     if (r >= rows || vec >= vecs) continue;
-    const bool moved = vec * EPL + EPL > a.dim;   // the row's last vector, moved back
-    const size_t at = moved ? a.dim - EPL : vec * EPL;
+    const size_t at = vec * EPL + EPL > a.dim ? a.dim - EPL : vec * EPL;
     const unsigned b = begin[r], e = end[r];
-    T *out = a.dW + (row0 + r) * a.dim + at;
-    const T *add = a.add ? a.add + (row0 + r) * a.dim + at : nullptr;
-    if (b == e && add == out) continue;
+    if (b == e && a.add == a.dW) continue;
     float acc[EPL];
 #pragma unroll
     for (int j = 0; j < EPL; ++j) acc[j] = 0.f;
-    if (!SCAN && e - b >= a.tile) {
-      const unsigned t0 = (b + a.tile - 1) / a.tile, t1 = e / a.tile;   // whole tiles of this row
-      if (t0 < t1) {
-        add_tokens<S, EPL>(a.dy, a.dim, at, place, b, t0 * a.tile, acc);
-        for (unsigned t = t0; t < t1; ++t) {
-          const float *p = a.partial + size_t(t) * a.dim + at;
+    add_tokens<S, EPL>(a.dy, a.dim, at, found, b, e, acc);
+    store_row<S, EPL>(a, row0 + r, at, vec, acc);
+  }
+}
+
+// ------------------------------------------------------------------------------------ many tokens
+
+// 1. The tokens are sorted by id, stable: passes of at most 9 bits from the lowest.  A pass counts the digits of each workgroup's stretch of
+//    tokens, turns the counts into the place of every stretch's first token with a digit, and moves the tokens there.  Up to kOneTokens
+//    one workgroup does all passes.  The workgroups that sort are few: beside them, in the same launches, others look through the ids for
+//    the rows that have no token and store those.
+// 2. Tiles of sorted tokens: a wavefront goes through the tokens of a tile (and a slice of the rows' elements), and stores each row whose
+//    tokens begin there.  Where a row's tokens hold a whole tile, that tile's sum is kept instead,
+// 3. and the tile in which they begin joins the sums.
+
+constexpr int kDigitBits = 9, kBins = 1 << kDigitBits;
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / SGH_WAVE;
+constexpr int kItems = 2;                              // tokens of a thread at a time
+constexpr unsigned kStretch = kSortThreads * kItems;
+constexpr int kMostStretches = 64;                     // each workgroup reads the counts of all
+constexpr unsigned kOneTokens = 8192;
+constexpr unsigned kFillRows = 8192;                   // rows that a workgroup looks out for
+
+struct Sort {
+  const int32_t *ids;                  // first pass
+  const Token *in;                     // later ones
+  Token *out;
+  unsigned *counts;                    // [stretches][bins]
+  unsigned tokens, vocab, per_stretch;
+  int pad, shift, bins, stretches;
+};
+struct Fill {
+  unsigned rows;               // of a workgroup
+  int launch, launches;
+  unsigned char *taken;        // [vocab]: rows with a token
+};
+
+struct SortSpace {
+  unsigned next[kBins];                  // where the next token with a digit goes
+  uint16_t in_wave[kSortWaves][kBins];   // tokens with a digit of each wavefront, then those of the wavefronts in front
+  unsigned sums[kSortWaves];
+};
+
+__device__ __forceinline__ unsigned key_of(int id, unsigned vocab, int pad) {
+  return id < 0 || unsigned(id) >= vocab || id == pad ? vocab : unsigned(id);
+}
+
+__device__ __forceinline__ void count_digits(const Sort &s, unsigned from, unsigned to, unsigned *h) {
+  constexpr unsigned U = 2;
+  for (size_t i = size_t(from) + threadIdx.x; i < to; i += U * kSortThreads) {
+    unsigned k[U];
 #pragma unroll
-          for (int j = 0; j < EPL; ++j) acc[j] += p[j];
-        }
-        add_tokens<S, EPL>(a.dy, a.dim, at, place, t1 * a.tile, e, acc);
-      } else {
-        add_tokens<S, EPL>(a.dy, a.dim, at, place, b, e, acc);
-      }
-    } else {
-      add_tokens<S, EPL>(a.dy, a.dim, at, place, b, e, acc);
+    for (unsigned u = 0; u < U; ++u) {
+      const size_t j = i + u * kSortThreads;
+      k[u] = j < to ? (s.ids ? unsigned(s.ids[j]) : s.in[j].key) : 0;
     }
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) acc[j] *= a.scale;
-    if (moved) {   // only what the vector before it leaves: `add` may be the result itself
-#pragma unroll
-      for (int j = 0; j < EPL; ++j)
-        if (at + j >= vec * EPL) S::st(out + j, add ? S::ld(add + j) + acc[j] : acc[j]);
-    } else {
-      if (add) {
-        float g[EPL];
-        sgh_load_any<S, EPL>(add, g);
-#pragma unroll
-        for (int j = 0; j < EPL; ++j) acc[j] += g[j];
+    for (unsigned u = 0; u < U; ++u)
+      if (i + u * kSortThreads < to) {
+        if (s.ids) k[u] = key_of(int(k[u]), s.vocab, s.pad);
+        atomicAdd(&h[(k[u] >> s.shift) & (s.bins - 1)], 1u);
       }
-      sgh_store_any<S, EPL>(out, acc);
+  }
+}
+
+// All tokens with a digit below this thread's, from every digit's total in thread `digit`
+__device__ __forceinline__ unsigned lower_digits(SortSpace &sp, unsigned total) {
+  const int lane = threadIdx.x & (SGH_WAVE - 1), wave = threadIdx.x >> 6;
+  const unsigned upto = wave_upto(total);
+  if (lane == SGH_WAVE - 1) sp.sums[wave] = upto;
+  __syncthreads();
+  unsigned lower = upto - total;
+  for (int w = 0; w < wave; ++w) lower += sp.sums[w];
+  return lower;
+}
+
+// Up to ITEMS * 64 tokens of every wavefront, neighbours each
+template <int ITEMS>
+struct Held {
+  unsigned key[ITEMS], place[ITEMS], rank[ITEMS];
+};
+constexpr unsigned kNoPlace = 0xffffffffu;
+
+// Ranks the held tokens among those of the wavefront with their digit, whose counts go to in_wave (zero before)
+template <int ITEMS>
+__device__ __forceinline__ void sort_rank(const Sort &s, unsigned per_wave, SortSpace &sp, Held<ITEMS> &h) {
+  const int wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int u = 0; u < ITEMS; ++u)
+    if (u * SGH_WAVE < per_wave) {
+      const bool there = h.place[u] != kNoPlace;
+      const unsigned digit = (h.key[u] >> s.shift) & (s.bins - 1);
+      const unsigned long long same = same_lanes<kDigitBits>(digit, there);
+      const int ahead = lanes_below(same);
+      const unsigned old = sp.in_wave[wave][digit];
+      h.rank[u] = old + ahead;
+      wave_sync();   // (every lane has read the count before one of them writes it)
+      if (there && ahead == 0) sp.in_wave[wave][digit] = uint16_t(old + __popcll(same));
+      wave_sync();
+    }
+}
+__device__ __forceinline__ void clear_counts(SortSpace &sp) {
+  unsigned *w = reinterpret_cast<unsigned *>(&sp.in_wave[0][0]);
+  for (int i = threadIdx.x; i < kSortWaves * kBins / 2; i += kSortThreads) w[i] = 0;
+}
+// in_wave from counts to those of the wavefronts in front: thread `digit`; returns the digit's total
+__device__ __forceinline__ unsigned front_counts(SortSpace &sp) {
+  unsigned at = 0;
+#pragma unroll
+  for (int w = 0; w < kSortWaves; ++w) {
+    const unsigned c = sp.in_wave[w][threadIdx.x];
+    sp.in_wave[w][threadIdx.x] = uint16_t(at);
+    at += c;
+  }
+  return at;
+}
+__device__ __forceinline__ unsigned place_of(const Sort &s, const SortSpace &sp, unsigned key, unsigned rank) {
+  const unsigned digit = (key >> s.shift) & (s.bins - 1);
+  return sp.next[digit] + sp.in_wave[threadIdx.x >> 6][digit] + rank;
+}
+__device__ __forceinline__ unsigned counted_key(const Sort &s, int id, bool there) {
+  const unsigned k = key_of(id, s.vocab, s.pad);
+  if (there && k == s.vocab && id != s.pad) atomicAdd(&g_index_errors, 1);
+  return k;
+}
+
+// The rows that have no token: zero, or `add`.  Workgroup `part` of each launch has the same `f.rows` rows and stores its share of them; in
+// the first launch it looks through the ids for all of them and leaves what it saw for the later ones.
+template <class S, int EPL>
+__device__ __forceinline__ void fill_rows(const Bwd<typename S::elem> &a, const Fill &f, unsigned part, unsigned char *taken) {
+  const size_t row0 = size_t(part) * f.rows;
+  const unsigned rows = a.vocab - row0 < f.rows ? unsigned(a.vocab - row0) : f.rows;
+  const unsigned tid = threadIdx.x, lane = tid & (SGH_WAVE - 1), wave = tid >> 6;
+  const unsigned lo = unsigned(size_t(rows) * f.launch / f.launches), hi = unsigned(size_t(rows) * (f.launch + 1) / f.launches);
+  if (f.launch == 0) {
+    for (unsigned r = tid; r < rows; r += kSortThreads) taken[r] = 0;
+    __syncthreads();
+    constexpr unsigned U = 8;
+    for (size_t i = tid; i < a.tokens; i += U * kSortThreads) {
+      int id[U];
+#pragma unroll
+      for (unsigned u = 0; u < U; ++u) id[u] = i + u * kSortThreads < a.tokens ? a.ids[i + u * kSortThreads] : a.pad;
+#pragma unroll
+      for (unsigned u = 0; u < U; ++u) {
+        const size_t r = size_t(id[u]) - row0;   // (an id below the rows, or below 0, is a large number)
+        if (id[u] >= 0 && r < rows && id[u] != a.pad) taken[r] = 1;
+      }
+    }
+    __syncthreads();
+    for (unsigned r = hi + tid; r < rows; r += kSortThreads) f.taken[row0 + r] = taken[r];
+  } else {
+    for (unsigned r = lo + tid; r < hi; r += kSortThreads) taken[r] = f.taken[row0 + r];
+    __syncthreads();
+  }
+  const size_t vecs = (a.dim + EPL - 1) / EPL;
+  const unsigned per_wave = SGH_WAVE / a.lanes;
+  constexpr int U = 4;
+  for (unsigned r = lo + wave * per_wave + lane / a.lanes; r < hi; r += kSortWaves * per_wave) {
+    if (taken[r]) continue;
+    for (size_t vec = lane & (a.lanes - 1); vec < vecs; vec += U * SGH_WAVE) {
+      float v[U][EPL];
+      size_t at[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        at[u] = (row0 + r) * a.dim + ((vec + u * SGH_WAVE) * EPL + EPL > a.dim ? a.dim - EPL : (vec + u * SGH_WAVE) * EPL);
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) v[u][j] = 0.f;
+        if (a.add && vec + u * SGH_WAVE < vecs) sgh_load_any<S, EPL>(a.add + at[u], v[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (vec + u * SGH_WAVE < vecs) sgh_store_any<S, EPL>(a.dW + at[u], v[u]);
     }
   }
 }
 
+// All passes by the first workgroup, every token in a register of it; they change places through LDS (as 2 x 8192 stores of single words
+// to global memory a pass took 12 us)
+struct OneSpace {
+  SortSpace sort;
+  unsigned key[kOneTokens];
+  uint16_t place[kOneTokens];
+};
+union OneLds {
+  OneSpace one;
+  unsigned char taken[kFillRows];
+};
+constexpr int kOneItems = int(kOneTokens) / kSortThreads;
+template <class S, int EPL>
+__global__ __launch_bounds__(kSortThreads) void k_embed_sort(Bwd<typename S::elem> a, Sort s, int passes, int digit_bits, Fill f) {
+  __shared__ OneLds lds;
+  if (blockIdx.x != 0) return fill_rows<S, EPL>(a, f, blockIdx.x - 1, lds.taken);
+  OneSpace &sp = lds.one;
+  const unsigned tid = threadIdx.x, lane = tid & (SGH_WAVE - 1), wave = tid >> 6;
+  const unsigned per_wave = (s.tokens + kSortThreads - 1) / kSortThreads * SGH_WAVE;
+  Held<kOneItems> h;
+#pragma unroll
+  for (int u = 0; u < kOneItems; ++u) {
+    const unsigned i = wave * per_wave + u * SGH_WAVE + lane;
+    const bool there = u * SGH_WAVE < per_wave && i < s.tokens;
+    h.place[u] = there ? i : kNoPlace;
+    h.key[u] = there ? unsigned(s.ids[i]) : 0;
+  }
+#pragma unroll
+  for (int u = 0; u < kOneItems; ++u) h.key[u] = counted_key(s, int(h.key[u]), h.place[u] != kNoPlace);
+  for (int pass = 0; pass < passes; ++pass) {
+    s.shift = pass * digit_bits;
+    clear_counts(sp.sort);
+    __syncthreads();
+    sort_rank(s, per_wave, sp.sort, h);
+    __syncthreads();
+    const unsigned lower = lower_digits(sp.sort, tid < unsigned(s.bins) ? front_counts(sp.sort) : 0);
+    if (tid < unsigned(s.bins)) sp.sort.next[tid] = lower;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kOneItems; ++u)
+      if (h.place[u] != kNoPlace) {
+        const unsigned to = place_of(s, sp.sort, h.key[u], h.rank[u]);
+        sp.key[to] = h.key[u];
+        sp.place[to] = uint16_t(h.place[u]);
+      }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kOneItems; ++u) {
+      const unsigned i = wave * per_wave + u * SGH_WAVE + lane;
+      if (h.place[u] != kNoPlace) h.key[u] = sp.key[i], h.place[u] = sp.place[i];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kOneItems; ++u)
+    if (h.place[u] != kNoPlace) s.out[wave * per_wave + u * SGH_WAVE + lane] = Token{h.key[u], h.place[u]};
+}
+
+union SortLds {
+  SortSpace sort;
+  unsigned char taken[kFillRows];
+};
+
+template <class S, int EPL>
+__global__ __launch_bounds__(kSortThreads) void k_embed_count(Bwd<typename S::elem> a, Sort s, Fill f) {
+  __shared__ SortLds lds;
+  if (blockIdx.x >= unsigned(s.stretches)) return fill_rows<S, EPL>(a, f, blockIdx.x - s.stretches, lds.taken);
+  unsigned *h = lds.sort.next;
+  for (int d = threadIdx.x; d < s.bins; d += kSortThreads) h[d] = 0;
+  __syncthreads();
+  const unsigned from = blockIdx.x * s.per_stretch, left = s.tokens - from;
+  count_digits(s, from, from + (left < s.per_stretch ? left : s.per_stretch), h);
+  __syncthreads();
+  for (int d = threadIdx.x; d < s.bins; d += kSortThreads) s.counts[blockIdx.x * s.bins + d] = h[d];
+}
+
+template <class S, int EPL>
+__global__ __launch_bounds__(kSortThreads) void k_embed_move(Bwd<typename S::elem> a, Sort s, Fill f) {
+  __shared__ SortLds lds;
+  if (blockIdx.x >= unsigned(s.stretches)) return fill_rows<S, EPL>(a, f, blockIdx.x - s.stretches, lds.taken);
+  SortSpace &sp = lds.sort;
+  const int tid = threadIdx.x;
+  // all tokens of a digit, and those of the stretches in front, by the threads that share it
+  const int digit = tid & (s.bins - 1), share = tid / s.bins, shares = kSortThreads / s.bins;
+  unsigned all = 0, before = 0;
+#pragma unroll 8
+  for (int b = share; b < s.stretches; b += shares) {
+    const unsigned c = s.counts[b * s.bins + digit];
+    all += c;
+    before += b < int(blockIdx.x) ? c : 0;
+  }
+  unsigned *of_thread = reinterpret_cast<unsigned *>(&sp.in_wave[0][0]);   // two values of every thread
+  of_thread[tid] = all;
+  of_thread[kSortThreads + tid] = before;
+  __syncthreads();
+  if (tid < s.bins)
+    for (int o = 1; o < shares; ++o) all += of_thread[o * s.bins + tid], before += of_thread[kSortThreads + o * s.bins + tid];
+  before += lower_digits(sp, tid < s.bins ? all : 0);
+  __syncthreads();
+  const unsigned from = blockIdx.x * s.per_stretch, left = s.tokens - from;
+  const size_t to = size_t(from) + (left < s.per_stretch ? left : s.per_stretch);
+  const unsigned lane = tid & (SGH_WAVE - 1), wave = tid >> 6, per_wave = SGH_WAVE * kItems;
+  if (tid < s.bins) sp.next[tid] = before;
+  for (size_t base = from; base < to; base += kStretch) {
+    clear_counts(sp);
+    Held<kItems> h;
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+      const size_t i = base + wave * per_wave + u * SGH_WAVE + lane;
+      Token t = {0, kNoPlace};
+      if (i < to) t = s.ids ? Token{unsigned(s.ids[i]), unsigned(i)} : s.in[i];
+      h.key[u] = t.key, h.place[u] = t.place;
+    }
+    if (s.ids) {
+#pragma unroll
+      for (int u = 0; u < kItems; ++u) h.key[u] = counted_key(s, int(h.key[u]), h.place[u] != kNoPlace);
+    }
+    __syncthreads();
+    sort_rank(s, per_wave, sp, h);
+    __syncthreads();
+    const unsigned total = tid < s.bins ? front_counts(sp) : 0;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kItems; ++u)
+      if (h.place[u] != kNoPlace) s.out[place_of(s, sp, h.key[u], h.rank[u])] = Token{h.key[u], h.place[u]};
+    __syncthreads();
+    if (tid < s.bins) sp.next[tid] += total;
+  }
+}
+
+constexpr unsigned kNoKey = 0xffffffffu;
+
+// Where a wavefront's lanes are: a tile of its own for every `lanes` of them, and a vector of the rows
+__host__ __device__ inline unsigned slices_at_once(int slices) { return slices < kWaves ? slices : kWaves; }   // of a workgroup
+__host__ __device__ inline unsigned tiles_at_once(int lanes, int slices) { return kWaves / slices_at_once(slices) * (SGH_WAVE / lanes); }
+struct Spot {
+  unsigned tile;   // of the workgroup's
+  size_t vec;
+};
+template <class T>
+__device__ __forceinline__ Spot spot_of(const Bwd<T> &a) {
+  const unsigned lane = threadIdx.x & (SGH_WAVE - 1), wave = threadIdx.x >> 6, each = slices_at_once(a.slices);
+  return {wave / each * (SGH_WAVE / a.lanes) + lane / a.lanes,
+          (size_t(blockIdx.y) * each + wave % each) * SGH_WAVE + (lane & (a.lanes - 1))};
+}
+
+// (LDS: the ids and places of the workgroup's tiles and of one tile behind them, the id in front first)
+template <class S, int EPL>
+__global__ __launch_bounds__(kBlock) void k_embed_tiles(Bwd<typename S::elem> a) {
+  extern __shared__ unsigned lds[];
+  const unsigned tiles = tiles_at_once(a.lanes, a.slices);
+  const size_t base = size_t(blockIdx.x) * tiles * a.tile;
+  const unsigned room = (tiles + 1) * a.tile, count = a.tokens - base < room ? unsigned(a.tokens - base) : room;
+  unsigned *keys = lds + 1, *places = lds + 1 + room;
+  if (threadIdx.x == 0) lds[0] = base ? a.sorted[base - 1].key : kNoKey;
+  for (unsigned i = threadIdx.x; i < count; i += kBlock) {
+    const Token t = a.sorted[base + i];
+    keys[i] = t.key, places[i] = t.place;
+  }
+  __syncthreads();
+  const Spot sp = spot_of(a);
+  const unsigned first = sp.tile * a.tile;
+  if (sp.tile >= tiles || first >= count || sp.vec * EPL >= a.dim) return;
+  const size_t at = sp.vec * EPL + EPL > a.dim ? a.dim - EPL : sp.vec * EPL;
+  const unsigned stop = count - first < a.tile ? count : first + a.tile, lead = lds[first], last = keys[stop - 1];
+  const bool goes_on = stop < count && keys[stop] == last;   // the last row's tokens go on behind the tile, ...
+  const bool joined = goes_on && count - stop >= a.tile && keys[stop + a.tile - 1] == last;   // ... and hold the next one whole
+  float acc[EPL];
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) acc[j] = 0.f;
+  const size_t index = size_t(blockIdx.x) * tiles + sp.tile;
+  float *sums = a.partial + index * 2 * a.pitch + at;
+  auto keep = [&](float *out) {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) out[j] = acc[j];
+  };
+  if (stop - first == a.tile && keys[first] == last) {   // all of one row
+    const bool begins = lead != last;
+    if (sp.vec == 0) a.tail[index] = begins && goes_on && last < a.vocab ? unsigned(2 * index) : kNoKey;
+    if (last >= a.vocab) return;
+    add_tokens<S, EPL>(a.dy, a.dim, at, places, first, stop, acc);
+    if (begins && !goes_on) return store_row<S, EPL>(a, last, at, sp.vec, acc);
+    return keep(sums);
+  }
+  // the rows whose tokens begin here, the last one's to their end (less than a tile further) or, where it is to be joined, to the end of
+  // the tile; and the head of a row that holds the tile in front whole
+  const bool led = base + first >= a.tile && a.sorted[base + first - a.tile].key == lead && lead < a.vocab;
+  constexpr int U = EPL == 8 ? 8 : 16;   // (64 floats: 16 vectors of 16-bit elements 115 -> 165 us at 65536 tokens of 2048)
+  unsigned row = kNoKey;
+  auto done = [&]() {
+    if (row == kNoKey) return;
+    if (row == lead) keep(sums);
+    else if (joined && row == last) keep(sums + a.pitch);
+    else store_row<S, EPL>(a, row, at, sp.vec, acc);
+  };
+  for (unsigned i = first;; i += U) {
+    unsigned key[U];
+    float v[U][EPL];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const unsigned k = i + u < count ? keys[i + u] : kNoKey;
+      const bool inside = i + u < stop;
+      const bool here = k < a.vocab && (k == lead ? inside && led : inside || (k == last && !joined));
+      key[u] = here ? k : kNoKey;
+      if (here) sgh_load_any<S, EPL>(a.dy + size_t(places[i + u]) * a.dim + at, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (key[u] != row) {
+        done();
+        row = key[u];
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) acc[j] = 0.f;
+      }
+      if (key[u] != kNoKey) {
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) acc[j] += v[u][j];
+      }
+    }
+    if (i + U >= stop && key[U - 1] == kNoKey) break;   // (behind the tile only its last row's tokens count)
+  }
+  done();
+  if (sp.vec == 0) a.tail[index] = joined && last < a.vocab ? unsigned(2 * index + 1) : kNoKey;
+}
+
+// Rows whose tokens hold whole tiles, from the tile in which they begin: the sum of their tokens there, of the whole tiles, and of the tokens
+// behind
+template <class S, int EPL>
+__global__ __launch_bounds__(kBlock) void k_embed_join(Bwd<typename S::elem> a) {
+  const unsigned tiles = tiles_at_once(a.lanes, a.slices);
+  const Spot sp = spot_of(a);
+  const size_t index = size_t(blockIdx.x) * tiles + sp.tile;
+  if (sp.tile >= tiles || index * a.tile >= a.tokens) return;
+  const unsigned from = a.tail[index];
+  if (from == kNoKey) return;
+  const unsigned lane = threadIdx.x & (SGH_WAVE - 1), of_tile = lane & (a.lanes - 1);
+  const size_t at = sp.vec * EPL + EPL > a.dim ? a.dim - EPL : sp.vec * EPL;
+  const unsigned row = a.sorted[(index + 1) * a.tile - 1].key;
+  // tiles behind this one that begin with a token of the row: a lane asks for one
+  size_t more = 0;
+  for (;;) {
+    const size_t begin = (index + 1 + more + of_tile) * a.tile;
+    const unsigned long long is = __ballot(begin < a.tokens && a.sorted[begin].key == row) >> (lane - of_tile);
+    const unsigned n = ~is ? unsigned(__builtin_ctzll(~is)) : SGH_WAVE;
+    more += n < unsigned(a.lanes) ? n : a.lanes;
+    if (n < unsigned(a.lanes)) break;
+  }
+  if (sp.vec * EPL >= a.dim) return;
+  float acc[EPL];
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) acc[j] = 0.f;
+  const float *p = a.partial + size_t(from) * a.pitch + at;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) acc[j] += p[j];
+  p = a.partial + (index + 1) * 2 * a.pitch + at;
+  constexpr int U = EPL == 8 ? 8 : 16;
+  for (size_t t = 0; t < more; t += U, p += U * 2 * a.pitch) {
+    float v[U][EPL];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (t + u < more) {
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) v[u][j] = p[u * 2 * a.pitch + j];
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (t + u < more) {
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) acc[j] += v[u][j];
+      }
+  }
+  store_row<S, EPL>(a, row, at, sp.vec, acc);
+}
+
 struct BwdPlan {
-  bool scan;
-  unsigned tile, tiles;             // whole tiles
+  bool scan, one;
+  unsigned tile, tiles;
   int passes, digit_bits, stretches;
   unsigned per_stretch;
-  size_t keys, places, keys2, places2, counts, partial, bytes;   // offsets into the workspace
+  size_t other, counts, tail, taken, partial, bytes;   // offsets into the workspace
 };
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
-BwdPlan bwd_plan(size_t tokens, size_t vocab, size_t dim) {
+BwdPlan bwd_plan(size_t tokens, size_t vocab, size_t dim, int vec) {
   BwdPlan p = {};
   p.scan = tokens <= kScanTokens;
   if (p.scan) return p;
-  p.tile = 64;   // near the root of the tokens: neither the tokens of a tile nor the tiles of a row are a long sum
-  while (size_t(p.tile) * p.tile * 16 < tokens) p.tile *= 2;
-  p.tiles = unsigned(tokens / p.tile);
+  p.one = tokens <= kOneTokens;
+  // tokens of a tile: few, so that neither a tile nor the tiles of one row are a long sum, more where there are wavefronts enough
+  const RowLanes r = row_lanes(dim, vec);
+  p.tile = 16;
+  while (p.tile < 128 && (tokens / p.tile) * r.slices / (SGH_WAVE / r.lanes) > size_t(8192)) p.tile *= 2;
+  p.tiles = unsigned((tokens + p.tile - 1) / p.tile);
   int bits = 1;
   while ((vocab >> bits) != 0) ++bits;   // (the largest key is `vocab`)
   p.passes = (bits + kDigitBits - 1) / kDigitBits;
@@ -479,61 +762,88 @@ BwdPlan bwd_plan(size_t tokens, size_t vocab, size_t dim) {
   const size_t each = (stretches + kMostStretches - 1) / kMostStretches;
   p.per_stretch = unsigned(each * kStretch);
   p.stretches = int((stretches + each - 1) / each);
-  const size_t list = up256(tokens * 4);
-  p.places = list;
-  p.keys2 = 2 * list;
-  p.places2 = 3 * list;
-  p.counts = 4 * list;
-  p.partial = p.counts + up256(size_t(p.stretches) * kBins * 4);
-  p.bytes = p.partial + up256(size_t(p.tiles) * dim * 4);
+  const size_t list = up256(tokens * sizeof(Token));
+  p.other = list;
+  p.counts = p.one ? list : 2 * list;
+  p.tail = p.counts + (p.one ? 0 : up256(size_t(p.stretches) * kBins * 4));
+  p.taken = p.tail + up256(size_t(p.tiles) * 4);
+  p.partial = p.taken + (p.one ? 0 : up256(vocab));
+  p.bytes = p.partial + 2 * size_t(p.tiles) * up256(dim * 4);
   return p;
 }
 
+// (enough for either size of element)
+size_t bwd_workspace(size_t tokens, size_t vocab, size_t dim) {
+  const size_t four = bwd_plan(tokens, vocab, dim, StF32::VEC).bytes, two = bwd_plan(tokens, vocab, dim, StF16::VEC).bytes;
+  return four > two ? four : two;
+}
+
 template <class S, int EPL>
-int launch_bwd(Rows<typename S::elem> a, const BwdPlan &p, void *workspace, hipStream_t s) {
-  constexpr size_t e = sizeof(typename S::elem);
-  if (!p.scan) {
-    char *ws = static_cast<char *>(workspace);
-    auto at = [&](size_t off) { return reinterpret_cast<unsigned *>(ws + off); };
-    const unsigned *keys = nullptr, *places = nullptr;
-    unsigned *counts = at(p.counts);
-    for (int pass = 0; pass < p.passes; ++pass) {
-      const int32_t *ids = pass == 0 ? a.ids : nullptr;
-      unsigned *k = at(pass % 2 ? p.keys2 : 0), *pl = at(pass % 2 ? p.places2 : p.places);
-      const int shift = pass * p.digit_bits, bins = 1 << p.digit_bits;
-      hipLaunchKernelGGL(k_embed_count, dim3(p.stretches), dim3(kSortThreads), 0, s, ids, keys, a.tokens, unsigned(a.vocab), a.pad, shift,
-                         bins, p.per_stretch, counts);
-      SGH_LAUNCH_CHECK();
-      hipLaunchKernelGGL(k_embed_move, dim3(p.stretches), dim3(kSortThreads), 0, s, ids, keys, places, a.tokens, unsigned(a.vocab), a.pad,
-                         shift, bins, p.per_stretch, counts, k, pl);
-      SGH_LAUNCH_CHECK();
-      keys = k, places = pl;
-    }
-    a.keys = keys, a.places = places;
-    a.partial = reinterpret_cast<float *>(ws + p.partial);
-    a.tile = p.tile;
-    const int ny = (a.slices + kWaves - 1) / kWaves;
-    hipLaunchKernelGGL((k_embed_tiles<S, EPL>), dim3(p.tiles, ny), dim3(kBlock), 0, s, a);
-    SGH_LAUNCH_CHECK();
-  }
+int launch_scan(const Bwd<typename S::elem> &a, hipStream_t s) {
   // about 32 KB of the result for a workgroup, the whole chip busy where the table is large enough
-  const int per_wave = SGH_WAVE / a.lanes;
-  size_t rows = (size_t(32) << 10) / (a.dim * e);
-  const size_t spread = a.vocab / (size_t(sgh_num_cus()) * 8);
+  const size_t per_wave = SGH_WAVE / a.lanes, cus = size_t(sgh_num_cus());
+  size_t rows = (size_t(32) << 10) / (a.dim * sizeof(typename S::elem));
+  const size_t spread = a.vocab / (cus * 8);
   if (rows > spread) rows = spread;
-  if (rows < size_t(per_wave)) rows = per_wave;
-  if (rows > size_t(kMostRows)) rows = kMostRows;
-  while ((a.vocab + rows - 1) / rows > (1u << 23)) rows *= 2;   // (2^31 rows at the most: 2^8 of them suffice)
-  if (rows > size_t(kMostRows)) rows = kMostRows;
-  a.rows = int(rows);
+  if (rows < per_wave) rows = per_wave;
+  while ((a.vocab + rows - 1) / rows > (1u << 23)) rows *= 2;
+  if (rows > size_t(kMostRows)) rows = kMostRows;   // (2^31 rows at the most: 2^23 workgroups)
   const size_t blocks = (a.vocab + rows - 1) / rows;
   const size_t units = (rows + per_wave - 1) / per_wave * size_t(a.slices);
-  size_t ny = blocks >= size_t(sgh_num_cus()) * 4 ? 1 : (size_t(sgh_num_cus()) * 4 + blocks - 1) / blocks;
+  size_t ny = blocks >= cus * 4 ? 1 : (cus * 4 + blocks - 1) / blocks;
   if (ny > (units + kWaves - 1) / kWaves) ny = (units + kWaves - 1) / kWaves;
-  if (p.scan)
-    hipLaunchKernelGGL((k_embed_rows<S, EPL, true>), dim3(unsigned(blocks), unsigned(ny)), dim3(kBlock), 0, s, a);
-  else
-    hipLaunchKernelGGL((k_embed_rows<S, EPL, false>), dim3(unsigned(blocks), unsigned(ny)), dim3(kBlock), 0, s, a);
+  hipLaunchKernelGGL((k_embed_rows<S, EPL>), dim3(unsigned(blocks), unsigned(ny)), dim3(kBlock), 0, s, a, int(rows));
+  SGH_LAUNCH_CHECK();
+  return SGH_OK;
+}
+
+template <class S, int EPL>
+int launch_bwd(Bwd<typename S::elem> a, const BwdPlan &p, void *workspace, hipStream_t s) {
+  if (p.scan) return launch_scan<S, EPL>(a, s);
+  char *ws = static_cast<char *>(workspace);
+  auto at = [&](size_t off) { return reinterpret_cast<unsigned *>(ws + off); };
+  Token *sorted = reinterpret_cast<Token *>(ws), *other = reinterpret_cast<Token *>(ws + p.other);
+  a.sorted = sorted, a.tail = at(p.tail);
+  a.partial = reinterpret_cast<float *>(ws + p.partial);
+  a.tile = p.tile, a.pitch = up256(a.dim * 4) / 4;
+  // the rows without a token, spread over the launches that sort: at least 64 KB of the result for a workgroup
+  Fill f = {0, 0, p.one ? 1 : 2 * p.passes, reinterpret_cast<unsigned char *>(ws + p.taken)};
+  unsigned fill_blocks = 0;
+  if (a.add != a.dW) {
+    size_t want = (a.vocab * a.dim * sizeof(typename S::elem) >> 16) / f.launches;
+    if (want > size_t(sgh_num_cus()) * 2) want = size_t(sgh_num_cus()) * 2;
+    if (want < 1) want = 1;
+    size_t rows = (a.vocab + want - 1) / want;
+    if (rows > kFillRows) rows = kFillRows;
+    f.rows = unsigned(rows);
+    fill_blocks = unsigned((a.vocab + rows - 1) / rows);
+  }
+  Sort so = {};
+  so.ids = a.ids, so.counts = at(p.counts), so.tokens = a.tokens, so.vocab = unsigned(a.vocab), so.pad = a.pad;
+  so.bins = 1 << p.digit_bits, so.stretches = p.stretches, so.per_stretch = p.per_stretch;
+  if (p.one) {
+    so.out = sorted;
+    hipLaunchKernelGGL((k_embed_sort<S, EPL>), dim3(1 + fill_blocks), dim3(kSortThreads), 0, s, a, so, p.passes, p.digit_bits, f);
+    SGH_LAUNCH_CHECK();
+  } else {
+    for (int pass = 0; pass < p.passes; ++pass) {
+      so.out = (p.passes - 1 - pass) & 1 ? other : sorted;
+      so.shift = pass * p.digit_bits;
+      hipLaunchKernelGGL((k_embed_count<S, EPL>), dim3(p.stretches + fill_blocks), dim3(kSortThreads), 0, s, a, so, f);
+      SGH_LAUNCH_CHECK();
+      ++f.launch;
+      hipLaunchKernelGGL((k_embed_move<S, EPL>), dim3(p.stretches + fill_blocks), dim3(kSortThreads), 0, s, a, so, f);
+      SGH_LAUNCH_CHECK();
+      ++f.launch;
+      so.ids = nullptr, so.in = so.out;
+    }
+  }
+  if (a.lanes < 8) a.lanes = 8;   // (LDS holds the tiles of a workgroup: 32 at most)
+  const unsigned tiles = tiles_at_once(a.lanes, a.slices), each = slices_at_once(a.slices);
+  const dim3 grid{(p.tiles + tiles - 1) / tiles, (a.slices + each - 1) / each};
+  hipLaunchKernelGGL((k_embed_tiles<S, EPL>), grid, dim3(kBlock), (2 * (tiles + 1) * p.tile + 1) * 4, s, a);
+  SGH_LAUNCH_CHECK();
+  hipLaunchKernelGGL((k_embed_join<S, EPL>), grid, dim3(kBlock), 0, s, a);
   SGH_LAUNCH_CHECK();
   return SGH_OK;
 }
@@ -548,13 +858,14 @@ int embed_bwd(const int32_t *ids, const typename S::elem *dy, const typename S::
   if ((tokens != 0 && (!ids || !dy)) || !dW) return SGH_EINVAL;
   if (sgh_ranges_meet(dW, bytes, dy, tokens * dim * e) || sgh_ranges_meet(dW, bytes, ids, tokens * 4)) return SGH_EINVAL;
   if (add && add != dW && sgh_ranges_meet(dW, bytes, add, bytes)) return SGH_EINVAL;
-  const BwdPlan p = bwd_plan(tokens, vocab, dim);
+  const BwdPlan p = bwd_plan(tokens, vocab, dim, S::VEC);
   if (p.bytes != 0 && (!workspace || ws_bytes < p.bytes)) return SGH_EWORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) % alignof(Token) != 0) return SGH_EINVAL;
   hipStream_t s = sgh_stream_of(stream);
   sgh_note_write(dW, bytes);
   sgh_prof_scope prof("embedding_bwd", double(tokens) * (4 + double(dim) * e) + double(bytes) * (add ? 2 : 1), s);
-  const RowLanes r = row_lanes<S>(dim);
-  Rows<typename S::elem> a = {};
+  const RowLanes r = row_lanes(dim, S::VEC);
+  Bwd<typename S::elem> a = {};
   a.dy = dy, a.add = add, a.dW = dW, a.ids = ids, a.dim = dim, a.vocab = vocab, a.tokens = unsigned(tokens), a.tile = 1;
   a.scale = scale, a.pad = pad, a.lanes = r.lanes, a.slices = r.slices;
   return r.epl == 1 ? launch_bwd<S, 1>(a, p, workspace, s) : launch_bwd<S, S::VEC>(a, p, workspace, s);
@@ -579,7 +890,7 @@ SGH_EMBEDDING(bf16, StBF16, uint16_t)
 #undef SGH_EMBEDDING
 
 size_t sgh_embedding_bwd_workspace_bytes(size_t tokens, size_t vocab, size_t dim) {
-  return sizes_ok(tokens, vocab, dim) && vocab != 0 && dim != 0 ? bwd_plan(tokens, vocab, dim).bytes : 0;
+  return sizes_ok(tokens, vocab, dim) && vocab != 0 && dim != 0 ? bwd_workspace(tokens, vocab, dim) : 0;
 }
 
 int sgh_embedding_index_errors(void *stream, int *count) {

@@ -190,6 +190,24 @@ def test_embedding_gradient_of_one_row_with_all_tokens(dev):
         assert np.array_equal(dW.to_numpy(), O.embedding_bwd(dy, ids, (4, 12)))
 
 
+def test_embedding_gradient_of_rows_that_end_with_a_tile(dev):
+    """Rows of whole tiles side by side, of whole tiles and some, and of less than a tile, in memory that held large numbers."""
+    from singa_amd import singa_wrap as singa
+    from singa_amd._lib import lib
+    r = np.random.default_rng(6)
+    for unit in (32, 64, 128):
+        for runs in ([2, 2, 2, 40], [1, 3, 0.5, 0.5, 2, 30, 1], [40, 1, 0.25, 1.75, 1], [0.5, 35, 0.5, 1, 1, 1, 1.5, 2.5]):
+            ids = r.permutation(np.repeat(np.arange(len(runs)), [int(n * unit) for n in runs]))
+            vocab, dim = len(runs) + 1, 20
+            dy = r.integers(-8, 9, (ids.size, dim)).astype(np.float32)
+            need = lib().sgh_embedding_bwd_workspace_bytes(ids.size, vocab, dim)
+            assert need
+            dirty = singa.from_numpy(np.full(need // 4, 0x7f7f7f7f, np.int32), dev)
+            del dirty    # (the pool hands this block to the call)
+            dW = singa.EmbeddingBackwardW(upload(singa, dev, "f32", dy), ints(singa, dev, ids), upload(singa, dev, "f32", np.zeros((vocab, dim))))
+            assert np.array_equal(dW.to_numpy(), O.embedding_bwd(dy, ids, (vocab, dim)))
+
+
 # ------------------------------------------------------------------------------------ distillation
 
 def make_case(r, t, n, v, k, masked=True):
