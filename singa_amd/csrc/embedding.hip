@@ -119,31 +119,31 @@ struct Bwd {
   float *partial;                  // [tiles][2][pitch]: sums of a row's tokens that hold whole tiles: a tile's head or all of it, its tail
   size_t pitch;
   size_t dim, vocab;
-  unsigned tokens, tile;           // sorted tokens that a wavefront goes through
+  unsigned tokens, tile, stretch;  // sorted tokens of a tile, of a workgroup
   float scale;
   int pad, lanes, slices;
 };
 
-// Stores one vector of a row: acc * scale on top of `add`.  `moved`: the row's last vector, moved back to end with the row; its first
-// elements are the vector's before it, which may be stored already where `add` is the result itself.
+// One vector of a row of `add` (zeros without one), asked for before the sums so that the two waits are one, and the store of acc * scale on
+// top of it.  The row's last vector is moved back to end with the row (at != vec * EPL): its first elements are the vector's before it,
+// which may be stored already where `add` is the result itself, and are left alone.
 template <class S, int EPL>
-__device__ __forceinline__ void store_row(const Bwd<typename S::elem> &a, size_t row, size_t at, size_t vec, float *acc) {
-  typename S::elem *out = a.dW + row * a.dim + at;
-  const typename S::elem *add = a.add ? a.add + row * a.dim + at : nullptr;
+__device__ __forceinline__ void load_add(const Bwd<typename S::elem> &a, size_t row, size_t at, float *g) {
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) acc[j] *= a.scale;
-  if (at != vec * EPL) {
+  for (int j = 0; j < EPL; ++j) g[j] = 0.f;
+  if (a.add) sgh_load_any<S, EPL>(a.add + row * a.dim + at, g);
+}
+template <class S, int EPL>
+__device__ __forceinline__ void store_row(const Bwd<typename S::elem> &a, size_t row, size_t at, size_t vec, float *acc, const float *g) {
+  typename S::elem *out = a.dW + row * a.dim + at;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) acc[j] = acc[j] * a.scale + g[j];
+  if (at == vec * EPL) {
+    sgh_store_any<S, EPL>(out, acc);
+  } else {
 #pragma unroll
     for (int j = 0; j < EPL; ++j)
-      if (at + j >= vec * EPL) S::st(out + j, add ? S::ld(add + j) + acc[j] : acc[j]);
-  } else {
-    if (add) {
-      float g[EPL];
-      sgh_load_any<S, EPL>(add, g);
-#pragma unroll
-      for (int j = 0; j < EPL; ++j) acc[j] += g[j];
-    }
-    sgh_store_any<S, EPL>(out, acc);
+      if (at + j >= vec * EPL) S::st(out + j, acc[j]);
   }
 }
 
@@ -287,7 +287,9 @@ __global__ __launch_bounds__(kBlock) void k_embed_rows(Bwd<typename S::elem> a, 
 #pragma unroll
     for (int j = 0; j < EPL; ++j) acc[j] = 0.f;
     add_tokens<S, EPL>(a.dy, a.dim, at, found, b, e, acc);
-    store_row<S, EPL>(a, row0 + r, at, vec, acc);
+    float g[EPL];
+    load_add<S, EPL>(a, row0 + r, at, g);
+    store_row<S, EPL>(a, row0 + r, at, vec, acc, g);
   }
 }
 
@@ -417,17 +419,17 @@ __device__ __forceinline__ unsigned counted_key(const Sort &s, int id, bool ther
 template <class S, int EPL>
 __device__ __forceinline__ void fill_rows(const Bwd<typename S::elem> &a, const Fill &f, unsigned part, unsigned char *taken) {
   const size_t row0 = size_t(part) * f.rows;
-  const unsigned rows = a.vocab - row0 < f.rows ? unsigned(a.vocab - row0) : f.rows;
+  const unsigned rows = a.vocab - row0 < f.rows ? unsigned(a.vocab - row0) : f.rows, threads = kSortThreads;
   const unsigned tid = threadIdx.x, lane = tid & (SGH_WAVE - 1), wave = tid >> 6;
-  const unsigned lo = unsigned(size_t(rows) * f.launch / f.launches), hi = unsigned(size_t(rows) * (f.launch + 1) / f.launches);
+  const unsigned lo = rows * f.launch / f.launches, hi = rows * (f.launch + 1) / f.launches;   // its share
   if (f.launch == 0) {
-    for (unsigned r = tid; r < rows; r += kSortThreads) taken[r] = 0;
+    for (unsigned r = tid; r < rows; r += threads) taken[r] = 0;
     __syncthreads();
     constexpr unsigned U = 8;
-    for (size_t i = tid; i < a.tokens; i += U * kSortThreads) {
+    for (size_t i = tid; i < a.tokens; i += U * threads) {
       int id[U];
 #pragma unroll
-      for (unsigned u = 0; u < U; ++u) id[u] = i + u * kSortThreads < a.tokens ? a.ids[i + u * kSortThreads] : a.pad;
+      for (unsigned u = 0; u < U; ++u) id[u] = i + u * threads < a.tokens ? a.ids[i + u * threads] : a.pad;
 #pragma unroll
       for (unsigned u = 0; u < U; ++u) {
         const size_t r = size_t(id[u]) - row0;   // (an id below the rows, or below 0, is a large number)
@@ -435,29 +437,36 @@ __device__ __forceinline__ void fill_rows(const Bwd<typename S::elem> &a, const 
       }
     }
     __syncthreads();
-    for (unsigned r = hi + tid; r < rows; r += kSortThreads) f.taken[row0 + r] = taken[r];
+    for (unsigned r = hi + tid; r < rows; r += threads) f.taken[row0 + r] = taken[r];
   } else {
-    for (unsigned r = lo + tid; r < hi; r += kSortThreads) taken[r] = f.taken[row0 + r];
+    for (unsigned r = lo + tid; r < hi; r += threads) taken[r] = f.taken[row0 + r];
     __syncthreads();
   }
   const size_t vecs = (a.dim + EPL - 1) / EPL;
   const unsigned per_wave = SGH_WAVE / a.lanes;
   constexpr int U = 4;
-  for (unsigned r = lo + wave * per_wave + lane / a.lanes; r < hi; r += kSortWaves * per_wave) {
-    if (taken[r]) continue;
-    for (size_t vec = lane & (a.lanes - 1); vec < vecs; vec += U * SGH_WAVE) {
-      float v[U][EPL];
-      size_t at[U];
+  const unsigned waves = threads / SGH_WAVE;
+  for (unsigned r0 = lo + wave; r0 < hi; r0 += threads) {   // every `waves`-th row is a wavefront's, a lane asks for each of 64
+    const unsigned asked = r0 + lane * waves;
+    const unsigned long long free = __ballot(asked < hi && !taken[asked]);
+    for (unsigned i = lane / a.lanes; i < SGH_WAVE && r0 + i * waves < hi; i += per_wave) {
+      if (!(free >> i & 1)) continue;
+      const size_t row = (row0 + r0 + i * waves) * a.dim;
+      for (size_t vec = lane & (a.lanes - 1); vec < vecs; vec += U * SGH_WAVE) {
+        float v[U][EPL];
+        size_t at[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        at[u] = (row0 + r) * a.dim + ((vec + u * SGH_WAVE) * EPL + EPL > a.dim ? a.dim - EPL : (vec + u * SGH_WAVE) * EPL);
+        for (int u = 0; u < U; ++u) {
+          const size_t n = vec + u * SGH_WAVE;
+          at[u] = row + (n * EPL + EPL > a.dim ? a.dim - EPL : n * EPL);
 #pragma unroll
-        for (int j = 0; j < EPL; ++j) v[u][j] = 0.f;
-        if (a.add && vec + u * SGH_WAVE < vecs) sgh_load_any<S, EPL>(a.add + at[u], v[u]);
+          for (int j = 0; j < EPL; ++j) v[u][j] = 0.f;
+          if (a.add && n < vecs) sgh_load_any<S, EPL>(a.add + at[u], v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (vec + u * SGH_WAVE < vecs) sgh_store_any<S, EPL>(a.dW + at[u], v[u]);
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (vec + u * SGH_WAVE < vecs) sgh_store_any<S, EPL>(a.dW + at[u], v[u]);
     }
   }
 }
@@ -607,83 +616,89 @@ __device__ __forceinline__ Spot spot_of(const Bwd<T> &a) {
           (size_t(blockIdx.y) * each + wave % each) * SGH_WAVE + (lane & (a.lanes - 1))};
 }
 
-// (LDS: the ids and places of the workgroup's tiles and of one tile behind them, the id in front first)
+// A workgroup has `a.stretch` neighbours of the sorted list (whole tiles).  Its threads first work out the jobs that begin there, each a sum
+// of neighbouring tokens that becomes a row of the result or is kept for joining: the tokens of a row that hold no whole tile (they may end
+// in the next one), or a row's piece of a tile.  Then the wavefronts take the jobs in turn, `lanes` lanes and a vector of each to a job.
+// (One wavefront that goes through a tile's tokens with loads of several jobs in flight needs its store once for each of them: the code no
+// longer fits the instruction cache, 6 -> 13 us at 2048 tokens of 64.)
 template <class S, int EPL>
 __global__ __launch_bounds__(kBlock) void k_embed_tiles(Bwd<typename S::elem> a) {
-  extern __shared__ unsigned lds[];
-  const unsigned tiles = tiles_at_once(a.lanes, a.slices);
-  const size_t base = size_t(blockIdx.x) * tiles * a.tile;
-  const unsigned room = (tiles + 1) * a.tile, count = a.tokens - base < room ? unsigned(a.tokens - base) : room;
-  unsigned *keys = lds + 1, *places = lds + 1 + room;
-  if (threadIdx.x == 0) lds[0] = base ? a.sorted[base - 1].key : kNoKey;
-  for (unsigned i = threadIdx.x; i < count; i += kBlock) {
-    const Token t = a.sorted[base + i];
+  extern __shared__ unsigned lds[];   // one key in front, the stretch, two tiles behind it; their places; the jobs
+  __shared__ unsigned jobs;
+  const unsigned room = a.stretch + 2 * a.tile;
+  unsigned *keys = lds + 1, *places = keys + room, *from_ = places + room, *to_ = from_ + a.stretch, *dest_ = to_ + a.stretch;
+  const size_t base = size_t(blockIdx.x) * a.stretch;
+  const unsigned count = a.tokens - base < room ? unsigned(a.tokens - base) : room;   // known keys
+  const unsigned mine = count < a.stretch ? count : a.stretch;
+  if (threadIdx.x == 0) {
+    lds[0] = base ? a.sorted[base - 1].key : kNoKey;
+    jobs = 0;
+  }
+  for (unsigned i = threadIdx.x; i < room; i += kBlock) {
+    const Token t = i < count ? a.sorted[base + i] : Token{kNoKey, 0};
     keys[i] = t.key, places[i] = t.place;
   }
+  const unsigned ahead = base >= a.tile ? a.sorted[base - a.tile].key : kNoKey;   // the first key of the tile in front
   __syncthreads();
-  const Spot sp = spot_of(a);
-  const unsigned first = sp.tile * a.tile;
-  if (sp.tile >= tiles || first >= count || sp.vec * EPL >= a.dim) return;
-  const size_t at = sp.vec * EPL + EPL > a.dim ? a.dim - EPL : sp.vec * EPL;
-  const unsigned stop = count - first < a.tile ? count : first + a.tile, lead = lds[first], last = keys[stop - 1];
-  const bool goes_on = stop < count && keys[stop] == last;   // the last row's tokens go on behind the tile, ...
-  const bool joined = goes_on && count - stop >= a.tile && keys[stop + a.tile - 1] == last;   // ... and hold the next one whole
-  float acc[EPL];
-#pragma unroll
-  for (int j = 0; j < EPL; ++j) acc[j] = 0.f;
-  const size_t index = size_t(blockIdx.x) * tiles + sp.tile;
-  float *sums = a.partial + index * 2 * a.pitch + at;
-  auto keep = [&](float *out) {
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) out[j] = acc[j];
-  };
-  if (stop - first == a.tile && keys[first] == last) {   // all of one row
-    const bool begins = lead != last;
-    if (sp.vec == 0) a.tail[index] = begins && goes_on && last < a.vocab ? unsigned(2 * index) : kNoKey;
-    if (last >= a.vocab) return;
-    add_tokens<S, EPL>(a.dy, a.dim, at, places, first, stop, acc);
-    if (begins && !goes_on) return store_row<S, EPL>(a, last, at, sp.vec, acc);
-    return keep(sums);
-  }
-  // the rows whose tokens begin here, the last one's to their end (less than a tile further) or, where it is to be joined, to the end of
-  // the tile; and the head of a row that holds the tile in front whole
-  const bool led = base + first >= a.tile && a.sorted[base + first - a.tile].key == lead && lead < a.vocab;
-  constexpr int U = EPL == 8 ? 8 : 16;   // (64 floats: 16 vectors of 16-bit elements 115 -> 165 us at 65536 tokens of 2048)
-  unsigned row = kNoKey;
-  auto done = [&]() {
-    if (row == kNoKey) return;
-    if (row == lead) keep(sums);
-    else if (joined && row == last) keep(sums + a.pitch);
-    else store_row<S, EPL>(a, row, at, sp.vec, acc);
-  };
-  for (unsigned i = first;; i += U) {
-    unsigned key[U];
-    float v[U][EPL];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const unsigned k = i + u < count ? keys[i + u] : kNoKey;
-      const bool inside = i + u < stop;
-      const bool here = k < a.vocab && (k == lead ? inside && led : inside || (k == last && !joined));
-      key[u] = here ? k : kNoKey;
-      if (here) sgh_load_any<S, EPL>(a.dy + size_t(places[i + u]) * a.dim + at, v[u]);
+  constexpr unsigned kRow = 0x80000000u;   // a job's destination: a row of the result (else one of the kept sums)
+  for (unsigned i = threadIdx.x; i < mine; i += kBlock) {
+    const unsigned k = keys[i], first = i & ~(a.tile - 1), tile = unsigned(base / a.tile) + first / a.tile;
+    if (i == first + a.tile - 1 || i + 1 == mine) {   // the tile's last row: does it begin here, hold a whole tile and go on?
+      const bool whole = i == first + a.tile - 1 && keys[first] == k;
+      const bool joined = keys[int(first) - 1] != k && k < a.vocab && i == first + a.tile - 1 &&
+                          (whole ? keys[i + 1] == k : keys[i + a.tile] == k);
+      if (blockIdx.y == 0) a.tail[tile] = joined ? 2 * tile + (whole ? 0 : 1) : kNoKey;
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (key[u] != row) {
-        done();
-        row = key[u];
-#pragma unroll
-        for (int j = 0; j < EPL; ++j) acc[j] = 0.f;
+    if (k >= a.vocab) continue;
+    const bool begins = keys[int(i) - 1] != k;
+    if (!begins && i != first) continue;
+    const unsigned next = begins ? (i + a.tile - 1) & ~(a.tile - 1) : i;   // where a whole tile could begin
+    const bool whole = keys[next + a.tile - 1] == k;
+    unsigned to, dest;
+    if (whole && next != i) {   // up to the first whole tile
+      to = next, dest = 2 * tile + 1;
+    } else {
+      if (whole) {
+        to = i + a.tile;
+      } else {
+        unsigned lo = i + 1, hi = next + a.tile - 1;   // the first token behind: keys[hi] is one
+        while (lo < hi) {
+          const unsigned mid = (lo + hi) / 2;
+          if (keys[mid] == k) lo = mid + 1;
+          else hi = mid;
+        }
+        to = lo;
       }
-      if (key[u] != kNoKey) {
-#pragma unroll
-        for (int j = 0; j < EPL; ++j) acc[j] += v[u][j];
+      if (begins && !(whole && keys[to] == k)) {
+        dest = kRow;
+      } else {
+        if (!whole && (first ? keys[first - a.tile] : ahead) != k) continue;   // taken by the tile in front
+        dest = 2 * tile;
       }
     }
-    if (i + U >= stop && key[U - 1] == kNoKey) break;   // (behind the tile only its last row's tokens count)
+    const unsigned slot = atomicAdd(&jobs, 1u);
+    from_[slot] = i, to_[slot] = to, dest_[slot] = dest;
   }
-  done();
-  if (sp.vec == 0) a.tail[index] = joined && last < a.vocab ? unsigned(2 * index + 1) : kNoKey;
+  __syncthreads();
+  const unsigned lane = threadIdx.x & (SGH_WAVE - 1), n = jobs, per_wave = SGH_WAVE / a.lanes;
+  const size_t vec = size_t(blockIdx.y) * SGH_WAVE + (lane & (a.lanes - 1));
+  if (vec * EPL >= a.dim) return;
+  const size_t at = vec * EPL + EPL > a.dim ? a.dim - EPL : vec * EPL;
+  for (unsigned j = (threadIdx.x >> 6) * per_wave + lane / a.lanes; j < n; j += kWaves * per_wave) {
+    const unsigned from = from_[j], dest = dest_[j];
+    float acc[EPL], g[EPL];
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) acc[e] = 0.f;
+    if (dest == kRow) load_add<S, EPL>(a, keys[from], at, g);
+    add_tokens<S, EPL>(a.dy, a.dim, at, places, from, to_[j], acc);
+    if (dest == kRow) {
+      store_row<S, EPL>(a, keys[from], at, vec, acc, g);
+    } else {
+      float *out = a.partial + size_t(dest) * a.pitch + at;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) out[e] = acc[e];
+    }
+  }
 }
 
 // Rows whose tokens hold whole tiles, from the tile in which they begin: the sum of their tokens there, of the whole tiles, and of the tokens
@@ -712,6 +727,8 @@ __global__ __launch_bounds__(kBlock) void k_embed_join(Bwd<typename S::elem> a) 
   float acc[EPL];
 #pragma unroll
   for (int j = 0; j < EPL; ++j) acc[j] = 0.f;
+  float g[EPL];
+  load_add<S, EPL>(a, row, at, g);
   const float *p = a.partial + size_t(from) * a.pitch + at;
 #pragma unroll
   for (int j = 0; j < EPL; ++j) acc[j] += p[j];
@@ -732,7 +749,7 @@ __global__ __launch_bounds__(kBlock) void k_embed_join(Bwd<typename S::elem> a) 
         for (int j = 0; j < EPL; ++j) acc[j] += v[u][j];
       }
   }
-  store_row<S, EPL>(a, row, at, sp.vec, acc);
+  store_row<S, EPL>(a, row, at, sp.vec, acc, g);
 }
 
 struct BwdPlan {
@@ -744,15 +761,12 @@ struct BwdPlan {
 };
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
-BwdPlan bwd_plan(size_t tokens, size_t vocab, size_t dim, int vec) {
+BwdPlan bwd_plan(size_t tokens, size_t vocab, size_t dim) {
   BwdPlan p = {};
   p.scan = tokens <= kScanTokens;
   if (p.scan) return p;
   p.one = tokens <= kOneTokens;
-  // tokens of a tile: few, so that neither a tile nor the tiles of one row are a long sum, more where there are wavefronts enough
-  const RowLanes r = row_lanes(dim, vec);
-  p.tile = 16;
-  while (p.tile < 128 && (tokens / p.tile) * r.slices / (SGH_WAVE / r.lanes) > size_t(8192)) p.tile *= 2;
+  p.tile = tokens <= 16384 ? 16 : 32;   // few, so that neither a tile nor the tiles of one row are a long sum
   p.tiles = unsigned((tokens + p.tile - 1) / p.tile);
   int bits = 1;
   while ((vocab >> bits) != 0) ++bits;   // (the largest key is `vocab`)
@@ -770,12 +784,6 @@ BwdPlan bwd_plan(size_t tokens, size_t vocab, size_t dim, int vec) {
   p.partial = p.taken + (p.one ? 0 : up256(vocab));
   p.bytes = p.partial + 2 * size_t(p.tiles) * up256(dim * 4);
   return p;
-}
-
-// (enough for either size of element)
-size_t bwd_workspace(size_t tokens, size_t vocab, size_t dim) {
-  const size_t four = bwd_plan(tokens, vocab, dim, StF32::VEC).bytes, two = bwd_plan(tokens, vocab, dim, StF16::VEC).bytes;
-  return four > two ? four : two;
 }
 
 template <class S, int EPL>
@@ -806,7 +814,8 @@ int launch_bwd(Bwd<typename S::elem> a, const BwdPlan &p, void *workspace, hipSt
   a.sorted = sorted, a.tail = at(p.tail);
   a.partial = reinterpret_cast<float *>(ws + p.partial);
   a.tile = p.tile, a.pitch = up256(a.dim * 4) / 4;
-  // the rows without a token, spread over the launches that sort: at least 64 KB of the result for a workgroup
+  // The rows without a token, spread over the launches that sort: at least 64 KB of the result for a workgroup and launch.  (Leaving a part
+  // for the launch of the tiles, whose own traffic they would run beside, was slower: 44.8 -> 48.9 and 337 -> 400 us for the cases below.)
   Fill f = {0, 0, p.one ? 1 : 2 * p.passes, reinterpret_cast<unsigned char *>(ws + p.taken)};
   unsigned fill_blocks = 0;
   if (a.add != a.dW) {
@@ -838,12 +847,19 @@ int launch_bwd(Bwd<typename S::elem> a, const BwdPlan &p, void *workspace, hipSt
       so.ids = nullptr, so.in = so.out;
     }
   }
-  if (a.lanes < 8) a.lanes = 8;   // (LDS holds the tiles of a workgroup: 32 at most)
-  const unsigned tiles = tiles_at_once(a.lanes, a.slices), each = slices_at_once(a.slices);
-  const dim3 grid{(p.tiles + tiles - 1) / tiles, (a.slices + each - 1) / each};
-  hipLaunchKernelGGL((k_embed_tiles<S, EPL>), grid, dim3(kBlock), (2 * (tiles + 1) * p.tile + 1) * 4, s, a);
+  Bwd<typename S::elem> t = a;
+  if (t.lanes < 8) t.lanes = 8;   // (LDS holds the tokens of a workgroup)
+  // Jobs a wavefront takes one after the other: 4 or fewer while that leaves CUs without work, more where the workgroups' own start counts
+  // (bf16, 65536 tokens of 2048: 351 us with 4, 337 with 8; f32, 8192 of 1024: 44.8 and 48.3)
+  const unsigned takers = kWaves * (SGH_WAVE / t.lanes);
+  t.stretch = takers * (size_t(a.tokens) / (takers * 4) * a.slices > size_t(sgh_num_cus()) * 32 ? 8 : 4);
+  if (t.stretch < t.tile) t.stretch = t.tile;
+  const unsigned lds = (2 * (t.stretch + 2 * t.tile) + 3 * t.stretch + 1) * 4, blocks = (t.tokens + t.stretch - 1) / t.stretch;
+  hipLaunchKernelGGL((k_embed_tiles<S, EPL>), dim3(blocks, unsigned(a.slices)), dim3(kBlock), lds, s, t);
   SGH_LAUNCH_CHECK();
-  hipLaunchKernelGGL((k_embed_join<S, EPL>), grid, dim3(kBlock), 0, s, a);
+  const unsigned tiles = tiles_at_once(t.lanes, t.slices), each = slices_at_once(t.slices);
+  const dim3 grid{(p.tiles + tiles - 1) / tiles, (t.slices + each - 1) / each};
+  hipLaunchKernelGGL((k_embed_join<S, EPL>), grid, dim3(kBlock), 0, s, t);
   SGH_LAUNCH_CHECK();
   return SGH_OK;
 }
@@ -858,7 +874,7 @@ int embed_bwd(const int32_t *ids, const typename S::elem *dy, const typename S::
   if ((tokens != 0 && (!ids || !dy)) || !dW) return SGH_EINVAL;
   if (sgh_ranges_meet(dW, bytes, dy, tokens * dim * e) || sgh_ranges_meet(dW, bytes, ids, tokens * 4)) return SGH_EINVAL;
   if (add && add != dW && sgh_ranges_meet(dW, bytes, add, bytes)) return SGH_EINVAL;
-  const BwdPlan p = bwd_plan(tokens, vocab, dim, S::VEC);
+  const BwdPlan p = bwd_plan(tokens, vocab, dim);
   if (p.bytes != 0 && (!workspace || ws_bytes < p.bytes)) return SGH_EWORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) % alignof(Token) != 0) return SGH_EINVAL;
   hipStream_t s = sgh_stream_of(stream);
@@ -890,7 +906,7 @@ SGH_EMBEDDING(bf16, StBF16, uint16_t)
 #undef SGH_EMBEDDING
 
 size_t sgh_embedding_bwd_workspace_bytes(size_t tokens, size_t vocab, size_t dim) {
-  return sizes_ok(tokens, vocab, dim) && vocab != 0 && dim != 0 ? bwd_workspace(tokens, vocab, dim) : 0;
+  return sizes_ok(tokens, vocab, dim) && vocab != 0 && dim != 0 ? bwd_plan(tokens, vocab, dim).bytes : 0;
 }
 
 int sgh_embedding_index_errors(void *stream, int *count) {

@@ -195,9 +195,11 @@ def test_embedding_gradient_of_rows_that_end_with_a_tile(dev):
     from singa_amd import singa_wrap as singa
     from singa_amd._lib import lib
     r = np.random.default_rng(6)
-    for unit in (32, 64, 128):
+    for unit in (16, 32, 64, 128, 1024):
         for runs in ([2, 2, 2, 40], [1, 3, 0.5, 0.5, 2, 30, 1], [40, 1, 0.25, 1.75, 1], [0.5, 35, 0.5, 1, 1, 1, 1.5, 2.5]):
             ids = r.permutation(np.repeat(np.arange(len(runs)), [int(n * unit) for n in runs]))
+            if ids.size <= 1024:
+                ids = np.concatenate([ids, np.full(1025 - ids.size, len(runs))])
             vocab, dim = len(runs) + 1, 20
             dy = r.integers(-8, 9, (ids.size, dim)).astype(np.float32)
             need = lib().sgh_embedding_bwd_workspace_bytes(ids.size, vocab, dim)
