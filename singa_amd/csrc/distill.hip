@@ -17,6 +17,7 @@
 namespace {
 
 constexpr int kBlock = 256;
+constexpr size_t kMostDim = size_t(1) << 28;   // a row's bytes and what is asked for behind it count in 32 bits
 constexpr float kLog2e = 1.44269504088896340736f;
 
 __device__ int g_list_errors = 0;
@@ -34,15 +35,49 @@ struct Rows {
   size_t batch, dim;
   int k;
   float tau, soft, hard, scale;
+  bool in_place;             // dx is x
 };
 
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// Over 16 neighbouring lanes without LDS, then over the four sixteens through scalar registers: every lane gets the result.  (Six shuffles
+// through LDS take ten times as long, and a row of a short vocabulary waits for a dozen of these.)
+template <int CTRL>
+__device__ __forceinline__ float lanes_of(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+constexpr int kSwap1 = 0xb1, kSwap2 = 0x4e, kHalfMirror = 0x141, kMirror = 0x140;   // lane ^ 1, ^ 2, 7 - lane of eight, 15 - lane of sixteen
+__device__ __forceinline__ float lane_value(float v, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+__device__ __forceinline__ float sum16(float v) {
+  v += lanes_of<kSwap1>(v);
+  v += lanes_of<kSwap2>(v);
+  v += lanes_of<kHalfMirror>(v);
+  return v + lanes_of<kMirror>(v);
+}
+__device__ __forceinline__ float max16(float v) {
+  v = fmaxf(v, lanes_of<kSwap1>(v));
+  v = fmaxf(v, lanes_of<kSwap2>(v));
+  v = fmaxf(v, lanes_of<kHalfMirror>(v));
+  return fmaxf(v, lanes_of<kMirror>(v));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  v = sum16(v);
+  return (lane_value(v, 0) + lane_value(v, 16)) + (lane_value(v, 32) + lane_value(v, 48));
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = max16(v);
+  return fmaxf(fmaxf(lane_value(v, 0), lane_value(v, 16)), fmaxf(lane_value(v, 32), lane_value(v, 48)));
+}
 
 // NT threads share a row: a wavefront (a workgroup then has several rows), or the workgroup
 template <int NT>
 struct Team {
   static constexpr int kPerBlock = NT == SGH_WAVE ? kBlock / SGH_WAVE : 1;
   static constexpr int kThreads = NT == SGH_WAVE ? kBlock : NT;
+  static constexpr int kWaves = NT / SGH_WAVE;
+  static constexpr int kLists = NT == SGH_WAVE ? 1 : 2;   // a row's list may still be read where the next one's is fetched
   static __device__ __forceinline__ int id() { return NT == SGH_WAVE ? threadIdx.x >> 6 : 0; }
   static __device__ __forceinline__ int tid() { return NT == SGH_WAVE ? threadIdx.x & 63 : threadIdx.x; }
   // what the team's threads stored (LDS and global memory) is seen by all of them behind this
@@ -55,279 +90,563 @@ struct Team {
       __syncthreads();
     }
   }
-  static __device__ __forceinline__ float max(float v, float *red) {
-    v = sgh_wave_max(v);
-    if constexpr (NT != SGH_WAVE) {
-      __syncthreads();
-      if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-      __syncthreads();
-      v = red[0];
-#pragma unroll
-      for (int i = 1; i < NT / 64; ++i) v = fmaxf(v, red[i]);
-    }
-    return v;
+};
+
+// A row's list in LDS; entry k is the label
+struct List {
+  int *at;       // column, -1: no entry
+  float *p, *x;  // the teacher's logit, later its share; the student's logit
+};
+__device__ __forceinline__ size_t list_bytes(int k) { return size_t(k + 1) * 12; }
+__device__ __forceinline__ List list_at(char *lds, int k) {
+  List l;
+  l.at = reinterpret_cast<int *>(lds);
+  l.p = reinterpret_cast<float *>(l.at + k + 1);
+  l.x = l.p + k + 1;
+  return l;
+}
+
+// What the teacher's list comes to: whether there is an entry, its largest logit, the sum of exp((logit - most) / tau)
+struct Teacher {
+  bool any;
+  float most, sum;
+};
+
+// The label of a row, or -1; `count`: those out of range
+template <class T>
+__device__ __forceinline__ int checked_label(const Rows<T> &a, int label, bool count) {
+  if (label < -1 || (label >= 0 && size_t(label) >= a.dim)) {
+    if (count) atomicAdd(&g_list_errors, 1);
+    return -1;
   }
-  static __device__ __forceinline__ float sum(float v, float *red) {
-    v = sgh_wave_sum(v);
-    if constexpr (NT != SGH_WAVE) {
-      __syncthreads();
-      if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-      __syncthreads();
-      v = red[0];
-#pragma unroll
-      for (int i = 1; i < NT / 64; ++i) v += red[i];
-    }
-    return v;
-  }
-};
+  return label;
+}
 
-// A list entry as the gradient needs it: its column, the student's logit there, and its share of -dx
-struct Entry {
-  int at;    // -1: none
-  float x, p;
+// A row's list comes into LDS by one wavefront of its team, in three steps, so that nothing else waits for its loads (the entries, then the
+// student's logits there): a lane's first entry stays in registers until it is needed.
+struct Early {
+  int at = -1;
+  float v = 0.f, x = 0.f, label_x = 0.f;
 };
-
-// What a row asks for, and its list in LDS (entry k is the label)
-struct RowTerms {
-  float w;
-  bool soft, hard;
-  float most, log_sum;   // the teacher's largest logit, the log of the sum of its exponentials relative to that one
-};
-
-template <int NT, class S>
-__device__ __forceinline__ RowTerms row_terms(const Rows<typename S::elem> &a, size_t row, Entry *list, float *red, bool count) {
-  typedef Team<NT> G;
-  const int tid = G::tid();
+// 1: the entries are asked for
+template <class T>
+__device__ __forceinline__ void ask_list(const Rows<T> &a, size_t row, Early &e) {
+  const int lane = threadIdx.x & (SGH_WAVE - 1);
+  if (a.soft != 0.f && lane < a.k) e.at = a.top[row * a.k + lane], e.v = a.teacher[row * a.k + lane];
+}
+// 2: they are there, and the student's logits are asked for; whether there is an entry.  `count`: those out of range
+template <class S>
+__device__ __forceinline__ bool gather_list(const Rows<typename S::elem> &a, size_t row, int label, bool count, const List &l, Early &e) {
+  const int lane = threadIdx.x & (SGH_WAVE - 1);
   const typename S::elem *x = a.x + row * a.dim;
-  RowTerms t;
-  t.w = a.weights ? a.weights[row] : 1.f;
-  t.hard = t.soft = false;
-  t.most = t.log_sum = 0.f;
-  int label = -1;
-  if (a.labels && a.hard != 0.f) {
-    label = a.labels[row];
-    if (label < -1 || (label >= 0 && size_t(label) >= a.dim)) {
-      if (count && tid == 0) atomicAdd(&g_list_errors, 1);
-      label = -1;
-    }
-    t.hard = label >= 0 && t.w != 0.f;
+  bool present = false;
+  if (lane == 0) {
+    l.at[a.k] = label;
+    l.p[a.k] = 1.f;
+    if (label >= 0) e.label_x = S::ld(x + label);
   }
-  G::sync();   // (the list of the row before is done with)
-  if (tid == 0) list[a.k] = Entry{t.hard ? label : -1, t.hard ? S::ld(x + label) : 0.f, 1.f};
-  if (a.k && a.soft != 0.f) {
-    float most = -__builtin_inff(), present = 0.f;
-    for (int k = tid; k < a.k; k += NT) {
-      int at = a.top[row * a.k + k];
-      const float v = a.teacher[row * a.k + k];
+  for (int k = lane; k < a.k; k += SGH_WAVE) {
+    int at = -1;
+    if (a.soft != 0.f) {
+      at = k == lane ? e.at : a.top[row * a.k + k];
+      const float v = k == lane ? e.v : a.teacher[row * a.k + k];
       if (at < -1 || (at >= 0 && size_t(at) >= a.dim)) {
         if (count) atomicAdd(&g_list_errors, 1);
         at = -1;
       }
       if (v == -__builtin_inff()) at = -1;   // (no share)
-      list[k] = Entry{at, at >= 0 && t.w != 0.f ? S::ld(x + at) : 0.f, v};
-      if (at >= 0) most = fmaxf(most, v), present = 1.f;
+      l.p[k] = v;
+      if (at >= 0) {
+        if (k == lane) e.x = S::ld(x + at);
+        else l.x[k] = S::ld(x + at);
+        present = true;
+      }
     }
-    t.soft = G::max(present, red) != 0.f && t.w != 0.f;
-    most = G::max(most, red);
-    float sum = 0.f;
-    const float c = kLog2e / a.tau;
-    for (int k = tid; k < a.k; k += NT)
-      if (list[k].at >= 0) sum += exp2_((list[k].p - most) * c);
-    sum = G::sum(sum, red);
-    t.most = most;
-    t.log_sum = logf(sum);
-    for (int k = tid; k < a.k; k += NT) {
-      if (!t.soft) list[k].at = -1;
-      if (list[k].at >= 0) list[k].p = exp2_((list[k].p - most) * c) / sum;
-    }
-  } else {
-    for (int k = tid; k < a.k; k += NT) list[k].at = -1;
+    l.at[k] = at;
   }
-  G::sync();
+  return __ballot(present) != 0;
+}
+// 3: those are there; what the teacher's logits come to
+template <class T>
+__device__ __forceinline__ Teacher finish_list(const Rows<T> &a, bool any, const List &l, const Early &e) {
+  const int lane = threadIdx.x & (SGH_WAVE - 1);
+  if (lane < a.k) l.x[lane] = e.x;
+  if (lane == 0) l.x[a.k] = e.label_x;
+  Teacher t = {any, -__builtin_inff(), 0.f};
+  if (!any) return t;
+  for (int k = lane; k < a.k; k += SGH_WAVE)
+    if (l.at[k] >= 0) t.most = fmaxf(t.most, l.p[k]);
+  t.most = wave_max(t.most);
+  const float c = kLog2e / a.tau;
+  for (int k = lane; k < a.k; k += SGH_WAVE)
+    if (l.at[k] >= 0) t.sum += exp2_((l.p[k] - t.most) * c);
+  t.sum = wave_sum(t.sum);
   return t;
 }
 
-// Running maximum and sums of exponentials relative to it.  tau = 1: both sums are one.
+// The teacher's shares in place of its logits, by the same wavefront; returns the divergence (LOSS)
+template <bool LOSS, class T>
+__device__ __forceinline__ float teacher_shares(const Rows<T> &a, const Teacher &t, float m, float log_st, const List &l) {
+  const int lane = threadIdx.x & (SGH_WAVE - 1);
+  const float log_sum = logf(t.sum), inv = 1.f / t.sum;
+  float kl = 0.f;
+  for (int k = lane; k < a.k; k += SGH_WAVE)
+    if (l.at[k] >= 0) {
+      const float d = (l.p[k] - t.most) / a.tau, p = exp2_((l.p[k] - t.most) * (kLog2e / a.tau)) * inv;
+      if (LOSS && p != 0.f) kl += p * (d - log_sum - ((l.x[k] - m) / a.tau - log_st));
+      l.p[k] = p;
+    }
+  return LOSS ? wave_sum(kl) : 0.f;
+}
+
+// Running maximum, and sums of exponentials relative to it: of d / tau where `t`, of d where `one` (tau = 1 makes one of both)
 struct Running {
   float m, st, s1;
 };
-template <int EPL>
-__device__ __forceinline__ void take(Running &r, const float *v, float ct, bool soft, bool hard) {
-  float most = v[0];
-#pragma unroll
-  for (int j = 1; j < EPL; ++j) most = fmaxf(most, v[j]);
-  if (most > r.m) {
-    const float d = r.m - most;   // (-inf at first: the sums are 0)
-    r.st *= exp2_(d * ct);
-    r.s1 *= exp2_(d * kLog2e);
-    r.m = most;
+struct Sums {
+  bool t, one;
+};
+// While a thread goes through its logits, its sums are relative to `ref`, which follows the maximum only when that is 2^8 above it: the sums
+// stay small enough, and they are rescaled next to never (after every vector that raised the maximum of one of 64 lanes it was a tenth
+// of the instructions)
+struct Lane {
+  float m, ref, far, st, s1;   // far: how far the maximum may be above ref
+  __device__ __forceinline__ void start(float ct, Sums want) {
+    m = ref = -__builtin_inff();
+    st = s1 = 0.f;
+    far = 8.f / (want.one ? fmaxf(ct, kLog2e) : ct);
   }
-  const float m = r.m == -__builtin_inff() ? 0.f : r.m;
-  if (soft) {
+  template <int N>
+  __device__ __forceinline__ void take(const float *v, float ct, Sums want) {
+    if constexpr (N == 1) {
+      m = fmaxf(m, v[0]);
+    } else {
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) r.st += exp2_((v[j] - m) * ct);
+      for (int j = 0; j < N; j += 2) m = fmaxf(fmaxf(m, v[j]), v[j + 1]);
+    }
+    if (m - ref > far) {   // (at first: -inf; where all are -inf still, no)
+      const float d = ref - m;
+      st *= exp2_(d * ct);
+      s1 *= exp2_(d * kLog2e);
+      ref = m;
+    }
+    const float r = ref == -__builtin_inff() ? 0.f : ref;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float d = v[j] - r;
+      if (want.t) st += exp2_(d * ct);
+      if (want.one) s1 += exp2_(d * kLog2e);
+    }
   }
-  if (hard) {
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) r.s1 += exp2_((v[j] - m) * kLog2e);
+};
+
+// The sums relative to the maximum of all; `of` is -inf where there was nothing but -inf
+__device__ __forceinline__ float rebased(float sum, float of, float m, float c) { return of == m ? sum : sum * exp2_((of - m) * c); }
+__device__ __forceinline__ Running wave_sums(const Lane &l, float ct) {
+  const float m = wave_max(l.m);
+  return {m, wave_sum(rebased(l.st, l.ref, m, ct)), wave_sum(rebased(l.s1, l.ref, m, kLog2e))};
+}
+
+// The gradient's factors of a row: dx = ft exp((x - m) / tau) + f1 exp(x - m), less the shares in the list's columns
+struct Slope {
+  float m, ct, ft, f1, share_t, share_1;
+  bool t, one;
+  __device__ __forceinline__ float operator()(float v) const {
+    const float d = v - m;
+    float o = 0.f;
+    if (t) o = ft * exp2_(d * ct);
+    if (one) o += f1 * exp2_(d * kLog2e);
+    return o;
+  }
+};
+template <class T>
+__device__ __forceinline__ Slope slope_of(const Rows<T> &a, float w, const Running &r, bool soft, bool hard) {
+  Slope s;
+  s.m = r.m, s.ct = kLog2e / a.tau;
+  s.share_t = soft ? a.scale * w * a.soft * a.tau : 0.f, s.share_1 = hard ? a.scale * w * a.hard : 0.f;
+  s.ft = soft ? s.share_t / r.st : 0.f, s.f1 = hard ? s.share_1 / r.s1 : 0.f;
+  s.t = soft, s.one = hard;
+  if (a.tau == 1.f && soft) s.f1 += s.ft, s.t = false, s.one = true;
+  return s;
+}
+
+// The columns of the list once more, behind a sync: a column that is there several times is its first entry's
+template <int NT, class S>
+__device__ __forceinline__ void list_columns(const Rows<typename S::elem> &a, size_t row, size_t from, size_t to, const Slope &s,
+                                             const List &l) {
+  for (int k = Team<NT>::tid(); k <= a.k; k += NT) {
+    const int at = l.at[k];
+    float p = 0.f;
+    bool first = true;
+#pragma unroll 8
+    for (int j = 0; j < a.k; ++j) {
+      const bool same = l.at[j] == at;
+      p += same ? l.p[j] : 0.f;
+      first = first && !(same && j < k);
+    }
+    float o = s(l.x[k]) - s.share_t * p;
+    if (l.at[a.k] == at) o -= s.share_1;
+    if (at >= 0 && size_t(at) >= from && size_t(at) < to && first) S::st(a.dx + row * a.dim + at, o);
   }
 }
 
+// A row's vectors through a buffer descriptor: what is behind the last of them reads as zero and is not stored, so that a load or a store needs no
+// branch around it, and waiting for one of them leaves the younger ones in flight.  (The offset is all in the lane's register: the
+// descriptor's limit is compared with that.)
+struct RowBuffer {
+  __amdgpu_buffer_rsrc_t r;
+  __device__ __forceinline__ RowBuffer(const void *p, unsigned bytes)
+      : r(__builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, int(bytes), 0x00020000)) {}
+  __device__ __forceinline__ sgh_v4u load(unsigned vec) const { return __builtin_amdgcn_raw_buffer_load_b128(r, int(vec * 16), 0, 0); }
+  __device__ __forceinline__ void store(sgh_v4u v, unsigned vec) const { __builtin_amdgcn_raw_buffer_store_b128(v, r, int(vec * 16), 0, 0); }
+};
+template <class S>
+__device__ __forceinline__ void unpack(const sgh_v4u &raw, float *v) {
+  sgh_load_any<S, S::VEC>(reinterpret_cast<const typename S::elem *>(&raw), v);
+}
+template <class S>
+__device__ __forceinline__ sgh_v4u packed(const float *v) {
+  sgh_v4u o;
+  sgh_store_any<S, S::VEC>(reinterpret_cast<typename S::elem *>(&o), v);
+  return o;
+}
+
+// A row's vectors, U of a thread at a time and the next U in flight: f(vector, its number, whether every thread of the team has one)
+constexpr int kAhead = 4;
+template <int NT>
+__device__ __forceinline__ void ask_vectors(const RowBuffer &x, unsigned from, sgh_v4u *v) {
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) v[u] = x.load(from + u * NT + Team<NT>::tid());
+}
+template <int NT, class F>
+__device__ __forceinline__ void stream_row(const RowBuffer &x, unsigned vecs, sgh_v4u *v, F f) {
+  for (unsigned c = 0; c < vecs; c += kAhead * NT) {
+    sgh_v4u then[kAhead];
+    ask_vectors<NT>(x, c + kAhead * NT, then);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (c + u * NT < vecs) f(v[u], c + u * NT + Team<NT>::tid(), c + (u + 1) * NT <= vecs);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) v[u] = then[u];
+  }
+}
+
+// A vector into a thread's sums; `all`: every thread of the team has one
+template <class S>
+__device__ __forceinline__ void take_vector(Lane &sum, const sgh_v4u &raw, unsigned vec, unsigned vecs, bool all, float ct, Sums want) {
+  float v[S::VEC];
+  unpack<S>(raw, v);
+  if (!all) {
+#pragma unroll
+    for (int j = 0; j < S::VEC; ++j) v[j] = vec < vecs ? v[j] : -__builtin_inff();
+  }
+  sum.take<S::VEC>(v, ct, want);
+}
+template <class S>
+__device__ __forceinline__ sgh_v4u slope_vector(const Slope &s, const sgh_v4u &raw) {
+  float v[S::VEC];
+  unpack<S>(raw, v);
+#pragma unroll
+  for (int j = 0; j < S::VEC; ++j) v[j] = s(v[j]);
+  return packed<S>(v);
+}
+
+// dx of a row's vectors [from, from + vecs) but for the list's columns, from memory (dx may be x: a thread stores what it has read); `none`: zeros
 template <int NT, class S>
-__device__ __forceinline__ Running row_statistics(const typename S::elem *x, size_t dim, float ct, bool soft, bool hard, float *red) {
-  typedef Team<NT> G;
-  constexpr int V = S::VEC, U = 4;
-  const int tid = G::tid();
-  Running r = {-__builtin_inff(), 0.f, 0.f};
-  const size_t vecs = dim / V;
-  size_t i = tid;
-  for (; i + (U - 1) * NT < vecs; i += U * NT) {
-    float v[U][V];
-#pragma unroll
-    for (int u = 0; u < U; ++u) sgh_load_any<S, V>(x + (i + u * NT) * V, v[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u) take<V>(r, v[u], ct, soft, hard);
+__device__ __forceinline__ void slope_row(const typename S::elem *x, typename S::elem *dx, unsigned vecs, bool none, const Slope &s) {
+  const RowBuffer from(x, none ? 0 : vecs * 16), to(dx, vecs * 16);
+  sgh_v4u v[kAhead];
+  ask_vectors<NT>(from, 0, v);
+  stream_row<NT>(from, vecs, v, [&](const sgh_v4u &raw, unsigned vec, bool) { to.store(slope_vector<S>(s, raw), vec); });
+}
+
+// The team's statistics from its threads'; `red`: one of each wavefront
+template <int NT, class T>
+__device__ __forceinline__ Running team_sums(const Rows<T> &a, const Lane &lane, float ct, Running *red) {
+  Running r = wave_sums(lane, ct);
+  constexpr int W = Team<NT>::kWaves;
+  static_assert(W <= 16, "a lane of sixteen takes a wavefront's");
+  if constexpr (W > 1) {
+    if ((threadIdx.x & (SGH_WAVE - 1)) == 0 && threadIdx.x < NT) red[threadIdx.x >> 6] = r;
+    __syncthreads();
+    const int of = threadIdx.x & 15;
+    r = of < W ? red[of] : Running{-__builtin_inff(), 0.f, 0.f};
+    const float m = max16(r.m);
+    r = {m, sum16(rebased(r.st, r.m, m, ct)), sum16(rebased(r.s1, r.m, m, kLog2e))};
   }
-  for (; i < vecs; i += NT) {
-    float v[V];
-    sgh_load_any<S, V>(x + i * V, v);
-    take<V>(r, v, ct, soft, hard);
-  }
-  const size_t last = vecs * V + tid;
-  if (last < dim) {
-    float v = S::ld(x + last);
-    take<1>(r, &v, ct, soft, hard);
-  }
-  const float m = G::max(r.m, red), d = r.m - m;
-  r.st = soft ? G::sum(r.st * exp2_(d * ct), red) : 0.f;
-  r.s1 = hard ? G::sum(r.s1 * exp2_(d * kLog2e), red) : 0.f;
-  r.m = m;
+  if (r.m == -__builtin_inff()) r.st = r.s1 = __builtin_nanf("");   // (no column with a probability)
+  if (a.tau == 1.f) r.st = r.s1;
   return r;
 }
 
-// dx of columns [from, to) of a row
-template <int NT, class S>
-__device__ __forceinline__ void row_gradient(const Rows<typename S::elem> &a, size_t row, size_t from, size_t to, const Running &r,
-                                             const RowTerms &t, const Entry *list) {
-  typedef Team<NT> G;
-  constexpr int V = S::VEC, U = 4;
-  const int tid = G::tid();
-  const typename S::elem *x = a.x + row * a.dim;
-  typename S::elem *dx = a.dx + row * a.dim;
-  const bool any = t.soft || t.hard;
-  const float ct = kLog2e / a.tau, g = a.scale * t.w;
-  const float share_t = t.soft ? g * a.soft * a.tau : 0.f, share_1 = t.hard ? g * a.hard : 0.f;
-  const float ft = t.soft ? share_t / r.st : 0.f, f1 = t.hard ? share_1 / r.s1 : 0.f;
-  auto value = [&](float v) {
-    const float d = v - r.m;
-    float o = 0.f;
-    if (t.soft) o = ft * exp2_(d * ct);
-    if (t.hard) o += f1 * exp2_(d * kLog2e);
-    return o;
-  };
-  const size_t vecs = (to - from) / V;
-  size_t i = tid;
-  for (; i + (U - 1) * NT < vecs; i += U * NT) {
-    float v[U][V];
-    if (any) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) sgh_load_any<S, V>(x + from + (i + u * NT) * V, v[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[u][j] = any ? value(v[u][j]) : 0.f;
-      sgh_store_any<S, V>(dx + from + (i + u * NT) * V, v[u]);
-    }
-  }
-  for (; i < vecs; i += NT) {
-    float v[V];
-    if (any) sgh_load_any<S, V>(x + from + i * V, v);
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = any ? value(v[j]) : 0.f;
-    sgh_store_any<S, V>(dx + from + i * V, v);
-  }
-  const size_t last = from + vecs * V + tid;
-  if (last < to) S::st(dx + last, any ? value(S::ld(x + last)) : 0.f);
-  if (!any) return;   // (the same for the whole team)
-  G::sync();   // the columns of the list again, now that the others are stored
-  for (int k = tid; k <= a.k; k += NT) {
-    const int at = list[k].at;
-    if (at < 0 || size_t(at) < from || size_t(at) >= to) continue;
-    bool first = true;
-    for (int j = 0; j < k; ++j) first &= list[j].at != at;
-    if (!first) continue;   // a column that is there twice is its first entry's
-    float o = value(list[k].x);
-    for (int j = k; j <= a.k; ++j)
-      if (list[j].at == at) o -= (j < a.k ? share_t : share_1) * list[j].p;
-    S::st(dx + at, o);
+// Loss and statistics of a row, by the wavefront that fetched its list; the teacher's shares are in the list then
+template <class T>
+__device__ __forceinline__ void store_loss(const Rows<T> &a, size_t row, float w, const Running &r, bool soft, bool hard,
+                                           const Teacher &teach, const List &list) {
+  float loss = 0.f;
+  if (soft) loss = a.soft * a.tau * a.tau * teacher_shares<true>(a, teach, r.m, logf(r.st), list);
+  if ((threadIdx.x & (SGH_WAVE - 1)) != 0) return;
+  if (hard) loss += a.hard * (logf(r.s1) - (list.x[a.k] - r.m));
+  a.loss[row] = soft || hard ? w * loss : 0.f;
+  if (a.stats) {
+    a.stats[row * 3] = soft || hard ? r.m : 0.f;
+    a.stats[row * 3 + 1] = soft ? r.st : 0.f;
+    a.stats[row * 3 + 2] = hard ? r.s1 : 0.f;
   }
 }
 
-// The loss and statistics of a row; GRAD: and its gradient
+// What a row asks for, known before its logits
+struct Row {
+  float w;
+  int label;
+  bool may_soft, hard;   // (whether the list has an entry is seen later)
+  __device__ __forceinline__ bool any() const { return may_soft || hard; }
+};
+template <class T>
+__device__ __forceinline__ Row row_at(const Rows<T> &a, size_t row, bool count) {
+  Row r;
+  r.w = a.weights ? a.weights[row] : 1.f;
+  r.label = a.labels && a.hard != 0.f ? checked_label(a, a.labels[row], count) : -1;
+  r.hard = r.label >= 0 && r.w != 0.f;
+  r.may_soft = a.k && a.soft != 0.f && r.w != 0.f;
+  return r;
+}
+
+// The loss and statistics of a row; GRAD: and its gradient, for which the row is read again.
 template <int NT, class S, bool GRAD>
 __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_fwd(Rows<typename S::elem> a) {
   typedef Team<NT> G;
+  typedef typename S::elem T;
   extern __shared__ char lds[];
-  __shared__ float red[16];
-  Entry *list = reinterpret_cast<Entry *>(lds) + G::id() * (a.k + 1);
-  for (size_t row = size_t(blockIdx.x) * G::kPerBlock + G::id(); row < a.batch; row += size_t(gridDim.x) * G::kPerBlock) {
-    const RowTerms t = row_terms<NT, S>(a, row, list, red, true);
+  __shared__ Running red[G::kWaves];
+  __shared__ int listed;
+  const int tid = G::tid();
+  const bool lister = tid < SGH_WAVE;
+  const float ct = kLog2e / a.tau;
+  const size_t step = size_t(gridDim.x) * G::kPerBlock;
+  const unsigned vecs = unsigned(a.dim / S::VEC), last = vecs * S::VEC + tid;   // the elements behind the last vector: one of a thread
+  int turn = 0;
+  for (size_t row = size_t(blockIdx.x) * G::kPerBlock + G::id(); row < a.batch; row += step) {
+    const T *x = a.x + row * a.dim;
+    // everything is asked for at once, the first vectors of a row that turns out to want nothing as well
+    Early early;
+    if (lister) ask_list(a, row, early);
+    const float tail = last < a.dim ? S::ld(x + last) : 0.f;
+    const RowBuffer from(x, vecs * 16);
+    sgh_v4u v[kAhead];
+    const Row q = row_at(a, row, tid == 0);
+    ask_vectors<NT>(from, 0, v);
+    const List list = list_at(lds + (G::id() * G::kLists + turn) * list_bytes(a.k), a.k);
+    bool any = false;
+    if (lister) {   // (entries out of range are counted whatever the weight)
+      any = gather_list<S>(a, row, q.hard ? q.label : -1, true, list, early);
+      if (tid == 0) listed = any;
+    }
+    const Sums want = {q.may_soft && a.tau != 1.f, q.hard || (q.may_soft && a.tau == 1.f)};
     Running r = {0.f, 0.f, 0.f};
-    if (t.soft || t.hard) r = row_statistics<NT, S>(a.x + row * a.dim, a.dim, kLog2e / a.tau, t.soft, t.hard, red);
-    float kl = 0.f;
-    if (t.soft) {
-      const float log_st = logf(r.st);
-      for (int k = G::tid(); k < a.k; k += NT)
-        if (list[k].at >= 0 && list[k].p != 0.f) {
-          const float log_p = (a.teacher[row * a.k + k] - t.most) / a.tau - t.log_sum;
-          kl += list[k].p * (log_p - ((list[k].x - r.m) / a.tau - log_st));
-        }
-      kl = G::sum(kl, red);
+    bool soft = false;
+    if (q.any()) {
+      Lane sum;
+      sum.start(ct, want);
+      stream_row<NT>(from, vecs, v, [&](const sgh_v4u &raw, unsigned vec, bool all) { take_vector<S>(sum, raw, vec, vecs, all, ct, want); });
+      if (last < a.dim) sum.take<1>(&tail, ct, want);
+      r = team_sums<NT>(a, sum, ct, red);
+      soft = q.may_soft && (NT == SGH_WAVE ? any : listed != 0);
     }
-    if (G::tid() == 0) {
-      float loss = 0.f;
-      if (t.soft) loss += a.soft * a.tau * a.tau * kl;
-      if (t.hard) loss += a.hard * (logf(r.s1) - (list[a.k].x - r.m));
-      a.loss[row] = t.w == 0.f ? 0.f : t.w * loss;
-      if (a.stats) {
-        a.stats[row * 3] = r.m;
-        a.stats[row * 3 + 1] = r.st;
-        a.stats[row * 3 + 2] = r.s1;
-      }
+    if (lister) {
+      const Teacher teach = finish_list(a, any, list, early);
+      store_loss(a, row, q.w, r, soft, q.hard, teach, list);
     }
-    if constexpr (GRAD) row_gradient<NT, S>(a, row, 0, a.dim, r, t, list);
+    if constexpr (GRAD) {
+      const Slope s = slope_of(a, q.w, r, soft, q.hard);
+      const bool none = !(soft || q.hard);
+      if (NT != SGH_WAVE) G::sync();   // (the list's logits are read: dx may be x)
+      slope_row<NT, S>(x, a.dx + row * a.dim, vecs, none, s);
+      if (last < a.dim) S::st(a.dx + row * a.dim + last, s(tail));
+      G::sync();
+      if (!none) list_columns<NT, S>(a, row, 0, a.dim, s, list);
+    } else {
+      G::sync();   // (`red` and `listed` are read)
+    }
+    turn = (turn + 1) % G::kLists;
   }
 }
 
-// The gradient from the statistics; a row may be several workgroups', `cols` columns each
-template <int NT, class S>
-__global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_bwd(Rows<typename S::elem> a, size_t cols) {
+// Both for rows of at most U * NT vectors, in registers.  A workgroup goes from row to row, and each of the next row's vectors is asked for when
+// the register it goes to is free, behind the store of this row's gradient there, so that the memory is at work while sums are joined and
+// the list is seen to.  What is small (weight, label, the first 64 of the list) is asked for in front of a row's vectors, a row or two ahead:
+// loads come back in order.
+template <int NT, int U, int PER_SIMD, class S>
+__global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(Rows<typename S::elem> a) {
   typedef Team<NT> G;
+  typedef typename S::elem T;
+  constexpr int V = S::VEC;
   extern __shared__ char lds[];
-  __shared__ float red[16];
-  Entry *list = reinterpret_cast<Entry *>(lds) + G::id() * (a.k + 1);
-  const size_t from = size_t(blockIdx.y) * cols, to = from + cols < a.dim ? from + cols : a.dim;
-  for (size_t row = size_t(blockIdx.x) * G::kPerBlock + G::id(); row < a.batch; row += size_t(gridDim.x) * G::kPerBlock) {
-    const RowTerms t = row_terms<NT, S>(a, row, list, red, false);
-    const Running r = {a.stats[row * 3], a.stats[row * 3 + 1], a.stats[row * 3 + 2]};
-    row_gradient<NT, S>(a, row, from, to, r, t, list);
+  __shared__ Running red[G::kWaves];
+  __shared__ int listed;
+  const int tid = G::tid();
+  const bool lister = tid < SGH_WAVE;   // the wavefront that sees to the list
+  const float ct = kLog2e / a.tau;
+  const size_t step = size_t(gridDim.x) * G::kPerBlock;
+  const unsigned vecs = unsigned(a.dim / V), bytes = vecs * 16, last = vecs * V + tid;   // the elements behind the last vector: one of a thread
+  const bool tails = last < a.dim;
+  size_t row = size_t(blockIdx.x) * G::kPerBlock + G::id();
+  if (row >= a.batch) return;
+  // weight and label as they are in memory
+  struct Raw {
+    float w;
+    int label;
+  };
+  auto raw_at = [&](size_t r) {
+    Raw q = {0.f, -1};
+    if (r < a.batch) {
+      q.w = a.weights ? a.weights[r] : 1.f;
+      if (a.labels && a.hard != 0.f) q.label = a.labels[r];
+    }
+    return q;
+  };
+  auto row_of = [&](const Raw &raw, bool count) {
+    Row q;
+    q.w = raw.w;
+    q.label = checked_label(a, raw.label, count);
+    q.hard = q.label >= 0 && q.w != 0.f;
+    q.may_soft = a.k && a.soft != 0.f && q.w != 0.f;
+    return q;
+  };
+  sgh_v4u held[U];
+  float tail = 0.f;
+  Early early;
+  if (lister) ask_list(a, row, early);
+  Row q = row_of(raw_at(row), tid == 0);
+  Raw next_raw = raw_at(row + step);
+  {
+    const RowBuffer x(a.x + row * a.dim, q.any() ? bytes : 0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) held[u] = x.load(u * NT + tid);
+    if (tails && q.any()) tail = S::ld(a.x + row * a.dim + last);
+  }
+  int turn = 0;
+  for (;;) {
+    const size_t next = row + step;
+    const bool goes_on = next < a.batch;
+    const Row nq = row_of(next_raw, tid == 0);   // (of nothing behind the last)
+    const T *nx = a.x + next * a.dim;
+    const List list = list_at(lds + (G::id() * G::kLists + turn) * list_bytes(a.k), a.k);
+    const RowBuffer to(a.dx + row * a.dim, bytes), then(nx, goes_on && nq.any() ? bytes : 0);
+    bool any = false;
+    if (lister) {
+      any = gather_list<S>(a, row, q.hard ? q.label : -1, true, list, early);
+      if (tid == 0) listed = any;
+    }
+    const Sums want = {q.may_soft && a.tau != 1.f, q.hard || (q.may_soft && a.tau == 1.f)};
+    Running r = {0.f, 0.f, 0.f};
+    bool soft = false;
+    if (q.any()) {
+      Lane sum;
+      sum.start(ct, want);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (unsigned(u * NT) < vecs) take_vector<S>(sum, held[u], u * NT + tid, vecs, unsigned(u * NT + NT) <= vecs, ct, want);
+      if (tails) sum.take<1>(&tail, ct, want);
+      r = team_sums<NT>(a, sum, ct, red);
+      soft = q.may_soft && (NT == SGH_WAVE ? any : listed != 0);
+    }
+    if (lister) {
+      const Teacher teach = finish_list(a, any, list, early);
+      store_loss(a, row, q.w, r, soft, q.hard, teach, list);
+      if (goes_on) ask_list(a, next, early);
+    }
+    next_raw = raw_at(next + step);
+    const Slope s = slope_of(a, q.w, r, soft, q.hard);
+    if (a.in_place && NT != SGH_WAVE) G::sync();   // (the list's logits are read)
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      to.store(slope_vector<S>(s, held[u]), u * NT + tid);
+      held[u] = then.load(u * NT + tid);
+    }
+    if (tails) {
+      S::st(a.dx + row * a.dim + last, s(tail));
+      if (goes_on && nq.any()) tail = S::ld(nx + last);
+    }
+    G::sync();
+    if (soft || q.hard) list_columns<NT, S>(a, row, 0, a.dim, s, list);
+    if (!goes_on) break;
+    row = next, q = nq;
+    turn = (turn + 1) % G::kLists;
   }
 }
 
+// The gradient from the statistics; a row may be several workgroups', `each` vectors of it
 template <int NT, class S>
-int launch(const Rows<typename S::elem> &a, bool fwd, bool grad, hipStream_t s) {
+__global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_bwd(Rows<typename S::elem> a, unsigned each) {
   typedef Team<NT> G;
-  size_t blocks = (a.batch + G::kPerBlock - 1) / G::kPerBlock;
-  if (blocks > (1u << 20)) blocks = 1u << 20;
-  const size_t lds = size_t(G::kPerBlock) * (a.k + 1) * sizeof(Entry);
-  const dim3 grid{unsigned(blocks)}, block{unsigned(G::kThreads)};
-  if (fwd && grad)
-    SGH_LAUNCH_TIMED((k_distill_fwd<NT, S, true>), grid, block, lds, s, a);
-  else if (fwd)
-    SGH_LAUNCH_TIMED((k_distill_fwd<NT, S, false>), grid, block, lds, s, a);
-  else
-    SGH_LAUNCH_TIMED((k_distill_bwd<NT, S>), grid, block, lds, s, a, a.dim);
+  typedef typename S::elem T;
+  extern __shared__ char lds[];
+  const int tid = G::tid();
+  const bool lister = tid < SGH_WAVE;
+  const unsigned all = unsigned(a.dim / S::VEC), first = blockIdx.y * each, vecs = all - first < each ? all - first : each;
+  const bool ends = blockIdx.y + 1 == gridDim.y;   // with the elements behind the last vector
+  const size_t from = size_t(first) * S::VEC, to = ends ? a.dim : from + size_t(vecs) * S::VEC, last = from + size_t(vecs) * S::VEC + tid;
+  const size_t step = size_t(gridDim.x) * G::kPerBlock;
+  int turn = 0;
+  for (size_t row = size_t(blockIdx.x) * G::kPerBlock + G::id(); row < a.batch; row += step) {
+    const T *x = a.x + row * a.dim;
+    T *dx = a.dx + row * a.dim;
+    Early early;
+    if (lister) ask_list(a, row, early);
+    const float tail = last < to ? S::ld(x + last) : 0.f;
+    const Running r = {a.stats[row * 3], a.stats[row * 3 + 1], a.stats[row * 3 + 2]};
+    Row q = row_at(a, row, false);
+    // (a sum of 0: the forward pass found no term)
+    const bool soft = q.may_soft && r.st != 0.f, hard = q.hard && r.s1 != 0.f, none = !(soft || hard);
+    const Slope s = slope_of(a, q.w, r, soft, hard);
+    const List list = list_at(lds + (G::id() * G::kLists + turn) * list_bytes(a.k), a.k);
+    bool any = false;
+    if (lister && !none) any = gather_list<S>(a, row, hard ? q.label : -1, false, list, early);
+    auto shares = [&]() {
+      if (!lister || none) return;
+      const Teacher t = finish_list(a, any, list, early);
+      if (soft) teacher_shares<false>(a, t, 0.f, 0.f, list);
+    };
+    if (a.in_place) {   // (the list's logits are read before any is stored over)
+      shares();
+      if (NT != SGH_WAVE) G::sync();
+    }
+    slope_row<NT, S>(x + from, dx + from, vecs, none, s);
+    if (last < to) S::st(dx + last, s(tail));
+    if (!a.in_place) shares();
+    G::sync();
+    if (!none) list_columns<NT, S>(a, row, from, to, s, list);
+    turn = (turn + 1) % G::kLists;
+  }
+}
+
+template <int NT>
+size_t lds_for(int k) {
+  return size_t(Team<NT>::kPerBlock) * Team<NT>::kLists * (k + 1) * 12;
+}
+template <int NT>
+unsigned blocks_for(size_t batch, size_t most) {
+  const size_t n = (batch + Team<NT>::kPerBlock - 1) / Team<NT>::kPerBlock;
+  return unsigned(n < most ? n : most);
+}
+template <int NT, class S, bool GRAD>
+int launch_fwd(const Rows<typename S::elem> &a, size_t most, hipStream_t s) {
+  SGH_LAUNCH_TIMED((k_distill_fwd<NT, S, GRAD>), dim3(blocks_for<NT>(a.batch, most)), dim3(Team<NT>::kThreads), lds_for<NT>(a.k), s, a);
+  SGH_LAUNCH_CHECK();
+  return SGH_OK;
+}
+template <int NT, int U, int PER_SIMD, class S>
+int launch_held(const Rows<typename S::elem> &a, hipStream_t s) {
+  const size_t at_once = size_t(sgh_num_cus()) * (PER_SIMD * 4 * SGH_WAVE / Team<NT>::kThreads);   // workgroups
+  SGH_LAUNCH_TIMED((k_distill_held<NT, U, PER_SIMD, S>), dim3(blocks_for<NT>(a.batch, at_once)), dim3(Team<NT>::kThreads), lds_for<NT>(a.k), s, a);
+  SGH_LAUNCH_CHECK();
+  return SGH_OK;
+}
+template <int NT, class S>
+int launch_bwd(const Rows<typename S::elem> &a, size_t most, unsigned each, hipStream_t s) {
+  const unsigned vecs = unsigned(a.dim / S::VEC), ny = vecs > each ? (vecs + each - 1) / each : 1;
+  SGH_LAUNCH_TIMED((k_distill_bwd<NT, S>), dim3(blocks_for<NT>(a.batch, most), ny), dim3(Team<NT>::kThreads), lds_for<NT>(a.k), s, a, each);
   SGH_LAUNCH_CHECK();
   return SGH_OK;
 }
@@ -336,7 +655,7 @@ int launch(const Rows<typename S::elem> &a, bool fwd, bool grad, hipStream_t s) 
 template <class T>
 int check(const Rows<T> &a, size_t k, bool fwd, bool grad, bool *empty) {
   *empty = false;
-  if (a.batch > 0x7fffffffu || a.dim > 0x7fffffffu) return SGH_EINVAL;
+  if (a.batch > 0x7fffffffu || a.dim > kMostDim) return SGH_EINVAL;
   if (!(a.tau > 0.f) || !__builtin_isfinite(a.tau) || !__builtin_isfinite(kLog2e / a.tau)) return SGH_EINVAL;
   if (k > SGH_DISTILL_MAX_TOP) return SGH_ELIMIT;
   if (a.batch == 0) return *empty = true, SGH_OK;
@@ -363,13 +682,25 @@ int distill(Rows<typename S::elem> a, size_t k, bool fwd, bool grad, void *strea
   const int rc = check(a, k, fwd, grad, &empty);
   if (rc != SGH_OK || empty) return rc;
   a.k = int(k);
+  a.in_place = grad && a.dx == a.x;
   hipStream_t s = sgh_stream_of(stream);
   const double bytes = double(a.batch) * a.dim * sizeof(typename S::elem);
   if (grad) sgh_note_write(a.dx, a.batch * a.dim * sizeof(typename S::elem));
   sgh_prof_kernel_scope prof(fwd && grad ? "distill/k_distill_fwd" : fwd ? "distill_fwd/k_distill_fwd" : "distill_bwd/k_distill_bwd",
                              bytes * (grad ? 2 : 1), s);
-  if (a.dim <= 2048) return launch<SGH_WAVE, S>(a, fwd, grad, s);
-  return launch<kBlock, S>(a, fwd, grad, s);
+  const size_t vecs = a.dim / S::VEC, many = size_t(1) << 20;
+  if (fwd && grad) {
+    if (vecs <= 64 * 4) return launch_held<64, 4, 6, S>(a, s);
+    if (vecs <= 64 * 8) return launch_held<64, 8, 5, S>(a, s);
+    if (vecs <= 64 * 16) return launch_held<64, 16, 4, S>(a, s);
+    if (vecs <= 256 * 8) return launch_held<256, 8, 5, S>(a, s);
+    if (vecs <= 256 * 16) return launch_held<256, 16, 4, S>(a, s);
+    if (vecs <= 512 * 16) return launch_held<512, 16, 4, S>(a, s);
+    if (vecs <= 1024 * 16) return launch_held<1024, 16, 4, S>(a, s);
+    return launch_fwd<512, S, true>(a, many, s);
+  }
+  if (fwd) return vecs <= 64 * 8 ? launch_fwd<64, S, false>(a, many, s) : launch_fwd<256, S, false>(a, many, s);
+  return vecs <= 64 * 8 ? launch_bwd<64, S>(a, many, vecs, s) : launch_bwd<256, S>(a, many, vecs, s);
 }
 
 }  // namespace
