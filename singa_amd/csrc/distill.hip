@@ -93,7 +93,7 @@ struct Team {
   }
 };
 
-// A row's list in LDS; entry k is the label
+// A row's list beyond 64 entries, in LDS; entry k is the label
 struct List {
   int *at;       // column, -1: no entry
   float *p, *x;  // the teacher's logit, later its share; the student's logit
@@ -123,80 +123,96 @@ __device__ __forceinline__ int checked_label(const Rows<T> &a, int label, bool c
   return label;
 }
 
-// A row's list comes into LDS by one wavefront of its team, in three steps, so that nothing else waits for its loads (the entries, then the
-// student's logits there): a lane's first entry stays in registers until it is needed.
-struct Early {
+// A row's list is seen to by one wavefront of its team, in three steps, so that nothing else waits for its loads (the entries, then the student's
+// logits there).  Up to 64 entries are a lane's each, in registers; a longer list goes to LDS, where the whole team ends up with it.
+struct Entry {
   int at = -1;
-  float v = 0.f, x = 0.f, label_x = 0.f;
+  float v = 0.f, x = 0.f, p = 0.f;   // the teacher's logit, the student's, the teacher's share
+  int label = -1;
+  float label_x = 0.f;               // (lane 0)
 };
+__host__ __device__ inline bool short_list(int k) { return k <= SGH_WAVE; }
 // 1: the entries are asked for
 template <class T>
-__device__ __forceinline__ void ask_list(const Rows<T> &a, size_t row, Early &e) {
+__device__ __forceinline__ void ask_list(const Rows<T> &a, size_t row, Entry &e) {
   const int lane = threadIdx.x & (SGH_WAVE - 1);
   if (a.soft != 0.f && lane < a.k) e.at = a.top[row * a.k + lane], e.v = a.teacher[row * a.k + lane];
 }
 // 2: they are there, and the student's logits are asked for; whether there is an entry.  `count`: those out of range
+template <class T>
+__device__ __forceinline__ int checked_entry(const Rows<T> &a, int at, float v, bool count) {
+  if (at < -1 || (at >= 0 && size_t(at) >= a.dim)) {
+    if (count) atomicAdd(&g_list_errors, 1);
+    return -1;
+  }
+  return v == -__builtin_inff() ? -1 : at;   // (no share)
+}
 template <class S>
-__device__ __forceinline__ bool gather_list(const Rows<typename S::elem> &a, size_t row, int label, bool count, const List &l, Early &e) {
+__device__ __forceinline__ bool gather_list(const Rows<typename S::elem> &a, size_t row, int label, bool count, const List &l, Entry &e) {
   const int lane = threadIdx.x & (SGH_WAVE - 1);
   const typename S::elem *x = a.x + row * a.dim;
-  bool present = false;
-  if (lane == 0) {
-    l.at[a.k] = label;
-    l.p[a.k] = 1.f;
-    if (label >= 0) e.label_x = S::ld(x + label);
-  }
-  for (int k = lane; k < a.k; k += SGH_WAVE) {
-    int at = -1;
-    if (a.soft != 0.f) {
-      at = k == lane ? e.at : a.top[row * a.k + k];
-      const float v = k == lane ? e.v : a.teacher[row * a.k + k];
-      if (at < -1 || (at >= 0 && size_t(at) >= a.dim)) {
-        if (count) atomicAdd(&g_list_errors, 1);
-        at = -1;
+  e.label = label;
+  if (lane == 0 && label >= 0) e.label_x = S::ld(x + label);
+  e.at = checked_entry(a, e.at, e.v, count);
+  if (e.at >= 0) e.x = S::ld(x + e.at);
+  bool present = e.at >= 0;
+  if (!short_list(a.k)) {
+    if (lane == 0) l.at[a.k] = label, l.p[a.k] = 1.f;
+    l.at[lane] = e.at, l.p[lane] = e.v;
+    for (int k = lane + SGH_WAVE; k < a.k; k += SGH_WAVE) {
+      int at = -1;
+      if (a.soft != 0.f) {
+        const float v = a.teacher[row * a.k + k];
+        at = checked_entry(a, a.top[row * a.k + k], v, count);
+        l.p[k] = v;
+        if (at >= 0) l.x[k] = S::ld(x + at), present = true;
       }
-      if (v == -__builtin_inff()) at = -1;   // (no share)
-      l.p[k] = v;
-      if (at >= 0) {
-        if (k == lane) e.x = S::ld(x + at);
-        else l.x[k] = S::ld(x + at);
-        present = true;
-      }
+      l.at[k] = at;
     }
-    l.at[k] = at;
   }
   return __ballot(present) != 0;
 }
 // 3: those are there; what the teacher's logits come to
 template <class T>
-__device__ __forceinline__ Teacher finish_list(const Rows<T> &a, bool any, const List &l, const Early &e) {
+__device__ __forceinline__ Teacher finish_list(const Rows<T> &a, bool any, const List &l, const Entry &e) {
   const int lane = threadIdx.x & (SGH_WAVE - 1);
-  if (lane < a.k) l.x[lane] = e.x;
-  if (lane == 0) l.x[a.k] = e.label_x;
   Teacher t = {any, -__builtin_inff(), 0.f};
+  const float c = kLog2e * a.inv_tau;
+  if (short_list(a.k)) {
+    if (!any) return t;
+    t.most = wave_max(e.at >= 0 ? e.v : -__builtin_inff());
+    t.sum = wave_sum(e.at >= 0 ? exp2_((e.v - t.most) * c) : 0.f);
+    return t;
+  }
+  l.x[lane] = e.x;
+  if (lane == 0) l.x[a.k] = e.label_x;
   if (!any) return t;
   for (int k = lane; k < a.k; k += SGH_WAVE)
     if (l.at[k] >= 0) t.most = fmaxf(t.most, l.p[k]);
   t.most = wave_max(t.most);
-  const float c = kLog2e * a.inv_tau;
   for (int k = lane; k < a.k; k += SGH_WAVE)
     if (l.at[k] >= 0) t.sum += exp2_((l.p[k] - t.most) * c);
   t.sum = wave_sum(t.sum);
   return t;
 }
 
-// The teacher's shares in place of its logits, by the same wavefront; returns the divergence (LOSS)
+// The teacher's shares, by the same wavefront; returns the divergence (LOSS)
 template <bool LOSS, class T>
-__device__ __forceinline__ float teacher_shares(const Rows<T> &a, const Teacher &t, float m, float log_st, const List &l) {
+__device__ __forceinline__ float teacher_shares(const Rows<T> &a, const Teacher &t, float m, float log_st, const List &l, Entry &e) {
   const int lane = threadIdx.x & (SGH_WAVE - 1);
   const float log_sum = logf(t.sum), inv = 1.f / t.sum;
   float kl = 0.f;
-  for (int k = lane; k < a.k; k += SGH_WAVE)
-    if (l.at[k] >= 0) {
-      const float d = (l.p[k] - t.most) * a.inv_tau, p = exp2_((l.p[k] - t.most) * (kLog2e * a.inv_tau)) * inv;
-      if (LOSS && p != 0.f) kl += p * (d - log_sum - ((l.x[k] - m) * a.inv_tau - log_st));
-      l.p[k] = p;
-    }
+  auto share = [&](float v, float x) {
+    const float d = (v - t.most) * a.inv_tau, p = exp2_((v - t.most) * (kLog2e * a.inv_tau)) * inv;
+    if (LOSS && p != 0.f) kl += p * (d - log_sum - ((x - m) * a.inv_tau - log_st));
+    return p;
+  };
+  if (short_list(a.k)) {
+    e.p = e.at >= 0 ? share(e.v, e.x) : 0.f;
+  } else {
+    for (int k = lane; k < a.k; k += SGH_WAVE)
+      if (l.at[k] >= 0) l.p[k] = share(l.p[k], l.x[k]);
+  }
   return LOSS ? wave_sum(kl) : 0.f;
 }
 
@@ -274,7 +290,31 @@ __device__ __forceinline__ Slope slope_of(const Rows<T> &a, float w, const Runni
 // The columns of the list once more, behind a sync: a column that is there several times is its first entry's
 template <int NT, class S>
 __device__ __forceinline__ void list_columns(const Rows<typename S::elem> &a, size_t row, size_t from, size_t to, const Slope &s,
-                                             const List &l) {
+                                             const List &l, const Entry &e) {
+  typename S::elem *dx = a.dx + row * a.dim;
+  auto mine = [&](int at) { return at >= 0 && size_t(at) >= from && size_t(at) < to; };
+  if (short_list(a.k)) {
+    if (Team<NT>::tid() >= SGH_WAVE) return;
+    unsigned long long same = __ballot(e.at >= 0);   // lanes with this one's column
+    for (unsigned rest = unsigned(a.dim - 1), b = 0; rest >> b; ++b) {
+      const unsigned bit = 0u - ((unsigned(e.at) >> b) & 1u);
+      const unsigned long long set = __ballot(bit != 0);
+      same &= ~(set ^ ((static_cast<unsigned long long>(bit) << 32) | bit));
+    }
+    const int first = __builtin_amdgcn_mbcnt_hi(unsigned(same >> 32), __builtin_amdgcn_mbcnt_lo(unsigned(same), 0)) == 0;
+    float p = e.p;
+    if (__ballot(e.at >= 0 && __popcll(same) > 1)) {
+      p = 0.f;
+      for (int j = 0; j < SGH_WAVE; ++j) {
+        const float of = lane_value(e.p, j);
+        if (same >> j & 1) p += of;
+      }
+    }
+    const bool labelled = e.at >= 0 && e.at == e.label;
+    if (first && mine(e.at)) S::st(dx + e.at, s(e.x) - s.share_t * p - (labelled ? s.share_1 : 0.f));
+    if (!__ballot(labelled) && Team<NT>::tid() == 0 && mine(e.label)) S::st(dx + e.label, s(e.label_x) - s.share_1);
+    return;
+  }
   for (int k = Team<NT>::tid(); k <= a.k; k += NT) {
     const int at = l.at[k];
     float p = 0.f;
@@ -287,7 +327,7 @@ __device__ __forceinline__ void list_columns(const Rows<typename S::elem> &a, si
     }
     float o = s(l.x[k]) - s.share_t * p;
     if (l.at[a.k] == at) o -= s.share_1;
-    if (at >= 0 && size_t(at) >= from && size_t(at) < to && first) S::st(a.dx + row * a.dim + at, o);
+    if (first && mine(at)) S::st(dx + at, o);
   }
 }
 
@@ -399,14 +439,14 @@ __device__ __forceinline__ Running team_sums(const Rows<T> &a, const Lane &lane,
   return r;
 }
 
-// Loss and statistics of a row, by the wavefront that fetched its list; the teacher's shares are in the list then
+// Loss and statistics of a row, by the wavefront that sees to its list; the teacher's shares are in the list then
 template <class T>
 __device__ __forceinline__ void store_loss(const Rows<T> &a, size_t row, float w, const Running &r, bool soft, bool hard,
-                                           const Teacher &teach, const List &list) {
+                                           const Teacher &teach, const List &list, Entry &entry) {
   float loss = 0.f;
-  if (soft) loss = a.soft * a.tau * a.tau * teacher_shares<true>(a, teach, r.m, logf(r.st), list);
+  if (soft) loss = a.soft * a.tau * a.tau * teacher_shares<true>(a, teach, r.m, logf(r.st), list, entry);
   if ((threadIdx.x & (SGH_WAVE - 1)) != 0) return;
-  if (hard) loss += a.hard * (logf(r.s1) - (list.x[a.k] - r.m));
+  if (hard) loss += a.hard * (logf(r.s1) - (entry.label_x - r.m));
   a.loss[row] = soft || hard ? w * loss : 0.f;
   if (a.stats) {
     a.stats[row * 3] = soft || hard ? r.m : 0.f;
@@ -450,8 +490,8 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_fwd(Rows<typenam
     const Lie lie = lie_of<S>(x, unsigned(a.dim), tid);
     const unsigned vecs = lie.vecs;
     // everything is asked for at once, the first vectors of a row that turns out to want nothing as well
-    Early early;
-    if (lister) ask_list(a, row, early);
+    Entry entry;
+    if (lister) ask_list(a, row, entry);
     const float tail = lie.odd != kNone ? S::ld(x + lie.odd) : 0.f;
     const RowBuffer from(x + lie.head, vecs * 16);
     sgh_v4u v[kAhead];
@@ -460,7 +500,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_fwd(Rows<typenam
     const List list = list_at(lds + (G::id() * G::kLists + turn) * list_bytes(a.k), a.k);
     bool any = false;
     if (lister) {   // (entries out of range are counted whatever the weight)
-      any = gather_list<S>(a, row, q.hard ? q.label : -1, true, list, early);
+      any = gather_list<S>(a, row, q.hard ? q.label : -1, true, list, entry);
       if (tid == 0) listed = any;
     }
     const Sums want = {q.may_soft && a.tau != 1.f, q.hard || (q.may_soft && a.tau == 1.f)};
@@ -475,8 +515,8 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_fwd(Rows<typenam
       soft = q.may_soft && (NT == SGH_WAVE ? any : listed != 0);
     }
     if (lister) {
-      const Teacher teach = finish_list(a, any, list, early);
-      store_loss(a, row, q.w, r, soft, q.hard, teach, list);
+      const Teacher teach = finish_list(a, any, list, entry);
+      store_loss(a, row, q.w, r, soft, q.hard, teach, list, entry);
     }
     if constexpr (GRAD) {
       const Slope s = slope_of(a, q.w, r, soft, q.hard);
@@ -485,7 +525,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_fwd(Rows<typenam
       slope_row<NT, S>(x + lie.head, a.dx + row * a.dim + lie.head, vecs, none, s);
       if (lie.odd != kNone) S::st(a.dx + row * a.dim + lie.odd, s(tail));
       G::sync();
-      if (!none) list_columns<NT, S>(a, row, 0, a.dim, s, list);
+      if (!none) list_columns<NT, S>(a, row, 0, a.dim, s, list, entry);
     } else {
       G::sync();   // (`red` and `listed` are read)
     }
@@ -533,8 +573,8 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
   };
   sgh_v4u held[U];
   float tail = 0.f;
-  Early early;
-  if (lister) ask_list(a, row, early);
+  Entry entry;
+  if (lister) ask_list(a, row, entry);
   Row q = row_of(raw_at(row), tid == 0);
   Raw next_raw = raw_at(row + step);
   Lie lie = lie_of<S>(a.x + row * a.dim, unsigned(a.dim), tid);
@@ -551,6 +591,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
     const bool goes_on = next < a.batch;
     const Row nq = row_of(next_raw, tid == 0);   // (of nothing behind the last)
     const T *nx = a.x + next * a.dim;
+    Entry next_entry;
     const List list = list_at(lds + (G::id() * G::kLists + turn) * list_bytes(a.k), a.k);
     const Lie next_lie = lie_of<S>(nx, unsigned(a.dim), tid);
     T *dx = a.dx + row * a.dim;
@@ -558,7 +599,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
     const RowBuffer to(dx + lie.head, vecs * 16), then(nx + next_lie.head, goes_on && nq.any() ? next_lie.vecs * 16 : 0);
     bool any = false;
     if (lister) {
-      any = gather_list<S>(a, row, q.hard ? q.label : -1, true, list, early);
+      any = gather_list<S>(a, row, q.hard ? q.label : -1, true, list, entry);
       if (tid == 0) listed = any;
     }
     const Sums want = {q.may_soft && a.tau != 1.f, q.hard || (q.may_soft && a.tau == 1.f)};
@@ -575,9 +616,9 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
       soft = q.may_soft && (NT == SGH_WAVE ? any : listed != 0);
     }
     if (lister) {
-      const Teacher teach = finish_list(a, any, list, early);
-      store_loss(a, row, q.w, r, soft, q.hard, teach, list);
-      if (goes_on) ask_list(a, next, early);
+      const Teacher teach = finish_list(a, any, list, entry);
+      store_loss(a, row, q.w, r, soft, q.hard, teach, list, entry);
+      if (goes_on) ask_list(a, next, next_entry);
     }
     next_raw = raw_at(next + step);
     const Slope s = slope_of(a, q.w, r, soft, q.hard);
@@ -590,9 +631,9 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
     if (lie.odd != kNone) S::st(dx + lie.odd, s(tail));
     if (next_lie.odd != kNone && goes_on && nq.any()) tail = S::ld(nx + next_lie.odd);
     G::sync();
-    if (soft || q.hard) list_columns<NT, S>(a, row, 0, a.dim, s, list);
+    if (soft || q.hard) list_columns<NT, S>(a, row, 0, a.dim, s, list, entry);
     if (!goes_on) break;
-    row = next, q = nq, lie = next_lie;
+    row = next, q = nq, lie = next_lie, entry = next_entry;
     turn = (turn + 1) % G::kLists;
   }
 }
@@ -616,8 +657,8 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_bwd(Rows<typenam
     const bool begins = blockIdx.y == 0, ends = blockIdx.y + 1 == gridDim.y;
     const size_t start = lie.head + size_t(first) * S::VEC, from = begins ? 0 : start, to = ends ? a.dim : start + size_t(vecs) * S::VEC;
     const bool odd = lie.odd != kNone && (lie.odd < lie.head ? begins : ends);
-    Early early;
-    if (lister) ask_list(a, row, early);
+    Entry entry;
+    if (lister) ask_list(a, row, entry);
     const float tail = odd ? S::ld(x + lie.odd) : 0.f;
     const Running r = {a.stats[row * 3], a.stats[row * 3 + 1], a.stats[row * 3 + 2]};
     Row q = row_at(a, row, false);
@@ -626,11 +667,11 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_bwd(Rows<typenam
     const Slope s = slope_of(a, q.w, r, soft, hard);
     const List list = list_at(lds + (G::id() * G::kLists + turn) * list_bytes(a.k), a.k);
     bool any = false;
-    if (lister && !none) any = gather_list<S>(a, row, hard ? q.label : -1, false, list, early);
+    if (lister && !none) any = gather_list<S>(a, row, hard ? q.label : -1, false, list, entry);
     auto shares = [&]() {
       if (!lister || none) return;
-      const Teacher t = finish_list(a, any, list, early);
-      if (soft) teacher_shares<false>(a, t, 0.f, 0.f, list);
+      const Teacher t = finish_list(a, any, list, entry);
+      if (soft) teacher_shares<false>(a, t, 0.f, 0.f, list, entry);
     };
     if (a.in_place) {   // (the list's logits are read before any is stored over)
       shares();
@@ -640,14 +681,14 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_bwd(Rows<typenam
     if (odd) S::st(dx + lie.odd, s(tail));
     if (!a.in_place) shares();
     G::sync();
-    if (!none) list_columns<NT, S>(a, row, from, to, s, list);
+    if (!none) list_columns<NT, S>(a, row, from, to, s, list, entry);
     turn = (turn + 1) % G::kLists;
   }
 }
 
 template <int NT>
 size_t lds_for(int k) {
-  return size_t(Team<NT>::kPerBlock) * Team<NT>::kLists * (k + 1) * 12;
+  return short_list(k) ? 0 : size_t(Team<NT>::kPerBlock) * Team<NT>::kLists * (k + 1) * 12;
 }
 template <int NT>
 unsigned blocks_for(size_t batch, size_t most) {
@@ -718,7 +759,7 @@ int distill(Rows<typename S::elem> a, size_t k, bool fwd, bool grad, void *strea
     if (vecs <= 64 * 4) return launch_held<64, 4, 6, S>(a, s);
     if (vecs <= 64 * 8) return launch_held<64, 8, 5, S>(a, s);
     if (vecs <= 64 * 16) return launch_held<64, 16, 4, S>(a, s);
-    if (vecs <= 256 * 8) return launch_held<256, 8, 5, S>(a, s);
+    if (vecs <= 128 * 16) return launch_held<128, 16, 4, S>(a, s);
     if (vecs <= 256 * 16) return launch_held<256, 16, 4, S>(a, s);
     if (vecs <= 512 * 16) return launch_held<512, 16, 4, S>(a, s);
     if (vecs <= 1024 * 16) return launch_held<1024, 16, 4, S>(a, s);
