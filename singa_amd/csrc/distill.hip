@@ -765,8 +765,19 @@ int distill(Rows<typename S::elem> a, size_t k, bool fwd, bool grad, void *strea
     if (vecs <= 1024 * 16) return launch_held<1024, 16, 4, S>(a, s);
     return launch_fwd<512, S, true>(a, many, s);
   }
-  if (fwd) return vecs <= 64 * 8 ? launch_fwd<64, S, false>(a, many, s) : launch_fwd<256, S, false>(a, many, s);
-  return vecs <= 64 * 8 ? launch_bwd<64, S>(a, many, vecs, s) : launch_bwd<256, S>(a, many, vecs, s);
+  const size_t cus = size_t(sgh_num_cus());
+  if (fwd) {
+    if (vecs <= 512) return launch_fwd<64, S, false>(a, many, s);
+    if (a.batch <= 2 * cus) return vecs <= 5120 ? launch_fwd<256, S, false>(a, many, s) : launch_fwd<512, S, false>(a, many, s);
+    return vecs <= 2560 ? launch_fwd<128, S, false>(a, many, s) : launch_fwd<256, S, false>(a, many, s);
+  }
+  if (vecs <= 512) return launch_bwd<64, S>(a, many, vecs, s);
+  // few rows: several workgroups to each, with a turn of every thread's vectors at least
+  auto each = [&](size_t threads) {
+    const size_t turns = (vecs + threads * kAhead - 1) / (threads * kAhead), want = (4 * cus + a.batch - 1) / a.batch, n = turns < want ? turns : want;
+    return unsigned((vecs + n - 1) / n);
+  };
+  return vecs <= 2048 ? launch_bwd<256, S>(a, many, each(256), s) : launch_bwd<512, S>(a, many, each(512), s);
 }
 
 }  // namespace
