@@ -338,9 +338,17 @@ struct RowBuffer {
   __amdgpu_buffer_rsrc_t r;
   __device__ __forceinline__ RowBuffer(const void *p, unsigned bytes)
       : r(__builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, int(bytes), 0x00020000)) {}
-  __device__ __forceinline__ sgh_v4u load(unsigned vec) const { return __builtin_amdgcn_raw_buffer_load_b128(r, int(vec * 16), 0, 0); }
-  __device__ __forceinline__ void store(sgh_v4u v, unsigned vec) const { __builtin_amdgcn_raw_buffer_store_b128(v, r, int(vec * 16), 0, 0); }
+  // (STREAM: past the caches, the "nt" bit)
+  template <bool STREAM>
+  __device__ __forceinline__ sgh_v4u load(unsigned vec) const {
+    return __builtin_amdgcn_raw_buffer_load_b128(r, int(vec * 16), 0, STREAM ? 2 : 0);
+  }
+  template <bool STREAM>
+  __device__ __forceinline__ void store(sgh_v4u v, unsigned vec) const {
+    __builtin_amdgcn_raw_buffer_store_b128(v, r, int(vec * 16), 0, STREAM ? 2 : 0);
+  }
 };
+
 // How a row lies: `head` elements up to the first 16-byte boundary, `vecs` vectors, and what is left.  (Vectors that begin between boundaries
 // cost a sixth of the rate: 83 -> 97 us for 4096 rows of 50000 and 50001 binary16 values.)  The elements around the vectors are a thread's each:
 // `odd` is this one's, or none.
@@ -373,16 +381,16 @@ __device__ __forceinline__ sgh_v4u packed(const float *v) {
 
 // A row's vectors, U of a thread at a time and the next U in flight: f(vector, its number, whether every thread of the team has one)
 constexpr int kAhead = 4;
-template <int NT>
+template <int NT, bool STREAM>
 __device__ __forceinline__ void ask_vectors(const RowBuffer &x, unsigned from, sgh_v4u *v) {
 #pragma unroll
-  for (int u = 0; u < kAhead; ++u) v[u] = x.load(from + u * NT + Team<NT>::tid());
+  for (int u = 0; u < kAhead; ++u) v[u] = x.load<STREAM>(from + u * NT + Team<NT>::tid());
 }
-template <int NT, class F>
+template <int NT, bool STREAM, class F>
 __device__ __forceinline__ void stream_row(const RowBuffer &x, unsigned vecs, sgh_v4u *v, F f) {
   for (unsigned c = 0; c < vecs; c += kAhead * NT) {
     sgh_v4u then[kAhead];
-    ask_vectors<NT>(x, c + kAhead * NT, then);
+    ask_vectors<NT, STREAM>(x, c + kAhead * NT, then);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
       if (c + u * NT < vecs) f(v[u], c + u * NT + Team<NT>::tid(), c + (u + 1) * NT <= vecs);
@@ -412,12 +420,12 @@ __device__ __forceinline__ sgh_v4u slope_vector(const Slope &s, const sgh_v4u &r
 }
 
 // dx of a row's vectors [from, from + vecs) but for the list's columns, from memory (dx may be x: a thread stores what it has read); `none`: zeros
-template <int NT, class S>
+template <int NT, class S, bool STREAM>
 __device__ __forceinline__ void slope_row(const typename S::elem *x, typename S::elem *dx, unsigned vecs, bool none, const Slope &s) {
   const RowBuffer from(x, none ? 0 : vecs * 16), to(dx, vecs * 16);
   sgh_v4u v[kAhead];
-  ask_vectors<NT>(from, 0, v);
-  stream_row<NT>(from, vecs, v, [&](const sgh_v4u &raw, unsigned vec, bool) { to.store(slope_vector<S>(s, raw), vec); });
+  ask_vectors<NT, STREAM>(from, 0, v);
+  stream_row<NT, STREAM>(from, vecs, v, [&](const sgh_v4u &raw, unsigned vec, bool) { to.store<STREAM>(slope_vector<S>(s, raw), vec); });
 }
 
 // The team's statistics from its threads'; `red`: one of each wavefront
@@ -473,7 +481,7 @@ __device__ __forceinline__ Row row_at(const Rows<T> &a, size_t row, bool count) 
 }
 
 // The loss and statistics of a row; GRAD: and its gradient, for which the row is read again.
-template <int NT, class S, bool GRAD>
+template <int NT, class S, bool GRAD, bool STREAM>
 __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_fwd(Rows<typename S::elem> a) {
   typedef Team<NT> G;
   typedef typename S::elem T;
@@ -496,7 +504,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_fwd(Rows<typenam
     const RowBuffer from(x + lie.head, vecs * 16);
     sgh_v4u v[kAhead];
     const Row q = row_at(a, row, tid == 0);
-    ask_vectors<NT>(from, 0, v);
+    ask_vectors<NT, STREAM && !GRAD>(from, 0, v);
     const List list = list_at(lds + (G::id() * G::kLists + turn) * list_bytes(a.k), a.k);
     bool any = false;
     if (lister) {   // (entries out of range are counted whatever the weight)
@@ -509,7 +517,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_fwd(Rows<typenam
     if (q.any()) {
       Lane sum;
       sum.start(ct, want);
-      stream_row<NT>(from, vecs, v, [&](const sgh_v4u &raw, unsigned vec, bool all) { take_vector<S>(sum, raw, vec, vecs, all, ct, want); });
+      stream_row<NT, STREAM && !GRAD>(from, vecs, v, [&](const sgh_v4u &raw, unsigned vec, bool all) { take_vector<S>(sum, raw, vec, vecs, all, ct, want); });
       if (lie.odd != kNone) sum.take<1>(&tail, ct, want);
       r = team_sums<NT>(a, sum, ct, red);
       soft = q.may_soft && (NT == SGH_WAVE ? any : listed != 0);
@@ -522,7 +530,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_fwd(Rows<typenam
       const Slope s = slope_of(a, q.w, r, soft, q.hard);
       const bool none = !(soft || q.hard);
       if (NT != SGH_WAVE) G::sync();   // (the list's logits are read: dx may be x)
-      slope_row<NT, S>(x + lie.head, a.dx + row * a.dim + lie.head, vecs, none, s);
+      slope_row<NT, S, STREAM>(x + lie.head, a.dx + row * a.dim + lie.head, vecs, none, s);
       if (lie.odd != kNone) S::st(a.dx + row * a.dim + lie.odd, s(tail));
       G::sync();
       if (!none) list_columns<NT, S>(a, row, 0, a.dim, s, list, entry);
@@ -537,7 +545,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_fwd(Rows<typenam
 // the register it goes to is free, behind the store of this row's gradient there, so that the memory is at work while sums are joined and
 // the list is seen to.  What is small (weight, label, the first 64 of the list) is asked for in front of a row's vectors, a row or two ahead:
 // loads come back in order.
-template <int NT, int U, int PER_SIMD, class S>
+template <int NT, int U, int PER_SIMD, class S, bool STREAM>
 __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(Rows<typename S::elem> a) {
   typedef Team<NT> G;
   typedef typename S::elem T;
@@ -582,7 +590,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
     const T *first = a.x + row * a.dim;
     const RowBuffer x(first + lie.head, q.any() ? lie.vecs * 16 : 0);
 #pragma unroll
-    for (int u = 0; u < U; ++u) held[u] = x.load(u * NT + tid);
+    for (int u = 0; u < U; ++u) held[u] = x.load<STREAM>(u * NT + tid);
     if (lie.odd != kNone && q.any()) tail = S::ld(first + lie.odd);
   }
   int turn = 0;
@@ -625,8 +633,8 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
     if (a.in_place && NT != SGH_WAVE) G::sync();   // (the list's logits are read)
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      to.store(slope_vector<S>(s, held[u]), u * NT + tid);
-      held[u] = then.load(u * NT + tid);
+      to.store<STREAM>(slope_vector<S>(s, held[u]), u * NT + tid);
+      held[u] = then.load<STREAM>(u * NT + tid);
     }
     if (lie.odd != kNone) S::st(dx + lie.odd, s(tail));
     if (next_lie.odd != kNone && goes_on && nq.any()) tail = S::ld(nx + next_lie.odd);
@@ -639,7 +647,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
 }
 
 // The gradient from the statistics; a row may be several workgroups', `each` vectors of it
-template <int NT, class S>
+template <int NT, class S, bool STREAM>
 __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_bwd(Rows<typename S::elem> a, unsigned each) {
   typedef Team<NT> G;
   typedef typename S::elem T;
@@ -677,7 +685,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_bwd(Rows<typenam
       shares();
       if (NT != SGH_WAVE) G::sync();
     }
-    slope_row<NT, S>(x + start, dx + start, vecs, none, s);
+    slope_row<NT, S, STREAM>(x + start, dx + start, vecs, none, s);
     if (odd) S::st(dx + lie.odd, s(tail));
     if (!a.in_place) shares();
     G::sync();
@@ -695,23 +703,31 @@ unsigned blocks_for(size_t batch, size_t most) {
   const size_t n = (batch + Team<NT>::kPerBlock - 1) / Team<NT>::kPerBlock;
   return unsigned(n < most ? n : most);
 }
+template <class T>
+bool streams(const Rows<T> &a) { return a.batch * a.dim * sizeof(T) >= kStreamBytes; }
 template <int NT, class S, bool GRAD>
-int launch_fwd(const Rows<typename S::elem> &a, size_t most, hipStream_t s) {
-  SGH_LAUNCH_TIMED((k_distill_fwd<NT, S, GRAD>), dim3(blocks_for<NT>(a.batch, most)), dim3(Team<NT>::kThreads), lds_for<NT>(a.k), s, a);
+int launch_fwd(const Rows<typename S::elem> &a, hipStream_t s) {
+  const dim3 grid{blocks_for<NT>(a.batch, size_t(1) << 20)}, block{unsigned(Team<NT>::kThreads)};
+  if (streams(a)) SGH_LAUNCH_TIMED((k_distill_fwd<NT, S, GRAD, true>), grid, block, lds_for<NT>(a.k), s, a);
+  else SGH_LAUNCH_TIMED((k_distill_fwd<NT, S, GRAD, false>), grid, block, lds_for<NT>(a.k), s, a);
   SGH_LAUNCH_CHECK();
   return SGH_OK;
 }
 template <int NT, int U, int PER_SIMD, class S>
 int launch_held(const Rows<typename S::elem> &a, hipStream_t s) {
   const size_t at_once = size_t(sgh_num_cus()) * (PER_SIMD * 4 * SGH_WAVE / Team<NT>::kThreads);   // workgroups
-  SGH_LAUNCH_TIMED((k_distill_held<NT, U, PER_SIMD, S>), dim3(blocks_for<NT>(a.batch, at_once)), dim3(Team<NT>::kThreads), lds_for<NT>(a.k), s, a);
+  const dim3 grid{blocks_for<NT>(a.batch, at_once)}, block{unsigned(Team<NT>::kThreads)};
+  if (streams(a)) SGH_LAUNCH_TIMED((k_distill_held<NT, U, PER_SIMD, S, true>), grid, block, lds_for<NT>(a.k), s, a);
+  else SGH_LAUNCH_TIMED((k_distill_held<NT, U, PER_SIMD, S, false>), grid, block, lds_for<NT>(a.k), s, a);
   SGH_LAUNCH_CHECK();
   return SGH_OK;
 }
 template <int NT, class S>
-int launch_bwd(const Rows<typename S::elem> &a, size_t most, unsigned each, hipStream_t s) {
+int launch_bwd(const Rows<typename S::elem> &a, unsigned each, hipStream_t s) {
   const unsigned vecs = unsigned(a.dim / S::VEC), ny = vecs > each ? (vecs + each - 1) / each : 1;
-  SGH_LAUNCH_TIMED((k_distill_bwd<NT, S>), dim3(blocks_for<NT>(a.batch, most), ny), dim3(Team<NT>::kThreads), lds_for<NT>(a.k), s, a, each);
+  const dim3 grid{blocks_for<NT>(a.batch, size_t(1) << 20), ny}, block{unsigned(Team<NT>::kThreads)};
+  if (streams(a)) SGH_LAUNCH_TIMED((k_distill_bwd<NT, S, true>), grid, block, lds_for<NT>(a.k), s, a, each);
+  else SGH_LAUNCH_TIMED((k_distill_bwd<NT, S, false>), grid, block, lds_for<NT>(a.k), s, a, each);
   SGH_LAUNCH_CHECK();
   return SGH_OK;
 }
@@ -754,7 +770,7 @@ int distill(Rows<typename S::elem> a, size_t k, bool fwd, bool grad, void *strea
   if (grad) sgh_note_write(a.dx, a.batch * a.dim * sizeof(typename S::elem));
   sgh_prof_kernel_scope prof(fwd && grad ? "distill/k_distill_fwd" : fwd ? "distill_fwd/k_distill_fwd" : "distill_bwd/k_distill_bwd",
                              bytes * (grad ? 2 : 1), s);
-  const size_t vecs = a.dim / S::VEC, many = size_t(1) << 20;
+  const size_t vecs = a.dim / S::VEC;
   if (fwd && grad) {
     if (vecs <= 64 * 4) return launch_held<64, 4, 6, S>(a, s);
     if (vecs <= 64 * 8) return launch_held<64, 8, 5, S>(a, s);
@@ -763,21 +779,21 @@ int distill(Rows<typename S::elem> a, size_t k, bool fwd, bool grad, void *strea
     if (vecs <= 256 * 16) return launch_held<256, 16, 4, S>(a, s);
     if (vecs <= 512 * 16) return launch_held<512, 16, 4, S>(a, s);
     if (vecs <= 1024 * 16) return launch_held<1024, 16, 4, S>(a, s);
-    return launch_fwd<512, S, true>(a, many, s);
+    return launch_fwd<512, S, true>(a, s);
   }
   const size_t cus = size_t(sgh_num_cus());
   if (fwd) {
-    if (vecs <= 512) return launch_fwd<64, S, false>(a, many, s);
-    if (a.batch <= 2 * cus) return vecs <= 5120 ? launch_fwd<256, S, false>(a, many, s) : launch_fwd<512, S, false>(a, many, s);
-    return vecs <= 2560 ? launch_fwd<128, S, false>(a, many, s) : launch_fwd<256, S, false>(a, many, s);
+    if (vecs <= 512) return launch_fwd<64, S, false>(a, s);
+    if (a.batch <= 2 * cus) return vecs <= 5120 ? launch_fwd<256, S, false>(a, s) : launch_fwd<512, S, false>(a, s);
+    return vecs <= 2560 ? launch_fwd<128, S, false>(a, s) : launch_fwd<256, S, false>(a, s);
   }
-  if (vecs <= 512) return launch_bwd<64, S>(a, many, vecs, s);
+  if (vecs <= 512) return launch_bwd<64, S>(a, unsigned(vecs), s);
   // few rows: several workgroups to each, with a turn of every thread's vectors at least
   auto each = [&](size_t threads) {
     const size_t turns = (vecs + threads * kAhead - 1) / (threads * kAhead), want = (4 * cus + a.batch - 1) / a.batch, n = turns < want ? turns : want;
     return unsigned((vecs + n - 1) / n);
   };
-  return vecs <= 2048 ? launch_bwd<256, S>(a, many, each(256), s) : launch_bwd<512, S>(a, many, each(512), s);
+  return vecs <= 2048 ? launch_bwd<256, S>(a, each(256), s) : launch_bwd<512, S>(a, each(512), s);
 }
 
 }  // namespace

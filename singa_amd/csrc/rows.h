@@ -31,6 +31,23 @@ __device__ __forceinline__ void sgh_store_any(typename S::elem *p, const float *
     __builtin_memcpy(p, e, 16);
   }
 }
+// The same; STREAM: past the caches
+template <class S, int EPL, bool STREAM>
+__device__ __forceinline__ void sgh_store_any(typename S::elem *p, const float *in) {
+  if constexpr (STREAM && EPL != 1) {
+    alignas(16) typename S::elem e[EPL];
+    S::store16(e, in);
+    sgh_v4u v;
+    __builtin_memcpy(&v, e, 16);
+    typedef sgh_v4u anywhere __attribute__((aligned(2)));
+    __builtin_nontemporal_store(v, reinterpret_cast<anywhere *>(p));
+  } else {
+    sgh_store_any<S, EPL>(p, in);
+  }
+}
+
+// Results of at least this many bytes are stored past the caches: they would not stay in the 256 MB of the last one until they are read
+constexpr size_t kStreamBytes = size_t(96) << 20;
 
 // [a, a + a_bytes) and [b, b + b_bytes) have a byte in common
 static inline bool sgh_ranges_meet(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
