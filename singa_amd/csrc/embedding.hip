@@ -152,7 +152,7 @@ __device__ __forceinline__ void store_row(const Bwd<typename S::elem> &a, size_t
 }
 
 // Sum of rows place[from .. to) of dy, ascending, on top of acc
-template <class S, int EPL>
+template <class S, int EPL, bool STREAM>
 __device__ __forceinline__ void add_tokens(const typename S::elem *dy, size_t dim, size_t at, const unsigned *place, unsigned from,
                                            unsigned to, float *acc) {
   constexpr int U = 4;   // (8: more code than it saves waits, 331 -> 326 us for 65536 tokens of 2048)
@@ -160,7 +160,7 @@ __device__ __forceinline__ void add_tokens(const typename S::elem *dy, size_t di
     float v[U][EPL];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (i + u < to) sgh_load_any<S, EPL>(dy + size_t(place[i + u]) * dim + at, v[u]);
+      if (i + u < to) sgh_load_any<S, EPL, STREAM>(dy + size_t(place[i + u]) * dim + at, v[u]);
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (i + u < to) {
@@ -290,7 +290,7 @@ __global__ __launch_bounds__(kBlock) void k_embed_rows(Bwd<typename S::elem> a, 
     float acc[EPL];
 #pragma unroll
     for (int j = 0; j < EPL; ++j) acc[j] = 0.f;
-    add_tokens<S, EPL>(a.dy, a.dim, at, found, b, e, acc);
+    add_tokens<S, EPL, false>(a.dy, a.dim, at, found, b, e, acc);
     float g[EPL];
     load_add<S, EPL>(a, row0 + r, at, g);
     store_row<S, EPL, STREAM>(a, row0 + r, at, vec, acc, g);
@@ -465,7 +465,7 @@ __device__ __forceinline__ void fill_rows(const Bwd<typename S::elem> &a, const 
           at[u] = row + (n * EPL + EPL > a.dim ? a.dim - EPL : n * EPL);
 #pragma unroll
           for (int j = 0; j < EPL; ++j) v[u][j] = 0.f;
-          if (a.add && n < vecs) sgh_load_any<S, EPL>(a.add + at[u], v[u]);
+          if (a.add && n < vecs) sgh_load_any<S, EPL, STREAM>(a.add + at[u], v[u]);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -625,7 +625,7 @@ __device__ __forceinline__ Spot spot_of(const Bwd<T> &a) {
 // in the next one), or a row's piece of a tile.  Then the wavefronts take the jobs in turn, `lanes` lanes and a vector of each to a job.
 // (One wavefront that goes through a tile's tokens with loads of several jobs in flight needs its store once for each of them: the code no
 // longer fits the instruction cache, 6 -> 13 us at 2048 tokens of 64.)
-template <class S, int EPL, bool STREAM>
+template <class S, int EPL, bool STREAM, bool STREAM_DY>
 __global__ __launch_bounds__(kBlock) void k_embed_tiles(Bwd<typename S::elem> a) {
   extern __shared__ unsigned lds[];   // one key in front, the stretch, two tiles behind it; their places; the jobs
   __shared__ unsigned jobs;
@@ -694,7 +694,7 @@ __global__ __launch_bounds__(kBlock) void k_embed_tiles(Bwd<typename S::elem> a)
 #pragma unroll
     for (int e = 0; e < EPL; ++e) acc[e] = 0.f;
     if (dest == kRow) load_add<S, EPL>(a, keys[from], at, g);
-    add_tokens<S, EPL>(a.dy, a.dim, at, places, from, to_[j], acc);
+    add_tokens<S, EPL, STREAM_DY>(a.dy, a.dim, at, places, from, to_[j], acc);
     if (dest == kRow) {
       store_row<S, EPL, STREAM>(a, keys[from], at, vec, acc, g);
     } else {
@@ -859,7 +859,12 @@ int launch_bwd(Bwd<typename S::elem> a, const BwdPlan &p, void *workspace, hipSt
   t.stretch = takers * (size_t(a.tokens) / (takers * 4) * a.slices > size_t(sgh_num_cus()) * 32 ? 8 : 4);
   if (t.stretch < t.tile) t.stretch = t.tile;
   const unsigned lds = (2 * (t.stretch + 2 * t.tile) + 3 * t.stretch + 1) * 4, blocks = (t.tokens + t.stretch - 1) / t.stretch;
-  hipLaunchKernelGGL((k_embed_tiles<S, EPL, STREAM>), dim3(blocks, unsigned(a.slices)), dim3(kBlock), lds, s, t);
+  // (dy past the caches: 65536 tokens of 2048 16-bit elements 321 -> 308 us; 33 MB of it, 39.6 -> 41.3)
+  const dim3 stretches{blocks, unsigned(a.slices)};
+  if (EPL != 1 && size_t(a.tokens) * a.dim * sizeof(typename S::elem) >= kStreamBytes)
+    hipLaunchKernelGGL((k_embed_tiles<S, EPL, STREAM, EPL != 1>), stretches, dim3(kBlock), lds, s, t);
+  else
+    hipLaunchKernelGGL((k_embed_tiles<S, EPL, STREAM, false>), stretches, dim3(kBlock), lds, s, t);
   SGH_LAUNCH_CHECK();
   const unsigned tiles = tiles_at_once(t.lanes, t.slices), each = slices_at_once(t.slices);
   const dim3 grid{(p.tiles + tiles - 1) / tiles, (t.slices + each - 1) / each};

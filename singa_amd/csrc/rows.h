@@ -20,6 +20,17 @@ __device__ __forceinline__ void sgh_load_any(const typename S::elem *p, float *o
     S::template load16<false>(e, out);
   }
 }
+// The same; STREAM: past the caches
+template <class S, int EPL, bool STREAM>
+__device__ __forceinline__ void sgh_load_any(const typename S::elem *p, float *out) {
+  if constexpr (STREAM && EPL != 1) {
+    typedef sgh_v4u anywhere __attribute__((aligned(2)));
+    const sgh_v4u v = __builtin_nontemporal_load(reinterpret_cast<const anywhere *>(p));
+    sgh_load_any<S, EPL>(reinterpret_cast<const typename S::elem *>(&v), out);
+  } else {
+    sgh_load_any<S, EPL>(p, out);
+  }
+}
 template <class S, int EPL>
 __device__ __forceinline__ void sgh_store_any(typename S::elem *p, const float *in) {
   if constexpr (EPL == 1) {
@@ -31,7 +42,6 @@ __device__ __forceinline__ void sgh_store_any(typename S::elem *p, const float *
     __builtin_memcpy(p, e, 16);
   }
 }
-// The same; STREAM: past the caches
 template <class S, int EPL, bool STREAM>
 __device__ __forceinline__ void sgh_store_any(typename S::elem *p, const float *in) {
   if constexpr (STREAM && EPL != 1) {
@@ -46,7 +56,7 @@ __device__ __forceinline__ void sgh_store_any(typename S::elem *p, const float *
   }
 }
 
-// Results of at least this many bytes are stored past the caches: they would not stay in the 256 MB of the last one until they are read
+// Tensors of at least this many bytes go past the caches: they would not stay in the 256 MB of the last one until they are read again
 constexpr size_t kStreamBytes = size_t(96) << 20;
 
 // [a, a + a_bytes) and [b, b + b_bytes) have a byte in common
