@@ -759,8 +759,8 @@ SGH_API int sgh_pool_bwd_bf16(const sgh_pool_geom *g, const uint16_t *dy, const 
  * ===================================================================================== */
 /* y[t] = scale * W[ids[t]]: rows of W [vocab, dim] by id, y [tokens, dim].  An id equal to padding_idx (any
  * number; -1 where there is no padding) gives a row of zeros, and so does one outside [0, vocab), which is also counted
- * (sgh_embedding_index_errors).  dim up to 2^24, tokens and vocab up to 2^31 - 1; rows need no alignment.  y must not overlap
- * W or ids. */
+ * (sgh_embedding_index_errors).  dim up to 2^21, tokens and vocab up to 2^31 - 1 (SGH_EINVAL beyond); rows need no alignment.  y must not
+ * overlap W or ids. */
 SGH_API int sgh_embedding_fwd_f32(const int32_t *ids, const float *W, float *y, size_t tokens, size_t vocab, size_t dim,
                                   float scale, int padding_idx, void *stream);
 SGH_API int sgh_embedding_fwd_f16(const int32_t *ids, const uint16_t *W, uint16_t *y, size_t tokens, size_t vocab, size_t dim,
@@ -771,7 +771,8 @@ SGH_API int sgh_embedding_fwd_bf16(const int32_t *ids, const uint16_t *W, uint16
  * forward pass gave zeros for take part in nothing.  add: NULL, a tensor of W's size, or dW itself (rows without a token then
  * stay as they are) -- the gradient that a matrix got elsewhere, as the weights of the output layer for one.  A row's tokens are
  * summed in fp32 in an order that follows from the ids alone: the same bits every time.  dW must not overlap dy, ids or a
- * part of add.  workspace: sgh_embedding_bwd_workspace_bytes (0 for few tokens, NULL is then taken). */
+ * part of add.  workspace: sgh_embedding_bwd_workspace_bytes, at a multiple of 8 bytes (0 for few tokens, NULL is then taken); calls on
+ * different streams need one each. */
 SGH_API size_t sgh_embedding_bwd_workspace_bytes(size_t tokens, size_t vocab, size_t dim);
 SGH_API int sgh_embedding_bwd_f32(const int32_t *ids, const float *dy, const float *add, float *dW, size_t tokens,
                                   size_t vocab, size_t dim, float scale, int padding_idx, void *workspace,
@@ -793,9 +794,12 @@ SGH_API int sgh_embedding_index_errors(void *stream, int *count);
  *   dx[n][j] = scale * weights[n] * (soft * temperature * (q_j - sum of p_k with top_k = j) + hard * (r_j - [j = label]))
  * A term without its list, its label or its factor (0) is left out; a row with no term, or of weight 0, has loss and gradient 0 and
  * its logits are not looked at.  An entry of logit -inf is none.  A column may be listed twice: its shares add up.  Entries and labels
- * below -1 or not below dim are treated as -1 and counted (sgh_distill_index_errors; the gradient alone does not count again).
+ * below -1 or not below dim are treated as -1 and counted (sgh_distill_index_errors; the gradient alone does not count again, and
+ * what a factor of 0 makes needless is not looked at).
  * k = 0 (top and teacher NULL) is a cross entropy that stores no probabilities.  x -inf has probability 0; a row of nothing else,
- * or with a NaN or +inf, has NaN results.  temperature > 0 and finite; k up to SGH_DISTILL_MAX_TOP (SGH_ELIMIT beyond).
+ * or with a NaN or +inf, has NaN results.  temperature > 0, its square and its inverse within fp32; dim from 1 to 2^28, batch up to
+ * 2^31 - 1 (SGH_EINVAL beyond); k up to SGH_DISTILL_MAX_TOP (SGH_ELIMIT beyond).  Rows need no alignment.  No result may overlap an
+ * argument or another result, but for dx that is x.
  *   _fwd      loss and stats [batch, 3] = the row's maximum m, sum exp((x - m) / temperature), sum exp(x - m): what the gradient
  *             needs of the forward pass; 0 where no term asks for it
  *   _bwd      dx from the stats of the same arguments; dx may be x itself

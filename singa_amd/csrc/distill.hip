@@ -509,7 +509,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_fwd(Rows<typenam
     bool any = false;
     if (lister) {   // (entries out of range are counted whatever the weight)
       any = gather_list<S>(a, row, q.hard ? q.label : -1, true, list, entry);
-      if (tid == 0) listed = any;
+      if (NT != SGH_WAVE && tid == 0) listed = any;
     }
     const Sums want = {q.may_soft && a.tau != 1.f, q.hard || (q.may_soft && a.tau == 1.f)};
     Running r = {0.f, 0.f, 0.f};
@@ -608,7 +608,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
     bool any = false;
     if (lister) {
       any = gather_list<S>(a, row, q.hard ? q.label : -1, true, list, entry);
-      if (tid == 0) listed = any;
+      if (NT != SGH_WAVE && tid == 0) listed = any;
     }
     const Sums want = {q.may_soft && a.tau != 1.f, q.hard || (q.may_soft && a.tau == 1.f)};
     Running r = {0.f, 0.f, 0.f};
@@ -737,23 +737,26 @@ template <class T>
 int check(const Rows<T> &a, size_t k, bool fwd, bool grad, bool *empty) {
   *empty = false;
   if (a.batch > 0x7fffffffu || a.dim > kMostDim) return SGH_EINVAL;
-  if (!(a.tau > 0.f) || !__builtin_isfinite(a.tau) || !__builtin_isfinite(kLog2e / a.tau)) return SGH_EINVAL;
+  if (!(a.tau > 0.f) || !__builtin_isfinite(a.tau * a.tau) || !__builtin_isfinite(kLog2e / a.tau)) return SGH_EINVAL;
   if (k > SGH_DISTILL_MAX_TOP) return SGH_ELIMIT;
   if (a.batch == 0) return *empty = true, SGH_OK;
   if (a.dim == 0) return SGH_EINVAL;   // (a row of no logits has no softmax)
   if (!a.x || (k != 0 && (!a.top || !a.teacher))) return SGH_EINVAL;
   if (fwd && !a.loss) return SGH_EINVAL;
   if ((!fwd || !grad) && !a.stats) return SGH_EINVAL;
-  const size_t bytes = a.batch * a.dim * sizeof(T);
-  if (grad) {
-    if (!a.dx) return SGH_EINVAL;
-    if (a.dx != a.x && sgh_ranges_meet(a.dx, bytes, a.x, bytes)) return SGH_EINVAL;
-    if (sgh_ranges_meet(a.dx, bytes, a.top, a.batch * k * 4) || sgh_ranges_meet(a.dx, bytes, a.teacher, a.batch * k * 4) ||
-        sgh_ranges_meet(a.dx, bytes, a.labels, a.labels ? a.batch * 4 : 0) ||
-        sgh_ranges_meet(a.dx, bytes, a.weights, a.weights ? a.batch * 4 : 0) ||
-        sgh_ranges_meet(a.dx, bytes, a.stats, a.stats ? a.batch * 12 : 0))
-      return SGH_EINVAL;
-  }
+  if (grad && !a.dx) return SGH_EINVAL;
+  // no result lies over an argument or another result, but for dx over the whole of x
+  const size_t bytes = a.batch * a.dim * sizeof(T), lists = a.batch * k * 4, each = a.batch * 4;
+  struct {
+    const void *p;
+    size_t bytes;
+  } const of[] = {{a.dx, grad ? bytes : 0}, {a.loss, fwd ? each : 0}, {a.stats, a.stats ? 3 * each : 0}, {a.x, bytes}, {a.top, lists},
+                  {a.teacher, lists}, {a.labels, a.labels ? each : 0}, {a.weights, a.weights ? each : 0}};
+  const int results = fwd ? 3 : 1;   // (the gradient alone reads stats)
+  for (int i = 0; i < results; ++i)
+    for (int j = i + 1; j < int(sizeof(of) / sizeof(of[0])); ++j)
+      if (sgh_ranges_meet(of[i].p, of[i].bytes, of[j].p, of[j].bytes) && !(i == 0 && of[j].p == a.x && a.dx == a.x))
+        return SGH_EINVAL;
   return SGH_OK;
 }
 

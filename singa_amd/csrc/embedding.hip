@@ -83,7 +83,7 @@ int launch_fwd(const int32_t *ids, const typename S::elem *W, typename S::elem *
   return SGH_OK;
 }
 
-constexpr size_t kMostDim = size_t(1) << 24;   // (the slices of a row are a grid's second dimension: at most 65535)
+constexpr size_t kMostDim = size_t(1) << 21;   // (the slices of a row, of 64 elements or more, are a grid's second dimension: at most 65535)
 
 bool sizes_ok(size_t tokens, size_t vocab, size_t dim) {
   return tokens <= 0x7fffffffu && vocab <= 0x7fffffffu && dim <= kMostDim;

@@ -888,7 +888,8 @@ def DistillationFwdBwd(x, top, teacher, labels=None, weights=None, temperature=1
     """(loss of ``DistillationFwd``, gradient of ``DistillationBwd``) in one call."""
     args = _distill_args("DistillationFwdBwd", x, top, teacher, labels, weights)
     fn, name = _fn("distill_fwd_bwd", x)
-    loss, dx = _empty(Tensor, x._shape[:1], x._dev, kFloat32), _distill_out("DistillationFwdBwd", x, out)
+    dx = _distill_out("DistillationFwdBwd", x, out)
+    loss = _empty(Tensor, x._shape[:1], x._dev, kFloat32)
     check(fn(x.ptr, *args, temperature, soft, hard, scale, loss.ptr, dx.ptr, x._dev.stream), name)
     return loss, dx
 
