@@ -97,7 +97,7 @@ def cpu_baseline(config, sample_batch, budget_s, single_thread_batch):
         ops = OracleOps()
         net = wl.build(config, ops)
         x, labels = wl.make_inputs(config, batch)
-        net.forward(ops.from_numpy(x), ops.from_numpy(labels))
+        net.forward(*net.inputs(x, labels))
         steps, t0 = 0, time.perf_counter()
         while True:
             net.backward_and_update()
@@ -172,9 +172,11 @@ def main():
     hip.set_fusion(not args.no_fusion)
     if args.no_overlap:
         hip.overlap_wgrad = False
+    if not args.with_forward:
+        hip.fuse_distill = False   # the loss's gradient belongs to what is timed
     net = wl.build(args.config, hip, lr=0.05, momentum=0.9)
     x, labels = wl.make_inputs(args.config, args.batch)
-    x_dev, labels_dev = hip.from_numpy(x), hip.from_numpy(labels)
+    x_dev, labels_dev = net.inputs(x, labels)
     net.forward(x_dev, labels_dev)
     fused = not args.per_parameter_update
     if args.with_forward and args.graph:
@@ -244,7 +246,7 @@ def main():
     if not (args.no_fusion or args.with_forward or args.no_reference_tape):
         saved = {f: getattr(hip, f) for f in ("fuse_bn_relu", "fuse_dgrad_add", "fuse_add_relu", "fuse_wgrad_bias",
                                               "batch_relayout", "overlap_wgrad", "fuse_forward", "fuse_linear", "fuse_dgrad_relu",
-                                              "fuse_pool_relu")}
+                                              "fuse_pool_relu", "fuse_distill")}
         hip.set_fusion(False)
         net.sgd.op_by_op = True     # SGD.apply's own tensor ops, three launches per parameter
         ref_steps = max(3, min(args.steps, 10))
@@ -306,7 +308,7 @@ def main():
 
     # the bandwidth-bound families: algorithmic bytes (minimal tensor traffic) / time between the two events
     hbm = {}
-    for k in ("bn_relu_bwd", "bn_bwd", "relu_bwd", "relu_bwd_add", "add", "pool_bwd", "sgd"):
+    for k in ("bn_relu_bwd", "bn_bwd", "relu_bwd", "relu_bwd_add", "add", "pool_bwd", "distill_bwd", "embedding_bwd", "sgd"):
         if k in prof and prof[k]["ms"] > 0:
             v = prof[k]
             gbs = v["work"] / (v["ms"] * 1e-3) / 1e9

@@ -4,6 +4,7 @@ TEST INFRASTRUCTURE ONLY (tests/, the smoke check, the CPU-baseline leg of bench
 import numpy as np
 
 from . import cpu_oracle as O
+from . import token_ops
 
 
 class _ConvH(object):
@@ -127,6 +128,22 @@ class OracleOps(object):
 
     def conv_bwd_b(self, dy, b, h):
         return O.conv_bgrad(dy)
+
+    def embedding(self, ids, W, scale):
+        return token_ops.embedding_fwd(ids, W, scale).astype(np.float32)
+
+    def embedding_bwd(self, dy, ids, W, scale):
+        return token_ops.embedding_bwd(dy, ids, W.shape, scale).astype(np.float32)
+
+    def _distill(self, x, t, batch):
+        return token_ops.distill(x, t.top, t.teacher, t.labels, t.weights, t.temperature, t.soft, t.hard, 1.0 / batch)
+
+    def distill_fwd(self, x, t):
+        loss, stats, _ = self._distill(x, t, 1)
+        return loss.astype(np.float32), stats.astype(np.float32)
+
+    def distill_bwd(self, x, stats, t, batch):
+        return self._distill(x, t, batch)[2].astype(np.float32)
 
     def accumulate(self, a, b):
         a[...] = O.add(a, b)

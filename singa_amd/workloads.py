@@ -143,6 +143,27 @@ class HipOps(object):
     def softmax_ce_fwd(self, x, t):
         return singa.SoftMaxCrossEntropyFwd(x, t)
 
+    # the two ends of a token model: vectors by id, and the loss against a teacher's top logits and labels
+    def embedding(self, ids, W, scale):
+        return singa.EmbeddingForward(ids, W, scale)
+
+    def embedding_bwd(self, dy, ids, W, scale):
+        return singa.EmbeddingBackwardW(dy, ids, W, scale)
+
+    def distill_fwd(self, x, t):
+        return singa.DistillationFwd(x, t.top, t.teacher, t.labels, t.weights, t.temperature, t.soft, t.hard)
+
+    def distill_bwd(self, x, stats, t, batch):
+        return singa.DistillationBwd(x, stats, t.top, t.teacher, t.labels, t.weights, t.temperature, t.soft, t.hard,
+                                     scale=float(np.float32(1.0) / np.float32(batch)))
+
+    # fusion the tape permits: nothing comes between the loss and its gradient, which is formed while the logits are at hand
+    fuse_distill = True
+
+    def distill_fwd_bwd(self, x, t, batch):
+        return singa.DistillationFwdBwd(x, t.top, t.teacher, t.labels, t.weights, t.temperature, t.soft, t.hard,
+                                        scale=float(np.float32(1.0) / np.float32(batch)))
+
     # backward
     def softmax_ce_bwd(self, p, t, batch):
         # SoftmaxCrossEntropyBwd followed by "dx /= N" (python/singa/autograd.py:1319-1322), fused
@@ -270,12 +291,12 @@ class HipOps(object):
             self._aux = None
 
     fusions = ("fuse_bn_relu", "fuse_dgrad_add", "fuse_wgrad_bias", "batch_relayout", "overlap_wgrad", "fuse_forward",
-               "fuse_linear", "fuse_pool_relu")   # what set_fusion(True) turns on
+               "fuse_linear", "fuse_pool_relu", "fuse_distill")   # what set_fusion(True) turns on
 
     def set_fusion(self, on):
         """All of this implementation's cross-op fusions on, or the reference's op-per-op tape."""
         for f in ("fuse_bn_relu", "fuse_dgrad_add", "fuse_add_relu", "fuse_wgrad_bias", "batch_relayout", "overlap_wgrad",
-                  "fuse_forward", "fuse_linear", "fuse_dgrad_relu", "fuse_pool_relu"):
+                  "fuse_forward", "fuse_linear", "fuse_dgrad_relu", "fuse_pool_relu", "fuse_distill"):
             setattr(self, f, bool(on) and f in self.fusions)
 
     def accumulate(self, a, b):
@@ -321,7 +342,7 @@ class HalfHipOps(HipOps):
     small_wgrad_group = 4
     fuse_pool_relu = False
     fusions = ("fuse_bn_relu", "fuse_add_relu", "fuse_wgrad_bias", "batch_relayout", "overlap_wgrad", "fuse_forward",
-               "fuse_linear", "fuse_dgrad_relu")
+               "fuse_linear", "fuse_dgrad_relu", "fuse_distill")
 
     def __init__(self, dev, dtype):
         HipOps.__init__(self, dev)
@@ -565,6 +586,23 @@ class Cast(_Layer):
         return self.ops.to_storage(dy) if hasattr(self.ops, "to_storage") else dy
 
 
+class Embedding(_Layer):
+    """Vectors of a table by token id, times `scale`.  Its input is whole numbers: ``bwd`` ends the tape."""
+
+    params = ("W",)
+
+    def __init__(self, ops, name, W, scale=1.0):
+        self.ops, self.name, self.W, self.scale = ops, name, ops.from_numpy(W), float(np.float32(scale))
+
+    def fwd(self, ids):
+        self.ids = ids
+        return self.ops.embedding(ids, self.W, self.scale)
+
+    def bwd(self, dy, grads):
+        grads(self.name + ".W", self.W, self.ops.embedding_bwd(dy, self.ids, self.W, self.scale))
+        return None
+
+
 class Linear(_Layer):
     params = ("W", "b")
 
@@ -773,11 +811,22 @@ class Net(object):
                 i += 1
         self.logits = x
         self.t = labels
+        return self.loss(x, labels)
+
+    def inputs(self, x, labels):
+        """A batch as ``make_inputs`` gives it, for ``forward``."""
+        return self.ops.from_numpy(x), self.ops.from_numpy(labels)
+
+    def loss(self, x, labels):
+        """Loss of the logits; keeps what its gradient needs."""
         if getattr(self.ops, "fuse_linear", False):
             self.p, loss = self.ops.softmax_ce_fwd(x, labels)
             return loss
         self.p = self.ops.softmax(x)
         return self.ops.ce_fwd(self.p, labels)
+
+    def loss_bwd(self):
+        return self.ops.softmax_ce_bwd(self.p, self.t, self.batch)
 
     def backward_and_update(self, keep_grads=False, fused_update=False):
         """The timed region: loss-gradient seed -> last parameter updated."""
@@ -797,7 +846,7 @@ class Net(object):
         if convs:
             ops.prepare_backward(convs, update_at_end=fused_update)   # (a layer's data gradient runs before its weights change)
         try:
-            dy = ops.softmax_ce_bwd(self.p, self.t, self.batch)
+            dy = self.loss_bwd()
             if keep_grads:
                 self.grad_log["logits"] = dy
             rev = list(reversed(self.layers))
@@ -824,12 +873,59 @@ class Net(object):
         finally:
             if convs:
                 ops.finish_backward(convs)
-        if keep_grads:
+        if keep_grads and dy is not None:
             self.grad_log["input"] = dy
         if fused_update:
             self.sgd.apply_all(pending)
         self.sgd.step()
         return dy
+
+
+class Targets(object):
+    """What a token model is trained towards: a label and a teacher's top logits for every row, see ``singa.DistillationFwd``."""
+
+    def __init__(self, labels, top, teacher, weights=None, temperature=2.0, soft=0.75, hard=0.25):
+        self.labels, self.top, self.teacher, self.weights = labels, top, teacher, weights
+        self.temperature, self.soft, self.hard = temperature, soft, hard
+
+
+class TokenNet(Net):
+    """A stack from token ids to logits, with the distillation loss."""
+
+    def inputs(self, x, labels):
+        from_numpy = self.ops.from_numpy
+        return from_numpy(x), Targets(from_numpy(labels.labels), from_numpy(labels.top), from_numpy(labels.teacher),
+                                      None if labels.weights is None else from_numpy(labels.weights), labels.temperature,
+                                      labels.soft, labels.hard)
+
+    def loss(self, x, targets):
+        self.dlogits = None
+        if getattr(self.ops, "fuse_distill", False):
+            loss, self.dlogits = self.ops.distill_fwd_bwd(x, targets, self.batch)
+            return loss
+        loss, self.p = self.ops.distill_fwd(x, targets)
+        return loss
+
+    def loss_bwd(self):
+        if self.dlogits is not None:
+            return self.dlogits
+        return self.ops.distill_bwd(self.logits, self.p, self.t, self.batch)
+
+    def adopt_saved_tensors(self, other):
+        Net.adopt_saved_tensors(self, other)
+        self.logits = self.ops.from_numpy(other.ops.to_numpy(other.logits))
+        self.dlogits = None
+
+
+def build_token_mlp(ops, rng, lr=0.05, momentum=0.9, vocab=10000, dim=64, context=4, hidden=256):
+    """The vectors of the last `context` tokens, one behind the other, through a hidden layer to the next token's logits."""
+    return TokenNet(ops, [
+        Embedding(ops, "embedding", (rng.standard_normal((vocab, dim)) / np.sqrt(dim)).astype(np.float32), np.sqrt(dim)),
+        Flatten(ops, "flatten"),
+        Linear(ops, "linear1", he_normal(rng, context * dim, hidden), np.zeros(hidden, np.float32)),
+        ReLU(ops, "relu"),
+        Linear(ops, "linear2", he_normal(rng, hidden, vocab), np.zeros(vocab, np.float32)),
+    ], lr, momentum)
 
 
 def build_mlp(ops, rng, lr=0.05, momentum=0.9, in_dim=784, hidden=1000, classes=10):
@@ -918,6 +1014,9 @@ CONFIGS = {
     "resnet50": (build_resnet50, {}, (3, 224, 224), 1000, 128),
     "resnet50_small": (build_resnet50, {"classes": 100, "final_pool": 2, "widths": (16, 32, 64, 128)},
                        (3, 64, 64), 100, 4),
+    # token ids to the next token's logits, distillation loss
+    "token_mlp": (build_token_mlp, {}, (4,), 10000, 256),
+    "token_mlp_small": (build_token_mlp, {"vocab": 1003, "dim": 20, "hidden": 48}, (4,), 1003, 24),
 }
 
 SEED_BASE = 0x5167A000
@@ -926,13 +1025,19 @@ SEED_BASE = 0x5167A000
 # splitmix64 -> Box-Muller), so the bytes do not depend on a library's random stream and a smaller batch is
 # a prefix of a larger one.  (Fixed numbers: adding a configuration leaves the inputs of the others unchanged.)
 _CONFIG_INDEX = {"mlp": 1, "conv": 2, "cnn": 3, "resnet18": 4, "resnet50": 5, "resnet18_small": 6, "smoke_cnn": 7,
-                 "resnet50_small": 8}
+                 "resnet50_small": 8, "token_mlp": 9, "token_mlp_small": 10}
+TOP_LOGITS = 16   # of a token model's teacher
 
 
 def make_inputs(name, batch=None):
     builder, kw, xshape, classes, default_batch = CONFIGS[name]
     batch = batch or default_batch
     base = SEED_BASE + 256 * _CONFIG_INDEX[name]
+    if builder is build_token_mlp:
+        # (tensors 0 and 1 as for the others; 254 and 255, behind the weights, are the teacher's)
+        labels = rng.integers(base + 1, (batch,), classes)
+        top = (rng.integers(base + 254, (batch, 1), classes) + 7 * np.arange(TOP_LOGITS)).astype(np.int32) % classes
+        return rng.integers(base + 0, (batch,) + xshape, classes), Targets(labels, top, 2 * rng.normal(base + 255, (batch, TOP_LOGITS)))
     x = rng.normal(base + 0, (batch,) + xshape)
     labels = rng.integers(base + 1, (batch,), classes)
     return x, labels
@@ -990,7 +1095,7 @@ def run_parity_case(name, dev, checker_ops, batch=None, steps=1, share_activatio
     for step in range(steps):
         losses = []
         for net in nets:
-            loss = net.forward(net.ops.from_numpy(x), net.ops.from_numpy(labels))
+            loss = net.forward(*net.inputs(x, labels))
             losses.append(net.ops.to_numpy(loss))
         errors["step%d.loss" % step] = _nl2(losses[0], losses[1])
         errors["step%d.logits" % step] = _nl2(hip.to_numpy(nets[0].logits), checker_ops.to_numpy(nets[1].logits))
