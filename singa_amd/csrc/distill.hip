@@ -334,10 +334,15 @@ __device__ __forceinline__ void list_columns(const Rows<typename S::elem> &a, si
 // A row's vectors through a buffer descriptor: what is behind the last of them reads as zero and is not stored, so that a load or a store needs no
 // branch around it, and waiting for one of them leaves the younger ones in flight.  (The offset is all in the lane's register: the
 // descriptor's limit is compared with that.)
+constexpr unsigned kOutside = 0x07ffffffu;   // (times 16: 2 GB behind the row's beginning; a row has 1 GB at the most)
 struct RowBuffer {
   __amdgpu_buffer_rsrc_t r;
   __device__ __forceinline__ RowBuffer(const void *p, unsigned bytes)
       : r(__builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, int(bytes), 0x00020000)) {}
+  // of `vecs` vectors behind `pad` places without one, which are asked for at kOutside instead
+  static __device__ __forceinline__ RowBuffer padded(const void *first, unsigned vecs, unsigned pad) {
+    return RowBuffer(static_cast<const char *>(first) - pad * 16, vecs ? (pad + vecs) * 16 : 0);
+  }
   // (STREAM: past the caches, the "nt" bit)
   template <bool STREAM>
   __device__ __forceinline__ sgh_v4u load(unsigned vec) const {
@@ -351,11 +356,14 @@ struct RowBuffer {
 
 // How a row lies: `head` elements up to the first 16-byte boundary, `vecs` vectors, and what is left.  (Vectors that begin between boundaries
 // cost a sixth of the rate: 83 -> 97 us for 4096 rows of 50000 and 50001 binary16 values.)  The elements around the vectors are a thread's each:
-// `odd` is this one's, or none.
+// `odd` is this one's, or none.  `pad` vectors are missing between a 128-byte line's beginning and the first: where a gradient is stored, the
+// first `pad` places of the row are no vectors, so that no line is stored in two
+// parts (4096 rows of 65001 bfloat16 values: the gradient 222 -> 194 us, both in one call 243 -> 232).
 struct Lie {
-  unsigned head, vecs, odd;
+  unsigned head, vecs, odd, pad;
 };
 constexpr unsigned kNone = 0xffffffffu;
+constexpr unsigned kLine = 128;
 template <class S>
 __device__ __forceinline__ Lie lie_of(const typename S::elem *x, unsigned dim, unsigned tid) {
   constexpr unsigned V = S::VEC, e = sizeof(typename S::elem);
@@ -366,6 +374,7 @@ __device__ __forceinline__ Lie lie_of(const typename S::elem *x, unsigned dim, u
   l.vecs = (dim - l.head) / V;
   const unsigned behind = l.head + l.vecs * V, left = dim - behind;
   l.odd = tid < l.head ? tid : tid >= V && tid - V < left ? behind + tid - V : kNone;
+  l.pad = unsigned(reinterpret_cast<uintptr_t>(x + l.head)) % kLine / 16;
   return l;
 }
 template <class S>
@@ -382,9 +391,12 @@ __device__ __forceinline__ sgh_v4u packed(const float *v) {
 // A row's vectors, U of a thread at a time and the next U in flight: f(vector, its number, whether every thread of the team has one)
 constexpr int kAhead = 4;
 template <int NT, bool STREAM>
-__device__ __forceinline__ void ask_vectors(const RowBuffer &x, unsigned from, sgh_v4u *v) {
+__device__ __forceinline__ void ask_vectors(const RowBuffer &x, unsigned from, sgh_v4u *v, unsigned pad = 0) {
 #pragma unroll
-  for (int u = 0; u < kAhead; ++u) v[u] = x.load<STREAM>(from + u * NT + Team<NT>::tid());
+  for (int u = 0; u < kAhead; ++u) {
+    const unsigned i = from + u * NT + Team<NT>::tid();
+    v[u] = x.load<STREAM>(u == 0 && i < pad ? kOutside : i);
+  }
 }
 template <int NT, bool STREAM, class F>
 __device__ __forceinline__ void stream_row(const RowBuffer &x, unsigned vecs, sgh_v4u *v, F f) {
@@ -421,11 +433,13 @@ __device__ __forceinline__ sgh_v4u slope_vector(const Slope &s, const sgh_v4u &r
 
 // dx of a row's vectors [from, from + vecs) but for the list's columns, from memory (dx may be x: a thread stores what it has read); `none`: zeros
 template <int NT, class S, bool STREAM>
-__device__ __forceinline__ void slope_row(const typename S::elem *x, typename S::elem *dx, unsigned vecs, bool none, const Slope &s) {
-  const RowBuffer from(x, none ? 0 : vecs * 16), to(dx, vecs * 16);
+__device__ __forceinline__ void slope_row(const typename S::elem *x, typename S::elem *dx, unsigned vecs, unsigned pad, bool none,
+                                          const Slope &s) {
+  const RowBuffer from = RowBuffer::padded(x, none ? 0 : vecs, pad), to = RowBuffer::padded(dx, vecs, pad);
   sgh_v4u v[kAhead];
-  ask_vectors<NT, STREAM>(from, 0, v);
-  stream_row<NT, STREAM>(from, vecs, v, [&](const sgh_v4u &raw, unsigned vec, bool) { to.store<STREAM>(slope_vector<S>(s, raw), vec); });
+  ask_vectors<NT, STREAM>(from, 0, v, pad);
+  stream_row<NT, STREAM>(from, vecs ? pad + vecs : 0, v,
+                         [&](const sgh_v4u &raw, unsigned i, bool) { to.store<STREAM>(slope_vector<S>(s, raw), i < pad ? kOutside : i); });
 }
 
 // The team's statistics from its threads'; `red`: one of each wavefront
@@ -530,7 +544,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_fwd(Rows<typenam
       const Slope s = slope_of(a, q.w, r, soft, q.hard);
       const bool none = !(soft || q.hard);
       if (NT != SGH_WAVE) G::sync();   // (the list's logits are read: dx may be x)
-      slope_row<NT, S, STREAM>(x + lie.head, a.dx + row * a.dim + lie.head, vecs, none, s);
+      slope_row<NT, S, STREAM>(x + lie.head, a.dx + row * a.dim + lie.head, vecs, lie.pad, none, s);
       if (lie.odd != kNone) S::st(a.dx + row * a.dim + lie.odd, s(tail));
       G::sync();
       if (!none) list_columns<NT, S>(a, row, 0, a.dim, s, list, entry);
@@ -579,6 +593,8 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
     q.may_soft = a.k && a.soft != 0.f && q.w != 0.f;
     return q;
   };
+  // a thread's first place in a row that lies like this
+  auto place = [&](const Lie &l) { return unsigned(tid) < l.pad ? kOutside : unsigned(tid); };
   sgh_v4u held[U];
   float tail = 0.f;
   Entry entry;
@@ -588,9 +604,9 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
   Lie lie = lie_of<S>(a.x + row * a.dim, unsigned(a.dim), tid);
   {
     const T *first = a.x + row * a.dim;
-    const RowBuffer x(first + lie.head, q.any() ? lie.vecs * 16 : 0);
+    const RowBuffer x = RowBuffer::padded(first + lie.head, q.any() ? lie.vecs : 0, lie.pad);
 #pragma unroll
-    for (int u = 0; u < U; ++u) held[u] = x.load<STREAM>(u * NT + tid);
+    for (int u = 0; u < U; ++u) held[u] = x.load<STREAM>(u == 0 ? place(lie) : u * NT + tid);
     if (lie.odd != kNone && q.any()) tail = S::ld(first + lie.odd);
   }
   int turn = 0;
@@ -603,8 +619,9 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
     const List list = list_at(lds + (G::id() * G::kLists + turn) * list_bytes(a.k), a.k);
     const Lie next_lie = lie_of<S>(nx, unsigned(a.dim), tid);
     T *dx = a.dx + row * a.dim;
-    const unsigned vecs = lie.vecs;
-    const RowBuffer to(dx + lie.head, vecs * 16), then(nx + next_lie.head, goes_on && nq.any() ? next_lie.vecs * 16 : 0);
+    const unsigned places = lie.pad + lie.vecs;
+    const RowBuffer to = RowBuffer::padded(dx + lie.head, lie.vecs, lie.pad);
+    const RowBuffer then = RowBuffer::padded(nx + next_lie.head, goes_on && nq.any() ? next_lie.vecs : 0, next_lie.pad);
     bool any = false;
     if (lister) {
       any = gather_list<S>(a, row, q.hard ? q.label : -1, true, list, entry);
@@ -618,7 +635,8 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
       sum.start(ct, want);
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (unsigned(u * NT) < vecs) take_vector<S>(sum, held[u], u * NT + tid, vecs, unsigned(u * NT + NT) <= vecs, ct, want);
+        if (unsigned(u * NT) < places)
+          take_vector<S>(sum, held[u], u == 0 ? place(lie) : u * NT + tid, places, (u != 0 || lie.pad == 0) && unsigned(u * NT + NT) <= places, ct, want);
       if (lie.odd != kNone) sum.take<1>(&tail, ct, want);
       r = team_sums<NT>(a, sum, ct, red);
       soft = q.may_soft && (NT == SGH_WAVE ? any : listed != 0);
@@ -631,10 +649,12 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
     next_raw = raw_at(next + step);
     const Slope s = slope_of(a, q.w, r, soft, q.hard);
     if (a.in_place && NT != SGH_WAVE) G::sync();   // (the list's logits are read)
+    unsigned i = tid;
+    asm("" : "+v"(i));   // (the places of a row are not kept in registers of their own from row to row: 20 of these went to scratch memory)
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      to.store<STREAM>(slope_vector<S>(s, held[u]), u * NT + tid);
-      held[u] = then.load<STREAM>(u * NT + tid);
+      to.store<STREAM>(slope_vector<S>(s, held[u]), u == 0 ? place(lie) : u * NT + i);
+      held[u] = then.load<STREAM>(u == 0 ? place(next_lie) : u * NT + i);
     }
     if (lie.odd != kNone) S::st(dx + lie.odd, s(tail));
     if (next_lie.odd != kNone && goes_on && nq.any()) tail = S::ld(nx + next_lie.odd);
@@ -685,7 +705,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_bwd(Rows<typenam
       shares();
       if (NT != SGH_WAVE) G::sync();
     }
-    slope_row<NT, S, STREAM>(x + start, dx + start, vecs, none, s);
+    slope_row<NT, S, STREAM>(x + start, dx + start, vecs, begins ? lie.pad : 0, none, s);
     if (odd) S::st(dx + lie.odd, s(tail));
     if (!a.in_place) shares();
     G::sync();
@@ -775,13 +795,16 @@ int distill(Rows<typename S::elem> a, size_t k, bool fwd, bool grad, void *strea
                              bytes * (grad ? 2 : 1), s);
   const size_t vecs = a.dim / S::VEC;
   if (fwd && grad) {
-    if (vecs <= 64 * 4) return launch_held<64, 4, 6, S>(a, s);
-    if (vecs <= 64 * 8) return launch_held<64, 8, 5, S>(a, s);
-    if (vecs <= 64 * 16) return launch_held<64, 16, 4, S>(a, s);
-    if (vecs <= 128 * 16) return launch_held<128, 16, 4, S>(a, s);
-    if (vecs <= 256 * 16) return launch_held<256, 16, 4, S>(a, s);
-    if (vecs <= 512 * 16) return launch_held<512, 16, 4, S>(a, s);
-    if (vecs <= 1024 * 16) return launch_held<1024, 16, 4, S>(a, s);
+    // places of a row's vectors
+    const bool lines = (reinterpret_cast<uintptr_t>(a.x) | a.dim * sizeof(typename S::elem)) % kLine == 0;
+    const size_t places = lines ? vecs : vecs + kLine / 16 - 1;
+    if (places <= 64 * 4) return launch_held<64, 4, 6, S>(a, s);
+    if (places <= 64 * 8) return launch_held<64, 8, 5, S>(a, s);
+    if (places <= 64 * 16) return launch_held<64, 16, 4, S>(a, s);
+    if (places <= 128 * 16) return launch_held<128, 16, 4, S>(a, s);
+    if (places <= 256 * 16) return launch_held<256, 16, 4, S>(a, s);
+    if (places <= 512 * 16) return launch_held<512, 16, 4, S>(a, s);
+    if (places <= 1024 * 16) return launch_held<1024, 16, 4, S>(a, s);
     return launch_fwd<512, S, true>(a, s);
   }
   const size_t cus = size_t(sgh_num_cus());
