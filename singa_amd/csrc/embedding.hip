@@ -299,20 +299,23 @@ __global__ __launch_bounds__(kBlock) void k_embed_rows(Bwd<typename S::elem> a, 
 
 // ------------------------------------------------------------------------------------ many tokens
 
-// 1. The tokens are sorted by id, stable: passes of at most 9 bits from the lowest.  A pass counts the digits of each workgroup's stretch of
-//    tokens, turns the counts into the place of every stretch's first token with a digit, and moves the tokens there.  Up to kOneTokens
-//    one workgroup does all passes.  The workgroups that sort are few: beside them, in the same launches, others look through the ids for
-//    the rows that have no token and store those.
+// 1. The tokens are sorted by id, stable.  Up to kRankTokens each token counts those that belong in front of it, in one launch.  More are sorted
+//    in passes of at most 9 bits from the lowest: a pass counts the digits of each workgroup's stretch of tokens, turns the counts into the
+//    place of every stretch's first token with a digit, and moves the tokens there.  Sorting leaves the memory idle: beside it, in the same
+//    launches, other workgroups store the rows that have no token.
 // 2. Tiles of sorted tokens: a wavefront goes through the tokens of a tile (and a slice of the rows' elements), and stores each row whose
 //    tokens begin there.  Where a row's tokens hold a whole tile, that tile's sum is kept instead,
 // 3. and the tile in which they begin joins the sums.
 
+constexpr unsigned kNoKey = 0xffffffffu;
 constexpr int kDigitBits = 9, kBins = 1 << kDigitBits;
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / SGH_WAVE;
 constexpr int kItems = 2;                              // tokens of a thread at a time
 constexpr unsigned kStretch = kSortThreads * kItems;
 constexpr int kMostStretches = 64;                     // each workgroup reads the counts of all
-constexpr unsigned kOneTokens = 8192;
+// (Counting is quadratic.  The whole gradient for a table of 131072 rows of 64 bfloat16 elements: 20.6 us for 8192 tokens counted, 29.4 sorted in
+// passes; 33.8 and 31.5 for 16384.)
+constexpr unsigned kRankTokens = 8192;
 constexpr unsigned kFillRows = 8192;                   // rows that a workgroup looks out for
 
 struct Sort {
@@ -323,10 +326,18 @@ struct Sort {
   unsigned tokens, vocab, per_stretch;
   int pad, shift, bins, stretches;
 };
+// Rows without a token: `rows` of them are looked after by each workgroup, the share `launch` of `launches` in this launch
+enum class Taken {
+  kIds,      // the rows that have one are found by looking through all ids,
+  kClear,    // or they are marked: the first launch clears the marks (and stores nothing), the first move sets them,
+  kMarks,    // the later launches read them;
+  kCounts    // with one digit they are in the counts
+};
 struct Fill {
-  unsigned rows;               // of a workgroup
+  unsigned rows;
   int launch, launches;
-  unsigned char *taken;        // [vocab]: rows with a token
+  Taken from;
+  unsigned char *taken;        // [vocab] or null
 };
 
 struct SortSpace {
@@ -418,15 +429,18 @@ __device__ __forceinline__ unsigned counted_key(const Sort &s, int id, bool ther
   return k;
 }
 
-// The rows that have no token: zero, or `add`.  Workgroup `part` of each launch has the same `f.rows` rows and stores its share of them; in
-// the first launch it looks through the ids for all of them and leaves what it saw for the later ones.
+// The rows that have no token: zero, or `add`
 template <class S, int EPL, bool STREAM>
-__device__ __forceinline__ void fill_rows(const Bwd<typename S::elem> &a, const Fill &f, unsigned part, unsigned char *taken) {
+__device__ __forceinline__ void fill_rows(const Bwd<typename S::elem> &a, const Sort &s, const Fill &f, unsigned part, unsigned char *taken) {
   const size_t row0 = size_t(part) * f.rows;
   const unsigned rows = a.vocab - row0 < f.rows ? unsigned(a.vocab - row0) : f.rows, threads = kSortThreads;
   const unsigned tid = threadIdx.x, lane = tid & (SGH_WAVE - 1), wave = tid >> 6;
   const unsigned lo = rows * f.launch / f.launches, hi = rows * (f.launch + 1) / f.launches;   // its share
-  if (f.launch == 0) {
+  if (f.from == Taken::kClear) {
+    for (unsigned r = tid; r < rows; r += threads) f.taken[row0 + r] = 0;
+    return;
+  }
+  if (f.from == Taken::kIds) {
     for (unsigned r = tid; r < rows; r += threads) taken[r] = 0;
     __syncthreads();
     constexpr unsigned U = 8;
@@ -440,12 +454,16 @@ __device__ __forceinline__ void fill_rows(const Bwd<typename S::elem> &a, const 
         if (id[u] >= 0 && r < rows && id[u] != a.pad) taken[r] = 1;
       }
     }
-    __syncthreads();
-    for (unsigned r = hi + tid; r < rows; r += threads) f.taken[row0 + r] = taken[r];
-  } else {
+  } else if (f.from == Taken::kMarks) {
     for (unsigned r = lo + tid; r < hi; r += threads) taken[r] = f.taken[row0 + r];
-    __syncthreads();
+  } else {
+    for (unsigned r = lo + tid; r < hi; r += threads) {
+      unsigned n = 0;
+      for (int b = 0; b < s.stretches; ++b) n |= s.counts[b * s.bins + row0 + r];
+      taken[r] = n != 0;
+    }
   }
+  __syncthreads();
   const size_t vecs = (a.dim + EPL - 1) / EPL;
   const unsigned per_wave = SGH_WAVE / a.lanes;
   constexpr int U = 4;
@@ -475,61 +493,77 @@ __device__ __forceinline__ void fill_rows(const Bwd<typename S::elem> &a, const 
   }
 }
 
-// All passes by the first workgroup, every token in a register of it; they change places through LDS (as 2 x 8192 stores of single words
-// to global memory a pass took 12 us)
-struct OneSpace {
-  SortSpace sort;
-  unsigned key[kOneTokens];
-  uint16_t place[kOneTokens];
-};
-union OneLds {
-  OneSpace one;
+// Up to kRankTokens tokens: the place of a token in the sorted list is the number of those with a smaller key, or with the same one further in
+// front.  A workgroup has all keys in LDS, where a wavefront goes through them for M tokens at a time, its lanes four neighbouring keys each:
+// two instructions for 64 comparisons, T^2 of these: 4.5 us for 1025 tokens, 6.3 for 4096, 8.4 for 8192.  (Passes by one workgroup, the tokens
+// in its registers: 12 us for 2048, 19 for 8192.)
+constexpr unsigned kChunk = 4 * SGH_WAVE;   // keys that a wavefront looks at at once
+union RankLds {
+  sgh_v4u keys[kRankTokens / 4];
   unsigned char taken[kFillRows];
 };
-constexpr int kOneItems = int(kOneTokens) / kSortThreads;
-template <class S, int EPL, bool STREAM>
-__global__ __launch_bounds__(kSortThreads) void k_embed_sort(Bwd<typename S::elem> a, Sort s, int passes, int digit_bits, Fill f) {
-  __shared__ OneLds lds;
-  if (blockIdx.x != 0) return fill_rows<S, EPL, STREAM>(a, f, blockIdx.x - 1, lds.taken);
-  OneSpace &sp = lds.one;
-  const unsigned tid = threadIdx.x, lane = tid & (SGH_WAVE - 1), wave = tid >> 6;
-  const unsigned per_wave = (s.tokens + kSortThreads - 1) / kSortThreads * SGH_WAVE;
-  Held<kOneItems> h;
+template <int M>
+__device__ __forceinline__ void rank_tokens(const Sort &s, const RankLds &lds, unsigned first) {
+  const unsigned *all = reinterpret_cast<const unsigned *>(lds.keys), lane = threadIdx.x & (SGH_WAVE - 1);
+  const sgh_v4u *keys = lds.keys + lane;
+  unsigned key[M], n[M];
 #pragma unroll
-  for (int u = 0; u < kOneItems; ++u) {
-    const unsigned i = wave * per_wave + u * SGH_WAVE + lane;
-    const bool there = u * SGH_WAVE < per_wave && i < s.tokens;
-    h.place[u] = there ? i : kNoPlace;
-    h.key[u] = there ? unsigned(s.ids[i]) : 0;
+  for (int m = 0; m < M; ++m) {
+    key[m] = __builtin_amdgcn_readfirstlane(all[first + m]);   // (kNoKey behind the last token)
+    n[m] = 0;
+  }
+  // `more`: 1 where equal keys are in front
+  auto count = [&](unsigned from, unsigned to, unsigned more) {
+#pragma unroll 4
+    for (unsigned c = from; c < to; ++c) {
+      const sgh_v4u k = keys[c * SGH_WAVE];
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) n[m] += k[e] < key[m] + more;
+    }
+  };
+  const unsigned here = first / kChunk, chunks = (s.tokens + kChunk - 1) / kChunk;   // (M divides kChunk and `first`)
+  count(0, here, 1);
+  count(here, chunks, 0);
+  const sgh_v4u k = keys[here * SGH_WAVE];
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) n[m] += k[e] == key[m] && here * kChunk + lane * 4 + e < first + m;
+#pragma unroll
+    for (int o = 1; o < SGH_WAVE; o <<= 1) n[m] += __shfl_xor(n[m], o, SGH_WAVE);
   }
 #pragma unroll
-  for (int u = 0; u < kOneItems; ++u) h.key[u] = counted_key(s, int(h.key[u]), h.place[u] != kNoPlace);
-  for (int pass = 0; pass < passes; ++pass) {
-    s.shift = pass * digit_bits;
-    clear_counts(sp.sort);
-    __syncthreads();
-    sort_rank(s, per_wave, sp.sort, h);
-    __syncthreads();
-    const unsigned lower = lower_digits(sp.sort, tid < unsigned(s.bins) ? front_counts(sp.sort) : 0);
-    if (tid < unsigned(s.bins)) sp.sort.next[tid] = lower;
-    __syncthreads();
+  for (int m = 0; m < M; ++m)
+    if (int(lane) == m && first + m < s.tokens) {
+      if (key[m] == s.vocab && s.ids[first + m] != s.pad) atomicAdd(&g_index_errors, 1);
+      s.out[n[m]] = Token{key[m], first + m};
+    }
+}
+template <class S, int EPL, bool STREAM>
+__global__ __launch_bounds__(kSortThreads) void k_embed_rank(Bwd<typename S::elem> a, Sort s, int per_wave, Fill f) {
+  __shared__ RankLds lds;
+  if (blockIdx.x >= unsigned(s.stretches)) return fill_rows<S, EPL, STREAM>(a, s, f, blockIdx.x - s.stretches, lds.taken);
+  unsigned *all = reinterpret_cast<unsigned *>(lds.keys);
+  const unsigned room = (s.tokens + kChunk - 1) / kChunk * kChunk;
+  constexpr unsigned U = 8;
+  for (unsigned i = threadIdx.x; i < room; i += U * kSortThreads) {
+    int id[U];
 #pragma unroll
-    for (int u = 0; u < kOneItems; ++u)
-      if (h.place[u] != kNoPlace) {
-        const unsigned to = place_of(s, sp.sort, h.key[u], h.rank[u]);
-        sp.key[to] = h.key[u];
-        sp.place[to] = uint16_t(h.place[u]);
-      }
-    __syncthreads();
+    for (unsigned u = 0; u < U; ++u) id[u] = i + u * kSortThreads < s.tokens ? s.ids[i + u * kSortThreads] : 0;
 #pragma unroll
-    for (int u = 0; u < kOneItems; ++u) {
-      const unsigned i = wave * per_wave + u * SGH_WAVE + lane;
-      if (h.place[u] != kNoPlace) h.key[u] = sp.key[i], h.place[u] = sp.place[i];
+    for (unsigned u = 0; u < U; ++u) {
+      const unsigned at = i + u * kSortThreads;
+      if (at < room) all[at] = at < s.tokens ? key_of(id[u], s.vocab, s.pad) : kNoKey;
     }
   }
-#pragma unroll
-  for (int u = 0; u < kOneItems; ++u)
-    if (h.place[u] != kNoPlace) s.out[wave * per_wave + u * SGH_WAVE + lane] = Token{h.key[u], h.place[u]};
+  __syncthreads();
+  const unsigned first = __builtin_amdgcn_readfirstlane((blockIdx.x * kSortWaves + (threadIdx.x >> 6)) * per_wave);
+  if (first >= s.tokens) return;
+  if (per_wave == 1) rank_tokens<1>(s, lds, first);
+  else if (per_wave == 2) rank_tokens<2>(s, lds, first);
+  else rank_tokens<4>(s, lds, first);
 }
 
 union SortLds {
@@ -540,7 +574,7 @@ union SortLds {
 template <class S, int EPL, bool STREAM>
 __global__ __launch_bounds__(kSortThreads) void k_embed_count(Bwd<typename S::elem> a, Sort s, Fill f) {
   __shared__ SortLds lds;
-  if (blockIdx.x >= unsigned(s.stretches)) return fill_rows<S, EPL, STREAM>(a, f, blockIdx.x - s.stretches, lds.taken);
+  if (blockIdx.x >= unsigned(s.stretches)) return fill_rows<S, EPL, STREAM>(a, s, f, blockIdx.x - s.stretches, lds.taken);
   unsigned *h = lds.sort.next;
   for (int d = threadIdx.x; d < s.bins; d += kSortThreads) h[d] = 0;
   __syncthreads();
@@ -553,9 +587,23 @@ __global__ __launch_bounds__(kSortThreads) void k_embed_count(Bwd<typename S::el
 template <class S, int EPL, bool STREAM>
 __global__ __launch_bounds__(kSortThreads) void k_embed_move(Bwd<typename S::elem> a, Sort s, Fill f) {
   __shared__ SortLds lds;
-  if (blockIdx.x >= unsigned(s.stretches)) return fill_rows<S, EPL, STREAM>(a, f, blockIdx.x - s.stretches, lds.taken);
+  if (blockIdx.x >= unsigned(s.stretches)) return fill_rows<S, EPL, STREAM>(a, s, f, blockIdx.x - s.stretches, lds.taken);
   SortSpace &sp = lds.sort;
   const int tid = threadIdx.x;
+  const unsigned from = blockIdx.x * s.per_stretch, left = s.tokens - from;
+  const size_t to = size_t(from) + (left < s.per_stretch ? left : s.per_stretch);
+  const unsigned lane = tid & (SGH_WAVE - 1), wave = tid >> 6, per_wave = SGH_WAVE * kItems;
+  Held<kItems> h;
+  auto ask = [&](size_t base) {
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+      const size_t i = base + wave * per_wave + u * SGH_WAVE + lane;
+      Token t = {0, kNoPlace};
+      if (i < to) t = s.ids ? Token{unsigned(s.ids[i]), unsigned(i)} : s.in[i];
+      h.key[u] = t.key, h.place[u] = t.place;
+    }
+  };
+  ask(from);
   // all tokens of a digit, and those of the stretches in front, by the threads that share it
   const int digit = tid & (s.bins - 1), share = tid / s.bins, shares = kSortThreads / s.bins;
   unsigned all = 0, before = 0;
@@ -573,23 +621,15 @@ __global__ __launch_bounds__(kSortThreads) void k_embed_move(Bwd<typename S::ele
     for (int o = 1; o < shares; ++o) all += of_thread[o * s.bins + tid], before += of_thread[kSortThreads + o * s.bins + tid];
   before += lower_digits(sp, tid < s.bins ? all : 0);
   __syncthreads();
-  const unsigned from = blockIdx.x * s.per_stretch, left = s.tokens - from;
-  const size_t to = size_t(from) + (left < s.per_stretch ? left : s.per_stretch);
-  const unsigned lane = tid & (SGH_WAVE - 1), wave = tid >> 6, per_wave = SGH_WAVE * kItems;
   if (tid < s.bins) sp.next[tid] = before;
   for (size_t base = from; base < to; base += kStretch) {
     clear_counts(sp);
-    Held<kItems> h;
-#pragma unroll
-    for (int u = 0; u < kItems; ++u) {
-      const size_t i = base + wave * per_wave + u * SGH_WAVE + lane;
-      Token t = {0, kNoPlace};
-      if (i < to) t = s.ids ? Token{unsigned(s.ids[i]), unsigned(i)} : s.in[i];
-      h.key[u] = t.key, h.place[u] = t.place;
-    }
     if (s.ids) {
 #pragma unroll
-      for (int u = 0; u < kItems; ++u) h.key[u] = counted_key(s, int(h.key[u]), h.place[u] != kNoPlace);
+      for (int u = 0; u < kItems; ++u) {
+        h.key[u] = counted_key(s, int(h.key[u]), h.place[u] != kNoPlace);
+        if (f.taken && h.place[u] != kNoPlace && h.key[u] < s.vocab) f.taken[h.key[u]] = 1;
+      }
     }
     __syncthreads();
     sort_rank(s, per_wave, sp, h);
@@ -599,12 +639,11 @@ __global__ __launch_bounds__(kSortThreads) void k_embed_move(Bwd<typename S::ele
 #pragma unroll
     for (int u = 0; u < kItems; ++u)
       if (h.place[u] != kNoPlace) s.out[place_of(s, sp, h.key[u], h.rank[u])] = Token{h.key[u], h.place[u]};
+    ask(base + kStretch);
     __syncthreads();
     if (tid < s.bins) sp.next[tid] += total;
   }
 }
-
-constexpr unsigned kNoKey = 0xffffffffu;
 
 // Where a wavefront's lanes are: a tile of its own for every `lanes` of them, and a vector of the rows
 __host__ __device__ inline unsigned slices_at_once(int slices) { return slices < kWaves ? slices : kWaves; }   // of a workgroup
@@ -757,7 +796,7 @@ __global__ __launch_bounds__(kBlock) void k_embed_join(Bwd<typename S::elem> a) 
 }
 
 struct BwdPlan {
-  bool scan, one;
+  bool scan, rank;
   unsigned tile, tiles;
   int passes, digit_bits, stretches;
   unsigned per_stretch;
@@ -769,7 +808,7 @@ BwdPlan bwd_plan(size_t tokens, size_t vocab, size_t dim) {
   BwdPlan p = {};
   p.scan = tokens <= kScanTokens;
   if (p.scan) return p;
-  p.one = tokens <= kOneTokens;
+  p.rank = tokens <= kRankTokens;
   p.tile = tokens <= 16384 ? 16 : 32;   // few, so that neither a tile nor the tiles of one row are a long sum
   p.tiles = unsigned((tokens + p.tile - 1) / p.tile);
   int bits = 1;
@@ -782,10 +821,10 @@ BwdPlan bwd_plan(size_t tokens, size_t vocab, size_t dim) {
   p.stretches = int((stretches + each - 1) / each);
   const size_t list = up256(tokens * sizeof(Token));
   p.other = list;
-  p.counts = p.one ? list : 2 * list;
-  p.tail = p.counts + (p.one ? 0 : up256(size_t(p.stretches) * kBins * 4));
+  p.counts = p.rank ? list : 2 * list;
+  p.tail = p.counts + (p.rank ? 0 : up256(size_t(p.stretches) * kBins * 4));
   p.taken = p.tail + up256(size_t(p.tiles) * 4);
-  p.partial = p.taken + (p.one ? 0 : up256(vocab));
+  p.partial = p.taken + (p.rank || p.passes == 1 ? 0 : up256(vocab));
   p.bytes = p.partial + 2 * size_t(p.tiles) * up256(dim * 4);
   return p;
 }
@@ -818,45 +857,60 @@ int launch_bwd(Bwd<typename S::elem> a, const BwdPlan &p, void *workspace, hipSt
   a.sorted = sorted, a.tail = at(p.tail);
   a.partial = reinterpret_cast<float *>(ws + p.partial);
   a.tile = p.tile, a.pitch = up256(a.dim * 4) / 4;
-  // The rows without a token, spread over the launches that sort: at least 64 KB of the result for a workgroup and launch.  (Leaving a part
-  // for the launch of the tiles, whose own traffic they would run beside, was slower: 44.8 -> 48.9 and 337 -> 400 us for the cases below.)
-  Fill f = {0, 0, p.one ? 1 : 2 * p.passes, reinterpret_cast<unsigned char *>(ws + p.taken)};
+  // The rows without a token, spread over the launches that sort and know them: at least 64 KB of the result for a workgroup and launch.
+  // (Leaving a part for the launch of the tiles, whose own traffic they would run beside, was slower: 44.8 -> 48.9 and 337 -> 400 us for 8192
+  // tokens of 1024 fp32 elements and 65536 of 2048 bfloat16.  Looking through the ids takes a workgroup 15 us for 131072 tokens; so the
+  // rows of more than kRankTokens are marked on the way: 82 -> 68 us for 131072 tokens, 32000 rows of 512 bfloat16.)
+  const bool marked = !p.rank && p.passes > 1;
+  Fill f = {0, 0, marked ? 2 * p.passes - 2 : 1, p.rank ? Taken::kIds : marked ? Taken::kClear : Taken::kCounts, nullptr};
+  Sort so = {};
+  so.ids = a.ids, so.counts = at(p.counts), so.tokens = a.tokens, so.vocab = unsigned(a.vocab), so.pad = a.pad;
+  so.bins = 1 << p.digit_bits, so.stretches = p.stretches, so.per_stretch = p.per_stretch;
+  const size_t cus = size_t(sgh_num_cus());
+  // Tokens that a wavefront ranks: one, or two where that leaves a workgroup for every CU; beside a table that takes longer to fill, four, for more
+  // room there (8192 tokens, 50000 rows of 1024 bfloat16: 34.5 -> 29.7 us; of 41 MB: 34.9 -> 36.6)
+  const size_t table = a.vocab * a.dim * sizeof(typename S::elem);
+  const int per_wave = a.add != a.dW && table >= size_t(64) << 20 ? 4 : a.tokens > cus * kSortWaves ? 2 : 1;
+  if (p.rank) so.stretches = int((a.tokens + kSortWaves * per_wave - 1) / (kSortWaves * per_wave));
   unsigned fill_blocks = 0;
   if (a.add != a.dW) {
-    size_t want = (a.vocab * a.dim * sizeof(typename S::elem) >> 16) / f.launches;
-    if (want > size_t(sgh_num_cus()) * 2) want = size_t(sgh_num_cus()) * 2;
+    size_t want = (table >> 16) / f.launches;
+    const size_t most = 2 * cus - (p.rank ? size_t(so.stretches) : 0);   // (two workgroups fit a CU)
+    if (want > most) want = most;
     if (want < 1) want = 1;
     size_t rows = (a.vocab + want - 1) / want;
     if (rows > kFillRows) rows = kFillRows;
     f.rows = unsigned(rows);
     fill_blocks = unsigned((a.vocab + rows - 1) / rows);
+    if (marked) f.taken = reinterpret_cast<unsigned char *>(ws + p.taken);
   }
-  Sort so = {};
-  so.ids = a.ids, so.counts = at(p.counts), so.tokens = a.tokens, so.vocab = unsigned(a.vocab), so.pad = a.pad;
-  so.bins = 1 << p.digit_bits, so.stretches = p.stretches, so.per_stretch = p.per_stretch;
-  if (p.one) {
+  if (p.rank) {
     so.out = sorted;
-    hipLaunchKernelGGL((k_embed_sort<S, EPL, STREAM>), dim3(1 + fill_blocks), dim3(kSortThreads), 0, s, a, so, p.passes, p.digit_bits, f);
+    hipLaunchKernelGGL((k_embed_rank<S, EPL, STREAM>), dim3(so.stretches + fill_blocks), dim3(kSortThreads), 0, s, a, so, per_wave, f);
     SGH_LAUNCH_CHECK();
   } else {
     for (int pass = 0; pass < p.passes; ++pass) {
       so.out = (p.passes - 1 - pass) & 1 ? other : sorted;
       so.shift = pass * p.digit_bits;
-      hipLaunchKernelGGL((k_embed_count<S, EPL, STREAM>), dim3(p.stretches + fill_blocks), dim3(kSortThreads), 0, s, a, so, f);
+      // the first count clears the marks, the first move sets them, or stores the rows if it is the last
+      const unsigned beside_count = pass != 0 || marked ? fill_blocks : 0, beside_move = pass != 0 || !marked ? fill_blocks : 0;
+      hipLaunchKernelGGL((k_embed_count<S, EPL, STREAM>), dim3(p.stretches + beside_count), dim3(kSortThreads), 0, s, a, so, f);
       SGH_LAUNCH_CHECK();
-      ++f.launch;
-      hipLaunchKernelGGL((k_embed_move<S, EPL, STREAM>), dim3(p.stretches + fill_blocks), dim3(kSortThreads), 0, s, a, so, f);
+      if (pass != 0) ++f.launch;
+      hipLaunchKernelGGL((k_embed_move<S, EPL, STREAM>), dim3(p.stretches + beside_move), dim3(kSortThreads), 0, s, a, so, f);
       SGH_LAUNCH_CHECK();
-      ++f.launch;
+      if (pass != 0) ++f.launch;
+      if (marked) f.from = Taken::kMarks;
       so.ids = nullptr, so.in = so.out;
     }
   }
   Bwd<typename S::elem> t = a;
   if (t.lanes < 8) t.lanes = 8;   // (LDS holds the tokens of a workgroup)
-  // Jobs a wavefront takes one after the other: 4 or fewer while that leaves CUs without work, more where the workgroups' own start counts
-  // (bf16, 65536 tokens of 2048: 351 us with 4, 337 with 8; f32, 8192 of 1024: 44.8 and 48.3)
+  // Jobs a wavefront takes one after the other, more where the workgroups' own start counts (bf16, 65536 tokens of 2048: 351 us with 4, 337 with 8;
+  // f32, 8192 of 1024: 44.8 and 48.3), one while that leaves CUs without work (bf16, 1025 tokens of 64: 16.3 -> 14.3)
   const unsigned takers = kWaves * (SGH_WAVE / t.lanes);
-  t.stretch = takers * (size_t(a.tokens) / (takers * 4) * a.slices > size_t(sgh_num_cus()) * 32 ? 8 : 4);
+  const size_t at_once = size_t(a.tokens) / takers * a.slices;   // workgroups of one job for each taker
+  t.stretch = takers * (at_once > cus * 128 ? 8 : at_once > cus * 2 ? 4 : 1);
   if (t.stretch < t.tile) t.stretch = t.tile;
   const unsigned lds = (2 * (t.stretch + 2 * t.tile) + 3 * t.stretch + 1) * 4, blocks = (t.tokens + t.stretch - 1) / t.stretch;
   // (dy past the caches: 65536 tokens of 2048 16-bit elements 321 -> 308 us; 33 MB of it, 39.6 -> 41.3)

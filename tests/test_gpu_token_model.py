@@ -115,7 +115,8 @@ def test_embedding_ids_outside_the_table_are_zeros_and_counted(dev):
 
 # few tokens (looked through), then sorted ones: one pass of digits, two, three; more than one stretch; whole tiles of one row
 BWD = [(0, 5, 3), (1, 1, 1), (3, 5, 3), (7, 5, 4), (9, 300, 7), (5, 3, 8), (64, 100, 16), (500, 1000, 201), (1024, 37, 100), (1000, 700, 513),
-       (1025, 3, 5), (1500, 300, 33), (3000, 10000, 64), (5000, 600, 129), (4097, 300000, 3), (9000, 77, 520), (20000, 1, 9), (12289, 5000, 40)]
+       (1025, 3, 5), (1500, 300, 33), (3000, 10000, 64), (5000, 600, 129), (4097, 300000, 3), (9000, 77, 520), (20000, 1, 9), (12289, 5000, 40),
+       (8192, 900, 20), (8193, 511, 33), (17001, 512, 64), (70000, 3000, 24), (18000, 262144, 2)]
 
 
 def bwd_bound(t, want, terms, counts, scale):
@@ -188,6 +189,25 @@ def test_embedding_gradient_of_one_row_with_all_tokens(dev):
         W = upload(singa, dev, "f32", np.zeros((4, 12)))
         dW = singa.EmbeddingBackwardW(upload(singa, dev, "f32", dy), ints(singa, dev, ids), W)
         assert np.array_equal(dW.to_numpy(), O.embedding_bwd(dy, ids, (4, 12)))
+
+
+@pytest.mark.parametrize("tokens", [1025, 5001, 8192, 9000])
+def test_embedding_gradient_beside_a_large_table(dev, tokens):
+    """Rows without a token of more than 64 MB beside the sort; sums of whole numbers are exact."""
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(8)
+    vocab, dim = 66001, 256
+    ids = np.where(r.random(tokens) < 0.3, r.integers(0, 5, tokens), r.integers(-2, vocab + 2, tokens))
+    dy = r.integers(-8, 9, (tokens, dim)).astype(np.float32)
+    want = np.zeros((vocab, dim), np.float32)
+    known = (ids >= 0) & (ids < vocab)
+    np.add.at(want, ids[known], dy[known])
+    singa.IndexErrors(dev)
+    out = singa.Tensor((vocab, dim), dev)
+    out.SetFloatValue(9.0)
+    assert singa.EmbeddingBackwardW(upload(singa, dev, "f32", dy), ints(singa, dev, ids), out, out=out) is out
+    assert np.array_equal(out.to_numpy(), want)
+    assert singa.IndexErrors(dev) == int((~known & (ids != -1)).sum())
 
 
 def test_embedding_gradient_of_rows_that_end_with_a_tile(dev):

@@ -177,7 +177,7 @@ def test_mirror_refusals():
 # ------------------------------------------------------------------------------------ launches
 
 def test_what_the_embedding_launches():
-    """Few tokens in one launch without a workspace, up to 8192 sorted by one workgroup, more by two launches for each 9 bits of the ids;
+    """Few tokens in one launch without a workspace, up to 8192 sorted by one more, others by two launches for each 9 bits of the ids;
     grids of the largest sizes stay within a launch."""
     few, one, two, three, largest = recorded("""
 S = SPACE
@@ -188,14 +188,14 @@ def run(t, v, d, add=None, fn=lib.sgh_embedding_bwd_bf16):
 most = (1 << 31) - 1
 largest = [lib.sgh_embedding_fwd_f32(S, 1 << 50, 1 << 55, most, most, 4, 1.0, -1, None), lib.sgh_embedding_fwd_f32(S, 1 << 50, 1 << 55, 5, 7, 1 << 21, 1.0, -1, None)]
 S2 = 1 << 50
-for t, v, d in ((5, most, 4), (most, 9, 4), (9000, 7, 1 << 21), (most, most, 1)):
+for t, v, d in ((5, most, 4), (most, 9, 4), (9000, 7, 1 << 21), (17000, 7, 1 << 21), (most, most, 1)):
     need = lib.sgh_embedding_bwd_workspace_bytes(t, v, d)
     largest.append(lib.sgh_embedding_bwd_f32(S2, 2 * S2, None, 3 * S2, t, v, d, 1.0, -1, 4 * S2, need, None))
 launched()
-answer([run(1024, 5000, 64), run(1025, 5000, 64), run(8193, 131071, 64), run(8193, 1 << 18, 64), largest])
+answer([run(1024, 5000, 64), run(8192, 5000, 64), run(8193, 131071, 64), run(8193, 1 << 18, 64), largest])
 """)
     assert few[:2] == [0, 0] and [k[:11] for k in few[2]] == ["k_embed_row"], few
-    assert one[0] == 0 and one[1] > 0 and [k[:11] for k in one[2]] == ["k_embed_sor", "k_embed_til", "k_embed_joi"], one
+    assert one[0] == 0 and one[1] > 0 and [k[:11] for k in one[2]] == ["k_embed_ran", "k_embed_til", "k_embed_joi"], one
     pair = ["k_embed_cou", "k_embed_mov"]
     assert [k[:11] for k in two[2]] == 2 * pair + ["k_embed_til", "k_embed_joi"], two
     assert [k[:11] for k in three[2]] == 3 * pair + ["k_embed_til", "k_embed_joi"], three
