@@ -803,35 +803,41 @@ SGH_API int sgh_embedding_index_errors(void *stream, int *count);
  *   _fwd      loss and stats [batch, 3] = the row's maximum m, sum exp((x - m) / temperature), sum exp(x - m): what the gradient
  *             needs of the forward pass; 0 where no term asks for it
  *   _bwd      dx from the stats of the same arguments; dx may be x itself
- *   _fwd_bwd  both in one call, the logits' row still at hand for the gradient; dx may be x itself */
+ *   _fwd_bwd  both in one call, the logits' row still at hand for the gradient; dx may be x itself
+ * workspace of _fwd and _fwd_bwd: sgh_distill_workspace_bytes, at a multiple of 16 bytes (0 but for few long rows, NULL is then taken);
+ * elem_bytes is 4 or 2, gradient is 1 for _fwd_bwd.  Calls on different streams need one each. */
 #define SGH_DISTILL_MAX_TOP 1024
+SGH_API size_t sgh_distill_workspace_bytes(size_t batch, size_t dim, size_t elem_bytes, int gradient);
 SGH_API int sgh_distill_fwd_f32(const float *x, const int32_t *top, const float *teacher, const int32_t *labels,
                                const float *weights, size_t batch, size_t dim, size_t k, float temperature, float soft,
-                               float hard, float *loss, float *stats, void *stream);
+                               float hard, float *loss, float *stats, void *workspace, size_t ws_bytes, void *stream);
 SGH_API int sgh_distill_bwd_f32(const float *x, const float *stats, const int32_t *top, const float *teacher,
                                const int32_t *labels, const float *weights, size_t batch, size_t dim, size_t k,
                                float temperature, float soft, float hard, float scale, float *dx, void *stream);
 SGH_API int sgh_distill_fwd_bwd_f32(const float *x, const int32_t *top, const float *teacher, const int32_t *labels,
                                    const float *weights, size_t batch, size_t dim, size_t k, float temperature,
-                                   float soft, float hard, float scale, float *loss, float *dx, void *stream);
+                                   float soft, float hard, float scale, float *loss, float *dx, void *workspace,
+                                   size_t ws_bytes, void *stream);
 SGH_API int sgh_distill_fwd_f16(const uint16_t *x, const int32_t *top, const float *teacher, const int32_t *labels,
                                const float *weights, size_t batch, size_t dim, size_t k, float temperature, float soft,
-                               float hard, float *loss, float *stats, void *stream);
+                               float hard, float *loss, float *stats, void *workspace, size_t ws_bytes, void *stream);
 SGH_API int sgh_distill_bwd_f16(const uint16_t *x, const float *stats, const int32_t *top, const float *teacher,
                                const int32_t *labels, const float *weights, size_t batch, size_t dim, size_t k,
                                float temperature, float soft, float hard, float scale, uint16_t *dx, void *stream);
 SGH_API int sgh_distill_fwd_bwd_f16(const uint16_t *x, const int32_t *top, const float *teacher, const int32_t *labels,
                                    const float *weights, size_t batch, size_t dim, size_t k, float temperature,
-                                   float soft, float hard, float scale, float *loss, uint16_t *dx, void *stream);
+                                   float soft, float hard, float scale, float *loss, uint16_t *dx, void *workspace,
+                                   size_t ws_bytes, void *stream);
 SGH_API int sgh_distill_fwd_bf16(const uint16_t *x, const int32_t *top, const float *teacher, const int32_t *labels,
                                const float *weights, size_t batch, size_t dim, size_t k, float temperature, float soft,
-                               float hard, float *loss, float *stats, void *stream);
+                               float hard, float *loss, float *stats, void *workspace, size_t ws_bytes, void *stream);
 SGH_API int sgh_distill_bwd_bf16(const uint16_t *x, const float *stats, const int32_t *top, const float *teacher,
                                const int32_t *labels, const float *weights, size_t batch, size_t dim, size_t k,
                                float temperature, float soft, float hard, float scale, uint16_t *dx, void *stream);
 SGH_API int sgh_distill_fwd_bwd_bf16(const uint16_t *x, const int32_t *top, const float *teacher, const int32_t *labels,
                                    const float *weights, size_t batch, size_t dim, size_t k, float temperature,
-                                   float soft, float hard, float scale, float *loss, uint16_t *dx, void *stream);
+                                   float soft, float hard, float scale, float *loss, uint16_t *dx, void *workspace,
+                                   size_t ws_bytes, void *stream);
 /* Number of list entries and labels outside the columns that the forward pass has met since the last call (synchronises the stream). */
 SGH_API int sgh_distill_index_errors(void *stream, int *count);
 

@@ -157,25 +157,26 @@ SIGNATURES = {
     "sgh_softmax_ce_fwd_f32": (C.c_int, [vp, vp, vp, vp, sz, sz, C.c_int, vp]),
     "sgh_embedding_bwd_workspace_bytes": (sz, [sz, sz, sz]),
     "sgh_embedding_index_errors": (C.c_int, [vp, C.POINTER(C.c_int)]),
+    "sgh_distill_workspace_bytes": (sz, [sz, sz, sz, C.c_int]),
     "sgh_distill_index_errors": (C.c_int, [vp, C.POINTER(C.c_int)]),
     "sgh_embedding_fwd_f32": (C.c_int, [vp, vp, vp, sz, sz, sz, C.c_float, C.c_int, vp]),
     "sgh_embedding_bwd_f32": (C.c_int, [vp, vp, vp, vp, sz, sz, sz, C.c_float, C.c_int, vp, sz, vp]),
-    "sgh_distill_fwd_f32": (C.c_int, [vp, vp, vp, vp, vp, sz, sz, sz, C.c_float, C.c_float, C.c_float, vp, vp, vp]),
+    "sgh_distill_fwd_f32": (C.c_int, [vp, vp, vp, vp, vp, sz, sz, sz, C.c_float, C.c_float, C.c_float, vp, vp, vp, sz, vp]),
     "sgh_distill_bwd_f32": (C.c_int, [vp, vp, vp, vp, vp, vp, sz, sz, sz, C.c_float, C.c_float, C.c_float, C.c_float, vp, vp]),
     "sgh_distill_fwd_bwd_f32": (C.c_int, [vp, vp, vp, vp, vp, sz, sz, sz, C.c_float, C.c_float, C.c_float, C.c_float, vp, vp,
-                                         vp]),
+                                         vp, sz, vp]),
     "sgh_embedding_fwd_f16": (C.c_int, [vp, vp, vp, sz, sz, sz, C.c_float, C.c_int, vp]),
     "sgh_embedding_bwd_f16": (C.c_int, [vp, vp, vp, vp, sz, sz, sz, C.c_float, C.c_int, vp, sz, vp]),
-    "sgh_distill_fwd_f16": (C.c_int, [vp, vp, vp, vp, vp, sz, sz, sz, C.c_float, C.c_float, C.c_float, vp, vp, vp]),
+    "sgh_distill_fwd_f16": (C.c_int, [vp, vp, vp, vp, vp, sz, sz, sz, C.c_float, C.c_float, C.c_float, vp, vp, vp, sz, vp]),
     "sgh_distill_bwd_f16": (C.c_int, [vp, vp, vp, vp, vp, vp, sz, sz, sz, C.c_float, C.c_float, C.c_float, C.c_float, vp, vp]),
     "sgh_distill_fwd_bwd_f16": (C.c_int, [vp, vp, vp, vp, vp, sz, sz, sz, C.c_float, C.c_float, C.c_float, C.c_float, vp, vp,
-                                         vp]),
+                                         vp, sz, vp]),
     "sgh_embedding_fwd_bf16": (C.c_int, [vp, vp, vp, sz, sz, sz, C.c_float, C.c_int, vp]),
     "sgh_embedding_bwd_bf16": (C.c_int, [vp, vp, vp, vp, sz, sz, sz, C.c_float, C.c_int, vp, sz, vp]),
-    "sgh_distill_fwd_bf16": (C.c_int, [vp, vp, vp, vp, vp, sz, sz, sz, C.c_float, C.c_float, C.c_float, vp, vp, vp]),
+    "sgh_distill_fwd_bf16": (C.c_int, [vp, vp, vp, vp, vp, sz, sz, sz, C.c_float, C.c_float, C.c_float, vp, vp, vp, sz, vp]),
     "sgh_distill_bwd_bf16": (C.c_int, [vp, vp, vp, vp, vp, vp, sz, sz, sz, C.c_float, C.c_float, C.c_float, C.c_float, vp, vp]),
     "sgh_distill_fwd_bwd_bf16": (C.c_int, [vp, vp, vp, vp, vp, sz, sz, sz, C.c_float, C.c_float, C.c_float, C.c_float, vp, vp,
-                                         vp]),
+                                         vp, sz, vp]),
     "sgh_sum_rows_f32": (C.c_int, [vp, vp, C.c_int, C.c_int, vp]),
     "sgh_add_row_f32": (C.c_int, [vp, vp, C.c_int, C.c_int, vp]),
     "sgh_conv_geom_init": (C.c_int, [C.POINTER(ConvGeom)] + [C.c_int] * 11),

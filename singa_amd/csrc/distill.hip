@@ -37,7 +37,10 @@ struct Rows {
   float tau, soft, hard, scale;
   float inv_tau;
   bool in_place;             // dx is x
+  float4 *parts;             // few long rows: of each a record, then its parts' maxima and sums
+  int per_row;               // parts of a row, or 0
 };
+constexpr int kMostParts = SGH_WAVE;   // (a lane each where they are joined)
 
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
 
@@ -72,12 +75,15 @@ __device__ __forceinline__ float wave_max(float v) {
   return fmaxf(fmaxf(lane_value(v, 0), lane_value(v, 16)), fmaxf(lane_value(v, 32), lane_value(v, 48)));
 }
 
-// NT threads share a row: a wavefront (a workgroup then has several rows), or the workgroup
+// NT threads share a row: a wavefront (a workgroup then has several rows), or the workgroup; kAny: whatever the workgroup's size
+constexpr int kAny = 0, kMostThreads = 1024;
+constexpr int kHeld = 16;   // vectors of a row that a thread holds
 template <int NT>
 struct Team {
   static constexpr int kPerBlock = NT == SGH_WAVE ? kBlock / SGH_WAVE : 1;
-  static constexpr int kThreads = NT == SGH_WAVE ? kBlock : NT;
-  static constexpr int kWaves = NT / SGH_WAVE;
+  static constexpr int kThreads = NT == SGH_WAVE ? kBlock : NT == kAny ? kMostThreads : NT;   // at the most
+  static constexpr int kWaves = (NT == kAny ? kMostThreads : NT) / SGH_WAVE;
+  static __device__ __forceinline__ unsigned size() { return NT == kAny ? blockDim.x : unsigned(NT); }
   static constexpr int kLists = NT == SGH_WAVE ? 1 : 2;   // a row's list may still be read where the next one's is fetched
   static __device__ __forceinline__ int id() { return NT == SGH_WAVE ? threadIdx.x >> 6 : 0; }
   static __device__ __forceinline__ int tid() { return NT == SGH_WAVE ? threadIdx.x & 63 : threadIdx.x; }
@@ -315,7 +321,7 @@ __device__ __forceinline__ void list_columns(const Rows<typename S::elem> &a, si
     if (!__ballot(labelled) && Team<NT>::tid() == 0 && mine(e.label)) S::st(dx + e.label, s(e.label_x) - s.share_1);
     return;
   }
-  for (int k = Team<NT>::tid(); k <= a.k; k += NT) {
+  for (int k = Team<NT>::tid(); k <= a.k; k += Team<NT>::size()) {
     const int at = l.at[k];
     float p = 0.f;
     bool first = true;
@@ -442,22 +448,27 @@ __device__ __forceinline__ void slope_row(const typename S::elem *x, typename S:
                          [&](const sgh_v4u &raw, unsigned i, bool) { to.store<STREAM>(slope_vector<S>(s, raw), i < pad ? kOutside : i); });
 }
 
+// The statistics of a whole row
+template <class T>
+__device__ __forceinline__ Running of_row(const Rows<T> &a, Running r) {
+  if (r.m == -__builtin_inff()) r.st = r.s1 = __builtin_nanf("");   // (no column with a probability)
+  if (a.tau == 1.f) r.st = r.s1;
+  return r;
+}
 // The team's statistics from its threads'; `red`: one of each wavefront
-template <int NT, class T>
-__device__ __forceinline__ Running team_sums(const Rows<T> &a, const Lane &lane, float ct, Running *red) {
+template <int NT>
+__device__ __forceinline__ Running team_sums(const Lane &lane, float ct, Running *red) {
   Running r = wave_sums(lane, ct);
   constexpr int W = Team<NT>::kWaves;
   static_assert(W <= 16, "a lane of sixteen takes a wavefront's");
   if constexpr (W > 1) {
-    if ((threadIdx.x & (SGH_WAVE - 1)) == 0 && threadIdx.x < NT) red[threadIdx.x >> 6] = r;
+    if ((threadIdx.x & (SGH_WAVE - 1)) == 0) red[threadIdx.x >> 6] = r;
     __syncthreads();
-    const int of = threadIdx.x & 15;
-    r = of < W ? red[of] : Running{-__builtin_inff(), 0.f, 0.f};
+    const unsigned of = threadIdx.x & 15;
+    r = of < Team<NT>::size() / SGH_WAVE ? red[of] : Running{-__builtin_inff(), 0.f, 0.f};
     const float m = max16(r.m);
     r = {m, sum16(rebased(r.st, r.m, m, ct)), sum16(rebased(r.s1, r.m, m, kLog2e))};
   }
-  if (r.m == -__builtin_inff()) r.st = r.s1 = __builtin_nanf("");   // (no column with a probability)
-  if (a.tau == 1.f) r.st = r.s1;
   return r;
 }
 
@@ -531,9 +542,10 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_fwd(Rows<typenam
     if (q.any()) {
       Lane sum;
       sum.start(ct, want);
-      stream_row<NT, STREAM && !GRAD>(from, vecs, v, [&](const sgh_v4u &raw, unsigned vec, bool all) { take_vector<S>(sum, raw, vec, vecs, all, ct, want); });
+      stream_row<NT, STREAM && !GRAD>(
+          from, vecs, v, [&](const sgh_v4u &raw, unsigned vec, bool all) { take_vector<S>(sum, raw, vec, vecs, all, ct, want); });
       if (lie.odd != kNone) sum.take<1>(&tail, ct, want);
-      r = team_sums<NT>(a, sum, ct, red);
+      r = of_row(a, team_sums<NT>(sum, ct, red));
       soft = q.may_soft && (NT == SGH_WAVE ? any : listed != 0);
     }
     if (lister) {
@@ -555,11 +567,113 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_fwd(Rows<typenam
   }
 }
 
-// Both for rows of at most U * NT vectors, in registers.  A workgroup goes from row to row, and each of the next row's vectors is asked for when
-// the register it goes to is free, behind the store of this row's gradient there, so that the memory is at work while sums are joined and
-// the list is seen to.  What is small (weight, label, the first 64 of the list) is asked for in front of a row's vectors, a row or two ahead:
-// loads come back in order.
-template <int NT, int U, int PER_SIMD, class S, bool STREAM>
+// Few long rows are cut in `per_row` parts, a workgroup each, whose statistics go to memory, and the next launch joins them.  What the list and
+// the label give to the loss is known but for those statistics: with `top` the largest of the student's logits there,
+//   sum_k p_k (log p_k - log q_k) = kl - (top - m) / tau + log S_tau,   kl = sum_k p_k (log p_k - (x_k - top) / tau)
+// so that the record of a row is {whether there is an entry, kl, top, x_label}.
+template <class T>
+__device__ __forceinline__ float4 row_record(const Rows<T> &a, const Teacher &t, const List &l, const Entry &e) {
+  const int lane = threadIdx.x & (SGH_WAVE - 1);
+  const float log_sum = logf(t.sum), inv = 1.f / t.sum;
+  auto share = [&](float v) { return exp2_((v - t.most) * (kLog2e * a.inv_tau)) * inv; };
+  auto each = [&](auto f) {   // f(the teacher's logit, the student's) for every entry with a share
+    if (short_list(a.k)) {
+      if (e.at >= 0 && share(e.v) != 0.f) f(e.v, e.x);
+    } else {
+      for (int k = lane; k < a.k; k += SGH_WAVE)
+        if (l.at[k] >= 0 && share(l.p[k]) != 0.f) f(l.p[k], l.x[k]);
+    }
+  };
+  float top = -__builtin_inff(), kl = 0.f;
+  each([&](float, float x) { top = fmaxf(top, x); });
+  top = wave_max(top);
+  each([&](float v, float x) { kl += share(v) * ((v - t.most) * a.inv_tau - log_sum - (x - top) * a.inv_tau); });
+  kl = wave_sum(kl);
+  if (top == -__builtin_inff()) kl = __builtin_inff(), top = 0.f;   // (the student gives none of them a probability)
+  return {t.any ? 1.f : 0.f, kl, top, e.label_x};
+}
+template <class S>
+__global__ __launch_bounds__(kBlock) void k_distill_part(Rows<typename S::elem> a, unsigned each) {
+  typedef typename S::elem T;
+  constexpr int NT = kBlock;
+  extern __shared__ char lds[];
+  __shared__ Running red[NT / SGH_WAVE];
+  const unsigned part = blockIdx.y;
+  const bool lister = part == 0 && threadIdx.x < SGH_WAVE, begins = part == 0, ends = part + 1 == gridDim.y;
+  const float ct = kLog2e * a.inv_tau;
+  const size_t row = blockIdx.x;
+  const T *x = a.x + row * a.dim;
+  const Lie lie = lie_of<S>(x, unsigned(a.dim), threadIdx.x);
+  const unsigned first = part * each < lie.vecs ? part * each : lie.vecs, vecs = lie.vecs - first < each ? lie.vecs - first : each;
+  const bool odd = lie.odd != kNone && (lie.odd < lie.head ? begins : ends);
+  Entry entry;
+  if (lister) ask_list(a, row, entry);
+  const float tail = odd ? S::ld(x + lie.odd) : 0.f;
+  const RowBuffer from(x + lie.head + size_t(first) * S::VEC, vecs * 16);
+  sgh_v4u v[kAhead];
+  const Row q = row_at(a, row, begins && threadIdx.x == 0);
+  ask_vectors<NT, false>(from, 0, v);
+  const List list = list_at(lds, a.k);
+  bool any = false;
+  if (lister) any = gather_list<S>(a, row, q.hard ? q.label : -1, true, list, entry);
+  float4 *out = a.parts + row * (a.per_row + 1);
+  if (q.any()) {
+    const Sums want = {q.may_soft && a.tau != 1.f, q.hard || (q.may_soft && a.tau == 1.f)};
+    Lane sum;
+    sum.start(ct, want);
+    stream_row<NT, false>(
+        from, vecs, v, [&](const sgh_v4u &raw, unsigned vec, bool all) { take_vector<S>(sum, raw, vec, vecs, all, ct, want); });
+    if (odd) sum.take<1>(&tail, ct, want);
+    const Running r = team_sums<NT>(sum, ct, red);
+    if (threadIdx.x == 0) out[1 + part] = {r.m, r.st, r.s1, 0.f};
+  }
+  if (lister) {
+    const Teacher teach = finish_list(a, any, list, entry);
+    float4 rec = {0.f, 0.f, 0.f, entry.label_x};
+    if (any) rec = row_record(a, teach, list, entry);
+    if (threadIdx.x == 0) out[0] = rec;
+  }
+}
+// A row's statistics from its parts', by every wavefront that asks
+template <class T>
+__device__ __forceinline__ Running joined(const Rows<T> &a, size_t row, float4 *record) {
+  const int lane = threadIdx.x & (SGH_WAVE - 1);
+  const float4 *p = a.parts + row * (a.per_row + 1);
+  *record = p[0];
+  const float4 of = lane < a.per_row ? p[1 + lane] : float4{-__builtin_inff(), 0.f, 0.f, 0.f};
+  const float m = wave_max(of.x);
+  return of_row(a, {m, wave_sum(rebased(of.y, of.x, m, kLog2e * a.inv_tau)), wave_sum(rebased(of.z, of.x, m, kLog2e))});
+}
+template <class T>
+__device__ __forceinline__ void store_joined(const Rows<T> &a, size_t row, float w, const Running &r, bool soft, bool hard, const float4 &record) {
+  float loss = 0.f;
+  if (soft) loss = a.soft * a.tau * a.tau * (record.y - (record.z - r.m) * a.inv_tau + logf(r.st));
+  if (hard) loss += a.hard * (logf(r.s1) - (record.w - r.m));
+  a.loss[row] = soft || hard ? w * loss : 0.f;
+  if (a.stats) {
+    a.stats[row * 3] = soft || hard ? r.m : 0.f;
+    a.stats[row * 3 + 1] = soft ? r.st : 0.f;
+    a.stats[row * 3 + 2] = hard ? r.s1 : 0.f;
+  }
+}
+// The loss of rows in parts, a wavefront each
+template <class T>
+__global__ __launch_bounds__(SGH_WAVE) void k_distill_join(Rows<T> a) {
+  const size_t row = blockIdx.x;
+  const Row q = row_at(a, row, false);
+  float4 record;
+  const Running r = joined(a, row, &record);
+  if (threadIdx.x == 0) store_joined(a, row, q.w, r, q.may_soft && record.x != 0.f, q.hard, record);
+}
+
+// Both for rows of at most U * NT vectors, in registers: what bounds it is the logits' way in and the gradient's out.
+// ONE: a workgroup for each row (a wavefront, of short ones), so that one's loads are in flight beside another's sums and stores.
+// Else a workgroup goes from row to row, and each of the next row's vectors is asked for when the register it goes to is free, behind the store
+// of this row's gradient there: for rows that leave a CU no second workgroup.  (Loads behind a row's stores wait for these: where there are
+// several workgroups, one for each row is faster, 530 -> 450 us for 16384 rows of 20001 fp32 values, 207 -> 186 for 4096 of 50304 bfloat16.)
+// What is small (weight, label, the first 64 of the list) is asked for in front of a row's vectors, a row or two ahead: loads come back in
+// order.  8192 rows of 131072 bfloat16 values with lists of 64, in turn: 4.5 TB/s; 2048 rows of 65001, labels alone: 107 us.
+template <int NT, int U, int PER_SIMD, bool ONE, class S, bool STREAM>
 __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(Rows<typename S::elem> a) {
   typedef Team<NT> G;
   typedef typename S::elem T;
@@ -567,6 +681,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
   __shared__ Running red[G::kWaves];
   __shared__ int listed;
   const int tid = G::tid();
+  const unsigned nt = G::size();
   const bool lister = tid < SGH_WAVE;   // the wavefront that sees to the list
   const float ct = kLog2e * a.inv_tau;
   const size_t step = size_t(gridDim.x) * G::kPerBlock;
@@ -600,19 +715,20 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
   Entry entry;
   if (lister) ask_list(a, row, entry);
   Row q = row_of(raw_at(row), tid == 0);
-  Raw next_raw = raw_at(row + step);
+  Raw next_raw = {0.f, -1};
+  if constexpr (!ONE) next_raw = raw_at(row + step);
   Lie lie = lie_of<S>(a.x + row * a.dim, unsigned(a.dim), tid);
   {
     const T *first = a.x + row * a.dim;
     const RowBuffer x = RowBuffer::padded(first + lie.head, q.any() ? lie.vecs : 0, lie.pad);
 #pragma unroll
-    for (int u = 0; u < U; ++u) held[u] = x.load<STREAM>(u == 0 ? place(lie) : u * NT + tid);
+    for (int u = 0; u < U; ++u) held[u] = x.load<STREAM>(u == 0 ? place(lie) : u * nt + tid);
     if (lie.odd != kNone && q.any()) tail = S::ld(first + lie.odd);
   }
   int turn = 0;
   for (;;) {
     const size_t next = row + step;
-    const bool goes_on = next < a.batch;
+    const bool goes_on = !ONE && next < a.batch;
     const Row nq = row_of(next_raw, tid == 0);   // (of nothing behind the last)
     const T *nx = a.x + next * a.dim;
     Entry next_entry;
@@ -635,10 +751,12 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
       sum.start(ct, want);
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (unsigned(u * NT) < places)
-          take_vector<S>(sum, held[u], u == 0 ? place(lie) : u * NT + tid, places, (u != 0 || lie.pad == 0) && unsigned(u * NT + NT) <= places, ct, want);
+        if (u * nt < places) {
+          const bool all = (u != 0 || lie.pad == 0) && (u + 1) * nt <= places;
+          take_vector<S>(sum, held[u], u == 0 ? place(lie) : u * nt + tid, places, all, ct, want);
+        }
       if (lie.odd != kNone) sum.take<1>(&tail, ct, want);
-      r = team_sums<NT>(a, sum, ct, red);
+      r = of_row(a, team_sums<NT>(sum, ct, red));
       soft = q.may_soft && (NT == SGH_WAVE ? any : listed != 0);
     }
     if (lister) {
@@ -646,15 +764,16 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
       store_loss(a, row, q.w, r, soft, q.hard, teach, list, entry);
       if (goes_on) ask_list(a, next, next_entry);
     }
-    next_raw = raw_at(next + step);
+    if constexpr (!ONE) next_raw = raw_at(next + step);
     const Slope s = slope_of(a, q.w, r, soft, q.hard);
     if (a.in_place && NT != SGH_WAVE) G::sync();   // (the list's logits are read)
     unsigned i = tid;
     asm("" : "+v"(i));   // (the places of a row are not kept in registers of their own from row to row: 20 of these went to scratch memory)
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      to.store<STREAM>(slope_vector<S>(s, held[u]), u == 0 ? place(lie) : u * NT + i);
-      held[u] = then.load<STREAM>(u == 0 ? place(next_lie) : u * NT + i);
+      if (u * nt < places) held[u] = slope_vector<S>(s, held[u]);   // (nothing but arithmetic in the branch)
+      to.store<STREAM>(held[u], u == 0 ? place(lie) : u * nt + i);
+      if constexpr (!ONE) held[u] = then.load<STREAM>(u == 0 ? place(next_lie) : u * nt + i);
     }
     if (lie.odd != kNone) S::st(dx + lie.odd, s(tail));
     if (next_lie.odd != kNone && goes_on && nq.any()) tail = S::ld(nx + next_lie.odd);
@@ -666,7 +785,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
   }
 }
 
-// The gradient from the statistics; a row may be several workgroups', `each` vectors of it
+// The gradient from the statistics, or from a row's parts, whose loss it stores then; a row may be several workgroups', `each` vectors of it
 template <int NT, class S, bool STREAM>
 __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_bwd(Rows<typename S::elem> a, unsigned each) {
   typedef Team<NT> G;
@@ -688,10 +807,19 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_bwd(Rows<typenam
     Entry entry;
     if (lister) ask_list(a, row, entry);
     const float tail = odd ? S::ld(x + lie.odd) : 0.f;
-    const Running r = {a.stats[row * 3], a.stats[row * 3 + 1], a.stats[row * 3 + 2]};
-    Row q = row_at(a, row, false);
-    // (a sum of 0: the forward pass found no term)
-    const bool soft = q.may_soft && r.st != 0.f, hard = q.hard && r.s1 != 0.f, none = !(soft || hard);
+    const Row q = row_at(a, row, false);
+    Running r;
+    bool soft = q.may_soft, hard = q.hard;
+    if (a.per_row) {
+      float4 record;
+      r = joined(a, row, &record);
+      soft = soft && record.x != 0.f;
+      if (begins && tid == 0) store_joined(a, row, q.w, r, soft, hard, record);
+    } else {   // (a sum of 0: the forward pass found no term)
+      r = {a.stats[row * 3], a.stats[row * 3 + 1], a.stats[row * 3 + 2]};
+      soft = soft && r.st != 0.f, hard = hard && r.s1 != 0.f;
+    }
+    const bool none = !(soft || hard);
     const Slope s = slope_of(a, q.w, r, soft, hard);
     const List list = list_at(lds + (G::id() * G::kLists + turn) * list_bytes(a.k), a.k);
     bool any = false;
@@ -733,12 +861,29 @@ int launch_fwd(const Rows<typename S::elem> &a, hipStream_t s) {
   SGH_LAUNCH_CHECK();
   return SGH_OK;
 }
-template <int NT, int U, int PER_SIMD, class S>
-int launch_held(const Rows<typename S::elem> &a, hipStream_t s) {
-  const size_t at_once = size_t(sgh_num_cus()) * (PER_SIMD * 4 * SGH_WAVE / Team<NT>::kThreads);   // workgroups
-  const dim3 grid{blocks_for<NT>(a.batch, at_once)}, block{unsigned(Team<NT>::kThreads)};
-  if (streams(a)) SGH_LAUNCH_TIMED((k_distill_held<NT, U, PER_SIMD, S, true>), grid, block, lds_for<NT>(a.k), s, a);
-  else SGH_LAUNCH_TIMED((k_distill_held<NT, U, PER_SIMD, S, false>), grid, block, lds_for<NT>(a.k), s, a);
+template <int NT, int U, int PER_SIMD, bool ONE, class S>
+int launch_held(Rows<typename S::elem> a, unsigned threads, hipStream_t s) {
+  const size_t at_once = size_t(sgh_num_cus()) * (PER_SIMD * 4 * SGH_WAVE / threads);   // workgroups
+  const bool stream = streams(a);
+  const size_t batch = a.batch, most = ONE ? size_t(1) << 20 : batch;   // (a launch has less than 2^32 threads)
+  for (size_t row = 0; row < batch; row += most) {
+    a.batch = batch - row < most ? batch - row : most;
+    const dim3 grid{blocks_for<NT>(a.batch, ONE ? a.batch : at_once)}, block{threads};
+    if (stream) SGH_LAUNCH_TIMED((k_distill_held<NT, U, PER_SIMD, ONE, S, true>), grid, block, lds_for<NT>(a.k), s, a);
+    else SGH_LAUNCH_TIMED((k_distill_held<NT, U, PER_SIMD, ONE, S, false>), grid, block, lds_for<NT>(a.k), s, a);
+    SGH_LAUNCH_CHECK();
+    a.x += a.batch * a.dim, a.dx += a.batch * a.dim, a.loss += a.batch;
+    if (a.k) a.top += a.batch * a.k, a.teacher += a.batch * a.k;
+    if (a.labels) a.labels += a.batch;
+    if (a.weights) a.weights += a.batch;
+  }
+  return SGH_OK;
+}
+template <class S>
+int launch_parts(const Rows<typename S::elem> &a, hipStream_t s) {
+  const unsigned vecs = unsigned(a.dim / S::VEC), each = (vecs + a.per_row - 1) / a.per_row;
+  const dim3 grid{unsigned(a.batch), unsigned(a.per_row)};
+  hipLaunchKernelGGL((k_distill_part<S>), grid, dim3(kBlock), lds_for<kBlock>(a.k), s, a, each);
   SGH_LAUNCH_CHECK();
   return SGH_OK;
 }
@@ -751,6 +896,20 @@ int launch_bwd(const Rows<typename S::elem> &a, unsigned each, hipStream_t s) {
   SGH_LAUNCH_CHECK();
   return SGH_OK;
 }
+
+// Parts that a row is cut in for the loss, 0: none.  Two launches that have the whole chip for few rows, against one that has a CU for each: a
+// row of 262144 bfloat16 values 26 -> 7 us, with its gradient 54 -> 10, 64 rows 27 -> 14 and 56 -> 28; 128 rows of 131072 15.9 -> 13.5 and 32.0 ->
+// 28.8.  Short rows have one launch: 16 of 32000 fp32 values 5.9 us, in parts 6.3, a bfloat16 row of 40000 6.7 and 7.0; with the gradient, a
+// bfloat16 row of 20001 8.2 and 9.6, of 40000 12.5 and 9.9, an fp32 row of 32000 10.5 and 9.1.
+int parts_of(size_t batch, size_t dim, size_t elem, bool grad) {
+  const size_t vecs = dim * elem / 16, cus = size_t(sgh_num_cus());
+  if (batch * 2 > cus || dim <= (grad ? 28000 : 40000)) return 0;
+  size_t n = (4 * cus + batch - 1) / batch;
+  const size_t most = vecs / (kBlock * kAhead);   // a turn of every thread at the least (3 parts and more)
+  if (n > most) n = most;
+  return int(n < size_t(kMostParts) ? n : size_t(kMostParts));
+}
+size_t parts_bytes(size_t batch, int per_row) { return per_row ? batch * size_t(per_row + 1) * sizeof(float4) : 0; }
 
 // The checks that the three entry points share; SGH_OK with `empty` set where there is nothing to do
 template <class T>
@@ -781,11 +940,17 @@ int check(const Rows<T> &a, size_t k, bool fwd, bool grad, bool *empty) {
 }
 
 template <class S>
-int distill(Rows<typename S::elem> a, size_t k, bool fwd, bool grad, void *stream) {
+int distill(Rows<typename S::elem> a, size_t k, bool fwd, bool grad, void *workspace, size_t ws_bytes, void *stream) {
   bool empty;
   const int rc = check(a, k, fwd, grad, &empty);
   if (rc != SGH_OK || empty) return rc;
   a.k = int(k);
+  a.per_row = fwd ? parts_of(a.batch, a.dim, sizeof(typename S::elem), grad) : 0;
+  if (a.per_row) {
+    if (!workspace || ws_bytes < parts_bytes(a.batch, a.per_row)) return SGH_EWORKSPACE;
+    if (reinterpret_cast<uintptr_t>(workspace) % alignof(float4) != 0) return SGH_EINVAL;
+    a.parts = static_cast<float4 *>(workspace);
+  }
   a.in_place = grad && a.dx == a.x;
   a.inv_tau = 1.f / a.tau;
   hipStream_t s = sgh_stream_of(stream);
@@ -793,33 +958,51 @@ int distill(Rows<typename S::elem> a, size_t k, bool fwd, bool grad, void *strea
   if (grad) sgh_note_write(a.dx, a.batch * a.dim * sizeof(typename S::elem));
   sgh_prof_kernel_scope prof(fwd && grad ? "distill/k_distill_fwd" : fwd ? "distill_fwd/k_distill_fwd" : "distill_bwd/k_distill_bwd",
                              bytes * (grad ? 2 : 1), s);
-  const size_t vecs = a.dim / S::VEC;
-  if (fwd && grad) {
+  const size_t vecs = a.dim / S::VEC, cus = size_t(sgh_num_cus());
+  if (a.per_row) {
+    prof.span();
+    const int failed = launch_parts<S>(a, s);
+    if (failed != SGH_OK) return failed;
+    if (!grad) {
+      hipLaunchKernelGGL((k_distill_join<typename S::elem>), dim3(unsigned(a.batch)), dim3(SGH_WAVE), 0, s, a);
+      SGH_LAUNCH_CHECK();
+      return SGH_OK;
+    }
+  } else if (fwd && grad) {
     // places of a row's vectors
     const bool lines = (reinterpret_cast<uintptr_t>(a.x) | a.dim * sizeof(typename S::elem)) % kLine == 0;
     const size_t places = lines ? vecs : vecs + kLine / 16 - 1;
-    if (places <= 64 * 4) return launch_held<64, 4, 6, S>(a, s);
-    if (places <= 64 * 8) return launch_held<64, 8, 5, S>(a, s);
-    if (places <= 64 * 16) return launch_held<64, 16, 4, S>(a, s);
-    if (places <= 128 * 16) return launch_held<128, 16, 4, S>(a, s);
-    if (places <= 256 * 16) return launch_held<256, 16, 4, S>(a, s);
-    if (places <= 512 * 16) return launch_held<512, 16, 4, S>(a, s);
-    if (places <= 1024 * 16) return launch_held<1024, 16, 4, S>(a, s);
+    if (places <= size_t(kMostThreads) * kHeld) {
+      // Vectors of a thread.  4, the shortest way through a row, while the wavefronts find room at once (1 row of 20001 bfloat16 values: 8.1 us, with
+      // 16 10.9; 1024 rows with 4, 8, 16: 31.8, 25.3, 27.7).  Then 8, while two workgroups fit a CU (4096 rows of 32000: 106 us, with 4 145;
+      // 16384 of 5000: 81, 93, with 16 89), or 16.  A wavefront for rows of up to 256 vectors: a workgroup's sum costs a microsecond.
+      auto waves = [&](size_t held) { return unsigned((places + SGH_WAVE * held - 1) / (SGH_WAVE * held)); };
+      if (places <= 64 * 4) return launch_held<64, 4, 6, true, S>(a, kBlock, s);
+      if (waves(4) <= 16 && a.batch * waves(4) <= cus * 24) return launch_held<kAny, 4, 6, true, S>(a, waves(4) * SGH_WAVE, s);
+      if (waves(8) <= 10) return launch_held<kAny, 8, 5, true, S>(a, waves(8) * SGH_WAVE, s);
+      if (waves(kHeld) <= 8 || a.batch <= cus) return launch_held<kAny, kHeld, 4, true, S>(a, waves(kHeld) * SGH_WAVE, s);
+      return launch_held<kAny, kHeld, 4, false, S>(a, waves(kHeld) * SGH_WAVE, s);
+    }
     return launch_fwd<512, S, true>(a, s);
   }
-  const size_t cus = size_t(sgh_num_cus());
-  if (fwd) {
-    if (vecs <= 512) return launch_fwd<64, S, false>(a, s);
-    if (a.batch <= 2 * cus) return vecs <= 5120 ? launch_fwd<256, S, false>(a, s) : launch_fwd<512, S, false>(a, s);
+  // Few rows have wide teams, many have teams that are not long at a row.  (The loss of 512 rows of 4096 bfloat16 values with 64, 256 threads
+  // each: 5.5, 4.7 us, of 4096 rows of 2000: 8.8, 12.0; 1024 rows of 20001 with 128, 256: 12.4, 13.3, 4096 of 50304: 84.8, 77.9; 64 of 20001 with
+  // 256, 512: 5.9, 5.5, 300: 7.5, 7.7.  The gradient of 512 rows of 4096 with 64, 256: 8.3, 6.9, of 4096 rows of 2000: 13.9, 20.0; 1024 rows of 20001
+  // with 256, 512: 17.5, 19.8, 512 of 50304: 20.6, 23.4, 64 of those: 7.7, 7.3,
+  // 4096: 158.6, 149.1.)
+  const bool few = a.batch <= 2 * cus;
+  if (vecs <= 128 || (vecs <= 512 && !few)) return grad ? launch_bwd<64, S>(a, unsigned(vecs), s) : launch_fwd<64, S, false>(a, s);
+  if (!grad) {
+    if (few) return a.batch * 2 <= cus && vecs > 1024 ? launch_fwd<512, S, false>(a, s) : launch_fwd<256, S, false>(a, s);
     return vecs <= 2560 ? launch_fwd<128, S, false>(a, s) : launch_fwd<256, S, false>(a, s);
   }
-  if (vecs <= 512) return launch_bwd<64, S>(a, unsigned(vecs), s);
   // few rows: several workgroups to each, with a turn of every thread's vectors at least
   auto each = [&](size_t threads) {
-    const size_t turns = (vecs + threads * kAhead - 1) / (threads * kAhead), want = (4 * cus + a.batch - 1) / a.batch, n = turns < want ? turns : want;
+    const size_t turns = (vecs + threads * kAhead - 1) / (threads * kAhead), want = (4 * cus + a.batch - 1) / a.batch;
+    const size_t n = turns < want ? turns : want;
     return unsigned((vecs + n - 1) / n);
   };
-  return vecs <= 2048 ? launch_bwd<256, S>(a, each(256), s) : launch_bwd<512, S>(a, each(512), s);
+  return vecs <= 4096 || (few && a.batch * 4 > cus && vecs <= 8192) ? launch_bwd<256, S>(a, each(256), s) : launch_bwd<512, S>(a, each(512), s);
 }
 
 }  // namespace
@@ -829,26 +1012,32 @@ extern "C" {
 #define SGH_DISTILL(SFX, S, T)                                                                                                     \
   int sgh_distill_fwd_##SFX(const T *x, const int32_t *top, const float *teacher, const int32_t *labels, const float *weights,     \
                             size_t batch, size_t dim, size_t k, float temperature, float soft, float hard, float *loss,            \
-                            float *stats, void *stream) {                                                                          \
+                            float *stats, void *workspace, size_t ws_bytes, void *stream) {                                        \
     return distill<S>({x, nullptr, top, teacher, labels, weights, loss, stats, batch, dim, 0, temperature, soft, hard, 0.f}, k,    \
-                      true, false, stream);                                                                                        \
+                      true, false, workspace, ws_bytes, stream);                                                                   \
   }                                                                                                                                \
   int sgh_distill_bwd_##SFX(const T *x, const float *stats, const int32_t *top, const float *teacher, const int32_t *labels,       \
                             const float *weights, size_t batch, size_t dim, size_t k, float temperature, float soft, float hard,   \
                             float scale, T *dx, void *stream) {                                                                    \
     return distill<S>({x, dx, top, teacher, labels, weights, nullptr, const_cast<float *>(stats), batch, dim, 0, temperature,      \
-                       soft, hard, scale}, k, false, true, stream);                                                                \
+                       soft, hard, scale}, k, false, true, nullptr, 0, stream);                                                    \
   }                                                                                                                                \
   int sgh_distill_fwd_bwd_##SFX(const T *x, const int32_t *top, const float *teacher, const int32_t *labels,                       \
                                 const float *weights, size_t batch, size_t dim, size_t k, float temperature, float soft,           \
-                                float hard, float scale, float *loss, T *dx, void *stream) {                                       \
+                                float hard, float scale, float *loss, T *dx, void *workspace, size_t ws_bytes,                     \
+                                void *stream) {                                                                                    \
     return distill<S>({x, dx, top, teacher, labels, weights, loss, nullptr, batch, dim, 0, temperature, soft, hard, scale}, k,     \
-                      true, true, stream);                                                                                         \
+                      true, true, workspace, ws_bytes, stream);                                                                    \
   }
 SGH_DISTILL(f32, StF32, float)
 SGH_DISTILL(f16, StF16, uint16_t)
 SGH_DISTILL(bf16, StBF16, uint16_t)
 #undef SGH_DISTILL
+
+size_t sgh_distill_workspace_bytes(size_t batch, size_t dim, size_t elem_bytes, int gradient) {
+  if (batch == 0 || batch > 0x7fffffffu || dim == 0 || dim > kMostDim || (elem_bytes != 2 && elem_bytes != 4)) return 0;
+  return parts_bytes(batch, parts_of(batch, dim, elem_bytes, gradient != 0));
+}
 
 int sgh_distill_index_errors(void *stream, int *count) {
   if (!count) return SGH_EINVAL;

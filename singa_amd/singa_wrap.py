@@ -18,6 +18,7 @@ host waits for it.  Errors raise ``SingaHipError`` (the reference aborts through
 There is no CPU path in this module: without the built library and a GPU it cannot run.
 """
 import ctypes as C
+import functools
 
 import numpy as np
 
@@ -767,6 +768,17 @@ def AddRow(v, m):
 
 # ------------------------------------------------------------------------------------ token models
 
+# (sizes follow from the arguments alone; a call through ctypes is a tenth of a short operation)
+@functools.lru_cache(maxsize=4096)
+def _embedding_bwd_bytes(tokens, vocab, dim):
+    return _L().sgh_embedding_bwd_workspace_bytes(tokens, vocab, dim)
+
+
+@functools.lru_cache(maxsize=4096)
+def _distill_bytes(batch, dim, elem_bytes, gradient):
+    return _L().sgh_distill_workspace_bytes(batch, dim, elem_bytes, gradient)
+
+
 def _plain(what, device, *tensors):
     """Dense tensors of one device (None: left out)."""
     for t in tensors:
@@ -807,7 +819,7 @@ def EmbeddingBackwardW(dy, ids, W, scale=1.0, padding_idx=-1, add=None, out=None
     vocab, dim = W._shape
     tokens, dev = ids.Size(), W._dev
     dW = _like(W) if out is None else out
-    need = _L().sgh_embedding_bwd_workspace_bytes(tokens, vocab, dim)
+    need = _embedding_bwd_bytes(tokens, vocab, dim)
     # (a block of the pool for this call: calls that are recorded or run side by side share none)
     ws = _empty(Tensor, (need // 4,), dev, kFloat32) if need else None
     check(fn(ids.ptr, dy.ptr, add.ptr if add is not None else None, dW.ptr, tokens, vocab, dim, scale, padding_idx,
@@ -848,6 +860,13 @@ def _distill_args(what, x, top, teacher, labels, weights):
             weights.ptr if weights is not None else None, batch, dim, k)
 
 
+def _distill_workspace(x, gradient):
+    """(tensor or None, its address, bytes): a block of the pool for this call."""
+    need = _distill_bytes(x._shape[0], x._shape[1], 4 if x._dtype == kFloat32 else 2, gradient)
+    ws = _empty(Tensor, (need // 4,), x._dev, kFloat32) if need else None
+    return ws, ws.ptr if need else None, need
+
+
 def DistillationFwd(x, top, teacher, labels=None, weights=None, temperature=1.0, soft=1.0, hard=0.0):
     """(loss, stats): for every row of the student's logits `x` [batch, dim] the divergence from a teacher known by its top logits,
     ``soft * temperature^2 * KL(p || q)`` with p the softmax of `teacher` [batch, k] (float32) / temperature over the columns `top`
@@ -858,7 +877,8 @@ def DistillationFwd(x, top, teacher, labels=None, weights=None, temperature=1.0,
     fn, name = _fn("distill_fwd", x)
     batch = x._shape[0]
     loss, stats = _empty(Tensor, (batch,), x._dev, kFloat32), _empty(Tensor, (batch, 3), x._dev, kFloat32)
-    check(fn(x.ptr, *args, temperature, soft, hard, loss.ptr, stats.ptr, x._dev.stream), name)
+    ws, at, need = _distill_workspace(x, 0)
+    check(fn(x.ptr, *args, temperature, soft, hard, loss.ptr, stats.ptr, at, need, x._dev.stream), name)
     return loss, stats
 
 
@@ -890,7 +910,8 @@ def DistillationFwdBwd(x, top, teacher, labels=None, weights=None, temperature=1
     fn, name = _fn("distill_fwd_bwd", x)
     dx = _distill_out("DistillationFwdBwd", x, out)
     loss = _empty(Tensor, x._shape[:1], x._dev, kFloat32)
-    check(fn(x.ptr, *args, temperature, soft, hard, scale, loss.ptr, dx.ptr, x._dev.stream), name)
+    ws, at, need = _distill_workspace(x, 1)
+    check(fn(x.ptr, *args, temperature, soft, hard, scale, loss.ptr, dx.ptr, at, need, x._dev.stream), name)
     return loss, dx
 
 

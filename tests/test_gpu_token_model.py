@@ -326,7 +326,7 @@ def check_case(singa, dev, t, case, scale=1.0, shift=0, temperature=1.0, soft=1.
 
 # (rows, columns, list): one column, less than a vector, odd ones, on both sides of every way to share a row out
 SIZES = [(1, 1, 1), (3, 2, 1), (5, 7, 3), (9, 64, 5), (2, 513, 40), (6, 1000, 5), (3, 2048, 16), (4, 2049, 64), (3, 4100, 7), (2, 10007, 8),
-         (3, 16385, 100), (1, 33000, 20), (2, 70001, 65)]
+         (3, 16385, 100), (1, 33000, 20), (2, 70001, 65), (128, 35001, 3), (1500, 520, 3), (700, 5003, 20), (2100, 1300, 70), (300, 19001, 2)]
 
 
 @pytest.mark.parametrize("t", TYPES)
@@ -364,7 +364,7 @@ def test_distillation_longest_list_and_one_longer(dev):
 
 
 @pytest.mark.parametrize("t", TYPES)
-@pytest.mark.parametrize("v", [300, 9001])
+@pytest.mark.parametrize("v", [300, 9001, 40003])
 def test_distillation_masked_columns_and_odd_values(dev, t, v):
     """Columns at -inf and at the type's lowest value, rows of nothing but the lowest value, NaN and infinities in rows that do not count."""
     from singa_amd import singa_wrap as singa
@@ -397,7 +397,7 @@ def test_distillation_masked_columns_and_odd_values(dev, t, v):
 def test_distillation_of_rows_without_a_softmax_is_nan(dev, t):
     from singa_amd import singa_wrap as singa
     r = np.random.default_rng(3)
-    for v in (100, 5000):
+    for v in (100, 5000, 50000):
         x, top, teacher, labels, _ = make_case(r, t, 4, v, 4, masked=False)
         x[0][:] = -np.inf
         x[1, v // 2] = np.nan
@@ -408,10 +408,58 @@ def test_distillation_of_rows_without_a_softmax_is_nan(dev, t):
             assert np.isnan(d[0]).all() and np.isnan(d[1]).all() and np.isnan(d[2, v - 1])
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("v", [300, 4000, 50000])
+def test_distillation_towards_columns_without_a_probability(dev, t, v):
+    """The teacher wants columns that the student masks: the loss is infinite, the gradient is not."""
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(13)
+    x, top, teacher, _, weights = make_case(r, t, 4, v, 5, masked=False)
+    top = np.tile(np.arange(5) * 11, (4, 1))
+    x[0, 11] = -np.inf                # one of the entries
+    x[1, top[1]] = -np.inf            # all of them
+    x[2, :], x[2, 200:] = -np.inf, 1  # and all else
+    teacher[3, :4] = -np.inf          # entries without a share may be anything
+    x[3, :44] = -np.inf
+    want = O.distill(x, top, teacher, None, weights, temperature=2.0)
+    loss, stats, dx, loss2, dx2 = run_all(singa, dev, t, x, top, teacher, None, weights, temperature=2.0)
+    b_loss, _, b_dx = bounds(t, x, top, teacher, None, weights, 1.0, 2.0, 1.0, 0.0)
+    for l, d in ((loss, dx), (loss2, dx2)):
+        assert (l[:3] == np.inf).all()
+        close(l[3:], want[0][3:], b_loss[3:], "loss")
+        close(d, want[2], b_dx, "dx")
+
+
+def test_distillation_of_many_long_rows(dev):
+    """More rows than the chip holds, each a workgroup's registers full, and some of them in smaller batches.  (Not the same
+    bits: a row of an odd length begins elsewhere in its 16 bytes there, and a thread's sum has other terms.)"""
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(17)
+    n, v, k = 700, 66003, 4
+    x = (r.standard_normal((n, v), dtype=np.float32) * 2).astype(np.float16)
+    top, labels = r.integers(0, v, (n, k)), r.integers(-1, v, n)
+    teacher = r.standard_normal((n, k)).astype(np.float32)
+    how = dict(temperature=2.0, soft=0.7, hard=0.3)
+
+    def both(rows):
+        d_x = upload(singa, dev, "f16", x[rows])
+        loss, dx = singa.DistillationFwdBwd(d_x, ints(singa, dev, top[rows]), singa.from_numpy(teacher[rows], dev), ints(singa, dev, labels[rows]), **how)
+        return loss.to_numpy(), dx.to_numpy()
+
+    loss, dx = both(slice(0, n))
+    for rows in ([0, 1, 255, 256, 257, 511, 512, 640, 699], list(range(3, n, 5))):
+        part_loss, part_dx = both(rows)
+        b = bounds("f16", x[rows].astype(np.float64), top[rows], teacher[rows], labels[rows], None, 1.0, 2.0, 0.7, 0.3)
+        want = O.distill(x[rows].astype(np.float64), top[rows], teacher[rows], labels[rows], None, **how)
+        for l, d in ((loss[rows], dx[rows]), (part_loss, part_dx)):
+            close(l, want[0], b[0], "loss")
+            close(d, want[2], b[2], "dx")
+
+
 def test_distillation_entries_out_of_range_are_left_out_and_counted(dev):
     from singa_amd import singa_wrap as singa
     r = np.random.default_rng(9)
-    for v in (50, 5000):
+    for v in (50, 5000, 50000):
         x, top, teacher, labels, weights = make_case(r, "f32", 3, v, 5, masked=False)
         top[0, 1], top[1, 2], top[2, 0] = v, -2, 2147483647
         labels[1], labels[2] = v, -5
@@ -430,7 +478,7 @@ def test_distillation_entries_out_of_range_are_left_out_and_counted(dev):
         close(dx.to_numpy(), want[2], b[2], "dx")
 
 
-@pytest.mark.parametrize("v", [200, 6000])
+@pytest.mark.parametrize("v", [200, 6000, 20000])
 def test_distillation_gradient_against_differences(dev, v):
     """Central differences of the loss along a direction of at most 1 in every place.  The third derivative of the logarithm of a sum of
     exponentials of y / tau along such a direction is a third central moment of a variable in [-1, 1], at most 1 by size, over tau^3."""
@@ -459,15 +507,18 @@ def test_recorded_calls_replay(dev):
     vocab, dim, n, k = 3000, 40, 1500, 4
     ids, table = ints(singa, dev, r.integers(0, vocab, n)), upload(singa, dev, "f32", r.standard_normal((vocab, dim)))
     few = ints(singa, dev, r.integers(0, vocab, 90))
+    long = upload(singa, dev, "bf16", r.standard_normal((3, 50000)))
     x = upload(singa, dev, "f32", r.standard_normal((n, vocab)))
     top, teacher = ints(singa, dev, r.integers(0, vocab, (n, k))), singa.from_numpy(r.standard_normal((n, k)).astype(np.float32), dev)
+    long_top, long_teacher = ints(singa, dev, r.integers(0, 50000, (3, k))), singa.from_numpy(r.standard_normal((3, k)).astype(np.float32), dev)
 
     def calls():
         y = singa.EmbeddingForward(ids, table)
         loss, stats = singa.DistillationFwd(x, top, teacher)
         dx = singa.DistillationBwd(x, stats, top, teacher, scale=1.0 / n)
         loss2, dx2 = singa.DistillationFwdBwd(x, top, teacher, scale=1.0 / n)
-        return [y, loss, stats, dx, loss2, dx2, singa.EmbeddingBackwardW(y, ids, table),
+        few_rows = [t for f in (singa.DistillationFwd, singa.DistillationFwdBwd) for t in f(long, long_top, long_teacher)]
+        return few_rows + [y, loss, stats, dx, loss2, dx2, singa.EmbeddingBackwardW(y, ids, table),
                 singa.EmbeddingBackwardW(singa.EmbeddingForward(few, table), few, table)]
 
     want = [t.to_numpy() for t in calls()]

@@ -111,16 +111,16 @@ answer([ok, refused, short, nothing])
 
 
 def test_distillation_refusals():
-    ok, refused, limit = recorded("""
+    ok, short, refused, limit = recorded("""
 S = SPACE
 N, V, K = 6, 700, 9
 inf, nan = float("inf"), float("nan")
-def fwd(x=S, top=2 * S, teacher=3 * S, labels=4 * S, w=5 * S, n=N, v=V, k=K, tau=2.0, loss=6 * S, stats=7 * S, sfx="f32"):
-    return getattr(lib, "sgh_distill_fwd_" + sfx)(x, top, teacher, labels, w, n, v, k, tau, 1.0, 1.0, loss, stats, None), len(kernels())
+def fwd(x=S, top=2 * S, teacher=3 * S, labels=4 * S, w=5 * S, n=N, v=V, k=K, tau=2.0, loss=6 * S, stats=7 * S, sfx="f32", ws=9 * S, wn=1 << 20):
+    return getattr(lib, "sgh_distill_fwd_" + sfx)(x, top, teacher, labels, w, n, v, k, tau, 1.0, 1.0, loss, stats, ws, wn, None), len(kernels())
 def bwd(x=S, stats=7 * S, top=2 * S, teacher=3 * S, labels=4 * S, w=5 * S, n=N, v=V, k=K, tau=2.0, dx=8 * S, sfx="f32"):
     return getattr(lib, "sgh_distill_bwd_" + sfx)(x, stats, top, teacher, labels, w, n, v, k, tau, 1.0, 1.0, 1.0, dx, None), len(kernels())
-def both(x=S, top=2 * S, teacher=3 * S, labels=4 * S, w=5 * S, n=N, v=V, k=K, tau=2.0, loss=6 * S, dx=8 * S, sfx="f32"):
-    return getattr(lib, "sgh_distill_fwd_bwd_" + sfx)(x, top, teacher, labels, w, n, v, k, tau, 1.0, 1.0, 1.0, loss, dx, None), len(kernels())
+def both(x=S, top=2 * S, teacher=3 * S, labels=4 * S, w=5 * S, n=N, v=V, k=K, tau=2.0, loss=6 * S, dx=8 * S, sfx="f32", ws=9 * S, wn=1 << 20):
+    return getattr(lib, "sgh_distill_fwd_bwd_" + sfx)(x, top, teacher, labels, w, n, v, k, tau, 1.0, 1.0, 1.0, loss, dx, ws, wn, None), len(kernels())
 size = N * V * 4
 ok = [f(**how) for f in (fwd, bwd, both) for how in ({}, {"k": 0, "top": None, "teacher": None}, {"labels": None, "w": None}, {"v": 1}, {"k": 1024},
                                                      {"v": 200000}, {"sfx": "f16"}, {"sfx": "bf16", "v": 50000})]
@@ -135,9 +135,16 @@ refused += [bwd(dx=7 * S), fwd(loss=S + size - 4), fwd(loss=2 * S), fwd(loss=7 *
 limit = [f(k=1025) for f in (fwd, bwd, both)]
 empty = [f(n=0) for f in (fwd, bwd, both)]
 ok += [(rc, 1 - n) for rc, n in empty]      # nothing to do, nothing launched
-answer([ok, refused, limit])
+ok += [f(ws=None, wn=0) for f in (fwd, both)]
+need = lib.sgh_distill_workspace_bytes(N, 200000, 4, 0)
+assert need == lib.sgh_distill_workspace_bytes(N, 200000, 4, 1)
+ok += [f(v=200000, wn=need) for f in (fwd, both)]
+short = [f(v=200000, **how) for f in (fwd, both) for how in ({"wn": need - 1}, {"ws": None}, {"sfx": "bf16", "wn": 0})]
+refused += [f(v=200000, ws=9 * S + 8) for f in (fwd, both)]
+answer([ok, short, refused, limit])
 """)
-    assert all(rc == 0 and n == 1 for rc, n in ok), ok
+    assert all(rc == 0 and n in (1, 2) for rc, n in ok), ok
+    assert all(r == [EWORKSPACE, 0] for r in short), short
     assert all(r == [EINVAL, 0] for r in refused), [(i, r) for i, r in enumerate(refused) if r != [EINVAL, 0]]
     assert all(r == [ELIMIT, 0] for r in limit), limit
 
@@ -203,16 +210,21 @@ answer([run(1024, 5000, 64), run(8192, 5000, 64), run(8193, 131071, 64), run(819
 
 
 def test_what_the_distillation_launches():
-    """One launch whatever the size; LDS only for lists that do not fit a wavefront's registers."""
+    """One launch; two for the loss of few long rows, which are cut in parts, and a workspace then."""
     got = recorded("""
 S = 1 << 50
 out = []
-for n, v, k in ((1, 1, 0), (3, 1000, 5), (1 << 20, 32, 64), ((1 << 31) - 1, 1, 0), (7, 1 << 28, 1024), (5000, 131072, 64)):
-    for sfx in ("f32", "f16", "bf16"):
+for n, v, k in ((1, 1, 0), (3, 1000, 5), (1 << 20, 32, 64), ((1 << 31) - 1, 1, 0), (5000, 131072, 64), (300, 300000, 3), (7, 1 << 28, 1024), (1, 131072, 16)):
+    for sfx, e in (("f32", 4), ("f16", 2), ("bf16", 2)):
+        need = lib.sgh_distill_workspace_bytes(n, v, e, 1)
         a = (S, 2 * S, 3 * S, 4 * S, 5 * S, n, v, k, 1.5, 1.0, 1.0)
-        rcs = [getattr(lib, "sgh_distill_fwd_" + sfx)(*a, 6 * S, 7 * S, None), getattr(lib, "sgh_distill_fwd_bwd_" + sfx)(*a, 1.0, 6 * S, 8 * S, None),
-               getattr(lib, "sgh_distill_bwd_" + sfx)(S, 7 * S, *a[1:], 1.0, 8 * S, None)]
-        out.append((rcs, len(kernels())))
+        ws = (9 * S if need else None, need, None)
+        rcs = [getattr(lib, "sgh_distill_fwd_" + sfx)(*a, 6 * S, 7 * S, *ws), len(kernels()), getattr(lib, "sgh_distill_fwd_bwd_" + sfx)(*a, 1.0, 6 * S, 8 * S, *ws),
+               len(kernels()), getattr(lib, "sgh_distill_bwd_" + sfx)(S, 7 * S, *a[1:], 1.0, 8 * S, None), len(kernels())]
+        out.append((n <= 7 and v > 100000, need, rcs))
 answer(out)
 """)
-    assert all(rcs == [0, 0, 0] and n == 3 for rcs, n in got), got
+    for parts, need, rcs in got:
+        if rcs[3] == 2048:   # (2^31 rows of one: 2^20 of them a launch)
+            rcs[3] = 1
+        assert (need > 0) == parts and rcs == ([0, 2, 0, 2, 0, 1] if parts else [0, 1, 0, 1, 0, 1]), got
