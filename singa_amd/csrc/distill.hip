@@ -85,7 +85,8 @@ struct Team {
   static constexpr int kWaves = (NT == kAny ? kMostThreads : NT) / SGH_WAVE;
   static __device__ __forceinline__ unsigned size() { return NT == kAny ? blockDim.x : unsigned(NT); }
   static constexpr int kLists = NT == SGH_WAVE ? 1 : 2;   // a row's list may still be read where the next one's is fetched
-  static __device__ __forceinline__ int id() { return NT == SGH_WAVE ? threadIdx.x >> 6 : 0; }
+  // (known to be the same for a wavefront's lanes: so are its row and what follows from that)
+  static __device__ __forceinline__ int id() { return NT == SGH_WAVE ? __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)) : 0; }
   static __device__ __forceinline__ int tid() { return NT == SGH_WAVE ? threadIdx.x & 63 : threadIdx.x; }
   // what the team's threads stored (LDS and global memory) is seen by all of them behind this
   static __device__ __forceinline__ void sync() {
@@ -131,16 +132,18 @@ __device__ __forceinline__ int checked_label(const Rows<T> &a, int label, bool c
 
 // A row's list is seen to by one wavefront of its team, in three steps, so that nothing else waits for its loads (the entries, then the student's
 // logits there).  Up to 64 entries are a lane's each, in registers; a longer list goes to LDS, where the whole team ends up with it.
+template <class T>
 struct Entry {
   int at = -1;
   float v = 0.f, x = 0.f, p = 0.f;   // the teacher's logit, the student's, the teacher's share
   int label = -1;
   float label_x = 0.f;               // (lane 0)
+  T x_raw = 0, label_raw = 0;        // as they are loaded: nothing waits for them before step 3
 };
 __host__ __device__ inline bool short_list(int k) { return k <= SGH_WAVE; }
 // 1: the entries are asked for
 template <class T>
-__device__ __forceinline__ void ask_list(const Rows<T> &a, size_t row, Entry &e) {
+__device__ __forceinline__ void ask_list(const Rows<T> &a, size_t row, Entry<T> &e) {
   const int lane = threadIdx.x & (SGH_WAVE - 1);
   if (a.soft != 0.f && lane < a.k) e.at = a.top[row * a.k + lane], e.v = a.teacher[row * a.k + lane];
 }
@@ -154,13 +157,14 @@ __device__ __forceinline__ int checked_entry(const Rows<T> &a, int at, float v, 
   return v == -__builtin_inff() ? -1 : at;   // (no share)
 }
 template <class S>
-__device__ __forceinline__ bool gather_list(const Rows<typename S::elem> &a, size_t row, int label, bool count, const List &l, Entry &e) {
+__device__ __forceinline__ bool gather_list(const Rows<typename S::elem> &a, size_t row, int label, bool count, const List &l,
+                                            Entry<typename S::elem> &e) {
   const int lane = threadIdx.x & (SGH_WAVE - 1);
   const typename S::elem *x = a.x + row * a.dim;
   e.label = label;
-  if (lane == 0 && label >= 0) e.label_x = S::ld(x + label);
+  if (lane == 0 && label >= 0) e.label_raw = x[label];
   e.at = checked_entry(a, e.at, e.v, count);
-  if (e.at >= 0) e.x = S::ld(x + e.at);
+  if (e.at >= 0) e.x_raw = x[e.at];
   bool present = e.at >= 0;
   if (!short_list(a.k)) {
     if (lane == 0) l.at[a.k] = label, l.p[a.k] = 1.f;
@@ -179,8 +183,10 @@ __device__ __forceinline__ bool gather_list(const Rows<typename S::elem> &a, siz
   return __ballot(present) != 0;
 }
 // 3: those are there; what the teacher's logits come to
-template <class T>
-__device__ __forceinline__ Teacher finish_list(const Rows<T> &a, bool any, const List &l, const Entry &e) {
+template <class S>
+__device__ __forceinline__ Teacher finish_list(const Rows<typename S::elem> &a, bool any, const List &l, Entry<typename S::elem> &e) {
+  if (e.at >= 0) e.x = S::ld(&e.x_raw);
+  if (e.label >= 0) e.label_x = S::ld(&e.label_raw);
   const int lane = threadIdx.x & (SGH_WAVE - 1);
   Teacher t = {any, -__builtin_inff(), 0.f};
   const float c = kLog2e * a.inv_tau;
@@ -204,7 +210,7 @@ __device__ __forceinline__ Teacher finish_list(const Rows<T> &a, bool any, const
 
 // The teacher's shares, by the same wavefront; returns the divergence (LOSS)
 template <bool LOSS, class T>
-__device__ __forceinline__ float teacher_shares(const Rows<T> &a, const Teacher &t, float m, float log_st, const List &l, Entry &e) {
+__device__ __forceinline__ float teacher_shares(const Rows<T> &a, const Teacher &t, float m, float log_st, const List &l, Entry<T> &e) {
   const int lane = threadIdx.x & (SGH_WAVE - 1);
   const float log_sum = logf(t.sum), inv = 1.f / t.sum;
   float kl = 0.f;
@@ -296,7 +302,7 @@ __device__ __forceinline__ Slope slope_of(const Rows<T> &a, float w, const Runni
 // The columns of the list once more, behind a sync: a column that is there several times is its first entry's
 template <int NT, class S>
 __device__ __forceinline__ void list_columns(const Rows<typename S::elem> &a, size_t row, size_t from, size_t to, const Slope &s,
-                                             const List &l, const Entry &e) {
+                                             const List &l, const Entry<typename S::elem> &e) {
   typename S::elem *dx = a.dx + row * a.dim;
   auto mine = [&](int at) { return at >= 0 && size_t(at) >= from && size_t(at) < to; };
   if (short_list(a.k)) {
@@ -344,7 +350,13 @@ constexpr unsigned kOutside = 0x07ffffffu;   // (times 16: 2 GB behind the row's
 struct RowBuffer {
   __amdgpu_buffer_rsrc_t r;
   __device__ __forceinline__ RowBuffer(const void *p, unsigned bytes)
-      : r(__builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, int(bytes), 0x00020000)) {}
+      : r(__builtin_amdgcn_make_buffer_rsrc(same(p), 0, __builtin_amdgcn_readfirstlane(int(bytes)), 0x00020000)) {}
+  // The same for all lanes, and known to be (each access is a loop over the lanes' descriptors else)
+  static __device__ __forceinline__ void *same(const void *p) {
+    const uintptr_t v = reinterpret_cast<uintptr_t>(p);
+    const unsigned lo = __builtin_amdgcn_readfirstlane(unsigned(v)), hi = __builtin_amdgcn_readfirstlane(unsigned(v >> 32));
+    return reinterpret_cast<void *>(uintptr_t(hi) << 32 | lo);
+  }
   // of `vecs` vectors behind `pad` places without one, which are asked for at kOutside instead
   static __device__ __forceinline__ RowBuffer padded(const void *first, unsigned vecs, unsigned pad) {
     return RowBuffer(static_cast<const char *>(first) - pad * 16, vecs ? (pad + vecs) * 16 : 0);
@@ -475,7 +487,7 @@ __device__ __forceinline__ Running team_sums(const Lane &lane, float ct, Running
 // Loss and statistics of a row, by the wavefront that sees to its list; the teacher's shares are in the list then
 template <class T>
 __device__ __forceinline__ void store_loss(const Rows<T> &a, size_t row, float w, const Running &r, bool soft, bool hard,
-                                           const Teacher &teach, const List &list, Entry &entry) {
+                                           const Teacher &teach, const List &list, Entry<T> &entry) {
   float loss = 0.f;
   if (soft) loss = a.soft * a.tau * a.tau * teacher_shares<true>(a, teach, r.m, logf(r.st), list, entry);
   if ((threadIdx.x & (SGH_WAVE - 1)) != 0) return;
@@ -523,9 +535,10 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_fwd(Rows<typenam
     const Lie lie = lie_of<S>(x, unsigned(a.dim), tid);
     const unsigned vecs = lie.vecs;
     // everything is asked for at once, the first vectors of a row that turns out to want nothing as well
-    Entry entry;
+    Entry<T> entry;
     if (lister) ask_list(a, row, entry);
-    const float tail = lie.odd != kNone ? S::ld(x + lie.odd) : 0.f;
+    T end = 0;
+    if (lie.odd != kNone) end = x[lie.odd];
     const RowBuffer from(x + lie.head, vecs * 16);
     sgh_v4u v[kAhead];
     const Row q = row_at(a, row, tid == 0);
@@ -544,12 +557,13 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_fwd(Rows<typenam
       sum.start(ct, want);
       stream_row<NT, STREAM && !GRAD>(
           from, vecs, v, [&](const sgh_v4u &raw, unsigned vec, bool all) { take_vector<S>(sum, raw, vec, vecs, all, ct, want); });
+      const float tail = S::ld(&end);
       if (lie.odd != kNone) sum.take<1>(&tail, ct, want);
       r = of_row(a, team_sums<NT>(sum, ct, red));
       soft = q.may_soft && (NT == SGH_WAVE ? any : listed != 0);
     }
     if (lister) {
-      const Teacher teach = finish_list(a, any, list, entry);
+      const Teacher teach = finish_list<S>(a, any, list, entry);
       store_loss(a, row, q.w, r, soft, q.hard, teach, list, entry);
     }
     if constexpr (GRAD) {
@@ -557,7 +571,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_fwd(Rows<typenam
       const bool none = !(soft || q.hard);
       if (NT != SGH_WAVE) G::sync();   // (the list's logits are read: dx may be x)
       slope_row<NT, S, STREAM>(x + lie.head, a.dx + row * a.dim + lie.head, vecs, lie.pad, none, s);
-      if (lie.odd != kNone) S::st(a.dx + row * a.dim + lie.odd, s(tail));
+      if (lie.odd != kNone) S::st(a.dx + row * a.dim + lie.odd, s(S::ld(&end)));
       G::sync();
       if (!none) list_columns<NT, S>(a, row, 0, a.dim, s, list, entry);
     } else {
@@ -572,7 +586,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_fwd(Rows<typenam
 //   sum_k p_k (log p_k - log q_k) = kl - (top - m) / tau + log S_tau,   kl = sum_k p_k (log p_k - (x_k - top) / tau)
 // so that the record of a row is {whether there is an entry, kl, top, x_label}.
 template <class T>
-__device__ __forceinline__ float4 row_record(const Rows<T> &a, const Teacher &t, const List &l, const Entry &e) {
+__device__ __forceinline__ float4 row_record(const Rows<T> &a, const Teacher &t, const List &l, const Entry<T> &e) {
   const int lane = threadIdx.x & (SGH_WAVE - 1);
   const float log_sum = logf(t.sum), inv = 1.f / t.sum;
   auto share = [&](float v) { return exp2_((v - t.most) * (kLog2e * a.inv_tau)) * inv; };
@@ -606,9 +620,10 @@ __global__ __launch_bounds__(kBlock) void k_distill_part(Rows<typename S::elem> 
   const Lie lie = lie_of<S>(x, unsigned(a.dim), threadIdx.x);
   const unsigned first = part * each < lie.vecs ? part * each : lie.vecs, vecs = lie.vecs - first < each ? lie.vecs - first : each;
   const bool odd = lie.odd != kNone && (lie.odd < lie.head ? begins : ends);
-  Entry entry;
+  Entry<T> entry;
   if (lister) ask_list(a, row, entry);
-  const float tail = odd ? S::ld(x + lie.odd) : 0.f;
+  T end = 0;
+  if (odd) end = x[lie.odd];
   const RowBuffer from(x + lie.head + size_t(first) * S::VEC, vecs * 16);
   sgh_v4u v[kAhead];
   const Row q = row_at(a, row, begins && threadIdx.x == 0);
@@ -623,12 +638,13 @@ __global__ __launch_bounds__(kBlock) void k_distill_part(Rows<typename S::elem> 
     sum.start(ct, want);
     stream_row<NT, false>(
         from, vecs, v, [&](const sgh_v4u &raw, unsigned vec, bool all) { take_vector<S>(sum, raw, vec, vecs, all, ct, want); });
+    const float tail = S::ld(&end);
     if (odd) sum.take<1>(&tail, ct, want);
     const Running r = team_sums<NT>(sum, ct, red);
     if (threadIdx.x == 0) out[1 + part] = {r.m, r.st, r.s1, 0.f};
   }
   if (lister) {
-    const Teacher teach = finish_list(a, any, list, entry);
+    const Teacher teach = finish_list<S>(a, any, list, entry);
     float4 rec = {0.f, 0.f, 0.f, entry.label_x};
     if (any) rec = row_record(a, teach, list, entry);
     if (threadIdx.x == 0) out[0] = rec;
@@ -666,14 +682,11 @@ __global__ __launch_bounds__(SGH_WAVE) void k_distill_join(Rows<T> a) {
   if (threadIdx.x == 0) store_joined(a, row, q.w, r, q.may_soft && record.x != 0.f, q.hard, record);
 }
 
-// Both for rows of at most U * NT vectors, in registers: what bounds it is the logits' way in and the gradient's out.
-// ONE: a workgroup for each row (a wavefront, of short ones), so that one's loads are in flight beside another's sums and stores.
-// Else a workgroup goes from row to row, and each of the next row's vectors is asked for when the register it goes to is free, behind the store
-// of this row's gradient there: for rows that leave a CU no second workgroup.  (Loads behind a row's stores wait for these: where there are
-// several workgroups, one for each row is faster, 530 -> 450 us for 16384 rows of 20001 fp32 values, 207 -> 186 for 4096 of 50304 bfloat16.)
-// What is small (weight, label, the first 64 of the list) is asked for in front of a row's vectors, a row or two ahead: loads come back in
-// order.  8192 rows of 131072 bfloat16 values with lists of 64, in turn: 4.5 TB/s; 2048 rows of 65001, labels alone: 107 us.
-template <int NT, int U, int PER_SIMD, bool ONE, class S, bool STREAM>
+// Both for rows of at most U * NT vectors, in registers: what bounds it is the logits' way in and the gradient's out.  A workgroup for each row (a
+// wavefront, of short ones), so that one's loads are in flight beside another's sums and stores.  (Going from row to row instead, with the
+// next row's loads behind this one's stores, these waited for the stores: 530 and 450 us for 16384 rows of 20001 fp32 values, 207 and 186
+// for 4096 of 50304 bfloat16.)  2048 rows of 65001 bfloat16 values, labels alone: 106 us; 4096 of 32000, with lists: 106 us, 4.9 TB/s.
+template <int NT, int U, int PER_SIMD, class S, bool STREAM>
 __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(Rows<typename S::elem> a) {
   typedef Team<NT> G;
   typedef typename S::elem T;
@@ -684,105 +697,61 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
   const unsigned nt = G::size();
   const bool lister = tid < SGH_WAVE;   // the wavefront that sees to the list
   const float ct = kLog2e * a.inv_tau;
-  const size_t step = size_t(gridDim.x) * G::kPerBlock;
-  size_t row = size_t(blockIdx.x) * G::kPerBlock + G::id();
+  const size_t row = size_t(blockIdx.x) * G::kPerBlock + G::id();
   if (row >= a.batch) return;
-  // weight and label as they are in memory
-  struct Raw {
-    float w;
-    int label;
-  };
-  auto raw_at = [&](size_t r) {
-    Raw q = {0.f, -1};
-    if (r < a.batch) {
-      q.w = a.weights ? a.weights[r] : 1.f;
-      if (a.labels && a.hard != 0.f) q.label = a.labels[r];
-    }
-    return q;
-  };
-  auto row_of = [&](const Raw &raw, bool count) {
-    Row q;
-    q.w = raw.w;
-    q.label = checked_label(a, raw.label, count);
-    q.hard = q.label >= 0 && q.w != 0.f;
-    q.may_soft = a.k && a.soft != 0.f && q.w != 0.f;
-    return q;
-  };
-  // a thread's first place in a row that lies like this
-  auto place = [&](const Lie &l) { return unsigned(tid) < l.pad ? kOutside : unsigned(tid); };
-  sgh_v4u held[U];
-  float tail = 0.f;
-  Entry entry;
+  const T *x = a.x + row * a.dim;
+  T *dx = a.dx + row * a.dim;
+  const Lie lie = lie_of<S>(x, unsigned(a.dim), tid);
+  const unsigned first = unsigned(tid) < lie.pad ? kOutside : unsigned(tid), places = lie.pad + lie.vecs;
+  // what is small is asked for in front of the row's vectors: loads come back in order
+  Entry<T> entry;
   if (lister) ask_list(a, row, entry);
-  Row q = row_of(raw_at(row), tid == 0);
-  Raw next_raw = {0.f, -1};
-  if constexpr (!ONE) next_raw = raw_at(row + step);
-  Lie lie = lie_of<S>(a.x + row * a.dim, unsigned(a.dim), tid);
-  {
-    const T *first = a.x + row * a.dim;
-    const RowBuffer x = RowBuffer::padded(first + lie.head, q.any() ? lie.vecs : 0, lie.pad);
+  const Row q = row_at(a, row, tid == 0);
+  const RowBuffer from = RowBuffer::padded(x + lie.head, q.any() ? lie.vecs : 0, lie.pad), to = RowBuffer::padded(dx + lie.head, lie.vecs, lie.pad);
+  sgh_v4u held[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) held[u] = x.load<STREAM>(u == 0 ? place(lie) : u * nt + tid);
-    if (lie.odd != kNone && q.any()) tail = S::ld(first + lie.odd);
+  for (int u = 0; u < U; ++u) held[u] = from.load<STREAM>(u == 0 ? first : u * nt + tid);
+  T end = 0;
+  if (lie.odd != kNone) end = x[lie.odd];
+  const List list = list_at(lds + G::id() * list_bytes(a.k), a.k);
+  bool any = false;
+  if (lister) {   // (entries out of range are counted whatever the weight)
+    any = gather_list<S>(a, row, q.hard ? q.label : -1, true, list, entry);
+    if (NT != SGH_WAVE && tid == 0) listed = any;
   }
-  int turn = 0;
-  for (;;) {
-    const size_t next = row + step;
-    const bool goes_on = !ONE && next < a.batch;
-    const Row nq = row_of(next_raw, tid == 0);   // (of nothing behind the last)
-    const T *nx = a.x + next * a.dim;
-    Entry next_entry;
-    const List list = list_at(lds + (G::id() * G::kLists + turn) * list_bytes(a.k), a.k);
-    const Lie next_lie = lie_of<S>(nx, unsigned(a.dim), tid);
-    T *dx = a.dx + row * a.dim;
-    const unsigned places = lie.pad + lie.vecs;
-    const RowBuffer to = RowBuffer::padded(dx + lie.head, lie.vecs, lie.pad);
-    const RowBuffer then = RowBuffer::padded(nx + next_lie.head, goes_on && nq.any() ? next_lie.vecs : 0, next_lie.pad);
-    bool any = false;
-    if (lister) {
-      any = gather_list<S>(a, row, q.hard ? q.label : -1, true, list, entry);
-      if (NT != SGH_WAVE && tid == 0) listed = any;
-    }
-    const Sums want = {q.may_soft && a.tau != 1.f, q.hard || (q.may_soft && a.tau == 1.f)};
-    Running r = {0.f, 0.f, 0.f};
-    bool soft = false;
-    if (q.any()) {
-      Lane sum;
-      sum.start(ct, want);
+  const Sums want = {q.may_soft && a.tau != 1.f, q.hard || (q.may_soft && a.tau == 1.f)};
+  Running r = {0.f, 0.f, 0.f};
+  bool soft = false;
+  if (q.any()) {
+    Lane sum;
+    sum.start(ct, want);
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (u * nt < places) {
-          const bool all = (u != 0 || lie.pad == 0) && (u + 1) * nt <= places;
-          take_vector<S>(sum, held[u], u == 0 ? place(lie) : u * nt + tid, places, all, ct, want);
-        }
-      if (lie.odd != kNone) sum.take<1>(&tail, ct, want);
-      r = of_row(a, team_sums<NT>(sum, ct, red));
-      soft = q.may_soft && (NT == SGH_WAVE ? any : listed != 0);
-    }
-    if (lister) {
-      const Teacher teach = finish_list(a, any, list, entry);
-      store_loss(a, row, q.w, r, soft, q.hard, teach, list, entry);
-      if (goes_on) ask_list(a, next, next_entry);
-    }
-    if constexpr (!ONE) next_raw = raw_at(next + step);
-    const Slope s = slope_of(a, q.w, r, soft, q.hard);
-    if (a.in_place && NT != SGH_WAVE) G::sync();   // (the list's logits are read)
-    unsigned i = tid;
-    asm("" : "+v"(i));   // (the places of a row are not kept in registers of their own from row to row: 20 of these went to scratch memory)
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (u * nt < places) held[u] = slope_vector<S>(s, held[u]);   // (nothing but arithmetic in the branch)
-      to.store<STREAM>(held[u], u == 0 ? place(lie) : u * nt + i);
-      if constexpr (!ONE) held[u] = then.load<STREAM>(u == 0 ? place(next_lie) : u * nt + i);
-    }
-    if (lie.odd != kNone) S::st(dx + lie.odd, s(tail));
-    if (next_lie.odd != kNone && goes_on && nq.any()) tail = S::ld(nx + next_lie.odd);
-    G::sync();
-    if (soft || q.hard) list_columns<NT, S>(a, row, 0, a.dim, s, list, entry);
-    if (!goes_on) break;
-    row = next, q = nq, lie = next_lie, entry = next_entry;
-    turn = (turn + 1) % G::kLists;
+    for (int u = 0; u < U; ++u)
+      if (u * nt < places) {
+        const bool all = (u != 0 || lie.pad == 0) && (u + 1) * nt <= places;
+        take_vector<S>(sum, held[u], u == 0 ? first : u * nt + tid, places, all, ct, want);
+      }
+    const float tail = S::ld(&end);
+    if (lie.odd != kNone) sum.take<1>(&tail, ct, want);
+    r = of_row(a, team_sums<NT>(sum, ct, red));
+    soft = q.may_soft && (NT == SGH_WAVE ? any : listed != 0);
   }
+  if (lister) {
+    const Teacher teach = finish_list<S>(a, any, list, entry);
+    store_loss(a, row, q.w, r, soft, q.hard, teach, list, entry);
+  }
+  const Slope s = slope_of(a, q.w, r, soft, q.hard);
+  if (a.in_place && NT != SGH_WAVE) G::sync();   // (the list's logits are read)
+  unsigned i = tid;
+  asm("" : "+v"(i));   // (the places are not kept in registers of their own from the loads on)
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (u * nt < places) held[u] = slope_vector<S>(s, held[u]);   // (nothing but arithmetic in the branch)
+    to.store<STREAM>(held[u], u == 0 ? first : u * nt + i);
+  }
+  if (lie.odd != kNone) S::st(dx + lie.odd, s(S::ld(&end)));
+  G::sync();
+  if (soft || q.hard) list_columns<NT, S>(a, row, 0, a.dim, s, list, entry);
 }
 
 // The gradient from the statistics, or from a row's parts, whose loss it stores then; a row may be several workgroups', `each` vectors of it
@@ -804,9 +773,10 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_bwd(Rows<typenam
     const bool begins = blockIdx.y == 0, ends = blockIdx.y + 1 == gridDim.y;
     const size_t start = lie.head + size_t(first) * S::VEC, from = begins ? 0 : start, to = ends ? a.dim : start + size_t(vecs) * S::VEC;
     const bool odd = lie.odd != kNone && (lie.odd < lie.head ? begins : ends);
-    Entry entry;
+    Entry<T> entry;
     if (lister) ask_list(a, row, entry);
-    const float tail = odd ? S::ld(x + lie.odd) : 0.f;
+    T end = 0;
+    if (odd) end = x[lie.odd];
     const Row q = row_at(a, row, false);
     Running r;
     bool soft = q.may_soft, hard = q.hard;
@@ -826,7 +796,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_bwd(Rows<typenam
     if (lister && !none) any = gather_list<S>(a, row, hard ? q.label : -1, false, list, entry);
     auto shares = [&]() {
       if (!lister || none) return;
-      const Teacher t = finish_list(a, any, list, entry);
+      const Teacher t = finish_list<S>(a, any, list, entry);
       if (soft) teacher_shares<false>(a, t, 0.f, 0.f, list, entry);
     };
     if (a.in_place) {   // (the list's logits are read before any is stored over)
@@ -834,7 +804,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_bwd(Rows<typenam
       if (NT != SGH_WAVE) G::sync();
     }
     slope_row<NT, S, STREAM>(x + start, dx + start, vecs, begins ? lie.pad : 0, none, s);
-    if (odd) S::st(dx + lie.odd, s(tail));
+    if (odd) S::st(dx + lie.odd, s(S::ld(&end)));
     if (!a.in_place) shares();
     G::sync();
     if (!none) list_columns<NT, S>(a, row, from, to, s, list, entry);
@@ -861,16 +831,15 @@ int launch_fwd(const Rows<typename S::elem> &a, hipStream_t s) {
   SGH_LAUNCH_CHECK();
   return SGH_OK;
 }
-template <int NT, int U, int PER_SIMD, bool ONE, class S>
+template <int NT, int U, int PER_SIMD, class S>
 int launch_held(Rows<typename S::elem> a, unsigned threads, hipStream_t s) {
-  const size_t at_once = size_t(sgh_num_cus()) * (PER_SIMD * 4 * SGH_WAVE / threads);   // workgroups
   const bool stream = streams(a);
-  const size_t batch = a.batch, most = ONE ? size_t(1) << 20 : batch;   // (a launch has less than 2^32 threads)
+  const size_t batch = a.batch, most = size_t(1) << 20;   // (a launch has less than 2^32 threads)
   for (size_t row = 0; row < batch; row += most) {
     a.batch = batch - row < most ? batch - row : most;
-    const dim3 grid{blocks_for<NT>(a.batch, ONE ? a.batch : at_once)}, block{threads};
-    if (stream) SGH_LAUNCH_TIMED((k_distill_held<NT, U, PER_SIMD, ONE, S, true>), grid, block, lds_for<NT>(a.k), s, a);
-    else SGH_LAUNCH_TIMED((k_distill_held<NT, U, PER_SIMD, ONE, S, false>), grid, block, lds_for<NT>(a.k), s, a);
+    const dim3 grid{blocks_for<NT>(a.batch, a.batch)}, block{threads};
+    if (stream) SGH_LAUNCH_TIMED((k_distill_held<NT, U, PER_SIMD, S, true>), grid, block, lds_for<NT>(a.k), s, a);
+    else SGH_LAUNCH_TIMED((k_distill_held<NT, U, PER_SIMD, S, false>), grid, block, lds_for<NT>(a.k), s, a);
     SGH_LAUNCH_CHECK();
     a.x += a.batch * a.dim, a.dx += a.batch * a.dim, a.loss += a.batch;
     if (a.k) a.top += a.batch * a.k, a.teacher += a.batch * a.k;
@@ -976,12 +945,13 @@ int distill(Rows<typename S::elem> a, size_t k, bool fwd, bool grad, void *works
       // Vectors of a thread.  4, the shortest way through a row, while the wavefronts find room at once (1 row of 20001 bfloat16 values: 8.1 us, with
       // 16 10.9; 1024 rows with 4, 8, 16: 31.8, 25.3, 27.7).  Then 8, while two workgroups fit a CU (4096 rows of 32000: 106 us, with 4 145;
       // 16384 of 5000: 81, 93, with 16 89), or 16.  A wavefront for rows of up to 256 vectors: a workgroup's sum costs a microsecond.
+      // Rows that leave no room for two are read twice, from cache the second time, by workgroups that hold nothing (2048 rows of 70001: 140 us,
+      // in registers 178; of 65001, which do leave room, 126 and 111), unless there are few.
       auto waves = [&](size_t held) { return unsigned((places + SGH_WAVE * held - 1) / (SGH_WAVE * held)); };
-      if (places <= 64 * 4) return launch_held<64, 4, 6, true, S>(a, kBlock, s);
-      if (waves(4) <= 16 && a.batch * waves(4) <= cus * 24) return launch_held<kAny, 4, 6, true, S>(a, waves(4) * SGH_WAVE, s);
-      if (waves(8) <= 10) return launch_held<kAny, 8, 5, true, S>(a, waves(8) * SGH_WAVE, s);
-      if (waves(kHeld) <= 8 || a.batch <= cus) return launch_held<kAny, kHeld, 4, true, S>(a, waves(kHeld) * SGH_WAVE, s);
-      return launch_held<kAny, kHeld, 4, false, S>(a, waves(kHeld) * SGH_WAVE, s);
+      if (places <= 64 * 4) return launch_held<64, 4, 6, S>(a, kBlock, s);
+      if (waves(4) <= 16 && a.batch * waves(4) <= cus * 24) return launch_held<kAny, 4, 6, S>(a, waves(4) * SGH_WAVE, s);
+      if (waves(8) <= 10) return launch_held<kAny, 8, 5, S>(a, waves(8) * SGH_WAVE, s);
+      if (waves(kHeld) <= 8 || a.batch <= cus) return launch_held<kAny, kHeld, 4, S>(a, waves(kHeld) * SGH_WAVE, s);
     }
     return launch_fwd<512, S, true>(a, s);
   }
