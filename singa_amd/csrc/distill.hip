@@ -742,12 +742,10 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
   }
   const Slope s = slope_of(a, q.w, r, soft, q.hard);
   if (a.in_place && NT != SGH_WAVE) G::sync();   // (the list's logits are read)
-  unsigned i = tid;
-  asm("" : "+v"(i));   // (the places are not kept in registers of their own from the loads on)
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     if (u * nt < places) held[u] = slope_vector<S>(s, held[u]);   // (nothing but arithmetic in the branch)
-    to.store<STREAM>(held[u], u == 0 ? first : u * nt + i);
+    to.store<STREAM>(held[u], u == 0 ? first : u * nt + tid);
   }
   if (lie.odd != kNone) S::st(dx + lie.odd, s(S::ld(&end)));
   G::sync();
@@ -943,14 +941,16 @@ int distill(Rows<typename S::elem> a, size_t k, bool fwd, bool grad, void *works
     const size_t places = lines ? vecs : vecs + kLine / 16 - 1;
     if (places <= size_t(kMostThreads) * kHeld) {
       // Vectors of a thread.  4, the shortest way through a row, while the wavefronts find room at once (1 row of 20001 bfloat16 values: 8.1 us, with
-      // 16 10.9; 1024 rows with 4, 8, 16: 31.8, 25.3, 27.7).  Then 8, while two workgroups fit a CU (4096 rows of 32000: 106 us, with 4 145;
-      // 16384 of 5000: 81, 93, with 16 89), or 16.  A wavefront for rows of up to 256 vectors: a workgroup's sum costs a microsecond.
-      // Rows that leave no room for two are read twice, from cache the second time, by workgroups that hold nothing (2048 rows of 70001: 140 us,
-      // in registers 178; of 65001, which do leave room, 126 and 111), unless there are few.
+      // 16 10.9; 1024 rows with 4, 8, 16: 31.8, 25.3, 27.7).  Then 8, 12 or 16, the fewest that leave a SIMD two of the workgroup's wavefronts, so
+      // that two workgroups and more fit a CU (4096 rows of 32000 with 8: 106 us, with 4 145; of 40000 with 8, 12: 161, 145; of 45000 with 12, 16:
+      // 145, 200).  A wavefront for rows of up to 256 vectors: a workgroup's sum costs a microsecond.  Rows that leave no room for two
+      // workgroups are read twice, from cache the second time, by workgroups that hold nothing (2048 rows of 70001: 135 us, in registers 178; of
+      // 65001, which do leave room, 126 and 107), unless there are few.
       auto waves = [&](size_t held) { return unsigned((places + SGH_WAVE * held - 1) / (SGH_WAVE * held)); };
       if (places <= 64 * 4) return launch_held<64, 4, 6, S>(a, kBlock, s);
       if (waves(4) <= 16 && a.batch * waves(4) <= cus * 24) return launch_held<kAny, 4, 6, S>(a, waves(4) * SGH_WAVE, s);
-      if (waves(8) <= 10) return launch_held<kAny, 8, 5, S>(a, waves(8) * SGH_WAVE, s);
+      if (waves(8) <= 8) return launch_held<kAny, 8, 5, S>(a, waves(8) * SGH_WAVE, s);
+      if (waves(12) <= 8) return launch_held<kAny, 12, 5, S>(a, waves(12) * SGH_WAVE, s);
       if (waves(kHeld) <= 8 || a.batch <= cus) return launch_held<kAny, kHeld, 4, S>(a, waves(kHeld) * SGH_WAVE, s);
     }
     return launch_fwd<512, S, true>(a, s);
