@@ -752,9 +752,10 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
   if (soft || q.hard) list_columns<NT, S>(a, row, 0, a.dim, s, list, entry);
 }
 
-// The gradient from the statistics, or from a row's parts, whose loss it stores then; a row may be several workgroups', `each` vectors of it
-template <int NT, class S, bool STREAM>
-__global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_bwd(Rows<typename S::elem> a, unsigned each) {
+// The gradient from the statistics, or (PARTS) from a row's parts, whose loss it stores then; a row may be several workgroups', `each` vectors of it
+// (Registers for 7 wavefronts of a SIMD where teams are small: 16384 rows of 5000 bfloat16 values 98.8 -> 83.1 us.)
+template <int NT, class S, bool STREAM, bool PARTS>
+__global__ __launch_bounds__(Team<NT>::kThreads, NT <= kBlock ? 7 : 4) void k_distill_bwd(Rows<typename S::elem> a, unsigned each) {
   typedef Team<NT> G;
   typedef typename S::elem T;
   extern __shared__ char lds[];
@@ -778,7 +779,7 @@ __global__ __launch_bounds__(Team<NT>::kThreads) void k_distill_bwd(Rows<typenam
     const Row q = row_at(a, row, false);
     Running r;
     bool soft = q.may_soft, hard = q.hard;
-    if (a.per_row) {
+    if constexpr (PARTS) {
       float4 record;
       r = joined(a, row, &record);
       soft = soft && record.x != 0.f;
@@ -858,8 +859,9 @@ template <int NT, class S>
 int launch_bwd(const Rows<typename S::elem> &a, unsigned each, hipStream_t s) {
   const unsigned vecs = unsigned(a.dim / S::VEC), ny = vecs > each ? (vecs + each - 1) / each : 1;
   const dim3 grid{blocks_for<NT>(a.batch, size_t(1) << 20), ny}, block{unsigned(Team<NT>::kThreads)};
-  if (streams(a)) SGH_LAUNCH_TIMED((k_distill_bwd<NT, S, true>), grid, block, lds_for<NT>(a.k), s, a, each);
-  else SGH_LAUNCH_TIMED((k_distill_bwd<NT, S, false>), grid, block, lds_for<NT>(a.k), s, a, each);
+  if (a.per_row) SGH_LAUNCH_TIMED((k_distill_bwd<NT, S, false, true>), grid, block, lds_for<NT>(a.k), s, a, each);   // (past no cache: read again)
+  else if (streams(a)) SGH_LAUNCH_TIMED((k_distill_bwd<NT, S, true, false>), grid, block, lds_for<NT>(a.k), s, a, each);
+  else SGH_LAUNCH_TIMED((k_distill_bwd<NT, S, false, false>), grid, block, lds_for<NT>(a.k), s, a, each);
   SGH_LAUNCH_CHECK();
   return SGH_OK;
 }
