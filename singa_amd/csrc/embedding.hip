@@ -953,7 +953,11 @@ int embed_bwd(const int32_t *ids, const typename S::elem *dy, const typename S::
   a.dy = dy, a.add = add, a.dW = dW, a.ids = ids, a.dim = dim, a.vocab = vocab, a.tokens = unsigned(tokens), a.tile = 1;
   a.scale = scale, a.pad = pad, a.lanes = r.lanes, a.slices = r.slices;
   if (r.epl == 1) return launch_bwd<S, 1, false>(a, p, workspace, s);
-  return bytes >= kStreamBytes ? launch_bwd<S, S::VEC, true>(a, p, workspace, s) : launch_bwd<S, S::VEC, false>(a, p, workspace, s);
+  // The result past the caches where it would push much dy out of the last of them, or is larger than that and of whole lines: those that are stored in
+  // two parts cost more there.  (131 MB, with 33 MB of dy: 36.9 us past, 42.2 through, with 8: 33.8 and 30.7; 262 and 8: 77.5 and 68.7; 410 and
+  // 80: 115 and 130; 525 and 2, rows of 4002 bytes: 136 and 115.)
+  const bool past = bytes >= kStreamBytes && (tokens * dim * e * 12 > bytes || (bytes >= 3 * kStreamBytes && dim * e % 128 == 0));
+  return past ? launch_bwd<S, S::VEC, true>(a, p, workspace, s) : launch_bwd<S, S::VEC, false>(a, p, workspace, s);
 }
 
 }  // namespace
