@@ -191,12 +191,12 @@ def test_embedding_gradient_of_one_row_with_all_tokens(dev):
         assert np.array_equal(dW.to_numpy(), O.embedding_bwd(dy, ids, (4, 12)))
 
 
-@pytest.mark.parametrize("tokens", [1025, 5001, 8192, 9000])
-def test_embedding_gradient_beside_a_large_table(dev, tokens):
-    """Rows without a token of more than 64 MB beside the sort; sums of whole numbers are exact."""
+@pytest.mark.parametrize("tokens,dim", [(1025, 256), (8192, 256), (700, 400), (5001, 400), (9000, 400)])
+def test_embedding_gradient_beside_a_large_table(dev, tokens, dim):
+    """Rows without a token of more than 64 and 96 MB beside the sort; sums of whole numbers are exact."""
     from singa_amd import singa_wrap as singa
     r = np.random.default_rng(8)
-    vocab, dim = 66001, 256
+    vocab = 66001
     ids = np.where(r.random(tokens) < 0.3, r.integers(0, 5, tokens), r.integers(-2, vocab + 2, tokens))
     dy = r.integers(-8, 9, (tokens, dim)).astype(np.float32)
     want = np.zeros((vocab, dim), np.float32)
@@ -208,6 +208,15 @@ def test_embedding_gradient_beside_a_large_table(dev, tokens):
     assert singa.EmbeddingBackwardW(upload(singa, dev, "f32", dy), ints(singa, dev, ids), out, out=out) is out
     assert np.array_equal(out.to_numpy(), want)
     assert singa.IndexErrors(dev) == int((~known & (ids != -1)).sum())
+
+
+@pytest.mark.parametrize("dim", [400, 403])
+def test_embedding_forward_of_more_than_the_caches(dev, dim):
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(9)
+    W, ids = r.standard_normal((900, dim)).astype(np.float32), r.integers(0, 900, 70000)
+    y = singa.EmbeddingForward(ints(singa, dev, ids), upload(singa, dev, "f32", W), scale=0.5)
+    assert np.array_equal(y.to_numpy(), (0.5 * W)[ids])
 
 
 def test_embedding_gradient_of_rows_that_end_with_a_tile(dev):
@@ -430,30 +439,36 @@ def test_distillation_towards_columns_without_a_probability(dev, t, v):
         close(d, want[2], b_dx, "dx")
 
 
-def test_distillation_of_many_long_rows(dev):
-    """More rows than the chip holds, each a workgroup's registers full, and some of them in smaller batches.  (Not the same
-    bits: a row of an odd length begins elsewhere in its 16 bytes there, and a thread's sum has other terms.)"""
+@pytest.mark.parametrize("n,v", [(110000, 500), (2700, 20001), (1300, 45000), (1000, 54000), (900, 66003)])
+def test_distillation_of_more_than_the_caches(dev, n, v):
+    """Logits of more than 96 MB and more rows than the chip holds: some of the rows, by each entry point, and in a smaller batch.  (Not the same bits
+    there: a row of an odd length begins elsewhere in its 16 bytes, and a thread's sum has other terms.)"""
     from singa_amd import singa_wrap as singa
     r = np.random.default_rng(17)
-    n, v, k = 700, 66003, 4
+    k = 4
     x = (r.standard_normal((n, v), dtype=np.float32) * 2).astype(np.float16)
     top, labels = r.integers(0, v, (n, k)), r.integers(-1, v, n)
     teacher = r.standard_normal((n, k)).astype(np.float32)
+    weights = np.where(r.random(n) < 0.3, 0, 1).astype(np.float32)
     how = dict(temperature=2.0, soft=0.7, hard=0.3)
 
-    def both(rows):
-        d_x = upload(singa, dev, "f16", x[rows])
-        loss, dx = singa.DistillationFwdBwd(d_x, ints(singa, dev, top[rows]), singa.from_numpy(teacher[rows], dev), ints(singa, dev, labels[rows]), **how)
-        return loss.to_numpy(), dx.to_numpy()
+    def run(rows):
+        d_x, d_top, d_teacher = upload(singa, dev, "f16", x[rows]), ints(singa, dev, top[rows]), singa.from_numpy(teacher[rows], dev)
+        rest = dict(labels=ints(singa, dev, labels[rows]), weights=singa.from_numpy(weights[rows], dev), **how)
+        loss, stats = singa.DistillationFwd(d_x, d_top, d_teacher, **rest)
+        dx = singa.DistillationBwd(d_x, stats, d_top, d_teacher, **rest)
+        return [t.to_numpy() for t in (loss, dx) + singa.DistillationFwdBwd(d_x, d_top, d_teacher, **rest)]
 
-    loss, dx = both(slice(0, n))
-    for rows in ([0, 1, 255, 256, 257, 511, 512, 640, 699], list(range(3, n, 5))):
-        part_loss, part_dx = both(rows)
-        b = bounds("f16", x[rows].astype(np.float64), top[rows], teacher[rows], labels[rows], None, 1.0, 2.0, 0.7, 0.3)
-        want = O.distill(x[rows].astype(np.float64), top[rows], teacher[rows], labels[rows], None, **how)
-        for l, d in ((loss[rows], dx[rows]), (part_loss, part_dx)):
-            close(l, want[0], b[0], "loss")
-            close(d, want[2], b[2], "dx")
+    whole = run(slice(0, n))
+    rows = np.unique(np.concatenate([[0, 1, 255, 256, 257, 511, 512, n - 2, n - 1], r.integers(0, n, 20)]))
+    part = run(rows)
+    x64 = x[rows].astype(np.float64)
+    want = O.distill(x64, top[rows], teacher[rows], labels[rows], weights[rows], **how)
+    b = bounds("f16", x64, top[rows], teacher[rows], labels[rows], weights[rows], 1.0, 2.0, 0.7, 0.3)
+    for got in ([a[rows] for a in whole], part):
+        for i in (0, 2):
+            close(got[i], want[0], b[0], "loss")
+            close(got[i + 1], want[2], b[2], "dx")
 
 
 def test_distillation_entries_out_of_range_are_left_out_and_counted(dev):

@@ -25,6 +25,13 @@ def test_steps_match_the_oracle(dev, fused, name, batch, steps):
     assert errors[worst] < 1e-3, (worst, errors[worst])
 
 
+def test_step_among_a_half_precision_models_operations(dev):
+    """The operations of a 16-bit tape leave a token model in fp32: the same step."""
+    from singa_amd import singa_wrap as singa
+    res = wl.run_parity_case("token_mlp_small", dev, OracleOps(), hip_ops=wl.HalfHipOps(dev, singa.kFloat16))
+    assert max(res["errors"].values()) < 1e-3
+
+
 def test_fused_and_separate_losses_train_alike(dev):
     """The gradient formed with the loss and the one formed from its statistics are the same formula: parameters after three steps differ by
     roundings alone."""
