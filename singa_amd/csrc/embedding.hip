@@ -222,7 +222,7 @@ constexpr unsigned kScanTokens = 1024;
 
 // Up to kScanTokens tokens, in one launch: a workgroup has a few consecutive rows, looks through all ids for theirs, sorts those in LDS and
 // sums and stores its rows, or slices of them; rows without a token become zero, or `add`.  A launch that waits for another costs more than the
-// ids, which every workgroup reads: 512 tokens, 10007 rows of 201 binary16 elements 8.0 us; 1024 tokens, 131072 rows of 64: 9.0, and 14.3 with
+// ids, which every workgroup reads: 512 tokens, 10007 rows of 201 binary16 elements 7.8 us; 1024 tokens, 131072 rows of 64: 9.1, and 14.2 with
 // 1025 sorted ones.  (32 KB of the result for a workgroup.  Beyond kScanTokens the rows of the commonest ids, which few workgroups have, are what
 // a call waits for.)
 template <class S, int EPL, bool STREAM>
@@ -673,7 +673,7 @@ __device__ __forceinline__ Spot spot_of(const Bwd<T> &a) {
 // of neighbouring tokens that becomes a row of the result or is kept for joining: the tokens of a row that hold no whole tile (they may end
 // in the next one), or a row's piece of a tile.  Then the wavefronts take the jobs in turn, `lanes` lanes and a vector of each to a job.
 // (One wavefront that goes through a tile's tokens with loads of several jobs in flight needs its store once for each of them: the code no
-// longer fits the instruction cache, 6 -> 13 us at 2048 tokens of 64.)  Bound by dy: 65536 tokens of 2048 bfloat16 elements 97 us, 319 MB read and
+// longer fits the instruction cache, 6 -> 13 us at 2048 tokens of 64.)  Bound by dy: 65536 tokens of 2048 bfloat16 elements 91 us, 319 MB read and
 // 84 written; few tokens by five loads one behind the other, 6 to 8 us.
 template <class S, int EPL, bool STREAM, bool STREAM_DY>
 __global__ __launch_bounds__(kBlock) void k_embed_tiles(Bwd<typename S::elem> a) {
