@@ -568,3 +568,32 @@ def test_entry_points_on_the_auxiliary_stream(dev):
     check(lib().sgh_embedding_bwd_f32(ids.ptr, dy.ptr, None, out.ptr, n, vocab, dim, 1.0, -1, ws.ptr, need, aux), "embedding_bwd")
     dev.Join()
     assert np.array_equal(out.to_numpy(), want)
+
+
+def test_two_streams_at_once(dev):
+    """Few long rows (in parts, a workspace each) and a sorted gradient on both streams at the same time."""
+    from singa_amd import singa_wrap as singa
+    from singa_amd._lib import check, lib
+    r = np.random.default_rng(33)
+    n, v, k, tokens, vocab, dim = 5, 60000, 6, 3000, 700, 40
+    L = lib()
+    x = [upload(singa, dev, "f32", r.standard_normal((n, v))) for _ in range(2)]
+    top, teacher = ints(singa, dev, r.integers(0, v, (n, k))), singa.from_numpy(r.standard_normal((n, k)).astype(np.float32), dev)
+    ids = [ints(singa, dev, r.integers(0, vocab, tokens)) for _ in range(2)]
+    dy, table = upload(singa, dev, "f32", r.standard_normal((tokens, dim))), singa.Tensor((vocab, dim), dev)
+    want = [[t.to_numpy() for t in singa.DistillationFwdBwd(x[i], top, teacher, temperature=2.0) + (singa.EmbeddingBackwardW(dy, ids[i], table),)]
+            for i in range(2)]
+    need, sort = L.sgh_distill_workspace_bytes(n, v, 4, 1), L.sgh_embedding_bwd_workspace_bytes(tokens, vocab, dim)
+    assert need and sort
+    out = [[singa.Tensor(s, dev) for s in ((n,), (n, v), (vocab, dim), (need // 4,), (sort // 4,))] for _ in range(2)]
+    aux = dev.Fork()
+    for _ in range(3):
+        for i, stream in enumerate((dev.stream, aux)):
+            loss, dx, dW, ws, ws_sort = out[i]
+            check(L.sgh_distill_fwd_bwd_f32(x[i].ptr, top.ptr, teacher.ptr, None, None, n, v, k, 2.0, 1.0, 0.0, 1.0, loss.ptr, dx.ptr, ws.ptr, need,
+                                            stream), "distill_fwd_bwd")
+            check(L.sgh_embedding_bwd_f32(ids[i].ptr, dy.ptr, None, dW.ptr, tokens, vocab, dim, 1.0, -1, ws_sort.ptr, sort, stream), "embedding_bwd")
+    dev.Join()
+    for i in range(2):
+        for t, w in zip(out[i], want[i]):
+            assert np.array_equal(t.to_numpy(), w)
