@@ -218,13 +218,13 @@ __device__ __forceinline__ unsigned long long same_lanes(unsigned v, bool there)
 // ------------------------------------------------------------------------------------ few tokens
 
 constexpr int kMostRows = 256;           // rows of a workgroup
-constexpr unsigned kScanTokens = 1024;
+constexpr unsigned kScanTokens = 512;
 
 // Up to kScanTokens tokens, in one launch: a workgroup has a few consecutive rows, looks through all ids for theirs, sorts those in LDS and
 // sums and stores its rows, or slices of them; rows without a token become zero, or `add`.  A launch that waits for another costs more than the
-// ids, which every workgroup reads: 512 tokens, 10007 rows of 201 binary16 elements 7.8 us; 1024 tokens, 131072 rows of 64: 9.1, and 14.2 with
-// 1025 sorted ones.  (32 KB of the result for a workgroup.  Beyond kScanTokens the rows of the commonest ids, which few workgroups have, are what
-// a call waits for.)
+// ids, which every workgroup reads: 512 tokens, 10007 rows of 201 binary16 elements 7.8 us; 131072 rows of 64: 8.0, sorted 14.  (32 KB of the result
+// for a workgroup.  Beyond kScanTokens a call waits for the rows of the commonest ids, which few workgroups have: 1024 tokens of text, 32000
+// rows of 512: 29.7 us, sorted 21.4; 512: 17.0 and 19.6; ids that are all one: 112 and 24, 57 and 21.)
 template <class S, int EPL, bool STREAM>
 __global__ __launch_bounds__(kBlock) void k_embed_rows(Bwd<typename S::elem> a, int rows_each) {
   __shared__ unsigned begin[kMostRows], end[kMostRows];

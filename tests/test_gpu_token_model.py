@@ -114,7 +114,7 @@ def test_embedding_ids_outside_the_table_are_zeros_and_counted(dev):
 
 
 # few tokens (looked through), then sorted ones: one pass of digits, two, three; more than one stretch; whole tiles of one row
-BWD = [(0, 5, 3), (1, 1, 1), (3, 5, 3), (7, 5, 4), (9, 300, 7), (5, 3, 8), (64, 100, 16), (500, 1000, 201), (1024, 37, 100), (1000, 700, 513),
+BWD = [(0, 5, 3), (1, 1, 1), (3, 5, 3), (7, 5, 4), (9, 300, 7), (5, 3, 8), (64, 100, 16), (500, 1000, 201), (1024, 37, 100), (1000, 700, 513), (512, 37, 100), (513, 37, 100), (512, 3, 600), (700, 2, 2100),
        (1025, 3, 5), (1500, 300, 33), (3000, 10000, 64), (5000, 600, 129), (4097, 300000, 3), (9000, 77, 520), (20000, 1, 9), (12289, 5000, 40),
        (8192, 900, 20), (8193, 511, 33), (17001, 512, 64), (70000, 3000, 24), (18000, 262144, 2)]
 
@@ -182,7 +182,7 @@ def test_embedding_gradient_of_one_row_with_all_tokens(dev):
     """Whole tiles of one row, their joining, and the ends of the row's tokens."""
     from singa_amd import singa_wrap as singa
     r = np.random.default_rng(5)
-    for tokens, other in ((4096, 0), (4097, 1), (70001, 63)):
+    for tokens, other in ((64, 0), (130, 65), (512, 0), (513, 0), (1000, 400), (4096, 0), (4097, 1), (70001, 63)):
         ids = np.full(tokens, 2)
         ids[:other] = 0
         dy = r.integers(-8, 9, (tokens, 12)).astype(np.float32)   # (sums of whole numbers: exact in any order)

@@ -199,7 +199,7 @@ for t, v, d in ((5, most, 4), (most, 9, 4), (9000, 7, 1 << 21), (17000, 7, 1 << 
     need = lib.sgh_embedding_bwd_workspace_bytes(t, v, d)
     largest.append(lib.sgh_embedding_bwd_f32(S2, 2 * S2, None, 3 * S2, t, v, d, 1.0, -1, 4 * S2, need, None))
 launched()
-answer([run(1024, 5000, 64), run(8192, 5000, 64), run(8193, 131071, 64), run(8193, 1 << 18, 64), largest])
+answer([run(512, 5000, 64), run(8192, 5000, 64), run(8193, 131071, 64), run(8193, 1 << 18, 64), largest])
 """)
     assert few[:2] == [0, 0] and [k[:11] for k in few[2]] == ["k_embed_row"], few
     assert one[0] == 0 and one[1] > 0 and [k[:11] for k in one[2]] == ["k_embed_ran", "k_embed_til", "k_embed_joi"], one
