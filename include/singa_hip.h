@@ -197,7 +197,7 @@ SGH_API int sgh_softmax_ce_bwd_f16(const uint16_t *p, const int32_t *t, uint16_t
                                    size_t dim, int int_target, float scale, void *stream);
 SGH_API int sgh_softmax_ce_bwd_bf16(const uint16_t *p, const int32_t *t, uint16_t *grad, size_t batch,
                                     size_t dim, int int_target, float scale, void *stream);
-/* Number of out-of-range labels seen since the last call (synchronises the stream). */
+/* Number of out-of-range labels seen since the last call (synchronises the stream; other streams as for sgh_embedding_index_errors). */
 SGH_API int sgh_softmax_ce_label_errors(void *stream, int *count);
 /* SoftMax<float, Lang> (rows) and ComputeCrossEntropy<float, Lang>: forward helpers,
  * tensor_math_cpp.h:361-379, :1058-1088; CUDA tensor_math_cuda.h:1274-1339. */
@@ -783,7 +783,8 @@ SGH_API int sgh_embedding_bwd_f16(const int32_t *ids, const uint16_t *dy, const 
 SGH_API int sgh_embedding_bwd_bf16(const int32_t *ids, const uint16_t *dy, const uint16_t *add, uint16_t *dW, size_t tokens,
                                    size_t vocab, size_t dim, float scale, int padding_idx, void *workspace,
                                    size_t ws_bytes, void *stream);
-/* Number of ids outside the table that were not padding, in both directions, since the last call (synchronises the stream). */
+/* Number of ids outside the table that were not padding, in both directions, since the last call (synchronises the stream).  What
+ * operators on other streams add is in this count or the next one's: join those streams for a count of all. */
 SGH_API int sgh_embedding_index_errors(void *stream, int *count);
 
 /* Distillation from a teacher's top logits, beside or instead of labels.  Row n of x [batch, dim] are the student's logits;
@@ -838,7 +839,8 @@ SGH_API int sgh_distill_fwd_bwd_bf16(const uint16_t *x, const int32_t *top, cons
                                    const float *weights, size_t batch, size_t dim, size_t k, float temperature,
                                    float soft, float hard, float scale, float *loss, uint16_t *dx, void *workspace,
                                    size_t ws_bytes, void *stream);
-/* Number of list entries and labels outside the columns that the forward pass has met since the last call (synchronises the stream). */
+/* Number of list entries and labels outside the columns that the forward pass has met since the last call (synchronises the stream; other
+ * streams as for sgh_embedding_index_errors). */
 SGH_API int sgh_distill_index_errors(void *stream, int *count);
 
 #ifdef __cplusplus

@@ -56,6 +56,10 @@ int sgh_bn_noalloc_setup();
 int sgh_bn_take_exchange_failures(int *count);
 void sgh_bn_mark_exchange_ran();
 
+// Reads a counter in device memory that kernels on any stream add to, and takes off what was read, both on `s` behind its work: what another
+// stream adds meanwhile is left for the next call (runtime.hip).  Waits for `s`.
+int sgh_take_count(int *counter, hipStream_t s, int *count);
+
 // Weight epoch: a host-side counter that every entry point which may change a weight tensor advances
 // (optimizer updates, Axpy, fills, casts, copies to the device, sgh_conv_weights_changed).  The note that
 // sgh_conv_dgrad_prepare_multi leaves in a geometry is honoured only within the epoch it was written in.

@@ -1016,13 +1016,9 @@ size_t sgh_distill_workspace_bytes(size_t batch, size_t dim, size_t elem_bytes, 
 
 int sgh_distill_index_errors(void *stream, int *count) {
   if (!count) return SGH_EINVAL;
-  SGH_HIP_TRY(hipStreamSynchronize(sgh_stream_of(stream)));
-  int v = 0;
-  SGH_HIP_TRY(hipMemcpyFromSymbol(&v, HIP_SYMBOL(g_list_errors), sizeof(int), 0, hipMemcpyDeviceToHost));
-  const int zero = 0;
-  SGH_HIP_TRY(hipMemcpyToSymbol(HIP_SYMBOL(g_list_errors), &zero, sizeof(int), 0, hipMemcpyHostToDevice));
-  *count = v;
-  return SGH_OK;
+  void *counter;
+  SGH_HIP_TRY(hipGetSymbolAddress(&counter, HIP_SYMBOL(g_list_errors)));
+  return sgh_take_count(static_cast<int *>(counter), sgh_stream_of(stream), count);
 }
 
 }  // extern "C"

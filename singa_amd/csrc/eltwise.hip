@@ -719,13 +719,9 @@ int sgh_softmax_ce_bwd_bf16(const uint16_t *p, const int32_t *t, uint16_t *grad,
 
 int sgh_softmax_ce_label_errors(void *stream, int *count) {
   if (!count) return SGH_EINVAL;
-  SGH_HIP_TRY(hipStreamSynchronize(sgh_stream_of(stream)));
-  int v = 0;
-  SGH_HIP_TRY(hipMemcpyFromSymbol(&v, HIP_SYMBOL(g_label_errors), sizeof(int), 0, hipMemcpyDeviceToHost));
-  const int zero = 0;
-  SGH_HIP_TRY(hipMemcpyToSymbol(HIP_SYMBOL(g_label_errors), &zero, sizeof(int), 0, hipMemcpyHostToDevice));
-  *count = v;
-  return SGH_OK;
+  void *counter;
+  SGH_HIP_TRY(hipGetSymbolAddress(&counter, HIP_SYMBOL(g_label_errors)));
+  return sgh_take_count(static_cast<int *>(counter), sgh_stream_of(stream), count);
 }
 
 int sgh_softmax_fwd_f32(const float *x, float *p, size_t batch, size_t dim, void *stream) {

@@ -990,13 +990,9 @@ size_t sgh_embedding_bwd_workspace_bytes(size_t tokens, size_t vocab, size_t dim
 
 int sgh_embedding_index_errors(void *stream, int *count) {
   if (!count) return SGH_EINVAL;
-  SGH_HIP_TRY(hipStreamSynchronize(sgh_stream_of(stream)));
-  int v = 0;
-  SGH_HIP_TRY(hipMemcpyFromSymbol(&v, HIP_SYMBOL(g_index_errors), sizeof(int), 0, hipMemcpyDeviceToHost));
-  const int zero = 0;
-  SGH_HIP_TRY(hipMemcpyToSymbol(HIP_SYMBOL(g_index_errors), &zero, sizeof(int), 0, hipMemcpyHostToDevice));
-  *count = v;
-  return SGH_OK;
+  void *counter;
+  SGH_HIP_TRY(hipGetSymbolAddress(&counter, HIP_SYMBOL(g_index_errors)));
+  return sgh_take_count(static_cast<int *>(counter), sgh_stream_of(stream), count);
 }
 
 }  // extern "C"

@@ -73,6 +73,26 @@ struct sgh_event {
 
 static int g_num_cus = 0;
 
+namespace {
+__global__ void k_subtract(int *counter, int v) { atomicSub(counter, v); }
+std::mutex g_take_mu;   // (two callers that read before either has taken off would both count the same)
+}  // namespace
+
+int sgh_take_count(int *counter, hipStream_t s, int *count) {
+  SGH_HIP_TRY(hipStreamSynchronize(s));
+  std::lock_guard<std::mutex> lk(g_take_mu);
+  int v = 0;
+  SGH_HIP_TRY(hipMemcpyAsync(&v, counter, sizeof(int), hipMemcpyDeviceToHost, s));
+  SGH_HIP_TRY(hipStreamSynchronize(s));
+  if (v != 0) {
+    hipLaunchKernelGGL(k_subtract, dim3(1), dim3(1), 0, s, counter, v);
+    SGH_LAUNCH_CHECK();
+    SGH_HIP_TRY(hipStreamSynchronize(s));
+  }
+  *count = v;
+  return SGH_OK;
+}
+
 int sgh_num_cus() {
   if (g_num_cus > 0) return g_num_cus;
   int dev = 0, n = 0;

@@ -829,7 +829,8 @@ def EmbeddingBackwardW(dy, ids, W, scale=1.0, padding_idx=-1, add=None, out=None
 
 def IndexErrors(device):
     """How many ids, list entries and labels outside their range ``EmbeddingForward``, ``EmbeddingBackwardW`` and the distillation's
-    forward pass have met since the last call."""
+    forward pass have met since the last call.  Waits for the device's stream; what operators on its auxiliary stream meet is in
+    this count or the next one's (``Join`` first for a count of all)."""
     total = 0
     for name in ("sgh_embedding_index_errors", "sgh_distill_index_errors"):
         n = C.c_int()

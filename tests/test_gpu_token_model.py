@@ -597,3 +597,25 @@ def test_two_streams_at_once(dev):
     for i in range(2):
         for t, w in zip(out[i], want[i]):
             assert np.array_equal(t.to_numpy(), w)
+
+
+def test_index_errors_of_two_streams(dev):
+    """Counted on the auxiliary stream while the main one reads the count: each once."""
+    from singa_amd import singa_wrap as singa
+    from singa_amd._lib import check, lib
+    L, tokens, vocab, dim, calls = lib(), 200, 50, 40, 400
+    ids, table = ints(singa, dev, np.where(np.arange(tokens) % 4 == 0, vocab + 1, 3)), upload(singa, dev, "f32", np.ones((vocab, dim)))
+    x, top = upload(singa, dev, "f32", np.zeros((3, vocab))), ints(singa, dev, np.full((3, 2), -5))
+    y, loss, stats = (singa.Tensor(s, dev) for s in ((tokens, dim), (3,), (3, 3)))
+    teacher = singa.from_numpy(np.zeros((3, 2), np.float32), dev)
+    dev.Sync()
+    singa.IndexErrors(dev)
+    aux, met = dev.Fork(), 0
+    for i in range(calls):
+        check(L.sgh_embedding_fwd_f32(ids.ptr, table.ptr, y.ptr, tokens, vocab, dim, 1.0, -1, aux), "embedding_fwd")
+        check(L.sgh_distill_fwd_f32(x.ptr, top.ptr, teacher.ptr, None, None, 3, vocab, 2, 1.0, 1.0, 0.0, loss.ptr, stats.ptr, None, 0, aux), "distill_fwd")
+        if i % 5 == 4:
+            met += singa.IndexErrors(dev)
+    dev.Join()
+    assert met + singa.IndexErrors(dev) == calls * (tokens // 4 + 6)
+    assert singa.IndexErrors(dev) == 0

@@ -228,3 +228,44 @@ answer(out)
         if rcs[3] == 2048:   # (2^31 rows of one: 2^20 of them a launch)
             rcs[3] = 1
         assert (need > 0) == parts and rcs == ([0, 2, 0, 2, 0, 1] if parts else [0, 1, 0, 1, 0, 1]), got
+
+
+# ------------------------------------------------------------------------------------ counts of what is out of range
+
+# A counter in memory, to which an operator on another stream adds 2 right behind each time that it is read
+COUNTER = r"""
+static int counter = 3;
+extern "C" {
+int hipStreamSynchronize(void *) { return 0; }
+int hipGetSymbolAddress(void **p, const void *) { *p = &counter; return 0; }
+static int copy(void *to, const void *from, size_t n) { memcpy(to, from, n); if (from == &counter) counter += 2; return 0; }
+int hipMemcpyAsync(void *to, const void *from, size_t n, int, void *) { return copy(to, from, n); }
+int hipMemcpy(void *to, const void *from, size_t n, int) { return copy(to, from, n); }
+int hipMemcpyFromSymbol(void *to, const void *, size_t n, size_t, int) { return copy(to, &counter, n); }
+int hipMemcpyToSymbol(const void *, const void *from, size_t n, size_t, int) { return copy(&counter, from, n); }
+int recorder_left() { return counter; }
+}
+// the one kernel that is run here: (counter, what is taken off)
+static int subtracting(const void *f, void **args) {
+  if (names()[f].find("k_subtract") != std::string::npos) **static_cast<int **>(args[0]) -= *static_cast<int *>(args[1]);
+  return 0;
+}
+"""
+
+
+@pytest.mark.parametrize("entry", ["sgh_embedding_index_errors", "sgh_distill_index_errors", "sgh_softmax_ce_label_errors"])
+def test_index_errors_met_while_they_are_read_are_counted_next_time(monkeypatch, entry):
+    import hip_recorder
+    launch = "int hipLaunchKernel(const void *f, Dim g, Dim b, void **, size_t, void *) { return launch(f, g, b); }"
+    assert launch in hip_recorder.SOURCE
+    source = hip_recorder.SOURCE.replace(launch, launch.replace("void **,", "void **args,").replace("{ ", "{ subtracting(f, args); "))
+    monkeypatch.setattr(hip_recorder, "SOURCE", source.replace('extern "C" {', COUNTER + 'extern "C" {', 1))
+    got = recorded("""
+n = C.c_int()
+out = []
+for _ in range(3):
+    assert lib.%s(None, C.byref(n)) == 0
+    out.append(n.value)
+answer([out, recorder.recorder_left(), lib.%s(None, None)])
+""" % (entry, entry))
+    assert got == [[3, 2, 2], 2, EINVAL]   # nothing is lost, nothing counted twice
