@@ -239,6 +239,67 @@ def test_embedding_gradient_of_rows_that_end_with_a_tile(dev):
             assert np.array_equal(dW.to_numpy(), O.embedding_bwd(dy, ids, (vocab, dim)))
 
 
+@pytest.mark.parametrize("t,tokens,dim", [("f16", 70000, 800), ("bf16", 70000, 807), ("f32", 8400001, 3)])
+def test_embedding_forward_past_the_caches(dev, t, tokens, dim):
+    """16-bit results of more than 96 MB, and rows of less than a vector."""
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(10)
+    W = r.integers(-100, 101, (900, dim)).astype(np.float32)   # (whole numbers of at most 8 bits: every type holds them and their halves)
+    ids = r.integers(-1, 900, tokens)
+    y = singa.EmbeddingForward(ints(singa, dev, ids), upload(singa, dev, t, W), scale=0.5).to_numpy()
+    want = np.concatenate([0.5 * W, np.zeros((1, dim), np.float32)])
+    for at in range(0, tokens, 1 << 20):
+        assert np.array_equal(y[at:at + (1 << 20)], want[ids[at:at + (1 << 20)]])
+
+
+def whole_gradient(singa, dev, t, r, tokens, vocab, dim, ids, add=False):
+    """Whole numbers of at most 3 bits: their sums are exact in fp32 in any order, the result one rounding of these."""
+    dy = r.integers(-4, 5, (tokens, dim), dtype=np.int8).astype(np.float32)
+    want = r.integers(-4, 5, (vocab, dim), dtype=np.int8).astype(np.float32) if add else np.zeros((vocab, dim), np.float32)
+    W = upload(singa, dev, t, want) if add else singa.Tensor((vocab, dim), dev, kind(singa, t))
+    known = (ids >= 0) & (ids < vocab)
+    order = np.argsort(ids[known], kind="stable")
+    rows, first = np.unique(ids[known][order], return_index=True)
+    want[rows] += np.add.reduceat(dy[known][order], first, axis=0)
+    singa.IndexErrors(dev)
+    got = singa.EmbeddingBackwardW(upload(singa, dev, t, dy), ints(singa, dev, ids), W, add=W if add else None)
+    assert np.array_equal(got.to_numpy().astype(np.float64), stored(t, want))
+    assert singa.IndexErrors(dev) == int((~known & (ids != -1)).sum())
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("tokens,vocab,dim", [(300, 300000, 8), (300, 300001, 16), (512, 140000, 3), (411, 262144, 1), (77, 600000, 5)])
+def test_embedding_gradient_of_few_tokens_in_a_long_table(dev, t, tokens, vocab, dim):
+    """Several groups of rows to a workgroup, tokens in more than one of them, more rows than a wavefront has lanes."""
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(41)
+    near = r.integers(0, 300, tokens) + 1000 * r.integers(0, 3, tokens)        # (many in the same workgroups, some more than once)
+    ids = np.where(r.random(tokens) < 0.7, near, r.integers(-3, vocab + 3, tokens))
+    for add in (False, True):
+        whole_gradient(singa, dev, t, r, tokens, vocab, dim, ids, add)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("tokens,vocab,dim", [(140000, 77, 8), (140001, 5000, 3), (270000, 5000, 7), (270001, 77, 4), (270000, 300000, 2)])
+def test_embedding_gradient_of_long_stretches(dev, t, tokens, vocab, dim):
+    """More tokens than 64 workgroups hold at once: each goes through its own in several turns."""
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(42)
+    ids = np.where(r.random(tokens) < 0.1, r.integers(0, 3, tokens), r.integers(-2, vocab + 2, tokens))
+    whole_gradient(singa, dev, t, r, tokens, vocab, dim, ids)
+
+
+# (fp32; 16 bits: dim is twice as long) of more than 96 MB: dy alone, in jobs of eight and of four; dy and the result; the result alone, and with few tokens
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("tokens,vocab,dim", [(97001, 3000, 260), (9601, 700, 2653), (9001, 12001, 2800), (7000, 70001, 400), (400, 72001, 1056)])
+def test_embedding_gradient_past_the_caches(dev, t, tokens, vocab, dim):
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(43)
+    dim *= 1 if t == "f32" else 2
+    ids = np.where(r.random(tokens) < 0.2, r.integers(0, 5, tokens), r.integers(-2, vocab + 2, tokens))
+    whole_gradient(singa, dev, t, r, tokens, vocab, dim, ids, add=tokens == 9601)
+
+
 # ------------------------------------------------------------------------------------ distillation
 
 def make_case(r, t, n, v, k, masked=True):
@@ -469,6 +530,40 @@ def test_distillation_of_more_than_the_caches(dev, n, v):
         for i in (0, 2):
             close(got[i], want[0], b[0], "loss")
             close(got[i + 1], want[2], b[2], "dx")
+
+
+# (fp32; 16 bits: twice the columns) a wavefront to a row, few and many vectors of a thread held, and rows that are read twice; of more than 96 MB and of less
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("n,v", [(110000, 240), (2700, 10001), (1700, 15001), (1100, 24001), (900, 30001), (700, 40003),
+                                 (1000, 15001), (600, 24001), (500, 30001), (300, 70001)])
+def test_distillation_of_many_long_rows(dev, t, n, v):
+    """Each way to share the rows out, in each type: some of the rows, by each entry point, in place too."""
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(19)
+    k, v = 4, v * (1 if t == "f32" else 2)
+    x = np.resize((r.standard_normal(1000003, dtype=np.float32) * 2).astype(np.float16), (n, v))
+    if t == "bf16":   # values that the type holds
+        x = (x.view(np.uint16) & 0xfff8).view(np.float16)
+    top, labels = r.integers(0, v, (n, k)), r.integers(-1, v, n)
+    teacher = r.standard_normal((n, k)).astype(np.float32)
+    weights = np.where(r.random(n) < 0.3, 0, 1).astype(np.float32)
+    how = dict(temperature=2.0, soft=0.7, hard=0.3)
+    d_x, d_top, d_teacher = upload(singa, dev, t, x), ints(singa, dev, top), singa.from_numpy(teacher, dev)
+    rest = dict(labels=ints(singa, dev, labels), weights=singa.from_numpy(weights, dev), **how)
+    loss, stats = singa.DistillationFwd(d_x, d_top, d_teacher, **rest)
+    got = [a.to_numpy() for a in (loss, singa.DistillationBwd(d_x, stats, d_top, d_teacher, **rest)) + singa.DistillationFwdBwd(d_x, d_top, d_teacher, **rest)]
+    in_place = singa.DistillationFwdBwd(d_x, d_top, d_teacher, out=d_x, **rest)
+    for a, b in zip(in_place, got[2:]):
+        assert np.array_equal(a.to_numpy(), b)
+    none = (weights == 0)
+    assert not got[0][none].any() and not got[1][none].any() and not got[3][none].any()
+    rows = np.unique(np.concatenate([[0, 1, 255, 256, 257, 299, n - 2, n - 1], r.integers(0, n, 12)]))
+    x64 = x[rows].astype(np.float64)
+    want = O.distill(x64, top[rows], teacher[rows], labels[rows], weights[rows], **how)
+    b = bounds(t, x64, top[rows], teacher[rows], labels[rows], weights[rows], 1.0, 2.0, 0.7, 0.3)
+    for i in (0, 2):
+        close(got[i][rows], want[0], b[0], "loss")
+        close(got[i + 1][rows], want[2], b[2], "dx")
 
 
 def test_distillation_entries_out_of_range_are_left_out_and_counted(dev):
