@@ -833,10 +833,11 @@ int launch_fwd(const Rows<typename S::elem> &a, hipStream_t s) {
   SGH_LAUNCH_CHECK();
   return SGH_OK;
 }
+constexpr size_t kRowsOfLaunch = size_t(1) << 20;   // (a launch has less than 2^32 threads)
 template <int NT, int U, int PER_SIMD, class S>
 int launch_held(Rows<typename S::elem> a, unsigned threads, hipStream_t s) {
   const bool stream = streams(a);
-  const size_t batch = a.batch, most = size_t(1) << 20;   // (a launch has less than 2^32 threads)
+  const size_t batch = a.batch, most = kRowsOfLaunch;
   for (size_t row = 0; row < batch; row += most) {
     a.batch = batch - row < most ? batch - row : most;
     const dim3 grid{blocks_for<NT>(a.batch, a.batch)}, block{threads};
@@ -944,6 +945,7 @@ int distill(Rows<typename S::elem> a, size_t k, bool fwd, bool grad, void *works
     // places of a row's vectors
     const bool lines = (reinterpret_cast<uintptr_t>(a.x) | a.dim * sizeof(typename S::elem)) % kLine == 0;
     const size_t places = lines ? vecs : vecs + kLine / 16 - 1;
+    if (a.batch > kRowsOfLaunch) prof.span();
     if (places <= size_t(kMostThreads) * kHeld) {
       // Vectors of a thread.  4, the shortest way through a row, while the wavefronts find room at once (1 row of 20001 bfloat16 values: 8.1 us, with
       // 16 10.9; 1024 rows with 4, 8, 16: 31.8, 25.3, 27.7).  Then 8, 12 or 16, the fewest that leave a SIMD two of the workgroup's wavefronts, so

@@ -566,6 +566,49 @@ def test_distillation_of_many_long_rows(dev, t, n, v):
         close(got[i + 1][rows], want[2], b[2], "dx")
 
 
+def record_of(dev, call):
+    """Milliseconds of the one profiling record that `call` leaves."""
+    import ctypes as C
+    from singa_amd._lib import check, lib
+    L, n, buf, ms, work = lib(), C.c_int(), C.create_string_buffer(64), C.c_float(), C.c_double()
+    dev.Sync()
+    check(L.sgh_prof_enable(1), "sgh_prof_enable")
+    try:
+        call()
+        dev.Sync()
+        check(L.sgh_prof_count(C.byref(n)), "sgh_prof_count")
+        assert n.value == 1
+        check(L.sgh_prof_get(0, buf, 64, C.byref(ms), C.byref(work)), "sgh_prof_get")
+    finally:
+        L.sgh_prof_enable(0)
+        L.sgh_prof_clear()
+    return ms.value
+
+
+def test_distillation_of_more_rows_than_a_launch_takes(dev):
+    """Both in one call for 3 * 2^20 rows and some: rows on both sides of every launch, and one profiling record around all of them."""
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(23)
+    one, n, v, k = 1 << 20, (3 << 20) + 5, 20, 2
+    x = np.resize(r.standard_normal(1000003, dtype=np.float32), (n, v))
+    top, labels, weights = r.integers(0, v, (n, k)), r.integers(-1, v, n), (r.random(n) < 0.8).astype(np.float32)
+    teacher = np.resize(r.standard_normal(999983, dtype=np.float32), (n, k))
+    how = dict(temperature=2.0, soft=0.7, hard=0.3)
+    d = [upload(singa, dev, "f32", x), ints(singa, dev, top), singa.from_numpy(teacher, dev), ints(singa, dev, labels), singa.from_numpy(weights, dev)]
+    part = [upload(singa, dev, "f32", x[:one]), ints(singa, dev, top[:one]), singa.from_numpy(teacher[:one], dev), ints(singa, dev, labels[:one]),
+            singa.from_numpy(weights[:one], dev)]
+    loss, dx = (a.to_numpy() for a in singa.DistillationFwdBwd(*d, **how))
+    singa.DistillationFwdBwd(*part, **how)
+    rows = np.unique(np.concatenate([[0, n - 1], *[[i * one - 1, i * one, i * one + 1] for i in (1, 2, 3)], r.integers(0, n, 30)]))
+    x64 = x[rows].astype(np.float64)
+    want = O.distill(x64, top[rows], teacher[rows], labels[rows], weights[rows], **how)
+    b = bounds("f32", x64, top[rows], teacher[rows], labels[rows], weights[rows], 1.0, 2.0, 0.7, 0.3)
+    close(loss[rows], want[0], b[0], "loss")
+    close(dx[rows], want[2], b[2], "dx")
+    times = [record_of(dev, lambda: singa.DistillationFwdBwd(*a, **how)) for a in (part, d)]
+    assert times[1] > 2 * times[0], times   # (three times the rows and more)
+
+
 def test_distillation_entries_out_of_range_are_left_out_and_counted(dev):
     from singa_amd import singa_wrap as singa
     r = np.random.default_rng(9)
