@@ -756,9 +756,9 @@ __global__ __launch_bounds__(Team<NT>::kThreads, PER_SIMD) void k_distill_held(R
 
 // The gradient from the statistics, or (PARTS) from a row's parts, whose loss it stores then; a row may be several workgroups', `each` vectors of it
 // Bound by memory: 8192 rows of 65536 bfloat16 values 364 us, 5.7 TB/s.  (Registers for 7 wavefronts of a SIMD where teams are small: 16384 rows of
-// 5000 bfloat16 values 98.8 -> 83.1 us.)
+// 5000 bfloat16 values 98.8 -> 83.1 us.  Rows in parts are few: no such limit, which the joining would not fit.)
 template <int NT, class S, bool STREAM, bool PARTS>
-__global__ __launch_bounds__(Team<NT>::kThreads, NT <= kBlock ? 7 : 4) void k_distill_bwd(Rows<typename S::elem> a, unsigned each) {
+__global__ __launch_bounds__(Team<NT>::kThreads, NT <= kBlock && !PARTS ? 7 : 4) void k_distill_bwd(Rows<typename S::elem> a, unsigned each) {
   typedef Team<NT> G;
   typedef typename S::elem T;
   extern __shared__ char lds[];
