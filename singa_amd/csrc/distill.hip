@@ -828,7 +828,8 @@ bool streams(const Rows<T> &a) { return a.batch * a.dim * sizeof(T) >= kStreamBy
 template <int NT, class S, bool GRAD>
 int launch_fwd(const Rows<typename S::elem> &a, hipStream_t s) {
   const dim3 grid{blocks_for<NT>(a.batch, size_t(1) << 20)}, block{unsigned(Team<NT>::kThreads)};
-  if (streams(a)) SGH_LAUNCH_TIMED((k_distill_fwd<NT, S, GRAD, true>), grid, block, lds_for<NT>(a.k), s, a);
+  constexpr bool small = NT == 512 && !GRAD;   // (the loss: at most half as many rows as CUs, of 40000 columns)
+  if (!small && streams(a)) SGH_LAUNCH_TIMED((k_distill_fwd<NT, S, GRAD, !small>), grid, block, lds_for<NT>(a.k), s, a);
   else SGH_LAUNCH_TIMED((k_distill_fwd<NT, S, GRAD, false>), grid, block, lds_for<NT>(a.k), s, a);
   SGH_LAUNCH_CHECK();
   return SGH_OK;
@@ -836,12 +837,13 @@ int launch_fwd(const Rows<typename S::elem> &a, hipStream_t s) {
 constexpr size_t kRowsOfLaunch = size_t(1) << 20;   // (a launch has less than 2^32 threads)
 template <int NT, int U, int PER_SIMD, class S>
 int launch_held(Rows<typename S::elem> a, unsigned threads, hipStream_t s) {
-  const bool stream = streams(a);
+  constexpr bool small = NT == kAny && U == 4;   // (at most 24 wavefronts' rows for each CU, 4 KB a wavefront)
+  const bool stream = !small && streams(a);
   const size_t batch = a.batch, most = kRowsOfLaunch;
   for (size_t row = 0; row < batch; row += most) {
     a.batch = batch - row < most ? batch - row : most;
     const dim3 grid{blocks_for<NT>(a.batch, a.batch)}, block{threads};
-    if (stream) SGH_LAUNCH_TIMED((k_distill_held<NT, U, PER_SIMD, S, true>), grid, block, lds_for<NT>(a.k), s, a);
+    if (stream) SGH_LAUNCH_TIMED((k_distill_held<NT, U, PER_SIMD, S, !small>), grid, block, lds_for<NT>(a.k), s, a);
     else SGH_LAUNCH_TIMED((k_distill_held<NT, U, PER_SIMD, S, false>), grid, block, lds_for<NT>(a.k), s, a);
     SGH_LAUNCH_CHECK();
     a.x += a.batch * a.dim, a.dx += a.batch * a.dim, a.loss += a.batch;
@@ -863,7 +865,8 @@ template <int NT, class S>
 int launch_bwd(const Rows<typename S::elem> &a, unsigned each, hipStream_t s) {
   const unsigned vecs = unsigned(a.dim / S::VEC), ny = vecs > each ? (vecs + each - 1) / each : 1;
   const dim3 grid{blocks_for<NT>(a.batch, size_t(1) << 20), ny}, block{unsigned(Team<NT>::kThreads)};
-  if (a.per_row) SGH_LAUNCH_TIMED((k_distill_bwd<NT, S, false, true>), grid, block, lds_for<NT>(a.k), s, a, each);   // (past no cache: read again)
+  constexpr bool parts = NT != SGH_WAVE;   // (rows in parts are long)
+  if (parts && a.per_row) SGH_LAUNCH_TIMED((k_distill_bwd<NT, S, false, parts>), grid, block, lds_for<NT>(a.k), s, a, each);   // (past no cache: read again)
   else if (streams(a)) SGH_LAUNCH_TIMED((k_distill_bwd<NT, S, true, false>), grid, block, lds_for<NT>(a.k), s, a, each);
   else SGH_LAUNCH_TIMED((k_distill_bwd<NT, S, false, false>), grid, block, lds_for<NT>(a.k), s, a, each);
   SGH_LAUNCH_CHECK();

@@ -269,3 +269,44 @@ for _ in range(3):
 answer([out, recorder.recorder_left(), lib.%s(None, None)])
 """ % (entry, entry))
     assert got == [[3, 2, 2], 2, EINVAL]   # nothing is lost, nothing counted twice
+
+
+# ------------------------------------------------------------------------------------ kernels
+
+def test_every_kernel_of_the_token_model_is_reached(monkeypatch):
+    """Each form that is built is what some call launches (256 compute units)."""
+    import hip_recorder
+    monkeypatch.setattr(hip_recorder, "SOURCE", hip_recorder.SOURCE + r"""
+extern "C" const char *recorder_built() {
+  static std::string out;
+  for (auto &n : names()) out += n.second + "\n";
+  return out.c_str();
+}
+""")
+    built, run = recorded("""
+S, out = 1 << 50, set()
+def note():
+    out.update(n for n, _, _ in launched())
+for sfx, e in (("f32", 4), ("f16", 2), ("bf16", 2)):
+    for n in (1, 16, 100, 200, 400, 1000, 3000, 20000, 300000):
+        for v in (2, 200, 1000, 3000, 7000, 15000, 20000, 30000, 40000, 60000, 120000, 300000):
+            for sizes in ((n, v, 0), (n, v, 100)):
+                need = [lib.sgh_distill_workspace_bytes(n, v, e, g) for g in (0, 1)]
+                a = (S, 2 * S, 3 * S, 4 * S, 5 * S) + sizes + (1.5, 1.0, 1.0)
+                assert getattr(lib, "sgh_distill_fwd_" + sfx)(*a, 6 * S, 7 * S, 9 * S, need[0], None) == 0
+                assert getattr(lib, "sgh_distill_fwd_bwd_" + sfx)(*a, 1.0, 6 * S, 8 * S, 9 * S, need[1], None) == 0
+                assert getattr(lib, "sgh_distill_bwd_" + sfx)(S, 7 * S, *a[1:], 1.0, 8 * S, None) == 0
+            note()
+    for t in (1, 300, 3000, 8193, 100000, 40000000):
+        for v, d in ((1000, 1), (1000, 100), (40000, 3), (40000, 1024), (300000, 100), (300000, 8), (300000, 1024), (1000, 8192)):
+            need = lib.sgh_embedding_bwd_workspace_bytes(t, v, d)
+            assert getattr(lib, "sgh_embedding_fwd_" + sfx)(S, 2 * S, 3 * S, t, v, d, 1.0, -1, None) == 0
+            assert getattr(lib, "sgh_embedding_bwd_" + sfx)(S, 2 * S, None, 3 * S, t, v, d, 1.0, -1, 4 * S, need, None) == 0
+        note()
+recorder.recorder_built.restype = C.c_char_p
+answer([recorder.recorder_built().decode().split(), sorted(out)])
+""")
+    ours = {n for n in built if "k_embed_" in n or "k_distill_" in n}
+    assert len(ours) > 100 and set(run) <= ours
+    left = sorted(ours - set(run))
+    assert not left, "\n" + "\n".join(left)
