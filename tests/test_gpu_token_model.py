@@ -300,6 +300,57 @@ def test_embedding_gradient_past_the_caches(dev, t, tokens, vocab, dim):
     whole_gradient(singa, dev, t, r, tokens, vocab, dim, ids, add=tokens == 9601)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("tokens", [300, 3000, 20000])   # (looked through, counted, sorted in passes)
+def test_embedding_of_nan_and_infinities_where_nothing_reads(dev, t, tokens):
+    """Rows of the table that are padding or that no id names, and gradients of tokens that take part in nothing."""
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(44)
+    vocab, dim, pad = 700, 24, 5
+    ids = r.integers(0, vocab // 2, tokens)
+    ids[::7], ids[3::11] = pad, vocab + 1
+    W = r.integers(-100, 101, (vocab, dim)).astype(np.float32)
+    W[pad], W[vocab // 2:] = np.nan, np.inf
+    d_ids, d_W = ints(singa, dev, ids), upload(singa, dev, t, W)
+    y = singa.EmbeddingForward(d_ids, d_W, scale=0.5, padding_idx=pad).to_numpy()
+    assert np.array_equal(y, O.embedding_fwd(ids, W, 0.5, pad)) and not y[::7].any()
+    dy = r.integers(-4, 5, (tokens, dim)).astype(np.float32)
+    out = (ids == pad) | (ids >= vocab)
+    dy[out] = np.where(r.random((out.sum(), 1)) < 0.5, np.nan, np.inf)
+    dy[np.flatnonzero(~out)[0]] = np.nan            # one that counts: its row alone
+    got = singa.EmbeddingBackwardW(upload(singa, dev, t, dy), d_ids, d_W, padding_idx=pad).to_numpy()
+    want = stored(t, O.embedding_bwd(np.where(out[:, None], 0, dy), ids, (vocab, dim), 1.0, pad))
+    assert np.isnan(want).any(1).sum() == 1 and np.array_equal(got, want, equal_nan=True)
+    singa.IndexErrors(dev)
+
+
+@pytest.mark.parametrize("tokens,vocab", [(9000, 300), (20000, 3000), (40000, 300000), (300, 100000)])
+def test_recorded_gradients_of_other_ids(dev, tokens, vocab):
+    """Recorded once, replayed on other ids and gradients each time, beside eager calls of the same sizes."""
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(45)
+    dim = 20
+    ids, dy, W = ints(singa, dev, np.zeros(tokens)), upload(singa, dev, "f32", np.zeros((tokens, dim))), singa.Tensor((vocab, dim), dev)
+    singa.EmbeddingBackwardW(dy, ids, W)
+    dev.Sync()
+    dev.EnableGraph(True)
+    out = singa.EmbeddingBackwardW(dy, ids, W)
+    dev.EnableGraph(False)
+    try:
+        for _ in range(4):
+            new_ids = np.where(r.random(tokens) < 0.3, r.integers(0, 4), r.integers(0, vocab, tokens)).astype(np.int32)
+            ids.CopyIntDataFromHostPtr(new_ids)
+            dy.CopyFloatDataFromHostPtr(r.standard_normal((tokens, dim)).astype(np.float32))
+            out.SetFloatValue(-77.0)
+            eager = singa.EmbeddingBackwardW(dy, ids, W).to_numpy()
+            dev.RunGraph()
+            assert np.array_equal(out.to_numpy(), eager)
+            counts = np.bincount(new_ids, minlength=vocab)
+            assert not eager[counts == 0].any() and eager[counts > 0].any(1).all()
+    finally:
+        dev.ResetGraph()
+
+
 # ------------------------------------------------------------------------------------ distillation
 
 def make_case(r, t, n, v, k, masked=True):
