@@ -351,6 +351,68 @@ def test_recorded_gradients_of_other_ids(dev, tokens, vocab):
         dev.ResetGraph()
 
 
+def row_of(singa, dev, t, tensor, row):
+    """One row of a matrix, as a tensor over its memory."""
+    dim = tensor.shape()[1]
+    return singa.from_device_pointer(tensor.ptr + row * dim * (4 if t == "f32" else 2), (1, dim), dev, kind(singa, t), keepalive=tensor)
+
+
+def put_row(singa, dev, t, tensor, row, values):
+    from singa_amd.singa_wrap import float_to_bf16_bits
+    assert t == "bf16"
+    row_of(singa, dev, t, tensor, row).CopyHalfDataFromHostPtr(float_to_bf16_bits(np.asarray(values, np.float32)))
+
+
+def test_embedding_of_more_than_32_bits_of_elements(dev):
+    """A table, a result and a gradient of 4.48e9 elements: rows on both sides of 2^31 and 2^32."""
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(46)
+    many, dim = 70000001, 64
+    far = np.array([0, 1, (1 << 25) - 1, 1 << 25, (1 << 26) - 1, 1 << 26, many - 1])
+    values = r.integers(-100, 101, (far.size, dim)).astype(np.float32)
+    big = singa.Tensor((many, dim), dev, singa.kBFloat16)
+    big.SetFloatValue(2.0)
+    for row, v in zip(far, values):
+        put_row(singa, dev, "bf16", big, row, v)
+    ids = np.concatenate([far, far + 5, far - 3, [many, -1]])
+    want = np.full((ids.size, dim), 2.0, np.float32)
+    want[:far.size] = values
+    want[(ids < 0) | (ids >= many)] = 0
+    got = singa.EmbeddingForward(ints(singa, dev, ids), big).to_numpy()
+    assert np.array_equal(got, want)
+    assert singa.IndexErrors(dev) == int((ids >= many).sum() + (ids < -1).sum())
+    # its gradient: looked through, counted and sorted
+    for tokens in (300, 3000, 9000):
+        ids = far[r.integers(0, far.size, tokens)]
+        dy = r.integers(-4, 5, (tokens, dim)).astype(np.float32)
+        big.SetFloatValue(9.0)
+        assert singa.EmbeddingBackwardW(upload(singa, dev, "bf16", dy), ints(singa, dev, ids), big, out=big) is big
+        want = stored("bf16", np.stack([dy[ids == f].sum(0) for f in far]))
+        for f, w in zip(far, want):
+            assert np.array_equal(row_of(singa, dev, "bf16", big, f).to_numpy()[0].astype(np.float64), w)
+            for near in (f - 2, f + 2):
+                if 0 <= near < many:
+                    assert not row_of(singa, dev, "bf16", big, near).to_numpy().any()
+    # and as many tokens: each row of a small table is the sum of 70000 and more (whole numbers, exact in fp32)
+    vocab = 997
+    ids = (np.arange(many) * 31 % vocab).astype(np.int32)
+    d_ids = ints(singa, dev, ids)
+    big.SetFloatValue(1.0)
+    for row, v in zip(far, values):
+        put_row(singa, dev, "bf16", big, row, v)
+    want = np.repeat(np.bincount(ids, minlength=vocab).astype(np.float32)[:, None], dim, 1)
+    np.add.at(want, ids[far], values - 1)
+    table = upload(singa, dev, "bf16", values[:1].repeat(vocab, 0) + np.arange(vocab)[:, None] % 100)
+    dW = singa.EmbeddingBackwardW(big, d_ids, table)
+    assert np.array_equal(dW.to_numpy().astype(np.float64), stored("bf16", want))
+    del big
+    y = singa.EmbeddingForward(d_ids, table)
+    rows = table.to_numpy()
+    for f in far:
+        assert np.array_equal(row_of(singa, dev, "bf16", y, f).to_numpy()[0], rows[ids[f]])
+    assert singa.IndexErrors(dev) == 0
+
+
 # ------------------------------------------------------------------------------------ distillation
 
 def make_case(r, t, n, v, k, masked=True):
@@ -615,6 +677,46 @@ def test_distillation_of_many_long_rows(dev, t, n, v):
     for i in (0, 2):
         close(got[i][rows], want[0], b[0], "loss")
         close(got[i + 1][rows], want[2], b[2], "dx")
+
+
+def test_distillation_of_more_than_32_bits_of_elements(dev):
+    """4.59e9 logits: rows on both sides of 2^31 and 2^32 elements, by each entry point and in place."""
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(24)
+    n, v, k = 70001, 65537, 3
+    rows = np.array([0, 32766, 32767, 32768, 65534, 65535, 65536, 70000])
+    top, labels = r.integers(0, v, (n, k)), r.integers(-1, v, n)
+    teacher = r.standard_normal((n, k)).astype(np.float32)
+    x64 = stored("bf16", r.standard_normal((rows.size, v)) * 3)
+    x64[3] = 0.5
+    x = singa.Tensor((n, v), dev, singa.kBFloat16)
+    x.SetFloatValue(0.5)
+    for row, a in zip(rows, x64):
+        put_row(singa, dev, "bf16", x, row, a)
+    how = dict(temperature=2.0, soft=0.7, hard=0.3)
+    d_top, d_teacher, d_labels = ints(singa, dev, top), singa.from_numpy(teacher, dev), ints(singa, dev, labels)
+    want = O.distill(x64, top[rows], teacher[rows], labels[rows], None, **how)
+    b = bounds("bf16", x64, top[rows], teacher[rows], labels[rows], None, 1.0, 2.0, 0.7, 0.3)
+
+    def look(loss, dx):
+        if loss is not None:
+            close(loss.to_numpy()[rows], want[0], b[0], "loss")
+        close(np.concatenate([row_of(singa, dev, "bf16", dx, i).to_numpy() for i in rows]), want[2], b[2], "dx")
+
+    loss, stats = singa.DistillationFwd(x, d_top, d_teacher, d_labels, **how)
+    look(loss, singa.DistillationBwd(x, stats, d_top, d_teacher, d_labels, **how))
+    look(*singa.DistillationFwdBwd(x, d_top, d_teacher, d_labels, **how))
+    look(None, singa.DistillationBwd(x, stats, d_top, d_teacher, d_labels, out=x, **how))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("n,v,k", [(9, 500, 1024), (9, 300, 700), (1030, 90, 65)])
+def test_distillation_of_long_lists_over_few_columns(dev, t, n, v, k):
+    """Lists longer than the row, every column there several times, a wavefront to a row."""
+    from singa_amd import singa_wrap as singa
+    case = make_case(np.random.default_rng(v), t, n, v, k)
+    check_case(singa, dev, t, case, temperature=2.0, soft=0.7, hard=0.3, scale=0.5)
+    check_case(singa, dev, t, case, shift=1)
 
 
 def record_of(dev, call):
