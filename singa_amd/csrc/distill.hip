@@ -875,8 +875,10 @@ int launch_bwd(const Rows<typename S::elem> &a, unsigned each, hipStream_t s) {
 
 // Parts that a row is cut in for the loss, 0: none.  Two launches that have the whole chip for few rows, against one that has a CU for each: a
 // row of 262144 bfloat16 values 26 -> 7 us, with its gradient 54 -> 10, 64 rows 27 -> 14 and 56 -> 28; 128 rows of 131072 15.9 -> 13.5 and 32.0 ->
-// 28.8.  Short rows have one launch: 16 of 32000 fp32 values 5.9 us, in parts 6.3, a bfloat16 row of 40000 6.7 and 7.0; with the gradient, a
-// bfloat16 row of 20001 8.2 and 9.6, of 40000 12.5 and 9.9, an fp32 row of 32000 10.5 and 9.1.
+// 28.8.  Short rows have one launch.  The border counts elements, not bytes: a workgroup waits for its row's exponentials as much as for the row.
+// One launch and parts, us, 16 rows: the loss of 28000 fp32 values 7.2 and 7.4, of 40000 8.4 and 7.4; of 40000 bfloat16 values 7.2 and 7.3, of 56000 8.6
+// and 7.3; with the gradient, 20001 fp32 values 8.9 and 10.1, 28000 10.5 and 10.0, 40000 13.6 and 10.2; 28000 bfloat16 values 9.9 and 10.6, 40000 12.8
+// and 11.1.  128 rows gain less (56000 bfloat16 values with the gradient 17.4 and 16.4) and some lose: 48000 fp32 values with it 16.3 and 20.1.
 int parts_of(size_t batch, size_t dim, size_t elem, bool grad) {
   const size_t vecs = dim * elem / 16, cus = size_t(sgh_num_cus());
   if (batch * 2 > cus || dim <= (grad ? 28000 : 40000)) return 0;
