@@ -843,6 +843,103 @@ SGH_API int sgh_distill_fwd_bwd_bf16(const uint16_t *x, const int32_t *top, cons
  * streams as for sgh_embedding_index_errors). */
 SGH_API int sgh_distill_index_errors(void *stream, int *count);
 
+/* =====================================================================================
+ * The middle of a token model (no counterpart in this reference version): attention between the
+ * tokens of a sequence, and what stands between two blocks.  fp32, and 16-bit tensors with fp32 statistics and sums.
+ * ===================================================================================== */
+/* Sizes of an attention, filled in by sgh_attn_geom_init.
+ *   q, o [batch, q_len, heads, dim];  k, v [batch, k_len, kv_heads, dim], head h reads the keys of head h / (heads / kv_heads)
+ * causal: the query at position p sees the keys up to p; it is at position q_starts[b] + its row, or k_len - q_len + its row where no
+ * q_starts are given.  scale: of the products q . k.
+ * A learned position bias is added to the scaled products if buckets is not 0: table[bucket][head] (fp32, [buckets, heads]) of the distance of
+ * key position minus query position.  With n buckets for a direction (bidirectional: half of them for keys up to the query's position, half for
+ * those behind it; else all of them for keys in front, and those behind have the bucket of distance 0) and e = n / 2 rounded down, distance m < e
+ * has bucket m, a longer one the bucket min(n - 1, e + floor((n - e) log(m / e) / log(max_distance / e))), borders exact in whole numbers.
+ * dim up to SGH_ATTN_MAX_DIM, n up to SGH_ATTN_MAX_BUCKETS and at least 2, max_distance above e and up to 1024, lengths up to 2^28,
+ * heads * dim up to 2^20, batch * heads * (q_len / 32 + 1) and batch * kv_heads * (k_len / 32 + 1) up to 2^22: SGH_ELIMIT beyond. */
+#define SGH_ATTN_MAX_DIM 128
+#define SGH_ATTN_MAX_BUCKETS 64
+typedef struct sgh_attn_geom {
+  int batch, q_len, k_len, heads, kv_heads, dim, causal;
+  float scale;
+  int buckets, max_distance, bidirectional;
+  int bounds;                        /* of one direction: where its buckets 1, 2, ... begin */
+  int bound[SGH_ATTN_MAX_BUCKETS];
+} sgh_attn_geom;
+SGH_API int sgh_attn_geom_init(sgh_attn_geom *g, int batch, int q_len, int k_len, int heads, int kv_heads, int dim, int causal,
+                               float scale, int buckets, int max_distance, int bidirectional);
+/* o = softmax(scale q k^T + bias) v, and lse [batch, heads, q_len] (fp32) = the logarithm of each row's sum of exponentials, which the
+ * backward pass needs.  q_lengths, k_lengths (int32, [batch], taken into [0, q_len] and [0, k_len]): how many rows of each sequence count, NULL: all.
+ * Rows behind them are not looked at; their results, and those of a query that sees no key, are 0 (lse: -inf).  q_starts (int32, [batch], within
+ * +-2^30): see above.  A value at a key that some query of a block sees may reach others of the block if it is infinite or NaN; what lies behind
+ * the lengths reaches nothing.
+ * _bwd: the gradients of q, k, v and of the table (dtable, with a table only) from dout, the gradient of o, and the o and lse of the same
+ * arguments.  The probabilities are computed anew.  Every sum has one order: the same bits every time.  The terms p and ds of the products
+ * over the keys and queries are rounded to the tensors' type (binary16: scaled into its range); statistics, sums and the table's
+ * gradient are fp32 throughout.
+ * Tensors need no alignment (whole 16-byte rows at multiples of 16 bytes are fastest).  No result may overlap an argument, another result or the
+ * workspace.  workspace: sgh_attn_{fwd,bwd}_workspace_bytes, at a multiple of 16 bytes (0: NULL is taken).  Calls on different streams need one
+ * each. */
+SGH_API size_t sgh_attn_fwd_workspace_bytes(const sgh_attn_geom *g);
+SGH_API size_t sgh_attn_bwd_workspace_bytes(const sgh_attn_geom *g);
+SGH_API int sgh_attn_fwd_f32(const sgh_attn_geom *g, const float *q, const float *k, const float *v, const float *table,
+                             const int32_t *q_lengths, const int32_t *k_lengths, const int32_t *q_starts, float *o, float *lse,
+                             void *workspace, size_t ws_bytes, void *stream);
+SGH_API int sgh_attn_bwd_f32(const sgh_attn_geom *g, const float *dout, const float *q, const float *k, const float *v,
+                             const float *o, const float *lse, const float *table, const int32_t *q_lengths,
+                             const int32_t *k_lengths, const int32_t *q_starts, float *dq, float *dk, float *dv, float *dtable,
+                             void *workspace, size_t ws_bytes, void *stream);
+SGH_API int sgh_attn_fwd_f16(const sgh_attn_geom *g, const uint16_t *q, const uint16_t *k, const uint16_t *v, const float *table,
+                             const int32_t *q_lengths, const int32_t *k_lengths, const int32_t *q_starts, uint16_t *o, float *lse,
+                             void *workspace, size_t ws_bytes, void *stream);
+SGH_API int sgh_attn_bwd_f16(const sgh_attn_geom *g, const uint16_t *dout, const uint16_t *q, const uint16_t *k, const uint16_t *v,
+                             const uint16_t *o, const float *lse, const float *table, const int32_t *q_lengths,
+                             const int32_t *k_lengths, const int32_t *q_starts, uint16_t *dq, uint16_t *dk, uint16_t *dv, float *dtable,
+                             void *workspace, size_t ws_bytes, void *stream);
+SGH_API int sgh_attn_fwd_bf16(const sgh_attn_geom *g, const uint16_t *q, const uint16_t *k, const uint16_t *v, const float *table,
+                             const int32_t *q_lengths, const int32_t *k_lengths, const int32_t *q_starts, uint16_t *o, float *lse,
+                             void *workspace, size_t ws_bytes, void *stream);
+SGH_API int sgh_attn_bwd_bf16(const sgh_attn_geom *g, const uint16_t *dout, const uint16_t *q, const uint16_t *k, const uint16_t *v,
+                             const uint16_t *o, const float *lse, const float *table, const int32_t *q_lengths,
+                             const int32_t *k_lengths, const int32_t *q_starts, uint16_t *dq, uint16_t *dk, uint16_t *dv, float *dtable,
+                             void *workspace, size_t ws_bytes, void *stream);
+
+/* The end of one block and the start of the next: x [rows, dim] is the stream that passes by the block, h [rows, dim] the block's result.
+ *   u = h * rsqrt(mean(h^2) + eps) * post      (the norm behind the block; post NULL: u = h)
+ *   y = x + scale * gate * u                   (h NULL: y is x and is not written)
+ *   n = y * rsqrt(mean(y^2) + eps) * pre       (the norm before the next block, of the unrounded y; pre NULL: none)
+ * post, pre [dim] fp32; gate [gates, dim] in the tensors' type, each row of it for rows / gates rows (gates divides rows: 1 is a gate for
+ * each channel, the number of sequences one for each sequence, rows one for each token), NULL: no gate.  h or pre has to be there, post and gate
+ * go with h.  stats [rows, 2] (fp32) are the two roots, 0 where there is none.
+ * _bwd: from dy (NULL: 0), the gradient of y that comes along the stream, and dn (with pre), the gradients of x (dx), h (dh), post, the gate
+ * and pre.  y is what the forward pass stored (x, if h is NULL).  Sums over rows are fp32 in an order that follows from the sizes: the same bits every
+ * time.
+ * dim up to 16384 (SGH_ELIMIT beyond), rows up to 2^31 - 1, eps >= 0.  Rows need no alignment.  No result may overlap an argument, another
+ * result or the workspace: sgh_residual_norm_bwd_workspace_bytes (gates 0: no gate), at a multiple of 16 bytes; calls on different streams
+ * need one each. */
+SGH_API size_t sgh_residual_norm_bwd_workspace_bytes(size_t rows, size_t dim, size_t gates, size_t elem_bytes);
+SGH_API int sgh_residual_norm_fwd_f32(const float *x, const float *h, const float *post, const float *gate,
+                                      const float *pre, size_t rows, size_t dim, size_t gates, float scale, float eps,
+                                      float *y, float *n, float *stats, void *stream);
+SGH_API int sgh_residual_norm_bwd_f32(const float *dy, const float *dn, const float *y, const float *stats,
+                                      const float *h, const float *post, const float *gate, const float *pre, size_t rows,
+                                      size_t dim, size_t gates, float scale, float *dx, float *dh, float *dpost,
+                                      float *dgate, float *dpre, void *workspace, size_t ws_bytes, void *stream);
+SGH_API int sgh_residual_norm_fwd_f16(const uint16_t *x, const uint16_t *h, const float *post, const uint16_t *gate,
+                                      const float *pre, size_t rows, size_t dim, size_t gates, float scale, float eps,
+                                      uint16_t *y, uint16_t *n, float *stats, void *stream);
+SGH_API int sgh_residual_norm_bwd_f16(const uint16_t *dy, const uint16_t *dn, const uint16_t *y, const float *stats,
+                                      const uint16_t *h, const float *post, const uint16_t *gate, const float *pre, size_t rows,
+                                      size_t dim, size_t gates, float scale, uint16_t *dx, uint16_t *dh, float *dpost,
+                                      uint16_t *dgate, float *dpre, void *workspace, size_t ws_bytes, void *stream);
+SGH_API int sgh_residual_norm_fwd_bf16(const uint16_t *x, const uint16_t *h, const float *post, const uint16_t *gate,
+                                      const float *pre, size_t rows, size_t dim, size_t gates, float scale, float eps,
+                                      uint16_t *y, uint16_t *n, float *stats, void *stream);
+SGH_API int sgh_residual_norm_bwd_bf16(const uint16_t *dy, const uint16_t *dn, const uint16_t *y, const float *stats,
+                                      const uint16_t *h, const float *post, const uint16_t *gate, const float *pre, size_t rows,
+                                      size_t dim, size_t gates, float scale, uint16_t *dx, uint16_t *dh, float *dpost,
+                                      uint16_t *dgate, float *dpre, void *workspace, size_t ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -3,6 +3,7 @@
 TEST INFRASTRUCTURE ONLY (tests/, the smoke check, the CPU-baseline leg of bench.py)."""
 import numpy as np
 
+from . import block_ops
 from . import cpu_oracle as O
 from . import token_ops
 
@@ -144,6 +145,22 @@ class OracleOps(object):
 
     def distill_bwd(self, x, stats, t, batch):
         return self._distill(x, t, batch)[2].astype(np.float32)
+
+    def attention_handle(self, q, k, causal, buckets, max_distance, bidirectional):
+        return block_ops.Attn(causal, None, buckets, max_distance, bidirectional)
+
+    def attention(self, h, q, k, v, table):
+        return tuple(t.astype(np.float32) for t in block_ops.attention(h, q, k, v, table))
+
+    def attention_bwd(self, h, do, q, k, v, o, lse, table):
+        return tuple(t.astype(np.float32) for t in block_ops.attention_bwd(h, do, q, k, v, o, lse, table))
+
+    def residual_norm(self, x, h, post, gate, scale, pre):
+        return tuple(t.astype(np.float32) for t in block_ops.residual_norm(x, h, post, gate, scale, pre))
+
+    def residual_norm_bwd(self, dy, dn, y, stats, h, post, gate, scale, pre):
+        return tuple(None if t is None else t.astype(np.float32)
+                     for t in block_ops.residual_norm_bwd(dy, dn, y, stats, h, post, gate, scale, pre))
 
     def accumulate(self, a, b):
         a[...] = O.add(a, b)

@@ -23,6 +23,12 @@ class ConvGeom(C.Structure):
                                       ("prelaid_ws_bytes", C.c_size_t), ("prelaid_epoch", C.c_ulonglong)]
 
 
+class AttnGeom(C.Structure):
+    """``sgh_attn_geom``"""
+    _fields_ = ([(n, C.c_int) for n in ("batch", "q_len", "k_len", "heads", "kv_heads", "dim", "causal")] + [("scale", C.c_float)] +
+                [(n, C.c_int) for n in ("buckets", "max_distance", "bidirectional", "bounds")] + [("bound", C.c_int * 64)])
+
+
 class ConvPrepareItem(C.Structure):
     """``sgh_conv_prepare_item``"""
     _fields_ = [("g", C.POINTER(ConvGeom)), ("W", vp), ("workspace", vp), ("ws_bytes", C.c_size_t)]
@@ -177,6 +183,22 @@ SIGNATURES = {
     "sgh_distill_bwd_bf16": (C.c_int, [vp, vp, vp, vp, vp, vp, sz, sz, sz, C.c_float, C.c_float, C.c_float, C.c_float, vp, vp]),
     "sgh_distill_fwd_bwd_bf16": (C.c_int, [vp, vp, vp, vp, vp, sz, sz, sz, C.c_float, C.c_float, C.c_float, C.c_float, vp, vp,
                                          vp, sz, vp]),
+    "sgh_attn_geom_init": (C.c_int, [C.POINTER(AttnGeom)] + [C.c_int] * 7 + [C.c_float] + [C.c_int] * 3),
+    "sgh_attn_fwd_workspace_bytes": (sz, [C.POINTER(AttnGeom)]),
+    "sgh_attn_bwd_workspace_bytes": (sz, [C.POINTER(AttnGeom)]),
+    "sgh_attn_fwd_f32": (C.c_int, [C.POINTER(AttnGeom)] + [vp] * 10 + [sz, vp]),
+    "sgh_attn_bwd_f32": (C.c_int, [C.POINTER(AttnGeom)] + [vp] * 15 + [sz, vp]),
+    "sgh_attn_fwd_f16": (C.c_int, [C.POINTER(AttnGeom)] + [vp] * 10 + [sz, vp]),
+    "sgh_attn_bwd_f16": (C.c_int, [C.POINTER(AttnGeom)] + [vp] * 15 + [sz, vp]),
+    "sgh_attn_fwd_bf16": (C.c_int, [C.POINTER(AttnGeom)] + [vp] * 10 + [sz, vp]),
+    "sgh_attn_bwd_bf16": (C.c_int, [C.POINTER(AttnGeom)] + [vp] * 15 + [sz, vp]),
+    "sgh_residual_norm_bwd_workspace_bytes": (sz, [sz, sz, sz, sz]),
+    "sgh_residual_norm_fwd_f32": (C.c_int, [vp] * 5 + [sz] * 3 + [C.c_float] * 2 + [vp] * 4),
+    "sgh_residual_norm_bwd_f32": (C.c_int, [vp] * 8 + [sz] * 3 + [C.c_float] + [vp] * 6 + [sz, vp]),
+    "sgh_residual_norm_fwd_f16": (C.c_int, [vp] * 5 + [sz] * 3 + [C.c_float] * 2 + [vp] * 4),
+    "sgh_residual_norm_bwd_f16": (C.c_int, [vp] * 8 + [sz] * 3 + [C.c_float] + [vp] * 6 + [sz, vp]),
+    "sgh_residual_norm_fwd_bf16": (C.c_int, [vp] * 5 + [sz] * 3 + [C.c_float] * 2 + [vp] * 4),
+    "sgh_residual_norm_bwd_bf16": (C.c_int, [vp] * 8 + [sz] * 3 + [C.c_float] + [vp] * 6 + [sz, vp]),
     "sgh_sum_rows_f32": (C.c_int, [vp, vp, C.c_int, C.c_int, vp]),
     "sgh_add_row_f32": (C.c_int, [vp, vp, C.c_int, C.c_int, vp]),
     "sgh_conv_geom_init": (C.c_int, [C.POINTER(ConvGeom)] + [C.c_int] * 11),

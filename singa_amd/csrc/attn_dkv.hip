@@ -1,0 +1,324 @@
+// Second half of attention's backward pass: the gradients of the keys and values.  A wavefront owns keys; the queries, the gradients of their
+// results and the statistics that the first half left run through LDS, for one head of the group after the other:
+//   dv = sum p do,  dk = scale sum ds q.
+// Each sum is one wavefront's, in the order of the heads and queries: the same bits every time, and nothing is added in memory.
+#include "attn_bwd.h"
+
+namespace {
+
+using namespace attn;
+
+constexpr int kStats = SGH_WAVE;   // places of a tile's statistics of a kind: a load writes one for each lane
+
+template <class T, int DP, int KW, bool BIAS>
+__global__ __launch_bounds__(kBlock, 1) void k_attn_dkv(BwdArgs a, Bounds bounds) {
+  typedef typename T::elem elem;
+  typedef Tile<T, DP> L;
+  constexpr int QR = T::half ? 64 : 32, SUB = QR / 32, ND = DP / 32, WAVE_KEYS = 32 * KW, KEYS = 4 * WAVE_KEYS;
+  constexpr int TILE = QR * L::BYTES_OF_ROW, SLOT = 2 * TILE + 2 * kStats * 4;
+  extern __shared__ __align__(16) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
+  const Shape &s = a.s;
+  const unsigned w = blockIdx.x / a.k_splits, split = blockIdx.x % a.k_splits;
+  unsigned tile, unit;
+  block_at(w, a.k_tiles, a.k_units, &tile, &unit);
+  const int b = unit / s.kv_heads, kv = unit % s.kv_heads, group = s.heads / s.kv_heads;
+  const Span span = span_of(s, b);
+  const int key0 = int(tile) * KEYS + wave * WAVE_KEYS;
+
+  int key[KW];
+  cols_t<T, DP> kf[KW], vf[KW];
+#pragma unroll
+  for (int t = 0; t < KW; ++t) {
+    key[t] = key0 + 32 * t + (lane & 31);
+    const size_t at = ((size_t(b) * s.k_len + key[t]) * s.kv_heads + kv) * s.dim;
+    const int n = key[t] < span.k ? s.dim : 0;
+    load_columns<T, DP>(kf[t], static_cast<const elem *>(a.k) + at, n, hi, a.direct);
+    load_columns<T, DP>(vf[t], static_cast<const elem *>(a.v) + at, n, hi, a.direct);
+  }
+  // queries [from, span.q) see a key of the block, [mine, span.q) one of the wavefront
+  const int from = s.causal ? max(int(tile) * KEYS - span.start, 0) / QR * QR : 0;
+  const int mine = s.causal ? key0 - span.start : 0, all_see = s.causal ? key0 + WAVE_KEYS - 1 - span.start : 0;
+  const int turns_of_head = int(tile) * KEYS < span.k && from < span.q ? (span.q - from + QR - 1) / QR : 0;
+  const int turns = turns_of_head * group, each = (turns + int(a.k_splits) - 1) / int(a.k_splits);
+  const int begin = min(turns, int(split) * each), end = min(turns, begin + each);
+
+  float *band = reinterpret_cast<float *>(lds + 2 * SLOT);
+  const size_t stride = size_t(s.heads) * s.dim;
+  Stage<T, DP, QR> stage;
+  stage.init(stride, s.dim, a.direct);
+  const size_t first_row = (size_t(b) * s.q_len * s.heads + size_t(kv) * group) * s.dim;
+  const elem *qp = static_cast<const elem *>(a.q) + first_row, *dp = static_cast<const elem *>(a.dout) + first_row;
+  const float *lse = a.stats + (size_t(b) * s.heads + size_t(kv) * group) * s.q_len;
+  const float *delta = lse + size_t(s.q_len) * s.heads * (a.k_units / s.kv_heads);
+
+  f32x16 dk[KW][ND], dv[KW][ND];
+  Range<T> range[KW];
+#pragma unroll
+  for (int t = 0; t < KW; ++t) zero(dk[t]), zero(dv[t]);
+  const float c = s.scale * kLog2e;
+  auto request = [&](int head, int q0, int slot) {
+    char *at = lds + slot * SLOT;
+    const size_t skip = q0 * stride + size_t(head) * s.dim;
+    stage(at, qp + skip, span.q - q0);
+    stage(at + TILE, dp + skip, span.q - q0);
+    if (wave < 2) {   // (rows behind the last query: 0, beside rows of zeros)
+      const float *p = (wave ? delta : lse) + size_t(head) * s.q_len + q0;
+      const rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(p), 0, max(span.q - q0, 0) * 4, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void *)(at + 2 * TILE + wave * kStats * 4), 4, lane < QR ? lane * 4 : kOOB, 0, 0, 0);
+    }
+  };
+  int head = turns_of_head ? begin / turns_of_head : 0, q0 = turns_of_head ? from + begin % turns_of_head * QR : 0, slot = 0;
+  bool other_head = true;
+  if (begin < end) request(head, q0, 0);
+  for (int turn = begin; turn < end; ++turn, slot ^= 1) {
+    tiles_arrive();
+    int next_head = head, next_q0 = q0 + QR;
+    if (next_q0 >= span.q) next_q0 = from, ++next_head;
+    if (turn + 1 < end) request(next_head, next_q0, slot ^ 1);
+    if constexpr (BIAS)
+      if (other_head) {
+        expand_bias(s, bounds, kv * group + head, band);
+        __syncthreads();
+      }
+    other_head = next_head != head;
+    const char *qt = lds + slot * SLOT, *dt = qt + TILE;
+    const float *st = reinterpret_cast<const float *>(dt + TILE);
+    if (q0 + QR > mine) {
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        f32x16 p[KW], ds[KW];
+        zero(p);
+        mul_rows<T, DP, KW>(qt, 32 * u, kf, p, lane);
+        float row_lse[16];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const sgh_v4f x = *reinterpret_cast<const sgh_v4f *>(st + 32 * u + 8 * g + 4 * hi);
+          const sgh_v4f y = *reinterpret_cast<const sgh_v4f *>(st + kStats + 32 * u + 8 * g + 4 * hi);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            row_lse[4 * g + i] = x[i];
+#pragma unroll
+            for (int t = 0; t < KW; ++t) ds[t][4 * g + i] = y[i];   // (the product starts from -delta)
+          }
+        }
+        mul_rows<T, DP, KW>(dt, 32 * u, vf, ds, lane);
+        const int q1 = q0 + 32 * u;
+#pragma unroll
+        for (int t = 0; t < KW; ++t) {
+          if constexpr (BIAS) {
+            const int first = key[t] - (span.start + q1) - 4 * hi;   // distance in row 0
+            const int lo = key0 + 32 * t - (span.start + q1 + 31), up = key0 + 32 * t + 31 - (span.start + q1);
+            const float *centre = band + s.reach;
+            if (up <= -s.reach || lo >= s.reach) {
+              const float far = centre[up <= -s.reach ? -s.reach : s.reach];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[t][i], c, far) - row_lse[i]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                p[t][i] = __builtin_amdgcn_exp2f(
+                    __builtin_fmaf(p[t][i], c, centre[min(max(first - row_of(i), -s.reach), s.reach)]) - row_lse[i]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[t][i], c, -row_lse[i]));
+          }
+          if (s.causal && q1 < all_see) {
+            const int seen_from = key[t] - span.start - q1 - 4 * hi;   // first row that sees the lane's key
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (row_of(i) < seen_from) p[t][i] = 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) ds[t][i] *= p[t][i];
+        }
+        Terms<T> terms[KW];
+#pragma unroll
+        for (int t = 0; t < KW; ++t) terms[t].set(p[t]);
+        mul_transposed<T, DP, KW>(dt, 32 * u, terms, dv, lane);
+#pragma unroll
+        for (int t = 0; t < KW; ++t) {
+          range[t].fit(ds[t], dk[t]);
+          terms[t].set(ds[t]);
+        }
+        mul_transposed<T, DP, KW>(qt, 32 * u, terms, dk, lane);
+      }
+    }
+    head = next_head, q0 = next_q0;
+  }
+
+#pragma unroll
+  for (int t = 0; t < KW; ++t) {
+    if (key[t] >= s.k_len) continue;
+    if (key[t] >= span.k) zero(dk[t]), zero(dv[t]);   // (what lies behind a sequence gets zeros)
+    constexpr float down = std::is_same<T, F16>::value ? 0x1p-14f : 1.f;
+    const float f = key[t] < span.k ? s.scale * range[t].inverse() * down : 0.f;
+    if (a.k_splits == 1) {
+      const size_t at = ((size_t(b) * s.k_len + key[t]) * s.kv_heads + kv) * s.dim;
+      store_column<T, DP>(static_cast<elem *>(a.dk) + at, dk[t], f, s.dim, hi, a.direct);
+      store_column<T, DP>(static_cast<elem *>(a.dv) + at, dv[t], down, s.dim, hi, a.direct);
+    } else {
+      const size_t n = size_t(a.k_units) * s.k_len, at = 2 * split * n + size_t(unit) * s.k_len + key[t];
+      store_partial<DP>(a.k_part + at * DP, dk[t], f, hi);
+      store_partial<DP>(a.k_part + (at + n) * DP, dv[t], down, hi);
+    }
+  }
+}
+
+// dk and dv of queries in parts: the parts' sums
+template <class T, int DP>
+__global__ __launch_bounds__(kBlock) void k_attn_dkv_join(BwdArgs a) {
+  constexpr int TEAM = DP / 4, PER = kBlock / TEAM;
+  const Shape &s = a.s;
+  const size_t n = size_t(a.k_units) * s.k_len, at = size_t(blockIdx.x) * PER + threadIdx.x / TEAM;
+  const int d = int(threadIdx.x % TEAM) * 4;
+  if (threadIdx.x >= PER * TEAM || at >= 2 * n) return;
+  sgh_v4f x = {0.f, 0.f, 0.f, 0.f};
+  for (unsigned i = 0; i < a.k_splits; ++i) x += *reinterpret_cast<const sgh_v4f *>(a.k_part + (2 * i * n + at) * DP + d);
+  const size_t row = at % n, unit = row / s.k_len, key = row % s.k_len, b = unit / s.kv_heads, kv = unit % s.kv_heads;
+  typename T::elem *out = static_cast<typename T::elem *>(at < n ? a.dk : a.dv) + ((b * s.k_len + key) * s.kv_heads + kv) * s.dim;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (d + i < s.dim) T::St::st(out + d + i, x[i]);
+}
+
+template <class T, int DP, int KW, bool BIAS>
+int launch(const BwdArgs &a, const Bounds &bounds, hipStream_t s) {
+  constexpr int QR = T::half ? 64 : 32;
+  const size_t lds = 4 * QR * Tile<T, DP>::BYTES_OF_ROW + 4 * kStats * 4 + (BIAS ? (2 * a.s.reach + 1) * sizeof(float) : 0);
+  static std::atomic<unsigned long long> asked{0};
+  SGH_HIP_TRY(allow_lds(reinterpret_cast<const void *>(k_attn_dkv<T, DP, KW, BIAS>), asked));
+  hipLaunchKernelGGL((k_attn_dkv<T, DP, KW, BIAS>), dim3(a.k_tiles * a.k_units * a.k_splits), dim3(kBlock), lds, s, a, bounds);
+  SGH_LAUNCH_CHECK();
+  if (a.k_splits > 1) {
+    const size_t n = 2 * size_t(a.k_units) * a.s.k_len, per = kBlock / (DP / 4);
+    hipLaunchKernelGGL((k_attn_dkv_join<T, DP>), dim3(unsigned((n + per - 1) / per)), dim3(kBlock), 0, s, a);
+    SGH_LAUNCH_CHECK();
+  }
+  return SGH_OK;
+}
+template <class T, int DP>
+int run_dim(const BwdArgs &a, const Bounds &bounds, hipStream_t s) {
+  if (a.s.buckets) return launch<T, DP, 1, true>(a, bounds, s);
+  return launch<T, DP, 1, false>(a, bounds, s);
+}
+
+template <class T>
+int run_dkv(const BwdArgs &a, const Bounds &bounds, hipStream_t s) {
+  switch ((a.s.dim + 31) / 32) {
+    case 1: return run_dim<T, 32>(a, bounds, s);
+    case 2: return run_dim<T, 64>(a, bounds, s);
+    case 3: return run_dim<T, 96>(a, bounds, s);
+    default: return run_dim<T, 128>(a, bounds, s);
+  }
+}
+
+// How a backward pass is cut
+struct Plan {
+  BwdArgs a;
+  size_t stats, q_part, bias_part, k_part;   // bytes
+  size_t bytes() const { return stats + q_part + bias_part + k_part; }
+};
+size_t up16(size_t n) { return (n + 15) / 16 * 16; }
+Plan plan_of(const sgh_attn_geom *g) {
+  Plan p;
+  BwdArgs &a = p.a;
+  const size_t dp = size_t(g->dim + 31) / 32 * 32, cus = size_t(sgh_num_cus());
+  const int group = g->heads / g->kv_heads;
+  a.pack = !g->buckets && size_t(g->q_len) * group <= size_t(kRows) ? group : 1;
+  a.q_tiles = unsigned((size_t(g->q_len) * a.pack + kRows - 1) / kRows);
+  a.q_units = unsigned(size_t(g->batch) * (g->heads / a.pack));
+  a.k_tiles = unsigned((size_t(g->k_len) + kRows - 1) / kRows);
+  a.k_units = unsigned(size_t(g->batch) * g->kv_heads);
+  // few blocks: several to the keys of a block of queries, and to the queries of a block of keys
+  a.q_splits = a.k_splits = 1, a.keys_each = 1 << 30;
+  const size_t q_blocks = size_t(a.q_tiles) * a.q_units, k_blocks = size_t(a.k_tiles) * a.k_units;
+  if (q_blocks * 2 <= 2 * cus && g->k_len > 256) {
+    size_t n = 2 * cus / q_blocks, most = (size_t(g->k_len) + 255) / 256;
+    if (n > most) n = most;
+    a.keys_each = int(((size_t(g->k_len) + n - 1) / n + 63) / 64 * 64);
+    a.q_splits = unsigned((g->k_len + a.keys_each - 1) / a.keys_each);
+  }
+  const size_t turns = size_t(group) * ((size_t(g->q_len) + 63) / 64);
+  if (k_blocks && k_blocks * 2 <= 2 * cus && turns > 2) {
+    size_t n = 2 * cus / k_blocks, most = turns / 2;
+    a.k_splits = unsigned(n < most ? n : most);
+  }
+  a.bias_blocks = size_t(g->batch) * a.q_tiles * a.q_splits;
+  p.stats = up16(2 * sizeof(float) * g->batch * g->heads * size_t(g->q_len));
+  p.q_part = a.q_splits > 1 ? a.q_splits * a.q_units * size_t(g->q_len) * a.pack * dp * sizeof(float) : 0;
+  p.bias_part = g->buckets ? up16(a.bias_blocks * g->heads * g->buckets * sizeof(float)) : 0;
+  p.k_part = a.k_splits > 1 ? 2 * a.k_splits * a.k_units * size_t(g->k_len) * dp * sizeof(float) : 0;
+  return p;
+}
+
+template <class T>
+int backward(const sgh_attn_geom *g, const void *dout, const void *q, const void *k, const void *v, const void *o, const float *lse,
+             const float *table, const int32_t *q_lengths, const int32_t *k_lengths, const int32_t *q_starts, void *dq, void *dk, void *dv,
+             float *dtable, void *workspace, size_t ws_bytes, void *stream) {
+  const int rc = check_geom(g);
+  if (rc != SGH_OK) return rc;
+  if (g->batch == 0) {   // (nothing but the table)
+    if (g->buckets == 0) return SGH_OK;
+    return dtable ? sgh_memset_f32(dtable, 0.f, size_t(g->buckets) * g->heads, stream) : SGH_EINVAL;
+  }
+  const size_t e = sizeof(typename T::elem), bq = size_t(g->batch) * g->q_len * g->heads, qn = bq * g->dim * e;
+  const size_t kn = size_t(g->batch) * g->k_len * g->kv_heads * g->dim * e, tn = g->buckets ? size_t(g->buckets) * g->heads * 4 : 0;
+  if (qn != 0 && (!dout || !q || !o || !lse || !dq)) return SGH_EINVAL;
+  if (kn != 0 && (!k || !v || !dk || !dv)) return SGH_EINVAL;
+  if (g->buckets != 0 && (!table || !dtable)) return SGH_EINVAL;
+  Plan p = plan_of(g);
+  if (p.bytes() && (!workspace || ws_bytes < p.bytes())) return SGH_EWORKSPACE;
+  if (p.bytes() && !sgh_aligned16(workspace)) return SGH_EINVAL;
+  const Extent results[] = {{dq, qn}, {dk, kn}, {dv, kn}, {dtable, tn}, {workspace, p.bytes()}};
+  const Extent arguments[] = {{dout, qn}, {q, qn}, {k, kn}, {v, kn}, {o, qn}, {lse, bq * 4}, {table, tn},
+                              {q_lengths, q_lengths ? size_t(g->batch) * 4 : 0}, {k_lengths, k_lengths ? size_t(g->batch) * 4 : 0},
+                              {q_starts, q_starts ? size_t(g->batch) * 4 : 0}};
+  if (any_overlap(results, arguments)) return SGH_EINVAL;
+  BwdArgs &a = p.a;
+  a.s = shape_of(g, table, q_lengths, k_lengths, q_starts);
+  a.q = q, a.k = k, a.v = v, a.o = o, a.dout = dout, a.lse = lse, a.dq = dq, a.dk = dk, a.dv = dv;
+  char *at = static_cast<char *>(workspace);
+  a.stats = reinterpret_cast<float *>(at), at += p.stats;
+  a.q_part = reinterpret_cast<float *>(at), at += p.q_part;
+  a.bias_part = reinterpret_cast<float *>(at), at += p.bias_part;
+  a.k_part = reinterpret_cast<float *>(at);
+  a.direct = g->dim % T::VEC == 0;
+  for (const void *x : {dout, q, k, v, o}) a.direct = a.direct && sgh_aligned16(x);
+  for (const void *x : {dq, dk, dv}) a.direct = a.direct && sgh_aligned16(x);
+  Bounds bounds;
+  bounds_of(g, &bounds);
+  hipStream_t s = sgh_stream_of(stream);
+  sgh_note_write(dq, qn), sgh_note_write(dk, kn), sgh_note_write(dv, kn), sgh_note_write(dtable, tn);
+  sgh_prof_kernel_scope prof("attn_bwd/k_attn_dq+k_attn_dkv", 10.0 * g->batch * g->heads * g->q_len * double(g->k_len) * g->dim, s);
+  prof.span();
+  if (g->q_len != 0) {
+    const int r = run_dq<T>(a, bounds, dtable, s);
+    if (r != SGH_OK) return r;
+  } else if (g->buckets != 0) {
+    const int r = sgh_memset_f32(dtable, 0.f, size_t(g->buckets) * g->heads, stream);
+    if (r != SGH_OK) return r;
+  }
+  return g->k_len != 0 ? run_dkv<T>(a, bounds, s) : SGH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t sgh_attn_bwd_workspace_bytes(const sgh_attn_geom *g) { return attn::check_geom(g) == SGH_OK && g->batch != 0 ? plan_of(g).bytes() : 0; }
+
+#define SGH_ATTN_BWD(SFX, S, E)                                                                                                        \
+  int sgh_attn_bwd_##SFX(const sgh_attn_geom *g, const E *dout, const E *q, const E *k, const E *v, const E *o, const float *lse,      \
+                         const float *table, const int32_t *q_lengths, const int32_t *k_lengths, const int32_t *q_starts, E *dq,       \
+                         E *dk, E *dv, float *dtable, void *workspace, size_t ws_bytes, void *stream) {                                \
+    return backward<S>(g, dout, q, k, v, o, lse, table, q_lengths, k_lengths, q_starts, dq, dk, dv, dtable, workspace, ws_bytes,       \
+                       stream);                                                                                                        \
+  }
+SGH_ATTN_BWD(f32, F32, float)
+SGH_ATTN_BWD(f16, F16, uint16_t)
+SGH_ATTN_BWD(bf16, BF16, uint16_t)
+#undef SGH_ATTN_BWD
+
+}  // extern "C"

@@ -1,0 +1,297 @@
+// First half of attention's backward pass: the gradients of the queries and of the position bias, and delta = do . o for the second half
+// (attn_dkv.hip).  A wavefront owns queries, keys and values run through LDS; the probabilities are computed anew from the logarithms of the row
+// sums:  p = e^(s - lse),  ds = p (do . v - delta),  dq = scale sum ds k.
+#include "attn_bwd.h"
+
+namespace {
+
+using namespace attn;
+
+template <class T, int DP, int QT, bool BIAS>
+__global__ __launch_bounds__(kBlock, 2) void k_attn_dq(BwdArgs a, Bounds bounds) {
+  typedef typename T::elem elem;
+  typedef Tile<T, DP> L;
+  constexpr int KT = T::half ? 64 : 32, SUB = KT / 32, ND = DP / 32, WAVE_ROWS = 32 * QT, ROWS = 4 * WAVE_ROWS;
+  constexpr int TILE = KT * L::BYTES_OF_ROW;
+  extern __shared__ __align__(16) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
+  const Shape &s = a.s;
+  const unsigned w = blockIdx.x / a.q_splits, split = blockIdx.x % a.q_splits;
+  unsigned tile, unit;
+  block_at(w, a.q_tiles, a.q_units, &tile, &unit);
+  tile = a.q_tiles - 1 - tile;
+  const int per_batch = s.heads / a.pack, b = unit / per_batch, head0 = int(unit % per_batch) * a.pack;
+  const int kv = head0 / (s.heads / s.kv_heads);
+  const Span span = span_of(s, b);
+  const int rows = s.q_len * a.pack, row0 = int(tile) * ROWS + wave * WAVE_ROWS;
+
+  int query[QT], head[QT], limit[QT], most = 0, least = 1 << 30;
+  float lse[QT], delta[QT];   // (with a bias, natural logarithms: the product with log2 e is rounded with the sum, which the bias's gradient is told by)
+  cols_t<T, DP> qf[QT], df[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = row0 + 32 * t + (lane & 31);
+    query[t] = a.pack == 1 ? r : r / a.pack;
+    head[t] = a.pack == 1 ? head0 : head0 + r % a.pack;
+    limit[t] = r < rows && query[t] < span.q ? (s.causal ? min(span.k, max(span.start + query[t] + 1, 0)) : span.k) : 0;
+    most = max(most, limit[t]), least = min(least, limit[t]);
+    const size_t at = ((size_t(b) * s.q_len + query[t]) * s.heads + head[t]) * s.dim;
+    const size_t stat = (size_t(b) * s.heads + head[t]) * s.q_len + query[t];
+    const int n = limit[t] ? s.dim : 0;
+    load_columns<T, DP>(qf[t], static_cast<const elem *>(a.q) + at, n, hi, a.direct);
+    load_columns<T, DP>(df[t], static_cast<const elem *>(a.dout) + at, n, hi, a.direct);
+    lse[t] = limit[t] ? a.lse[stat] : kNegInf;
+    if (lse[t] == kNegInf) lse[t] = -kNegInf;
+    const float lse2 = lse[t] * kLog2e;
+    if (!BIAS) lse[t] = lse2;
+    float x = 0.f;
+    cols_t<T, DP> of;
+    load_columns<T, DP>(of, static_cast<const elem *>(a.o) + at, n, hi, a.direct);
+#pragma unroll
+    for (int k = 0; k < kSteps<T, DP>; ++k) {
+      float o[T::VEC], d[T::VEC];
+      T::St::template load16<false>(reinterpret_cast<const elem *>(&of[k]), o);
+      T::St::template load16<false>(reinterpret_cast<const elem *>(&df[t][k]), d);
+#pragma unroll
+      for (int i = 0; i < T::VEC; ++i) x = __builtin_fmaf(o[i], d[i], x);
+    }
+    delta[t] = sum_of_pair(x);
+    if (r < rows && hi == 0 && split == 0) {
+      a.stats[stat] = lse2 - term_bits<T>();
+      a.stats[size_t(a.q_units) * rows + stat] = -delta[t];
+    }
+  }
+  for (int m = 1; m < 32; m *= 2) most = max(most, __shfl_xor(most, m)), least = min(least, __shfl_xor(least, m));
+  most = __builtin_amdgcn_readfirstlane(most), least = __builtin_amdgcn_readfirstlane(least);
+  int end = span.k;
+  if (s.causal) {
+    const int last = min(int(tile + 1) * ROWS, rows) - 1;
+    end = min(end, max(span.start + min(last / a.pack, span.q - 1) + 1, 0));
+  }
+  if (int(tile) * ROWS >= span.q * a.pack) end = 0;
+  const int begin = int(split) * a.keys_each;
+  end = min(end, begin + a.keys_each);
+
+  const int band_len = 2 * s.reach + 1;
+  float *band = reinterpret_cast<float *>(lds + 4 * TILE), *sums = band + band_len + wave * band_len;   // sums: a wavefront's own
+  float far_back = 0.f, far_on = 0.f;
+  if constexpr (BIAS) {
+    expand_bias(s, bounds, head0, band);
+    for (int i = lane; i < band_len; i += SGH_WAVE) sums[i] = 0.f;
+  }
+
+  const size_t stride = size_t(s.kv_heads) * s.dim;
+  Stage<T, DP, KT> stage;
+  stage.init(stride, s.dim, a.direct);
+  const elem *kp = static_cast<const elem *>(a.k) + (size_t(b) * s.k_len * s.kv_heads + kv) * s.dim;
+  const elem *vp = static_cast<const elem *>(a.v) + (size_t(b) * s.k_len * s.kv_heads + kv) * s.dim;
+  f32x16 acc[QT][ND];
+  Range<T> range[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) zero(acc[t]);
+  const float c = s.scale * kLog2e;
+  auto request = [&](int k0, int slot) {
+    stage(lds + slot * 2 * TILE, kp + k0 * stride, span.k - k0);
+    stage(lds + slot * 2 * TILE + TILE, vp + k0 * stride, span.k - k0);
+  };
+  if (begin < end) request(begin, 0);
+  int slot = 0;
+  for (int k0 = begin; k0 < end; k0 += KT, slot ^= 1) {
+    tiles_arrive();
+    if (k0 + KT < end) request(k0 + KT, slot ^ 1);
+    const char *kt = lds + slot * 2 * TILE, *vt = kt + TILE;
+    if (k0 >= most) continue;
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+      f32x16 p[QT], ds[QT];
+      zero(p);
+      mul_rows<T, DP, QT>(kt, 32 * u, qf, p, lane);
+      // (the product starts from -delta)
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ds[t][i] = -delta[t];
+      mul_rows<T, DP, QT>(vt, 32 * u, df, ds, lane);
+      const int k1 = k0 + 32 * u;
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        const int first = k1 - (span.start + query[t]) + 4 * hi;
+        if constexpr (BIAS) {
+          const int lo = k1 - (span.start + row0 + 32 * t + 31), up = k1 + 31 - (span.start + row0 + 32 * t);
+          const float *mine = band + s.reach;
+          if (up <= -s.reach || lo >= s.reach) {
+            const float far = __builtin_fmaf(-lse[t], kLog2e, mine[up <= -s.reach ? -s.reach : s.reach]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[t][i], c, far));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              p[t][i] = __builtin_amdgcn_exp2f(
+                  __builtin_fmaf(p[t][i], c, __builtin_fmaf(-lse[t], kLog2e, mine[min(max(first + row_of(i), -s.reach), s.reach)])));
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[t][i], c, -lse[t]));
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ds[t][i] *= p[t][i];
+        if (k1 + 32 > least) {
+          const int left = limit[t] - k1 - 4 * hi;
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (row_of(i) >= left) ds[t][i] = 0.f;
+        }
+        if constexpr (BIAS) {
+          const int lo = k1 - (span.start + row0 + 32 * t + 31), up = k1 + 31 - (span.start + row0 + 32 * t);
+          if (up <= -s.reach || lo >= s.reach) {
+            float x = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x += ds[t][i];
+            if (up <= -s.reach) far_back += x;
+            else far_on += x;
+          } else {
+            // Sums of the diagonals.  Lane j gets from row r the column (r - j) mod 32, whose distance is j or j - 32 on from the block's
+            // corner: two sums for each lane, in the order of the rows.
+            float on = 0.f, back = 0.f;
+            const int j = lane & 31;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int r = row_of(i) + 4 * hi;
+              const float x = __shfl(ds[t][i], ((r - j) & 31) + 32 * hi);
+              if (r >= j) on += x;
+              else back += x;
+            }
+            on = sum_of_pair(on), back = sum_of_pair(back);
+            const int d = lo + 31 + (hi ? j - 32 : j);
+            const float x = hi ? back : on;
+            if (d < -s.reach) far_back += x;
+            else if (d > s.reach) far_on += x;
+            else sums[d + s.reach] += x;
+            __builtin_amdgcn_wave_barrier();
+          }
+        }
+        range[t].fit(ds[t], acc[t]);
+      }
+      Terms<T> terms[QT];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) terms[t].set(ds[t]);
+      mul_transposed<T, DP, QT>(kt, 32 * u, terms, acc, lane);
+    }
+  }
+
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = row0 + 32 * t + (lane & 31);
+    if (r >= rows) continue;
+    if (!limit[t]) zero(acc[t]);
+    const float f = s.scale * range[t].inverse();
+    if (a.q_splits == 1) {
+      store_column<T, DP>(static_cast<elem *>(a.dq) + ((size_t(b) * s.q_len + query[t]) * s.heads + head[t]) * s.dim, acc[t], f, s.dim, hi,
+                          a.direct);
+    } else {
+      const size_t n = size_t(a.q_units) * rows;
+      store_partial<DP>(a.q_part + (split * n + size_t(unit) * rows + r) * DP, acc[t], f, hi);
+    }
+  }
+  if constexpr (BIAS) {
+    // the block's sums of the buckets: distances in order, the wavefronts' sums of each one behind the other
+    for (int m = 1; m < SGH_WAVE; m *= 2) far_back += __shfl_xor(far_back, m), far_on += __shfl_xor(far_on, m);
+    __builtin_amdgcn_wave_barrier();
+    if (lane == 0) sums[0] += far_back, sums[2 * s.reach] += far_on;
+    __syncthreads();
+    float *out = a.bias_part + (size_t(head0) * a.bias_blocks + (size_t(b) * a.q_tiles + tile) * a.q_splits + split) * s.buckets;
+    const float *all = band + band_len;
+    for (int e = tid; e < s.buckets; e += kBlock) {
+      const int half = s.bidirectional ? s.buckets / 2 : s.buckets, n = e % half, side = e / half;
+      const int from = n == 0 ? 0 : bounds.at[n - 1], to = n == half - 1 ? s.reach : bounds.at[n] - 1;
+      float x = 0.f;
+      for (int m = from; m <= to && m <= s.reach; ++m) {
+        const int d = side ? m : -m;
+        if (!side || m > 0)
+          for (int v = 0; v < 4; ++v) x += all[v * band_len + d + s.reach];
+      }
+      if (!s.bidirectional && n == 0)   // (one direction: all keys in front have the bucket of distance 0)
+        for (int d = 1; d <= s.reach; ++d)
+          for (int v = 0; v < 4; ++v) x += all[v * band_len + d + s.reach];
+      out[e] = x;
+    }
+  }
+}
+
+// dq of keys in parts: the parts' sum
+template <class T, int DP>
+__global__ __launch_bounds__(kBlock) void k_attn_dq_join(BwdArgs a) {
+  constexpr int TEAM = DP / 4, PER = kBlock / TEAM;
+  const Shape &s = a.s;
+  const size_t rows = size_t(s.q_len) * a.pack, n = a.q_units * rows, at = size_t(blockIdx.x) * PER + threadIdx.x / TEAM;
+  const int d = int(threadIdx.x % TEAM) * 4;
+  if (threadIdx.x >= PER * TEAM || at >= n) return;
+  sgh_v4f x = {0.f, 0.f, 0.f, 0.f};
+  for (unsigned i = 0; i < a.q_splits; ++i) x += *reinterpret_cast<const sgh_v4f *>(a.q_part + (i * n + at) * DP + d);
+  const size_t unit = at / rows;
+  const int r = int(at % rows), per_batch = s.heads / a.pack, b = int(unit / per_batch);
+  const int query = r / a.pack, head = int(unit % per_batch) * a.pack + r % a.pack;
+  typename T::elem *out = static_cast<typename T::elem *>(a.dq) + ((size_t(b) * s.q_len + query) * s.heads + head) * s.dim;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (d + i < s.dim) T::St::st(out + d + i, x[i]);
+}
+
+// dtable[e][h]: the sum over all blocks of head h, each thread's in order, then the threads' by halves
+__global__ __launch_bounds__(kBlock) void k_attn_dtable(BwdArgs a, float *dtable) {
+  __shared__ float part[kBlock];
+  const int h = blockIdx.x % a.s.heads, e = blockIdx.x / a.s.heads;
+  const float *p = a.bias_part + size_t(h) * a.bias_blocks * a.s.buckets + e;
+  float x = 0.f;
+  for (size_t i = threadIdx.x; i < a.bias_blocks; i += kBlock) x += p[i * a.s.buckets];
+  part[threadIdx.x] = x;
+  for (int m = kBlock / 2; m > 0; m /= 2) {
+    __syncthreads();
+    if (int(threadIdx.x) < m) part[threadIdx.x] += part[threadIdx.x + m];
+  }
+  if (threadIdx.x == 0) dtable[size_t(e) * a.s.heads + h] = part[0];
+}
+
+template <class T, int DP, int QT, bool BIAS>
+int launch(const BwdArgs &a, const Bounds &bounds, float *dtable, hipStream_t s) {
+  constexpr int KT = T::half ? 64 : 32;
+  const size_t lds = 4 * KT * Tile<T, DP>::BYTES_OF_ROW + (BIAS ? 5 * (2 * a.s.reach + 1) * sizeof(float) : 0);
+  static std::atomic<unsigned long long> asked{0};
+  SGH_HIP_TRY(allow_lds(reinterpret_cast<const void *>(k_attn_dq<T, DP, QT, BIAS>), asked));
+  hipLaunchKernelGGL((k_attn_dq<T, DP, QT, BIAS>), dim3(a.q_tiles * a.q_units * a.q_splits), dim3(kBlock), lds, s, a, bounds);
+  SGH_LAUNCH_CHECK();
+  if (a.q_splits > 1) {
+    const size_t n = size_t(a.q_units) * a.s.q_len * a.pack, per = kBlock / (DP / 4);
+    hipLaunchKernelGGL((k_attn_dq_join<T, DP>), dim3(unsigned((n + per - 1) / per)), dim3(kBlock), 0, s, a);
+    SGH_LAUNCH_CHECK();
+  }
+  if (BIAS) {
+    hipLaunchKernelGGL(k_attn_dtable, dim3(unsigned(a.s.heads * a.s.buckets)), dim3(kBlock), 0, s, a, dtable);
+    SGH_LAUNCH_CHECK();
+  }
+  return SGH_OK;
+}
+template <class T, int DP>
+int run_dim(const BwdArgs &a, const Bounds &bounds, float *dtable, hipStream_t s) {
+  if (a.s.buckets) return launch<T, DP, 1, true>(a, bounds, dtable, s);
+  return launch<T, DP, 1, false>(a, bounds, dtable, s);
+}
+
+}  // namespace
+
+namespace attn {
+
+template <class T>
+int run_dq(const BwdArgs &a, const Bounds &bounds, float *dtable, hipStream_t s) {
+  switch ((a.s.dim + 31) / 32) {
+    case 1: return run_dim<T, 32>(a, bounds, dtable, s);
+    case 2: return run_dim<T, 64>(a, bounds, dtable, s);
+    case 3: return run_dim<T, 96>(a, bounds, dtable, s);
+    default: return run_dim<T, 128>(a, bounds, dtable, s);
+  }
+}
+template int run_dq<F32>(const BwdArgs &, const Bounds &, float *, hipStream_t);
+template int run_dq<F16>(const BwdArgs &, const Bounds &, float *, hipStream_t);
+template int run_dq<BF16>(const BwdArgs &, const Bounds &, float *, hipStream_t);
+
+}  // namespace attn

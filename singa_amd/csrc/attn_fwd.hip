@@ -1,0 +1,336 @@
+// Forward pass of attention: o = softmax(scale q k^T + bias) v in one pass over the keys, and the logarithm of every row's sum.
+//
+// s and the probabilities of a 32x32 block live in one wavefront's registers, queries in the lanes: a running maximum m and sum l for each query,
+// o rescaled when m grows.  Exponentials are powers of two (scale and bias times log2 e).
+#include "attn.h"
+#include "attn_run.h"
+
+namespace {
+
+using namespace attn;
+
+struct FwdArgs {
+  Shape s;
+  const void *q, *k, *v;
+  void *o;
+  float *lse;
+  float *part;        // [splits][units][rows][DP + 1]: results of a part of the keys, and the logarithms of their sums
+  unsigned tiles, units, splits;
+  int pack;           // heads of a group that share a tile: row r is query r / pack, head r % pack of the group
+  int keys_each;      // keys of a split, a multiple of 64
+  bool direct;
+};
+
+// m moves only when a row's maximum has grown by more than 2^8: the terms then stay within 2^8 of one, and o is rescaled seldom
+constexpr float kGrowth = 8.f;
+
+template <class T, int DP, int QT, bool BIAS>
+__global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds) {
+  typedef typename T::elem elem;
+  typedef Tile<T, DP> L;
+  constexpr int KT = T::half ? 64 : 32, SUB = KT / 32, ND = DP / 32, WAVE_ROWS = 32 * QT, ROWS = 4 * WAVE_ROWS;
+  constexpr int TILE = KT * L::BYTES_OF_ROW;
+  // binary16: terms from 2^-14 to 2^14 with all their bits
+  constexpr float kShift = std::is_same<T, F16>::value ? 6.f : 0.f;
+  extern __shared__ __align__(16) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
+  const Shape &s = a.s;
+  const unsigned w = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+  unsigned tile, unit;
+  block_at(w, a.tiles, a.units, &tile, &unit);
+  tile = a.tiles - 1 - tile;   // (with a causal mask the last tiles are the longest)
+  const int per_batch = s.heads / a.pack, b = unit / per_batch, head0 = int(unit % per_batch) * a.pack;
+  const int kv = head0 / (s.heads / s.kv_heads);
+  const Span span = span_of(s, b);
+  const int rows = s.q_len * a.pack, row0 = int(tile) * ROWS + wave * WAVE_ROWS;
+
+  // the lane's queries: keys [0, limit) are seen
+  int query[QT], head[QT], limit[QT], most = 0, least = 1 << 30;
+  cols_t<T, DP> qf[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = row0 + 32 * t + (lane & 31);
+    query[t] = a.pack == 1 ? r : r / a.pack;
+    head[t] = a.pack == 1 ? head0 : head0 + r % a.pack;
+    limit[t] = r < rows && query[t] < span.q ? (s.causal ? min(span.k, max(span.start + query[t] + 1, 0)) : span.k) : 0;
+    most = max(most, limit[t]), least = min(least, limit[t]);
+    load_columns<T, DP>(qf[t], static_cast<const elem *>(a.q) + ((size_t(b) * s.q_len + query[t]) * s.heads + head[t]) * s.dim,
+                        limit[t] ? s.dim : 0, hi, a.direct);
+  }
+  for (int m = 1; m < 32; m *= 2) most = max(most, __shfl_xor(most, m)), least = min(least, __shfl_xor(least, m));
+  most = __builtin_amdgcn_readfirstlane(most), least = __builtin_amdgcn_readfirstlane(least);
+  // of the whole block: the last row's
+  int end = span.k;
+  if (s.causal) {
+    const int last = min(int(tile + 1) * ROWS, rows) - 1;
+    end = min(end, max(span.start + min(last / a.pack, span.q - 1) + 1, 0));
+  }
+  if (int(tile) * ROWS >= span.q * a.pack) end = 0;
+  const int begin = int(split) * a.keys_each;
+  end = min(end, begin + a.keys_each);
+
+  float *band = reinterpret_cast<float *>(lds + 4 * TILE);
+  const int band_len = 2 * s.reach + 1;
+  if constexpr (BIAS)
+    for (int g = 0; g < a.pack; ++g) expand_bias(s, bounds, head0 + g, band + g * band_len);
+
+  const size_t stride = size_t(s.kv_heads) * s.dim;
+  Stage<T, DP, KT> stage;
+  stage.init(stride, s.dim, a.direct);
+  const elem *kp = static_cast<const elem *>(a.k) + (size_t(b) * s.k_len * s.kv_heads + kv) * s.dim;
+  const elem *vp = static_cast<const elem *>(a.v) + (size_t(b) * s.k_len * s.kv_heads + kv) * s.dim;
+
+  f32x16 acc[QT][ND];
+  float m[QT], l[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    zero(acc[t]);
+    m[t] = -3e38f, l[t] = 0.f;
+  }
+  const float c = s.scale * kLog2e;
+  auto request = [&](int k0, int slot) {
+    stage(lds + slot * 2 * TILE, kp + k0 * stride, span.k - k0);
+    stage(lds + slot * 2 * TILE + TILE, vp + k0 * stride, span.k - k0);
+  };
+  if (begin < end) request(begin, 0);
+  int slot = 0;
+  for (int k0 = begin; k0 < end; k0 += KT, slot ^= 1) {
+    tiles_arrive();
+    if (k0 + KT < end) request(k0 + KT, slot ^ 1);
+    const char *kt = lds + slot * 2 * TILE, *vt = kt + TILE;
+    if (k0 >= most) continue;   // (no row of this wavefront sees any of them)
+    f32x16 p[SUB][QT];
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+      zero(p[u]);
+      mul_rows<T, DP, QT>(kt, 32 * u, qf, p[u], lane);
+    }
+    // scores in units of log2, -inf where the mask is
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      float top = kNegInf;
+      if constexpr (BIAS) {
+        const int first = k0 - (span.start + query[t]);   // the distance of key k0
+        const int lo = k0 - (span.start + (row0 + 32 * t + 31) / a.pack), up = k0 + KT - 1 - (span.start + (row0 + 32 * t) / a.pack);
+        const float *mine = band + (head[t] - head0) * band_len + s.reach;
+        if (up <= -s.reach || lo >= s.reach) {   // far away the bias is one number
+          const float far = mine[up <= -s.reach ? -s.reach : s.reach];
+#pragma unroll
+          for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[u][t][i] = __builtin_fmaf(p[u][t][i], c, far);
+        } else {
+#pragma unroll
+          for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int d = first + 32 * u + row_of(i) + 4 * hi;
+              p[u][t][i] = __builtin_fmaf(p[u][t][i], c, mine[min(max(d, -s.reach), s.reach)]);
+            }
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) p[u][t][i] *= c;
+      }
+      if (k0 + KT > least) {
+        const int left = limit[t] - k0 - 4 * hi;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (32 * u + row_of(i) >= left) p[u][t][i] = kNegInf;
+      }
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, p[u][t][i]);
+      top = max_of_pair(top);
+      if (__ballot(top > m[t] + kGrowth)) {
+        const float now = fmaxf(m[t], top), f = __builtin_amdgcn_exp2f(m[t] - now);
+        m[t] = now, l[t] *= f;
+#pragma unroll
+        for (int n = 0; n < ND; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[t][n][i] *= f;
+      }
+      const float from = m[t] - kShift;
+      float sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          p[u][t][i] = __builtin_amdgcn_exp2f(p[u][t][i] - from);
+          sum += p[u][t][i];
+        }
+      l[t] += sum;
+    }
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+      Terms<T> terms[QT];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) terms[t].set(p[u][t]);
+      mul_transposed<T, DP, QT>(vt, 32 * u, terms, acc, lane);
+    }
+  }
+
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = row0 + 32 * t + (lane & 31);
+    if (r >= rows) continue;
+    const float sum = sum_of_pair(l[t]);
+    // (a row that sees nothing has o = 0 and the logarithm of 0)
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (sum == 0.f) zero(acc[t]);
+    const float lse = sum == 0.f ? kNegInf : (m[t] - kShift + __builtin_amdgcn_logf(sum)) * kLn2;
+    if (a.splits == 1) {
+      store_column<T, DP>(static_cast<elem *>(a.o) + ((size_t(b) * s.q_len + query[t]) * s.heads + head[t]) * s.dim, acc[t], inv, s.dim, hi,
+                          a.direct);
+      if (hi == 0) a.lse[(size_t(b) * s.heads + head[t]) * s.q_len + query[t]] = lse;
+    } else {
+      const size_t n = size_t(a.units) * rows, at = split * n + size_t(unit) * rows + r;
+      store_partial<DP>(a.part + at * DP, acc[t], inv, hi);
+      if (hi == 0) a.part[a.splits * n * DP + at] = lse;
+    }
+  }
+}
+
+// Joins the parts of the keys, DP / 4 lanes to a row: o = sum e^(lse_s - lse) o_s
+template <class T, int DP>
+__global__ __launch_bounds__(kBlock) void k_attn_join(FwdArgs a) {
+  typedef typename T::elem elem;
+  constexpr int TEAM = DP / 4, PER = kBlock / TEAM;
+  const Shape &s = a.s;
+  const size_t rows = size_t(s.q_len) * a.pack, n = a.units * rows, at = size_t(blockIdx.x) * PER + threadIdx.x / TEAM;
+  const int d = int(threadIdx.x % TEAM) * 4;
+  if (threadIdx.x >= PER * TEAM || at >= n) return;
+  const float *lses = a.part + a.splits * n * DP + at;
+  float top = kNegInf, sum = 0.f;
+  for (unsigned i = 0; i < a.splits; ++i) top = fmaxf(top, lses[i * n]);
+  sgh_v4f o = {0.f, 0.f, 0.f, 0.f};
+  for (unsigned i = 0; i < a.splits; ++i) {
+    const float lse = lses[i * n];
+    const float f = lse == kNegInf ? 0.f : __builtin_amdgcn_exp2f((lse - top) * kLog2e);
+    const sgh_v4f x = *reinterpret_cast<const sgh_v4f *>(a.part + (i * n + at) * DP + d);
+    sum += f;
+    o += x * f;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const size_t unit = at / rows;
+  const int r = int(at % rows), per_batch = s.heads / a.pack, b = int(unit / per_batch);
+  const int query = r / a.pack, head = int(unit % per_batch) * a.pack + r % a.pack;
+  elem *out = static_cast<elem *>(a.o) + ((size_t(b) * s.q_len + query) * s.heads + head) * s.dim;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (d + i < s.dim) T::St::st(out + d + i, o[i] * inv);
+  if (d == 0) a.lse[(size_t(b) * s.heads + head) * s.q_len + query] = sum == 0.f ? kNegInf : top + __builtin_amdgcn_logf(sum) * kLn2;
+}
+
+template <class T, int DP, int QT, bool BIAS>
+int launch(const FwdArgs &a, const Bounds &bounds, size_t lds, hipStream_t s) {
+  static std::atomic<unsigned long long> asked{0};
+  SGH_HIP_TRY(allow_lds(reinterpret_cast<const void *>(k_attn_fwd<T, DP, QT, BIAS>), asked));
+  SGH_LAUNCH_TIMED((k_attn_fwd<T, DP, QT, BIAS>), dim3(a.tiles * a.units * a.splits), dim3(kBlock), lds, s, a, bounds);
+  SGH_LAUNCH_CHECK();
+  if (a.splits > 1) {
+    const size_t n = size_t(a.units) * a.s.q_len * a.pack, per = kBlock / (DP / 4);
+    hipLaunchKernelGGL((k_attn_join<T, DP>), dim3(unsigned((n + per - 1) / per)), dim3(kBlock), 0, s, a);
+    SGH_LAUNCH_CHECK();
+  }
+  return SGH_OK;
+}
+
+// How a forward pass is cut
+struct Plan {
+  int dp, pack;
+  unsigned tiles, units, splits;
+  int keys_each;
+  size_t ws;
+};
+constexpr int kRows = 128;   // of a block
+Plan plan_of(const sgh_attn_geom *g) {
+  Plan p;
+  p.dp = (g->dim + 31) / 32 * 32;
+  const int group = g->heads / g->kv_heads;
+  // few queries: the heads of a group read their keys together
+  p.pack = size_t(g->q_len) * group <= kRows && band_bytes(g) * group <= kMostBand ? group : 1;
+  p.tiles = unsigned((size_t(g->q_len) * p.pack + kRows - 1) / kRows);
+  p.units = unsigned(size_t(g->batch) * (g->heads / p.pack));
+  // few rows: several blocks to the keys of each, of 256 keys at the least
+  p.splits = 1, p.keys_each = 1 << 30;
+  const size_t blocks = size_t(p.tiles) * p.units, want = 4 * size_t(sgh_num_cus());
+  if (blocks * 2 <= want && g->k_len > 256) {
+    size_t n = want / blocks, most = (size_t(g->k_len) + 255) / 256;
+    if (n > most) n = most;
+    p.keys_each = int(((size_t(g->k_len) + n - 1) / n + 63) / 64 * 64);
+    p.splits = unsigned((g->k_len + p.keys_each - 1) / p.keys_each);
+  }
+  p.ws = p.splits > 1 ? size_t(p.splits) * p.units * g->q_len * p.pack * (p.dp + 1) * sizeof(float) : 0;
+  return p;
+}
+
+template <class T, int DP>
+int run_dim(const FwdArgs &a, const Bounds &bounds, hipStream_t s) {
+  constexpr int KT = T::half ? 64 : 32;
+  const size_t tiles = 4 * KT * Tile<T, DP>::BYTES_OF_ROW;
+  if (a.s.buckets) return launch<T, DP, 1, true>(a, bounds, tiles + a.pack * (2 * a.s.reach + 1) * sizeof(float), s);
+  return launch<T, DP, 1, false>(a, bounds, tiles, s);
+}
+
+template <class T>
+int forward(const sgh_attn_geom *g, const void *q, const void *k, const void *v, const float *table, const int32_t *q_lengths,
+            const int32_t *k_lengths, const int32_t *q_starts, void *o, float *lse, void *workspace, size_t ws_bytes, void *stream) {
+  const int rc = check_geom(g);
+  if (rc != SGH_OK) return rc;
+  if (g->batch == 0 || g->q_len == 0) return SGH_OK;
+  const size_t e = sizeof(typename T::elem), bq = size_t(g->batch) * g->q_len * g->heads, qn = bq * g->dim * e;
+  const size_t kn = size_t(g->batch) * g->k_len * g->kv_heads * g->dim * e;
+  if (!q || !o || !lse || (g->k_len != 0 && (!k || !v)) || (g->buckets != 0 && !table)) return SGH_EINVAL;
+  const Plan p = plan_of(g);
+  if (p.ws && (!workspace || ws_bytes < p.ws)) return SGH_EWORKSPACE;
+  if (p.ws && !sgh_aligned16(workspace)) return SGH_EINVAL;
+  const Extent results[] = {{o, qn}, {lse, bq * 4}, {workspace, p.ws}};
+  const Extent arguments[] = {{q, qn}, {k, kn}, {v, kn}, {table, g->buckets ? size_t(g->buckets) * g->heads * 4 : 0},
+                              {q_lengths, q_lengths ? size_t(g->batch) * 4 : 0}, {k_lengths, k_lengths ? size_t(g->batch) * 4 : 0},
+                              {q_starts, q_starts ? size_t(g->batch) * 4 : 0}};
+  if (any_overlap(results, arguments)) return SGH_EINVAL;
+  FwdArgs a;
+  a.s = shape_of(g, table, q_lengths, k_lengths, q_starts);
+  a.q = q, a.k = k, a.v = v, a.o = o, a.lse = lse, a.part = static_cast<float *>(workspace);
+  a.tiles = p.tiles, a.units = p.units, a.splits = p.splits, a.pack = p.pack, a.keys_each = p.keys_each;
+  a.direct = g->dim % T::VEC == 0 && sgh_aligned16(q) && sgh_aligned16(k) && sgh_aligned16(v) && sgh_aligned16(o);
+  Bounds bounds;
+  bounds_of(g, &bounds);
+  hipStream_t s = sgh_stream_of(stream);
+  sgh_note_write(o, qn);
+  sgh_prof_kernel_scope prof("attn_fwd/k_attn_fwd", 4.0 * g->batch * g->heads * g->q_len * double(g->k_len) * g->dim, s);
+  if (p.splits > 1) prof.span();
+  switch (p.dp) {
+    case 32: return run_dim<T, 32>(a, bounds, s);
+    case 64: return run_dim<T, 64>(a, bounds, s);
+    case 96: return run_dim<T, 96>(a, bounds, s);
+    default: return run_dim<T, 128>(a, bounds, s);
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t sgh_attn_fwd_workspace_bytes(const sgh_attn_geom *g) {
+  return check_geom(g) == SGH_OK && g->batch != 0 && g->q_len != 0 ? plan_of(g).ws : 0;
+}
+
+#define SGH_ATTN_FWD(SFX, S, E)                                                                                                        \
+  int sgh_attn_fwd_##SFX(const sgh_attn_geom *g, const E *q, const E *k, const E *v, const float *table, const int32_t *q_lengths,     \
+                         const int32_t *k_lengths, const int32_t *q_starts, E *o, float *lse, void *workspace, size_t ws_bytes,        \
+                         void *stream) {                                                                                               \
+    return forward<S>(g, q, k, v, table, q_lengths, k_lengths, q_starts, o, lse, workspace, ws_bytes, stream);                         \
+  }
+SGH_ATTN_FWD(f32, F32, float)
+SGH_ATTN_FWD(f16, F16, uint16_t)
+SGH_ATTN_FWD(bf16, BF16, uint16_t)
+#undef SGH_ATTN_FWD
+
+}  // extern "C"

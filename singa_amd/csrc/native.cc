@@ -77,7 +77,8 @@ struct EntryOf {
   ONE(sgh_conv_wgrad_bias_f32) ALL(sgh_bn_fwd_train) ALL(sgh_bn_relu_fwd_train) \
   ALL(sgh_bn_add_relu_fwd_train) ALL(sgh_bn_fwd_infer) ALL(sgh_bn_bwd) ALL(sgh_bn_relu_bwd) ALL(sgh_pool_fwd) ALL(sgh_pool_bwd) \
   ONE(sgh_pool_relu_fwd_f32) ONE(sgh_pool_relu_bwd_f32) ALL(sgh_embedding_fwd) ALL(sgh_embedding_bwd) ALL(sgh_distill_fwd)       \
-  ALL(sgh_distill_bwd) ALL(sgh_distill_fwd_bwd)
+  ALL(sgh_distill_bwd) ALL(sgh_distill_fwd_bwd) ALL(sgh_attn_fwd) ALL(sgh_attn_bwd)                               \
+  ALL(sgh_residual_norm_fwd) ALL(sgh_residual_norm_bwd)
 SGH_CALLS(SGH_ENTRY, SGH_ENTRY3)
 SGH_ENTRY(sgh_malloc)
 SGH_ENTRY(sgh_free)

@@ -916,6 +916,163 @@ def DistillationFwdBwd(x, top, teacher, labels=None, weights=None, temperature=1
     return loss, dx
 
 
+class AttentionHandle(object):
+    """Sizes of an attention between the queries `q` [batch, q_len, heads, dim] and the keys `k` [batch, k_len, kv_heads, dim] (of the values
+    as well), head h reading the keys of head ``h // (heads // kv_heads)``, with its mask, the scale of its products (None:
+    ``dim ** -0.5``) and, if `buckets` is not 0, the buckets of a learned position bias:
+
+    * `causal`: a query sees the keys up to its own position, which is its row plus ``k_len - q_len`` (or `q_starts`, see
+      ``AttentionForward``).
+    * the bias is ``table[bucket, head]`` of the distance from the query's position to the key's.  Half of a direction's buckets are one
+      distance each, the others grow in equal ratios up to `max_distance`.  `bidirectional`: half of the buckets for keys behind the query's
+      position; otherwise those have the bucket of distance 0."""
+
+    def __init__(self, q, k, causal=False, scale=None, buckets=0, max_distance=128, bidirectional=True):
+        if q.nDim() != 4 or k.nDim() != 4 or q._shape[0] != k._shape[0] or q._shape[3] != k._shape[3]:
+            raise SingaHipError("AttentionHandle: [batch, length, heads, dim] is expected of q and k, got %s, %s" % (q.shape(), k.shape()))
+        if q._dtype != k._dtype or q._dtype not in _SUFFIX:
+            raise SingaHipError("AttentionHandle: q and k of one floating type are expected")
+        self.q_shape, self.k_shape, self.dtype = q._shape, k._shape, q._dtype
+        self.batch, self.q_len, self.heads, self.dim = q._shape
+        self.k_len, self.kv_heads = k._shape[1:3]
+        self.scale = float(self.dim) ** -0.5 if scale is None and self.dim else float(scale or 0.0)
+        self.causal, self.buckets = bool(causal), int(buckets)
+        self.geom = _lib.AttnGeom()
+        check(_L().sgh_attn_geom_init(C.byref(self.geom), self.batch, self.q_len, self.k_len, self.heads, self.kv_heads, self.dim,
+                                      int(self.causal), self.scale, self.buckets, int(max_distance), int(bidirectional)),
+              "sgh_attn_geom_init")
+        self._at = C.addressof(self.geom)
+        self._forward_bytes = _L().sgh_attn_fwd_workspace_bytes(C.byref(self.geom))
+        self._backward_bytes = _L().sgh_attn_bwd_workspace_bytes(C.byref(self.geom))
+
+
+def _attn_args(what, h, q_like, k_like, table, lengths):
+    """The checks of both directions; the addresses of the table and of the three tensors of lengths."""
+    dev = q_like[0]._dev
+    for t in q_like:
+        if t._shape != h.q_shape or t._dtype != h.dtype:
+            raise SingaHipError("%s: a tensor of the queries' shape and type is expected, got %s" % (what, t.shape()))
+    for t in k_like:
+        if t._shape != h.k_shape or t._dtype != h.dtype:
+            raise SingaHipError("%s: a tensor of the keys' shape and type is expected, got %s" % (what, t.shape()))
+    _plain(what, dev, table, *q_like, *k_like, *lengths)
+    if (table is not None) != (h.buckets != 0):
+        raise SingaHipError("%s: a handle with buckets and a table belong together" % what)
+    if table is not None and (table._dtype != kFloat32 or table._shape != (h.buckets, h.heads)):
+        raise SingaHipError("%s: a float32 table [buckets, heads] is expected, got %s" % (what, table.shape()))
+    for t in lengths:
+        if t is not None and (t._dtype != kInt or t.Size() != h.batch):
+            raise SingaHipError("%s: an int32 number for every sequence is expected" % what)
+    return tuple(None if t is None else t.ptr for t in (table,) + lengths)
+
+
+def _workspace(need, dev):
+    """(tensor or None, its address): a block of the pool for this call, so that calls that are recorded or run side by side share none."""
+    ws = _empty(Tensor, (need // 4,), dev, kFloat32) if need else None
+    return ws, ws.ptr if need else None
+
+
+def AttentionForward(h, q, k, v, table=None, q_lengths=None, k_lengths=None, q_starts=None):
+    """(o, lse): ``softmax(scale * q k^T + bias) v`` for every head of the handle `h`, and the logarithm of every row's sum of exponentials,
+    float32 [batch, heads, q_len], which ``AttentionBackward`` needs.  `table`: the position bias, float32 [buckets, heads].  `q_lengths`,
+    `k_lengths` (int32, [batch]): how many queries and keys of each sequence count; what lies behind them is not looked at, and its
+    results are 0 (lse: -inf), as are those of a query that sees no key.  `q_starts` (int32, [batch]): the position of each sequence's
+    first query among its keys, as of a new token behind a cache of `k_len` places."""
+    args = _attn_args("AttentionForward", h, (q,), (k, v), table, (q_lengths, k_lengths, q_starts))
+    fn, name = _fn("attn_fwd", q)
+    dev = q._dev
+    o, lse = _like(q), _empty(Tensor, (h.batch, h.heads, h.q_len), dev, kFloat32)
+    ws, at = _workspace(h._forward_bytes, dev)
+    check(fn(h._at, q.ptr, k.ptr, v.ptr, *args, o.ptr, lse.ptr, at, h._forward_bytes, dev.stream), name)
+    return o, lse
+
+
+def AttentionBackward(h, do, q, k, v, o, lse, table=None, q_lengths=None, k_lengths=None, q_starts=None):
+    """(dq, dk, dv, dtable) from `do`, the gradient of `o`, and the `o` and `lse` of ``AttentionForward`` on the same arguments; `dtable`
+    (float32) is None without a table.  Rows behind the lengths get gradients of 0."""
+    args = _attn_args("AttentionBackward", h, (q, do, o), (k, v), table, (q_lengths, k_lengths, q_starts))
+    _plain("AttentionBackward", q._dev, lse)
+    if lse._dtype != kFloat32 or lse._shape != (h.batch, h.heads, h.q_len):
+        raise SingaHipError("AttentionBackward: the row sums do not match: %s" % lse.shape())
+    fn, name = _fn("attn_bwd", q)
+    dev = q._dev
+    dq, dk, dv = _like(q), _like(k), _like(v)
+    dtable = None if table is None else _like(table)
+    ws, at = _workspace(h._backward_bytes, dev)
+    check(fn(h._at, do.ptr, q.ptr, k.ptr, v.ptr, o.ptr, lse.ptr, *args, dq.ptr, dk.ptr, dv.ptr, None if dtable is None else dtable.ptr,
+             at, h._backward_bytes, dev.stream), name)
+    return dq, dk, dv, dtable
+
+
+@functools.lru_cache(maxsize=4096)
+def _residual_norm_bytes(rows, dim, gates, elem_bytes):
+    return _L().sgh_residual_norm_bwd_workspace_bytes(rows, dim, gates, elem_bytes)
+
+
+def _norm_args(what, x, rows_tensors, h, post, gate, pre):
+    """The checks of both directions; (rows, dim, gates)."""
+    if not x._shape:
+        raise SingaHipError("%s: rows are expected" % what)
+    dim = x._shape[-1]
+    rows = x.Size() // dim if dim else 0
+    _plain(what, x._dev, x, h, post, gate, pre, *rows_tensors)
+    for t in (h,) + rows_tensors:
+        if t is not None and (t._shape != x._shape or t._dtype != x._dtype):
+            raise SingaHipError("%s: a tensor of the stream's shape and type is expected, got %s" % (what, t.shape()))
+    if h is None and (pre is None or post is not None or gate is not None):
+        raise SingaHipError("%s: a block's result, or else only the norm before a block, is expected" % what)
+    for t in (post, pre):
+        if t is not None and (t._dtype != kFloat32 or t._shape != (dim,)):
+            raise SingaHipError("%s: a float32 weight for each channel is expected, got %s" % (what, t.shape()))
+    gates = 0
+    if gate is not None:
+        gates = gate._shape[0] if len(gate._shape) == 2 else 0
+        if gate._dtype != x._dtype or gate._shape != (gates, dim) or (rows % gates if gates else rows):
+            raise SingaHipError("%s: a gate [gates, dim] of the stream's type whose rows divide the stream's is expected, got %s" %
+                                (what, gate.shape()))
+    return rows, dim, gates
+
+
+def _ptr(t):
+    return None if t is None else t.ptr
+
+
+def ResidualNormForward(x, h=None, post=None, gate=None, scale=1.0, pre=None, eps=1e-5):
+    """(y, n, stats): the end of one block and the start of the next.  `x` [..., dim] is the stream that passes by the block, `h` the block's
+    result; ``u = h / rms(h) * post`` (`post` None: h itself), ``y = x + scale * gate * u`` (`h` None: y is x), ``n = y / rms(y) * pre``
+    (`pre` None: n is None) with ``rms(a) = sqrt(mean(a * a) + eps)`` over a row.  `post`, `pre`: float32 [dim].  `gate` [gates, dim] of the
+    stream's type, each row for a stretch of rows / gates rows: one row for all, one for each sequence or one for each token.  `stats`
+    [rows, 2] is what ``ResidualNormBackward`` needs."""
+    rows, dim, gates = _norm_args("ResidualNormForward", x, (), h, post, gate, pre)
+    fn, name = _fn("residual_norm_fwd", x)
+    dev = x._dev
+    y = x if h is None else _like(x)
+    n = None if pre is None else _like(x)
+    stats = _empty(Tensor, (rows, 2), dev, kFloat32)
+    check(fn(x.ptr, _ptr(h), _ptr(post), _ptr(gate), _ptr(pre), rows, dim, gates, scale, eps, None if h is None else y.ptr, _ptr(n),
+             stats.ptr, dev.stream), name)
+    return y, n, stats
+
+
+def ResidualNormBackward(dy, dn, y, stats, h=None, post=None, gate=None, scale=1.0, pre=None):
+    """(dx, dh, dpost, dgate, dpre) of ``ResidualNormForward``, None where there is no such argument, from the gradients `dy` (None: 0) and
+    `dn` of its results, its `y` and its `stats`."""
+    rows, dim, gates = _norm_args("ResidualNormBackward", y, tuple(t for t in (dy, dn) if t is not None), h, post, gate, pre)
+    if (dn is None) != (pre is None) or (dy is None and dn is None):
+        raise SingaHipError("ResidualNormBackward: dn belongs to pre, and one of dy and dn is expected")
+    _plain("ResidualNormBackward", y._dev, stats)
+    if stats._dtype != kFloat32 or stats._shape != (rows, 2):
+        raise SingaHipError("ResidualNormBackward: the statistics do not match: %s" % stats.shape())
+    fn, name = _fn("residual_norm_bwd", y)
+    dev = y._dev
+    dx, dh, dpost, dgate, dpre = _like(y), *(None if t is None else _like(t) for t in (h, post, gate, pre))
+    need = _residual_norm_bytes(rows, dim, gates, 4 if y._dtype == kFloat32 else 2)
+    ws, at = _workspace(need, dev)
+    check(fn(_ptr(dy), _ptr(dn), y.ptr, stats.ptr, _ptr(h), _ptr(post), _ptr(gate), _ptr(pre), rows, dim, gates, scale, dx.ptr, _ptr(dh),
+             _ptr(dpost), _ptr(dgate), _ptr(dpre), at, need, dev.stream), name)
+    return dx, dh, dpost, dgate, dpre
+
+
 # ------------------------------------------------------------------------------------ operations
 
 # A handle's geometry goes to the library by address.  The address is asked for at every call: a copied or unpickled handle,

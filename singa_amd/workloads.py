@@ -164,6 +164,22 @@ class HipOps(object):
         return singa.DistillationFwdBwd(x, t.top, t.teacher, t.labels, t.weights, t.temperature, t.soft, t.hard,
                                         scale=float(np.float32(1.0) / np.float32(batch)))
 
+    # the middle of a token model: attention within sequences, and the norms, gate, scale and sum around a block
+    def attention_handle(self, q, k, causal, buckets, max_distance, bidirectional):
+        return singa.AttentionHandle(q, k, causal=causal, buckets=buckets, max_distance=max_distance, bidirectional=bidirectional)
+
+    def attention(self, h, q, k, v, table):
+        return singa.AttentionForward(h, q, k, v, table)
+
+    def attention_bwd(self, h, do, q, k, v, o, lse, table):
+        return singa.AttentionBackward(h, do, q, k, v, o, lse, table)
+
+    def residual_norm(self, x, h, post, gate, scale, pre):
+        return singa.ResidualNormForward(x, h, post, gate, scale, pre)
+
+    def residual_norm_bwd(self, dy, dn, y, stats, h, post, gate, scale, pre):
+        return singa.ResidualNormBackward(dy, dn, y, stats, h, post, gate, scale, pre)
+
     # backward
     def softmax_ce_bwd(self, p, t, batch):
         # SoftmaxCrossEntropyBwd followed by "dx /= N" (python/singa/autograd.py:1319-1322), fused
@@ -928,6 +944,145 @@ def build_token_mlp(ops, rng, lr=0.05, momentum=0.9, vocab=10000, dim=64, contex
     ], lr, momentum)
 
 
+class ResidualNorm(_Layer):
+    """The end of one block and the start of the next, see ``singa.ResidualNormForward``: without a block, the norm before the first."""
+
+    def __init__(self, ops, name, dim, block=True, scale=1.0):
+        self.ops, self.name, self.scale = ops, name, float(np.float32(scale))
+        ones = np.ones(dim, np.float32)
+        self.pre, self.post, self.gate = ops.from_numpy(ones), None, None
+        self.params = ("pre",)
+        if block:
+            self.post, self.gate = ops.from_numpy(ones), ops.from_numpy(ones[None, :])
+            self.params = ("post", "gate", "pre")
+
+    def fwd(self, x, h=None):
+        self.h = h
+        self.y, n, self.stats = self.ops.residual_norm(x, h, self.post, self.gate, self.scale, self.pre)
+        return self.y, n
+
+    def bwd(self, dy, dn, grads):
+        """(gradient of the stream, gradient of the block's result) from those of the stream behind the block (None: nothing reads it) and
+        of the normalised stream."""
+        dx, dh, dpost, dgate, dpre = self.ops.residual_norm_bwd(dy, dn, self.y, self.stats, self.h, self.post, self.gate, self.scale,
+                                                                self.pre)
+        for k, g in (("post", dpost), ("gate", dgate), ("pre", dpre)):
+            if g is not None:
+                grads(self.name + "." + k, getattr(self, k), g)
+        return dx, dh
+
+
+class Attention(_Layer):
+    """Attention between the tokens of each of `length` rows, with a learned position bias; one product for each of q, k, v and the result."""
+
+    def __init__(self, ops, name, rng, dim, length, heads, kv_heads, causal=True, buckets=16, max_distance=64):
+        self.ops, self.name, self.length, self.heads, self.kv_heads = ops, name, length, heads, kv_heads
+        self.mask = (causal, buckets, max_distance, not causal)
+        each = dim // heads
+
+        def linear(k, n_in, n_out):
+            return Linear(ops, name + "." + k, he_normal(rng, n_in, n_out) / np.float32(np.sqrt(2)), np.zeros(n_out, np.float32))
+
+        self.q, self.k, self.v = linear("q", dim, dim), linear("k", dim, kv_heads * each), linear("v", dim, kv_heads * each)
+        self.out = linear("out", dim, dim)
+        self.table = ops.from_numpy(rng.standard_normal((buckets, heads)).astype(np.float32))
+        self.params, self.h = ("table",), None
+
+    def sublayers(self):
+        return [self.q, self.k, self.v, self, self.out]
+
+    def _rows(self, t):
+        shape = self.ops.shape(t)
+        return self.ops.reshape(t, (shape[0] * shape[1], shape[2] * shape[3]))
+
+    def fwd(self, n):
+        def heads(t, count):
+            rows, width = self.ops.shape(t)
+            return self.ops.reshape(t, (rows // self.length, self.length, count, width // count))
+
+        self.saved = heads(self.q.fwd(n), self.heads), heads(self.k.fwd(n), self.kv_heads), heads(self.v.fwd(n), self.kv_heads)
+        if self.h is None:
+            self.h = self.ops.attention_handle(self.saved[0], self.saved[1], *self.mask)
+        self.o, self.lse = self.ops.attention(self.h, *self.saved, self.table)
+        return self.out.fwd(self._rows(self.o))
+
+    def bwd(self, dy, grads):
+        do = self.ops.reshape(self.out.bwd(dy, grads), self.ops.shape(self.o))
+        dq, dk, dv, dtable = self.ops.attention_bwd(self.h, do, *self.saved, self.o, self.lse, self.table)
+        grads(self.name + ".table", self.table, dtable)
+        dn = self.q.bwd(self._rows(dq), grads)
+        for layer, d in ((self.k, dk), (self.v, dv)):
+            dn = self.ops.accumulate(dn, layer.bwd(self._rows(d), grads))
+        return dn
+
+
+class FeedForward(_Layer):
+    """Two dense layers with a ReLU between them."""
+
+    def __init__(self, ops, name, rng, dim, hidden):
+        self.up = Linear(ops, name + ".up", he_normal(rng, dim, hidden), np.zeros(hidden, np.float32))
+        self.relu = ReLU(ops, name + ".relu")
+        self.down = Linear(ops, name + ".down", he_normal(rng, hidden, dim), np.zeros(dim, np.float32))
+
+    def sublayers(self):
+        return [self.up, self.relu, self.down]
+
+    def fwd(self, n):
+        return self.down.fwd(self.up.fwd_through_relu(self.relu, n))
+
+    def bwd(self, dy, grads):
+        return self.up.bwd(self.down.bwd_behind_relu(self.relu, dy, grads), grads)
+
+
+class Blocks(_Layer):
+    """Attention and feed-forward blocks along a stream of rows, a norm before and behind each; the result is the normalised stream."""
+
+    def __init__(self, ops, name, rng, dim, blocks, scale, **attention):
+        self.ops, self.first = ops, ResidualNorm(ops, name + ".norm", dim, block=False)
+        self.blocks = []
+        for i in range(blocks):
+            at = "%s.%d" % (name, i)
+            for block in (Attention(ops, at + ".attention", rng, dim, **attention), FeedForward(ops, at + ".dense", rng, dim, 4 * dim)):
+                self.blocks.append((block, ResidualNorm(ops, "%s.%d.norm%d" % (name, i, len(self.blocks) % 2), dim, scale=scale)))
+
+    def sublayers(self):
+        out = [self.first]
+        for block, norm in self.blocks:
+            out += block.sublayers() + [norm]
+        return out
+
+    def fwd(self, x):
+        self.shape = self.ops.shape(x)
+        x, n = self.first.fwd(self.ops.reshape(x, (int(np.prod(self.shape[:-1])), self.shape[-1])))
+        for block, norm in self.blocks:
+            x, n = norm.fwd(x, block.fwd(n))
+        return n
+
+    def bwd(self, dn, grads):
+        dy = None
+        for block, norm in reversed(self.blocks):
+            dy, dh = norm.bwd(dy, dn, grads)
+            dn = block.bwd(dh, grads)
+        return self.ops.reshape(self.first.bwd(dy, dn, grads)[0], self.shape)
+
+
+class SequenceNet(TokenNet):
+    """A ``TokenNet`` that learns the next token of every place of its sequences: the loss is the mean over all of them."""
+
+    def loss(self, x, targets):
+        self.batch = self.ops.shape(x)[0]
+        return TokenNet.loss(self, x, targets)
+
+
+def build_token_attention(ops, rng, lr=0.05, momentum=0.9, vocab=10000, dim=64, length=64, heads=4, kv_heads=2, blocks=2):
+    """Sequences of `length` tokens through blocks of causal attention and dense layers to every next token's logits."""
+    return SequenceNet(ops, [
+        Embedding(ops, "embedding", (rng.standard_normal((vocab, dim)) / np.sqrt(dim)).astype(np.float32), np.sqrt(dim)),
+        Blocks(ops, "blocks", rng, dim, blocks, scale=1.0 / np.sqrt(2 * blocks), length=length, heads=heads, kv_heads=kv_heads),
+        Linear(ops, "linear", he_normal(rng, dim, vocab) / np.float32(np.sqrt(2)), np.zeros(vocab, np.float32)),
+    ], lr, momentum)
+
+
 def build_mlp(ops, rng, lr=0.05, momentum=0.9, in_dim=784, hidden=1000, classes=10):
     return Net(ops, [
         Linear(ops, "linear1", he_normal(rng, in_dim, hidden), np.zeros(hidden, np.float32)),
@@ -1017,6 +1172,9 @@ CONFIGS = {
     # token ids to the next token's logits, distillation loss
     "token_mlp": (build_token_mlp, {}, (4,), 10000, 256),
     "token_mlp_small": (build_token_mlp, {"vocab": 1003, "dim": 20, "hidden": 48}, (4,), 1003, 24),
+    # sequences of token ids to all next tokens' logits, attention and dense blocks
+    "token_attention": (build_token_attention, {}, (64,), 10000, 32),
+    "token_attention_small": (build_token_attention, {"vocab": 301, "dim": 24, "length": 11, "heads": 3, "kv_heads": 1, "blocks": 1}, (11,), 301, 5),
 }
 
 SEED_BASE = 0x5167A000
@@ -1025,7 +1183,7 @@ SEED_BASE = 0x5167A000
 # splitmix64 -> Box-Muller), so the bytes do not depend on a library's random stream and a smaller batch is
 # a prefix of a larger one.  (Fixed numbers: adding a configuration leaves the inputs of the others unchanged.)
 _CONFIG_INDEX = {"mlp": 1, "conv": 2, "cnn": 3, "resnet18": 4, "resnet50": 5, "resnet18_small": 6, "smoke_cnn": 7,
-                 "resnet50_small": 8, "token_mlp": 9, "token_mlp_small": 10}
+                 "resnet50_small": 8, "token_mlp": 9, "token_mlp_small": 10, "token_attention": 11, "token_attention_small": 12}
 TOP_LOGITS = 16   # of a token model's teacher
 
 
@@ -1033,11 +1191,12 @@ def make_inputs(name, batch=None):
     builder, kw, xshape, classes, default_batch = CONFIGS[name]
     batch = batch or default_batch
     base = SEED_BASE + 256 * _CONFIG_INDEX[name]
-    if builder is build_token_mlp:
+    if builder in (build_token_mlp, build_token_attention):
         # (tensors 0 and 1 as for the others; 254 and 255, behind the weights, are the teacher's)
-        labels = rng.integers(base + 1, (batch,), classes)
-        top = (rng.integers(base + 254, (batch, 1), classes) + 7 * np.arange(TOP_LOGITS)).astype(np.int32) % classes
-        return rng.integers(base + 0, (batch,) + xshape, classes), Targets(labels, top, 2 * rng.normal(base + 255, (batch, TOP_LOGITS)))
+        rows = batch if builder is build_token_mlp else batch * xshape[0]
+        labels = rng.integers(base + 1, (rows,), classes)
+        top = (rng.integers(base + 254, (rows, 1), classes) + 7 * np.arange(TOP_LOGITS)).astype(np.int32) % classes
+        return rng.integers(base + 0, (batch,) + xshape, classes), Targets(labels, top, 2 * rng.normal(base + 255, (rows, TOP_LOGITS)))
     x = rng.normal(base + 0, (batch,) + xshape)
     labels = rng.integers(base + 1, (batch,), classes)
     return x, labels

@@ -1,0 +1,347 @@
+"""Attention and its gradients on the GPU against their definitions in 64 bits (oracle/block_ops.py), at the sizes, types, head layouts and masks
+where they can go wrong.
+
+Tolerances, first order, u = 2^-24 half a step of fp32 and h half a step of the tensors' type.  A score is a product of D terms and two sums: off
+by (D + 4) u sum |scale q k| + 4 u (|score| + |bias| + |lse|), and the power of two is good to 2 u; that, E, is a probability's relative error.
+In 16-bit tensors p and ds are rounded once more before the products over them (h; binary16 is scaled so that what is below its range is
+at most 2^-31 of a row's largest), sums of n terms are off by n u of their sizes, and results by h."""
+import numpy as np
+import pytest
+
+from oracle import block_ops as O
+from test_gpu_token_model import HALF, TINY, TYPES, U, close, ints, shifted, stored, upload
+
+pytestmark = pytest.mark.gpu
+
+
+def handle(singa, q, k, a):
+    return singa.AttentionHandle(q, k, causal=a.causal, scale=a.scale, buckets=a.buckets, max_distance=a.max_distance, bidirectional=a.bidirectional)
+
+
+def bounds(t, a, do, q, k, v, o, table, q_lengths, k_lengths, q_starts):
+    """(of o, lse, dq, dk, dv, dtable), terms as in the module's description."""
+    b, sq, h, d = q.shape
+    sk = k.shape[1]
+    half = 0.0 if t == "f32" else HALF[t]
+    scale = d ** -0.5 if a.scale is None else a.scale
+    n = sk + 64
+    eo, el = np.zeros(q.shape), np.zeros((b, h, sq))
+    eq, ek, ev, et = np.zeros(q.shape), np.zeros(k.shape), np.zeros(v.shape), None if table is None else np.zeros(table.shape)
+    group = h // k.shape[2]
+    for i, head, kv, s, mask, which in O._each(a, q, k, table, q_lengths, k_lengths, q_starts):
+        row, key = mask.any(1), mask.any(0)
+        some = np.isfinite(s).any(1)
+        top = np.where(some, s.max(1, initial=-np.inf), 0.0)
+        lse = np.where(some, top + np.log(np.where(some, np.exp(s - top[:, None]).sum(1), 1.0)), 0.0)
+        p = np.exp(s - lse[:, None])
+        Q, K, V = (np.abs(O._rows(x, keep)) for x, keep in ((q[i, :, head], row), (k[i, :, kv], key), (v[i, :, kv], key)))
+        size = np.where(mask & np.isfinite(s), np.abs(s), 0.0)
+        extra = 0.0 if which is None else np.abs(np.where(np.isfinite(table[:, head]), table[:, head], 0.0))[which]
+        E = (d + 4) * U * abs(scale) * (Q @ K.T) + 4 * U * (size + extra + np.abs(lse)[:, None]) + 4 * U
+        Er = np.where(mask, E, 0.0).max(1, initial=0.0)[:, None]
+        el[i, head] = Er[:, 0] + n * U + 2 * U * np.abs(lse)
+        eo[i, :, head] = (2 * Er + half + n * U) * (p @ V) + 2.0 ** -31 * V.sum(0)
+        if do is None:
+            continue
+        dd, x = O._rows(do[i, :, head], row), O._rows(o[i, :, head], row)
+        D, X = np.abs(dd), np.abs(x)
+        gap = dd @ O._rows(v[i, :, kv], key).T - (dd * x).sum(1)[:, None]
+        Ep = E + 2 * U * np.abs(lse)[:, None]
+        Es = p * (np.abs(gap) * (Ep + 2 * U) + (d + 4) * U * (D @ V.T + (D * X).sum(1)[:, None]))
+        ds = np.abs(p * gap)
+        lost = 2.0 ** -33
+        eq[i, :, head] = abs(scale) * ((Es + (half + n * U) * ds + lost * ds.max(1, initial=0.0)[:, None]) @ K)
+        ek[i, :, kv] += abs(scale) * ((Es + (half + (group * sq + 64) * U) * ds + lost * ds.max(0, initial=0.0)[None]).T @ Q)
+        ev[i, :, kv] += (p * (Ep + half + (group * sq + 64) * U) + 2.0 ** -38).T @ D
+        if which is not None:
+            np.add.at(et[:, head], which[mask], (Es + (b * sq * sk / 16 + 400) * U * ds)[mask])
+    return eo, el, eq, ek, ev, et
+
+
+def check(singa, dev, t, a, b, sq, sk, h, g, d, lengths=(None, None, None), seed=0, shift=0, sharp=1.5, grads=True, case=None):
+    r = np.random.default_rng(seed + sq + 7 * sk + 31 * h + d)
+    if case is None:
+        q, k, v, do = (stored(t, s * r.standard_normal(shape)) for s, shape in ((sharp, (b, sq, h, d)), (1, (b, sk, g, d)), (1, (b, sk, g, d)), (1, (b, sq, h, d))))
+        table = stored("f32", r.standard_normal((a.buckets, h))) if a.buckets else None
+    else:
+        q, k, v, do, table = case
+    put = (lambda x: shifted(singa, dev, t, x, shift)) if shift else (lambda x: upload(singa, dev, t, x))
+    dq_, dk_, dv_, ddo = (put(x) for x in (q, k, v, do))
+    dt = None if table is None else upload(singa, dev, "f32", table)
+    dl = dict(zip(("q_lengths", "k_lengths", "q_starts"), (None if x is None else ints(singa, dev, x) for x in lengths)))
+    H = handle(singa, dq_, dk_, a)
+    go, gl = singa.AttentionForward(H, dq_, dk_, dv_, dt, **dl)
+    wo, wl = O.attention(a, q, k, v, table, *lengths)
+    o = go.to_numpy().astype(np.float64)
+    eo, el, eq, ek, ev, et = bounds(t, a, do if grads else None, q, k, v, o, table, *lengths)
+
+    def rounded(bound, want):
+        return bound * 1.01 + HALF[t] * np.abs(want) * 1.01 + TINY[t]
+
+    close(o, wo, rounded(eo, wo), "o")
+    close(gl.to_numpy(), wl, el * 1.01, "lse")
+    if not grads:
+        return go, gl
+    got = singa.AttentionBackward(H, ddo, dq_, dk_, dv_, go, gl, dt, **dl)
+    want = O.attention_bwd(a, do, q, k, v, o, gl.to_numpy().astype(np.float64), table, *lengths)
+    for name, x, w, e in zip(("dq", "dk", "dv"), got, want, (eq, ek, ev)):
+        close(x.to_numpy(), w, rounded(e, w), name)
+    if table is not None:
+        close(got[3].to_numpy(), want[3], et * 1.01 + U * np.abs(want[3]), "dtable")
+    else:
+        assert got[3] is None
+    again = singa.AttentionBackward(H, ddo, dq_, dk_, dv_, go, gl, dt, **dl)
+    for x, y in zip(got, again):
+        assert x is y is None or np.array_equal(x.to_numpy(), y.to_numpy(), equal_nan=True)   # the same bits every time
+    return go, gl
+
+
+# (batch, queries, keys, heads, heads of keys, dim): one of everything, tiles that are not full, one more than full, long ones, groups
+SIZES = [(1, 1, 1, 1, 1, 1), (2, 3, 5, 2, 2, 8), (1, 33, 31, 3, 1, 16), (2, 64, 64, 2, 2, 32), (1, 65, 129, 4, 2, 33), (3, 128, 128, 1, 1, 64),
+         (1, 129, 257, 2, 1, 63), (2, 37, 37, 4, 4, 40), (1, 300, 300, 2, 2, 96), (1, 200, 333, 3, 3, 100), (1, 257, 130, 4, 1, 128),
+         (1, 5, 700, 8, 1, 65), (1, 1, 1500, 6, 2, 64), (2, 2, 900, 4, 4, 127), (1, 700, 40, 2, 2, 24), (1, 515, 515, 1, 1, 72)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("size", SIZES)
+def test_attention(dev, t, causal, size):
+    from singa_amd import singa_wrap as singa
+    check(singa, dev, t, O.Attn(causal), *size)
+
+
+# few buckets, a band that ends inside a tile, one that reaches over all distances, no gap between the buckets' borders
+BIAS = [(4, 3, True), (8, 20, True), (32, 128, True), (2, 5, False), (16, 64, False), (32, 100, False), (128, 1024, True)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("buckets,distance,both", BIAS)
+@pytest.mark.parametrize("causal,size", [(False, (2, 70, 70, 2, 2, 16)), (True, (1, 200, 200, 4, 2, 40)), (False, (1, 150, 301, 2, 1, 64)),
+                                         (True, (1, 1, 600, 8, 2, 32)), (False, (1, 400, 17, 3, 3, 128))])
+def test_attention_with_a_position_bias(dev, t, buckets, distance, both, causal, size):
+    from singa_amd import singa_wrap as singa
+    check(singa, dev, t, O.Attn(causal, buckets=buckets, max_distance=distance, bidirectional=both), *size)
+
+
+# lengths of zero, one and all; more than there is and less than none; queries in front of every key, and behind
+LENGTHS = [((0, 1, 90, 64), (0, 1, 90, 64), None), (None, (90, 0, 33, 1), None), ((90, 500, -3, 64), (1000, 90, 90, -1), None),
+           (None, None, (0, 60, -40, -200)), ((5, 90, 90, 90), (90, 70, 90, 0), (-(1 << 30), 1 << 30, 17, 0))]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("causal,buckets", [(False, 0), (True, 0), (True, 16), (False, 16)])
+@pytest.mark.parametrize("lengths", LENGTHS)
+def test_padded_batches(dev, t, causal, buckets, lengths):
+    """Rows behind a sequence hold NaN and infinities: they reach nothing, and their results are 0."""
+    from singa_amd import singa_wrap as singa
+    if buckets and lengths[2] is not None:
+        lengths = (lengths[0], lengths[1], tuple(max(-300, min(300, x)) for x in lengths[2]))   # (the oracle lists the distances)
+    r = np.random.default_rng(5)
+    b, sq, sk, h, g, d = 4, 90, 90, 4, 2, 24
+    case = [stored(t, r.standard_normal(s)) for s in ((b, sq, h, d), (b, sk, g, d), (b, sk, g, d), (b, sq, h, d))]
+    for i in range(b):
+        for which, n in ((0, lengths[0]), (3, lengths[0]), (1, lengths[1]), (2, lengths[1])):
+            if n is not None:
+                rest = case[which][i, max(0, n[i]):]
+                rest[...] = np.resize([np.nan, np.inf, -np.inf], rest.shape)
+    case.append(stored("f32", r.standard_normal((buckets, h))) if buckets else None)
+    check(singa, dev, t, O.Attn(causal, buckets=buckets, max_distance=40), b, sq, sk, h, g, d, lengths=lengths, case=case)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_one_new_token_over_caches_of_different_lengths(dev, t):
+    from singa_amd import singa_wrap as singa
+    keys = (1, 3000, 64, 1999, 0)
+    starts = tuple(n - 1 for n in keys)
+    for buckets, (h, g) in ((0, (8, 2)), (32, (8, 2)), (32, (3, 3))):
+        check(singa, dev, t, O.Attn(True, buckets=buckets, bidirectional=False), 5, 1, 3000, h, g, 48, lengths=(None, keys, starts))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("d", [1, 7, 8, 64, 70])
+def test_tensors_at_any_element(dev, t, d):
+    from singa_amd import singa_wrap as singa
+    for shift in (1, 2, 8):
+        check(singa, dev, t, O.Attn(True, buckets=8, max_distance=30), 2, 70, 100, 2, 1, d, shift=shift)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_no_queries_no_keys_no_sequences(dev, t):
+    from singa_amd import singa_wrap as singa
+    for a in (O.Attn(), O.Attn(True, buckets=4, max_distance=9)):
+        for size in ((2, 0, 5, 2, 1, 16), (2, 5, 0, 2, 1, 16), (0, 5, 5, 2, 1, 16)):
+            b, sq, sk, h, g, d = size
+            q, k = singa.Tensor((b, sq, h, d), dev, upload(singa, dev, t, [0.0]).data_type()), singa.Tensor((b, sk, g, d), dev, upload(singa, dev, t, [0.0]).data_type())
+            table = upload(singa, dev, "f32", np.ones((a.buckets, h))) if a.buckets else None
+            if q.Size():
+                q.SetFloatValue(1.0)
+            if k.Size():
+                k.SetFloatValue(1.0)
+            H = handle(singa, q, k, a)
+            o, lse = singa.AttentionForward(H, q, k, k, table)
+            dq, dk, dv, dtable = singa.AttentionBackward(H, q, q, k, k, o, lse, table)
+            for x in (o, dq, dk, dv) + ((dtable,) if table is not None else ()):
+                assert not x.to_numpy().any()
+            assert (lse.to_numpy() == -np.inf).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_peaked_and_flat_rows(dev, t):
+    """Scores far apart (one key takes all), equal ones, and a bias of -inf for some buckets (those keys take nothing)."""
+    from singa_amd import singa_wrap as singa
+    check(singa, dev, t, O.Attn(), 1, 130, 260, 2, 2, 64, sharp=12.0)
+    check(singa, dev, t, O.Attn(True, scale=0.0), 1, 130, 260, 2, 2, 64)
+    check(singa, dev, t, O.Attn(scale=-0.3), 1, 40, 50, 2, 2, 20)
+    r = np.random.default_rng(1)
+    a = O.Attn(buckets=8, max_distance=16)
+    case = [stored(t, r.standard_normal(s)) for s in ((1, 90, 2, 16),) * 4] + [stored("f32", r.standard_normal((8, 2)))]
+    case[4][0, 0] = case[4][3, 1] = case[4][6, 1] = -np.inf
+    check(singa, dev, t, a, 1, 90, 90, 2, 2, 16, case=case, grads=False)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("size", [1e-6, 1.0, 3e3])
+def test_gradients_of_any_size(dev, t, size):
+    """The products over the probabilities' gradients keep their bits whatever the size of the result's gradient: halves' small ones as well.  The
+    bound on what leaves the type is the type's own (half of its smallest step), on top of the usual one."""
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(3)
+    q, k, v = (stored(t, 0.5 * r.standard_normal((1, 300, 2, 64))) for _ in range(3))
+    do = stored(t, size * r.standard_normal((1, 300, 2, 64)))
+    do[:, ::3] *= 0.125
+    do = stored(t, do)   # (what the device holds: the small ones lose bits)
+    check(singa, dev, t, O.Attn(True), 1, 300, 300, 2, 2, 64, case=(q, k, v, do, None))
+
+
+def test_gradients_against_differences(dev):
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(2)
+    a = O.Attn(True, buckets=6, max_distance=11)
+    q, k, v, do = (stored("f32", r.standard_normal(s)) for s in ((2, 40, 4, 16), (2, 45, 2, 16), (2, 45, 2, 16), (2, 40, 4, 16)))
+    table = stored("f32", r.standard_normal((6, 4)))
+    lengths = ((40, 31), (45, 37), None)
+    dl = dict(q_lengths=ints(singa, dev, lengths[0]), k_lengths=ints(singa, dev, lengths[1]))
+    dq, dk, dv, ddo, dt = (upload(singa, dev, "f32", x) for x in (q, k, v, do, table))
+    H = handle(singa, dq, dk, a)
+    o, lse = singa.AttentionForward(H, dq, dk, dv, dt, **dl)
+    grads = singa.AttentionBackward(H, ddo, dq, dk, dv, o, lse, dt, **dl)
+    args, step = [q, k, v, table], 1e-4
+    for i, g in enumerate(grads):
+        along = r.standard_normal(args[i].shape)
+        along /= np.linalg.norm(along)
+        ends = []
+        for sign in (1, -1):
+            moved = [x + sign * step * along if j == i else x for j, x in enumerate(args)]
+            ends.append((O.attention(a, *moved, *lengths)[0] * do).sum())
+        got = (g.to_numpy().astype(np.float64) * along).sum()
+        # the third derivative over step^2 / 6 is below 1e3 * 1e-8 / 6 of |do| |v|; fp32 gradients of up to 45 terms: 1e-5
+        assert abs(got - (ends[0] - ends[1]) / (2 * step)) < 1e-4 * max(1.0, np.linalg.norm(g.to_numpy())), i
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_recorded_calls_replay(dev, t):
+    """A forward and a backward pass of two sizes in one recording, replayed on other values with the program's own calls in between."""
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(4)
+    a = O.Attn(True, buckets=16, max_distance=50, bidirectional=False)
+    sizes = [(2, 150, 150, 4, 2, 32), (1, 1, 1300, 8, 2, 64), (1, 20, 900, 2, 2, 40)]
+    made = []
+    for b, sq, sk, h, g, d in sizes:
+        ts = [upload(singa, dev, t, r.standard_normal(s)) for s in ((b, sq, h, d), (b, sk, g, d), (b, sk, g, d), (b, sq, h, d))]
+        made.append((handle(singa, ts[0], ts[1], a), ts, upload(singa, dev, "f32", r.standard_normal((16, h)))))
+
+    def run():
+        out = []
+        for H, (q, k, v, do), table in made:
+            o, lse = singa.AttentionForward(H, q, k, v, table)
+            out += [o, lse, *singa.AttentionBackward(H, do, q, k, v, o, lse, table)]
+        return out
+
+    run()
+    dev.Sync()
+    dev.EnableGraph(True)
+    kept = run()
+    dev.EnableGraph(False)
+    try:
+        for turn in range(4):
+            for _, ts, table in made:
+                for x in ts:
+                    fresh = stored(t, r.standard_normal(x.shape()))
+                    if t == "f32":
+                        x.CopyFloatDataFromHostPtr(fresh)
+                    else:
+                        x.CopyHalfDataFromHostPtr(fresh.astype(np.float16) if t == "f16" else singa.float_to_bf16_bits(fresh))
+            dev.RunGraph()
+            want = run()
+            dev.Sync()
+            for x, y in zip(kept, want):
+                x, y = x.to_numpy(), y.to_numpy()
+                assert np.isfinite(y).all() and np.array_equal(x, y), turn
+    finally:
+        dev.ResetGraph()
+
+
+def test_two_streams_at_once(dev):
+    """Calls on the auxiliary stream beside others on the main one: each has its own workspace."""
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(6)
+    q, k, do = (upload(singa, dev, "bf16", r.standard_normal(s)) for s in ((1, 300, 4, 64), (1, 700, 2, 64), (1, 300, 4, 64)))
+    H = singa.AttentionHandle(q, k, causal=True)
+    o, lse = singa.AttentionForward(H, q, k, k)
+    want = [o, lse, *singa.AttentionBackward(H, do, q, k, k, o, lse)[:3]]
+    want = [x.to_numpy() for x in want]
+
+    class _Beside(object):
+        def __init__(self, stream):
+            self.__dict__.update(dev.__dict__)
+            self.stream = stream
+
+    for _ in range(3):
+        aux = dev.Fork()
+        held, out = [], []
+        main = dev.stream
+        for turn in range(4):
+            dev.stream = aux if turn % 2 else main
+            try:
+                o, lse = singa.AttentionForward(H, q, k, k)
+                out.append([o, lse, *singa.AttentionBackward(H, do, q, k, k, o, lse)[:3]])
+            finally:
+                dev.stream = main
+            held.append(out[-1])
+            if turn % 2:
+                dev.UsedOn(aux, q, k, do, *out[-1])
+            dev.Join() if turn == 3 else None
+        dev.Sync()
+        for each in out:
+            for x, w in zip(each, want):
+                assert np.array_equal(x.to_numpy(), w)
+
+
+def test_a_long_cache_with_offsets_beyond_32_bits(dev):
+    """Keys of more than 2^32 bytes in all and for one sequence: the last sequence's and the last rows' are the ones that count."""
+    from singa_amd import singa_wrap as singa
+    sk, g, d = 1 << 20, 16, 128          # 4 GB of bfloat16 for a sequence
+    b = 2
+    k = singa.Tensor((b, sk, g, d), dev, singa.kBFloat16)
+    k.SetFloatValue(0.0)
+    r = np.random.default_rng(8)
+    rows = 300
+    tail = stored("bf16", r.standard_normal((rows, g, d)))
+    bits = singa.float_to_bf16_bits(tail)
+    at = k.ptr + (k.Size() - tail.size) * 2
+    view = singa.from_device_pointer(at, tail.shape, dev, singa.kBFloat16, keepalive=k)
+    view.CopyHalfDataFromHostPtr(bits)
+    q = stored("bf16", r.standard_normal((b, 1, g, d)))
+    dq = upload(singa, dev, "bf16", q)
+    H = singa.AttentionHandle(dq, k)
+    o, lse = singa.AttentionForward(H, dq, k, k)
+    s = np.einsum("hd,rhd->hr", q[1, 0], tail) * d ** -0.5
+    e = np.exp(s)
+    total = e.sum(1) + (sk - rows)       # keys of zeros have a score of 0
+    want = np.einsum("hr,rhd->hd", e, tail) / total[:, None]
+    got = o.to_numpy().astype(np.float64)
+    assert not got[0].any()
+    # the sums of up to 2^20 equal terms in chains of at most 2^14: 2^-10; a probability's and the result's rounding
+    size = np.einsum("hr,rhd->hd", e, np.abs(tail)) / total[:, None]
+    assert (np.abs(got[1, 0] - want) <= 3 * 2.0 ** -8 * size).all()
+    np.testing.assert_allclose(lse.to_numpy()[:, :, 0], np.stack([np.full(g, np.log(sk)), np.log(total)]), rtol=0, atol=2.0 ** -10)
