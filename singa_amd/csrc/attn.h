@@ -21,7 +21,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef __amdgpu_buffer_rsrc_t rsrc_t;
 
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 constexpr float kNegInf = -__builtin_inff();
@@ -100,37 +99,56 @@ typedef u32x4 frag_t;
 
 // ------------------------------------------------------------------------------------ tiles in LDS
 
-// A tile holds rows of DP values, 16-byte chunks [row][RS], RS a power of two.  Chunk c of row r lies at place c ^ turn(r), so that
-// neither the reads of one chunk of 32 rows nor those of 64 bytes of four rows meet in a bank.
+// A tile holds rows of DP values, 16-byte chunks [row][RS], RS a power of two, in groups of 1024 bytes (what one load of a wavefront writes) that
+// are 1040 bytes apart.  Chunk c of row r lies at place c ^ turn(r) of its row.  With both, the two ways in which a tile is read meet in no bank
+// (64 of 4 bytes): one chunk of 16 rows, and four chunks of four rows.  turn() moves two bits of a chunk's number and is the same 8 rows on
+// (but for the shortest rows), so that a lane has a handful of addresses, and all others are those and a constant.  (Without the 16 bytes, by three
+// turned bits, half of the LDS's cycles were conflicts.)
 template <class T, int DP>
 struct Tile {
   static constexpr int CH = DP / T::VEC;                       // chunks of a row that are used
   static constexpr int RS = CH <= 4 ? 4 : CH <= 8 ? 8 : CH <= 16 ? 16 : 32;
-  static constexpr int BYTES_OF_ROW = RS * 16;
-  static __device__ __forceinline__ int turn(int r) {
-    if constexpr (!T::half) return RS >= 16 ? (((r >> 2) & 1) << 3) | ((r & 3) << 1) | ((r >> 3) & 1) : (r >> 1) & (RS - 1);
-    if constexpr (RS == 16) return ((r & 3) << 2) | ((r >> 2) & 3);
-    if constexpr (RS == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
-    return (r >> 2) & 3;
+  static constexpr int G = 64 / RS, GROUP = 1040;              // rows of a group
+  static constexpr int bytes(int rows) { return rows / G * GROUP; }
+  static __device__ __forceinline__ constexpr int turn(int r) {
+    if constexpr (RS == 4) return (r >> 2) & 3;
+    if constexpr (RS == 8) return ((r >> 1) & 1) << 2 | ((r >> 2) & 1) << 1;
+    if constexpr (RS == 16) return (r & 3) << 2;
+    return (r & 1) << 3;
   }
-  static __device__ __forceinline__ int place(int r, int c) { return (r * RS + (c ^ turn(r))) * 16; }
+  static __device__ __forceinline__ int place(int r, int c) { return r / G * GROUP + (r % G * RS + (c ^ turn(r))) * 16; }
 };
 
-typedef __attribute__((address_space(3))) void lds_void;
-// 16 bytes for each lane, one behind the other from `lds` on
-__device__ __forceinline__ void load_lds16(rsrc_t rs, lds_void *lds, int voff) {
-#ifdef __HIP_DEVICE_COMPILE__   // (the host's pass takes this size for an error, and then drops kernels that call it, without a word)
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds, 16, voff, 0, 0, 0);
-#endif
+// Loads that write LDS: what the compiler knows of them it waits for in front of every transposed read, whichever tile that reads, so they are
+// assembly (with no register to wait for), and tiles_arrive() waits for them.
+typedef unsigned rsrc4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ rsrc4_t buffer_of(const void *p, int bytes) {
+  const unsigned long long a = reinterpret_cast<unsigned long long>(p);
+  return rsrc4_t{unsigned(a), unsigned(a >> 32) & 0xffffu, unsigned(bytes), 0x00020000u};   // (the same for all lanes)
+}
+__device__ __forceinline__ unsigned lds_offset(const void *lds) {
+  typedef __attribute__((address_space(3))) const void lds_void;
+  return unsigned(size_t((lds_void *)lds));
+}
+// (m0 is the compiler's to set wherever it needs it, as here: it keeps nothing there.)
+// 16 (4) bytes for each lane, one behind the other from `lds` on, the same for the whole wavefront; offsets behind the buffer give zeros
+__device__ __forceinline__ void load_lds16(rsrc4_t buffer, unsigned lds, int offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(int(lds))), "v"(offset), "s"(buffer)
+               : "memory");
+}
+__device__ __forceinline__ void load_lds4(rsrc4_t buffer, unsigned lds, int offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(int(lds))), "v"(offset), "s"(buffer)
+               : "memory");
 }
 
 // Copies rows of a matrix into a tile.  Rows from `rows` on and values from `dim` on become zeros, whatever lies there.
-template <class T, int DP, int ROWS>
+template <class T, int DP, int ROWS, int NT = kBlock>
 struct Stage {
   typedef typename T::elem elem;
   typedef Tile<T, DP> L;
-  static constexpr int N = ROWS * L::RS / kBlock;   // chunks of a thread
-  static_assert(N * kBlock == ROWS * L::RS, "whole rounds");
+  static constexpr int N = (ROWS * L::RS + NT - 1) / NT;   // chunks of a thread
+  static_assert(ROWS * L::RS % SGH_WAVE == 0, "whole wavefronts");
+  static constexpr bool kPart = N * NT != ROWS * L::RS;    // (the last wavefronts have one less)
   int voff[N];
   size_t stride;   // elements from row to row
   int dim;
@@ -140,23 +158,32 @@ struct Stage {
     stride = stride_, dim = dim_, direct = direct_;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int p = j * kBlock + int(threadIdx.x), r = p / L::RS, c = (p % L::RS) ^ L::turn(r);
+      const int p = j * NT + int(threadIdx.x), r = p / L::RS, c = (p % L::RS) ^ L::turn(r);
       voff[j] = c * T::VEC < dim ? int((r * stride + size_t(c) * T::VEC) * sizeof(elem)) : kOOB;
     }
+  }
+  // loads of a wavefront
+  __device__ __forceinline__ int loads(int wave) const {
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) n += !kPart || j * NT + wave * SGH_WAVE < ROWS * L::RS;
+    return n;
   }
   __device__ __forceinline__ void operator()(char *lds, const elem *p, int rows) const {
     rows = min(rows, ROWS);
     if (direct) {
-      const int bytes = rows > 0 ? int(((rows - 1) * stride + dim) * sizeof(elem)) : 0;
-      const rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<elem *>(p), 0, bytes, 0x00020000);
-      char *at = lds + __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6) * 1024;
+      const int bytes = rows > 0 ? ((rows - 1) * int(stride) + dim) * int(sizeof(elem)) : 0;   // (heads * dim is at most 2^20)
+      const rsrc4_t buffer = buffer_of(p, bytes);
+      const unsigned to = lds_offset(lds);
+      const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
 #pragma unroll
-      for (int j = 0; j < N; ++j) load_lds16(rs, (lds_void *)(at + j * kBlock * 16), voff[j]);
+      for (int j = 0; j < N; ++j)
+        if (!kPart || j * NT + wave * SGH_WAVE < ROWS * L::RS) load_lds16(buffer, to + (wave + j * NT / SGH_WAVE) * L::GROUP, voff[j]);
     } else {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const int q = j * kBlock + int(threadIdx.x), r = q / L::RS, c = (q % L::RS) ^ L::turn(r);
-        *reinterpret_cast<u32x4 *>(lds + q * 16) = chunk(p + r * stride, c * T::VEC, r < rows ? dim : 0);
+        const int q = j * NT + int(threadIdx.x), r = q / L::RS, c = (q % L::RS) ^ L::turn(r);
+        if (!kPart || q < ROWS * L::RS) *reinterpret_cast<u32x4 *>(lds + q / SGH_WAVE * L::GROUP + q % SGH_WAVE * 16) = chunk(p + r * stride, c * T::VEC, r < rows ? dim : 0);
       }
     }
   }
@@ -175,6 +202,22 @@ struct Stage {
     return v;
   }
 };
+// Loads into registers have arrived (vmcnt(0)).  In front of a loop that requests tiles: the compiler would otherwise wait for them inside, where they are used,
+// and with that for every tile on its way.
+__device__ __forceinline__ void registers_arrive() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
+// The same where up to `behind` later loads of this wavefront may be under way (0 to 15)
+__device__ __forceinline__ void tiles_arrive(int behind) {
+#define SGH_WAIT(N) case N: asm volatile("s_waitcnt vmcnt(" #N ") lgkmcnt(0)" ::: "memory"); break;
+  switch (behind) {
+    SGH_WAIT(1) SGH_WAIT(2) SGH_WAIT(3) SGH_WAIT(4) SGH_WAIT(5) SGH_WAIT(6) SGH_WAIT(7) SGH_WAIT(8) SGH_WAIT(9) SGH_WAIT(10) SGH_WAIT(11) SGH_WAIT(12)
+    SGH_WAIT(13) SGH_WAIT(14) SGH_WAIT(15)
+    default: asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  }
+#undef SGH_WAIT
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 // tiles that the block's threads have requested are there, and everybody is done with what was read before
 __device__ __forceinline__ void tiles_arrive() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -213,19 +256,6 @@ __device__ __forceinline__ f32x16 mul_step(frag_t a, frag_t b, f32x16 c) {
   }
 }
 
-// c[q] += rows [row0, row0 + 32) of the tile x columns f[q]
-template <class T, int DP, int Q>
-__device__ __forceinline__ void mul_rows(const char *tile, int row0, const cols_t<T, DP> (&f)[Q], f32x16 (&c)[Q], int lane) {
-  typedef Tile<T, DP> L;
-  const int r = row0 + (lane & 31), hi = lane >> 5;
-#pragma unroll
-  for (int k = 0; k < kSteps<T, DP>; ++k) {
-    const frag_t a = *reinterpret_cast<const frag_t *>(tile + L::place(r, 2 * k + hi));
-#pragma unroll
-    for (int q = 0; q < Q; ++q) c[q] = mul_step<T>(a, f[q][k], c[q]);
-  }
-}
-
 // Row of register i of a 32x32 result, without the 4 * (lane / 32)
 __device__ __forceinline__ constexpr int row_of(int i) { return (i & 3) + 8 * (i >> 2); }
 
@@ -246,42 +276,157 @@ struct Terms<F32> {
   __device__ __forceinline__ void set(const f32x16 &x) { v = x; }
 };
 
-// c[q][n] += (rows [row0, row0 + 32) of the tile, transposed: values 32 n ..) x t[q]
-template <class T, int DP, int Q>
-__device__ __forceinline__ void mul_transposed(const char *tile, int row0, const Terms<T> (&t)[Q], f32x16 (&c)[Q][DP / 32], int lane) {
+// Nothing is moved across: the loads in front are issued before what follows uses the first of them.  (Left to itself the compiler loaded one
+// fragment, waited for it, used it and loaded the next.)
+__device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
+
+// A lane's places in a tile, and the products that read it
+template <class T, int DP>
+struct Reader {
   typedef Tile<T, DP> L;
-  const int hi = lane >> 5;
-  if constexpr (T::half) {
-    // 16 lanes take four rows of 16 values and return them by columns
-    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    const int r = 4 * hi + ((lane >> 2) & 3), sub = (lane >> 4) & 1;
+  // Row reads take chunk 2 k + hi of row lane % 32: of the bits of k, those that turn() moves make an address, the others are a constant
+  static constexpr int LOW = L::RS >= 32 ? 4 : L::RS == 16 ? 2 : 1;   // what k counts before its first turned bit
+  static constexpr int ROWS = L::RS >= 32 ? 2 : L::RS == 4 ? 2 : 4;
+  int row[ROWS];
+  static __device__ __forceinline__ constexpr int which(int k) { return k / LOW % ROWS; }
+  static __device__ __forceinline__ constexpr int beyond(int k) { return (k % LOW + k / (LOW * ROWS) * (LOW * ROWS)) * 32; }
+  // Transposed reads.  16-bit: 16 lanes take four rows of 16 values and get them by columns, for values 32 n and on; fp32: a value of row i + 4 hi
+  static constexpr int COLS = T::half ? (L::RS == 4 ? 1 : L::RS == 8 ? 2 : 4) : L::RS == 8 ? 1 : 2;
+  int col[T::half ? (L::RS == 4 ? 2 : 1) : 4][COLS];
+  __device__ __forceinline__ explicit Reader(int lane) {
+    const int hi = lane >> 5;
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int k = 0; k < ROWS; ++k) row[k] = L::place(lane & 31, 2 * k * LOW + hi);
 #pragma unroll
-      for (int n = 0; n < DP / 32; ++n) {
-        const int c0 = 4 * n + 2 * sub + ((lane >> 1) & 1), within = (lane & 1) * 8;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(tile + L::place(row0 + 16 * s + r, c0) + within));
-        const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(tile + L::place(row0 + 16 * s + 8 + r, c0) + within));
-        const u32x2 l = __builtin_bit_cast(u32x2, lo), u = __builtin_bit_cast(u32x2, up);
-        const frag_t a = {l[0], l[1], u[0], u[1]};
+    for (int n = 0; n < COLS; ++n)
+      if constexpr (T::half) {
+        const int r = 4 * hi + ((lane >> 2) & 3), c = 4 * n + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+        col[0][n] = L::place(r, c) + (lane & 1) * 8;
+        if constexpr (L::RS == 4) col[1][n] = L::place(r + 8, c) + (lane & 1) * 8;
+      } else {
 #pragma unroll
-        for (int q = 0; q < Q; ++q) c[q][n] = T::mfma(a, t[q].v[s], c[q][n]);
+        for (int i = 0; i < 4; ++i) col[i][n] = L::place(i + 4 * hi, 8 * n + ((lane & 31) >> 2)) + (lane & 3) * 4;
       }
-  } else {
-    const int d = lane & 31;
+  }
+  // What a product reads of a tile: rows [row0, row0 + 32), or the same rows transposed.  Loaded apart from the product where the order of
+  // the loads matters (pin()).
+  struct Rows {
+    frag_t v[kSteps<T, DP>];
+  };
+  struct Cols {
+    typename std::conditional<T::half, frag_t, float>::type v[T::half ? 2 : 16][DP / 32];
+  };
+  __device__ __forceinline__ frag_t row_chunk(const char *tile, int row0, int k) const {
+    return *reinterpret_cast<const frag_t *>(tile + row[which(k)] + (row0 / L::G * L::GROUP + beyond(k)));
+  }
+  template <class V>
+  __device__ __forceinline__ void col_chunk(const char *tile, int row0, int s, int n, V *v) const {
+    if constexpr (T::half) {
+      typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+      const char *at = tile + (row0 + 16 * s) / L::G * L::GROUP;
+      const char *on = L::RS == 4 ? at + col[L::RS == 4][n] : at + col[0][n] + 8 / L::G * L::GROUP;
+      const u32x2 l = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at + col[0][n])));
+      const u32x2 u = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)on));
+      *v = frag_t{l[0], l[1], u[0], u[1]};
+    } else {
+      *v = *reinterpret_cast<const float *>(tile + col[s & 3][n % COLS] + ((row0 + (s >> 2) * 8) / L::G * L::GROUP + n / COLS * COLS * 128));
+    }
+  }
+  __device__ __forceinline__ void load(const char *tile, int row0, Rows &a) const {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int r = row0 + row_of(i) + 4 * hi;
+    for (int k = 0; k < kSteps<T, DP>; ++k) a.v[k] = row_chunk(tile, row0, k);
+  }
+  __device__ __forceinline__ void load(const char *tile, int row0, Cols &a) const {
+#pragma unroll
+    for (int s = 0; s < (T::half ? 2 : 16); ++s)
+#pragma unroll
+      for (int n = 0; n < DP / 32; ++n) col_chunk(tile, row0, s, n, &a.v[s][n]);
+  }
+  // c[q] += rows x columns f[q]
+  template <int Q>
+  static __device__ __forceinline__ void mul(const Rows &a, const cols_t<T, DP> (&f)[Q], f32x16 (&c)[Q]) {
+#pragma unroll
+    for (int k = 0; k < kSteps<T, DP>; ++k)
+#pragma unroll
+      for (int q = 0; q < Q; ++q) c[q] = mul_step<T>(a.v[k], f[q][k], c[q]);
+  }
+  // c[q][n] += (rows, transposed: values 32 n ..) x t[q]
+  template <int Q>
+  static __device__ __forceinline__ void mul(const Cols &a, const Terms<T> (&t)[Q], f32x16 (&c)[Q][DP / 32]) {
+#pragma unroll
+    for (int s = 0; s < (T::half ? 2 : 16); ++s)
+#pragma unroll
+      for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          if constexpr (T::half) c[q][n] = T::mfma(a.v[s][n], t[q].v[s], c[q][n]);
+          else c[q][n] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[s][n], t[q].v[s], c[q][n], 0, 0, 0);
+        }
+  }
+  template <int Q>
+  __device__ __forceinline__ void rows(const char *tile, int row0, const cols_t<T, DP> (&f)[Q], f32x16 (&c)[Q]) const {
+    Rows a;
+    load(tile, row0, a);
+    mul(a, f, c);
+  }
+  // The same with few registers: four chunk pairs at a time, the columns' last ones (from HELD on) from another tile, of 32 values
+  template <int HELD>
+  __device__ __forceinline__ void rows_by_four(const char *tile, int row0, const frag_t (&f)[HELD], const Reader<T, 32> &rest, const char *columns,
+                                               f32x16 &c) const {
+    constexpr int STEP = kSteps<T, DP> < 4 ? kSteps<T, DP> : 4;
+#pragma unroll
+    for (int k0 = 0; k0 < kSteps<T, DP>; k0 += STEP) {
+      frag_t a[STEP], b[STEP];
+#pragma unroll
+      for (int k = 0; k < STEP; ++k)
+        if (k0 + k < kSteps<T, DP>) {
+          a[k] = row_chunk(tile, row0, k0 + k);
+          if (k0 + k >= HELD) b[k] = rest.row_chunk(columns, 0, k0 + k - HELD);
+        }
+      pin();
+#pragma unroll
+      for (int k = 0; k < STEP; ++k)
+        if (k0 + k < kSteps<T, DP>) c = mul_step<T>(a[k], k0 + k < HELD ? f[k0 + k < HELD ? k0 + k : 0] : b[k], c);
+      pin();
+    }
+  }
+  __device__ __forceinline__ void transposed_by_four(const char *tile, int row0, const Terms<T> &t, f32x16 (&c)[DP / 32]) const {
+#pragma unroll
+    for (int s = 0; s < (T::half ? 2 : 16); ++s) {
+      typename std::conditional<T::half, frag_t, float>::type a[DP / 32];
+#pragma unroll
+      for (int n = 0; n < DP / 32; ++n) col_chunk(tile, row0, s, n, &a[n]);
+      if (T::half || s % 4 == 3) pin();
 #pragma unroll
       for (int n = 0; n < DP / 32; ++n) {
-        const float a = *reinterpret_cast<const float *>(tile + L::place(r, 8 * n + (d >> 2)) + (d & 3) * 4);
-#pragma unroll
-        for (int q = 0; q < Q; ++q) c[q][n] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, t[q].v[i], c[q][n], 0, 0, 0);
+        if constexpr (T::half) c[n] = T::mfma(a[n], t.v[s], c[n]);
+        else c[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[n], t.v[s], c[n], 0, 0, 0);
       }
     }
   }
-}
-
+  // c += rows [row0, row0 + 32) of the tile x rows [own, own + 32) of another one as columns, four chunk pairs at a time
+  __device__ __forceinline__ void rows(const char *tile, int row0, const char *columns, int own, f32x16 &c) const {
+    constexpr int STEP = kSteps<T, DP> < 4 ? kSteps<T, DP> : DP == 128 ? 2 : 4;
+#pragma unroll
+    for (int k0 = 0; k0 < kSteps<T, DP>; k0 += STEP) {
+      frag_t a[STEP], b[STEP];
+#pragma unroll
+      for (int k = 0; k < STEP; ++k)
+        if (k0 + k < kSteps<T, DP>) a[k] = row_chunk(tile, row0, k0 + k), b[k] = row_chunk(columns + own / L::G * L::GROUP, 0, k0 + k);
+      pin();
+#pragma unroll
+      for (int k = 0; k < STEP; ++k)
+        if (k0 + k < kSteps<T, DP>) c = mul_step<T>(a[k], b[k], c);
+      pin();
+    }
+  }
+  template <int Q>
+  __device__ __forceinline__ void transposed(const char *tile, int row0, const Terms<T> (&t)[Q], f32x16 (&c)[Q][DP / 32]) const {
+    Cols a;
+    load(tile, row0, a);
+    mul(a, t, c);
+  }
+};
 // The value of the lane 32 lanes on or back, together with the lane's own
 __device__ __forceinline__ float max_of_pair(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
@@ -339,7 +484,7 @@ __device__ __forceinline__ void store_partial(float *row, const f32x16 (&c)[DP /
 
 // The bias of distances -reach .. reach for head h, times log2(e), in LDS
 __device__ __forceinline__ void expand_bias(const Shape &s, const Bounds &bounds, int h, float *band) {
-  for (int i = threadIdx.x; i <= 2 * s.reach; i += kBlock)
+  for (int i = threadIdx.x; i <= 2 * s.reach; i += int(blockDim.x))
     band[i] = s.table[size_t(bucket_of(s, bounds, i - s.reach)) * s.heads + h] * kLog2e;
 }
 

@@ -10,12 +10,26 @@ using namespace attn;
 
 constexpr int kStats = SGH_WAVE;   // places of a tile's statistics of a kind: a load writes one for each lane
 
+// A block's form.  VL: its values lie in LDS, where registers for two wavefronts of a SIMD would not do otherwise; the tiles are then 32 rows.
+template <class T, int DP>
+struct Form {
+  static constexpr bool VL = T::half ? DP >= 96 : DP >= 64;
+  static constexpr int QR = T::half && !VL ? 64 : 32;
+  static constexpr int TILE = Tile<T, DP>::bytes(QR), SLOT = 2 * TILE + 2 * kStats * 4;
+  static constexpr int VALUES = VL ? Tile<T, DP>::bytes(kRows) : 0;
+  // of the longest rows the last 32 values of a key as well
+  static constexpr bool KL = T::half && DP == 128;
+  static constexpr int HELD = KL ? kSteps<T, DP> - kSteps<T, 32> : kSteps<T, DP>, REST = KL ? Tile<T, 32>::bytes(kRows) : 0;
+  static constexpr int PER_SIMD = T::half || DP <= 64 ? 2 : 1;
+  static constexpr size_t lds(int reach, bool bias) { return 2 * SLOT + VALUES + REST + (bias ? (2 * reach + 1) * sizeof(float) : 0); }
+};
+
 template <class T, int DP, int KW, bool BIAS>
-__global__ __launch_bounds__(kBlock, 1) void k_attn_dkv(BwdArgs a, Bounds bounds) {
+__global__ __launch_bounds__(kBlock, (Form<T, DP>::PER_SIMD)) void k_attn_dkv(BwdArgs a, Bounds bounds) {
   typedef typename T::elem elem;
-  typedef Tile<T, DP> L;
-  constexpr int QR = T::half ? 64 : 32, SUB = QR / 32, ND = DP / 32, WAVE_KEYS = 32 * KW, KEYS = 4 * WAVE_KEYS;
-  constexpr int TILE = QR * L::BYTES_OF_ROW, SLOT = 2 * TILE + 2 * kStats * 4;
+  typedef Form<T, DP> F;
+  constexpr int QR = F::QR, SUB = QR / 32, ND = DP / 32, WAVE_KEYS = 32 * KW, KEYS = 4 * WAVE_KEYS, TILE = F::TILE, SLOT = F::SLOT;
+  constexpr bool VL = F::VL;
   extern __shared__ __align__(16) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
   const Shape &s = a.s;
@@ -27,14 +41,15 @@ __global__ __launch_bounds__(kBlock, 1) void k_attn_dkv(BwdArgs a, Bounds bounds
   const int key0 = int(tile) * KEYS + wave * WAVE_KEYS;
 
   int key[KW];
-  cols_t<T, DP> kf[KW], vf[KW];
+  frag_t kf[KW][F::HELD];
+  cols_t<T, DP> vf[VL ? 1 : KW];
 #pragma unroll
   for (int t = 0; t < KW; ++t) {
     key[t] = key0 + 32 * t + (lane & 31);
     const size_t at = ((size_t(b) * s.k_len + key[t]) * s.kv_heads + kv) * s.dim;
     const int n = key[t] < span.k ? s.dim : 0;
-    load_columns<T, DP>(kf[t], static_cast<const elem *>(a.k) + at, n, hi, a.direct);
-    load_columns<T, DP>(vf[t], static_cast<const elem *>(a.v) + at, n, hi, a.direct);
+    load_columns<T, F::HELD * 2 * T::VEC>(kf[t], static_cast<const elem *>(a.k) + at, n, hi, a.direct);
+    if (!VL) load_columns<T, DP>(vf[t], static_cast<const elem *>(a.v) + at, n, hi, a.direct);
   }
   // queries [from, span.q) see a key of the block, [mine, span.q) one of the wavefront
   const int from = s.causal ? max(int(tile) * KEYS - span.start, 0) / QR * QR : 0;
@@ -43,7 +58,9 @@ __global__ __launch_bounds__(kBlock, 1) void k_attn_dkv(BwdArgs a, Bounds bounds
   const int turns = turns_of_head * group, each = (turns + int(a.k_splits) - 1) / int(a.k_splits);
   const int begin = min(turns, int(split) * each), end = min(turns, begin + each);
 
-  float *band = reinterpret_cast<float *>(lds + 2 * SLOT);
+  char *const values = lds + 2 * SLOT;
+  char *const rest = values + F::VALUES;
+  float *band = reinterpret_cast<float *>(rest + F::REST);
   const size_t stride = size_t(s.heads) * s.dim;
   Stage<T, DP, QR> stage;
   stage.init(stride, s.dim, a.direct);
@@ -57,25 +74,46 @@ __global__ __launch_bounds__(kBlock, 1) void k_attn_dkv(BwdArgs a, Bounds bounds
 #pragma unroll
   for (int t = 0; t < KW; ++t) zero(dk[t]), zero(dv[t]);
   const float c = s.scale * kLog2e;
-  auto request = [&](int head, int q0, int slot) {
+  const Reader<T, DP> reader(lane);
+  const Reader<T, 32> short_reader(lane);
+  // A turn is QR queries of a head of the group.  Where the next one to be requested begins in the matrices and the statistics:
+  int head = 0, q0 = 0, ahead_head = 0, ahead_q0 = 0, slot = 0;
+  size_t skip = 0, stat = 0;
+  auto request = [&](int slot) {
     char *at = lds + slot * SLOT;
-    const size_t skip = q0 * stride + size_t(head) * s.dim;
-    stage(at, qp + skip, span.q - q0);
-    stage(at + TILE, dp + skip, span.q - q0);
-    if (wave < 2) {   // (rows behind the last query: 0, beside rows of zeros)
-      const float *p = (wave ? delta : lse) + size_t(head) * s.q_len + q0;
-      const rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(p), 0, max(span.q - q0, 0) * 4, 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void *)(at + 2 * TILE + wave * kStats * 4), 4, lane < QR ? lane * 4 : kOOB, 0, 0, 0);
+    const int rows = span.q - ahead_q0;
+    stage(at, qp + skip, rows);
+    stage(at + TILE, dp + skip, rows);
+    if (wave < 2)   // (rows behind the last query: 0, beside rows of zeros)
+      load_lds4(buffer_of((wave ? delta : lse) + stat, rows * 4), lds_offset(at) + 2 * TILE + wave * kStats * 4, lane < QR ? lane * 4 : kOOB);
+    ahead_q0 += QR, skip += QR * stride, stat += QR;
+    if (ahead_q0 >= span.q) {
+      ahead_q0 = from, ++ahead_head;
+      skip = size_t(ahead_head) * s.dim + from * stride, stat = size_t(ahead_head) * s.q_len + from;
     }
   };
-  int head = turns_of_head ? begin / turns_of_head : 0, q0 = turns_of_head ? from + begin % turns_of_head * QR : 0, slot = 0;
   bool other_head = true;
-  if (begin < end) request(head, q0, 0);
+  registers_arrive();
+  if (begin < end) {
+    if constexpr (VL) {
+      Stage<T, DP, KEYS> all;
+      all.init(size_t(s.kv_heads) * s.dim, s.dim, a.direct);
+      all(values, static_cast<const elem *>(a.v) + ((size_t(b) * s.k_len + size_t(tile) * KEYS) * s.kv_heads + kv) * s.dim, span.k - int(tile) * KEYS);
+    }
+    if constexpr (F::KL) {
+      Stage<T, 32, KEYS> last;
+      last.init(size_t(s.kv_heads) * s.dim, s.dim - (DP - 32), a.direct);
+      last(rest, static_cast<const elem *>(a.k) + ((size_t(b) * s.k_len + size_t(tile) * KEYS) * s.kv_heads + kv) * s.dim + (DP - 32),
+           span.k - int(tile) * KEYS);
+    }
+    ahead_head = head = begin / turns_of_head, ahead_q0 = q0 = from + begin % turns_of_head * QR;
+    skip = size_t(head) * s.dim + q0 * stride, stat = size_t(head) * s.q_len + q0;
+    request(0);
+  }
   for (int turn = begin; turn < end; ++turn, slot ^= 1) {
     tiles_arrive();
-    int next_head = head, next_q0 = q0 + QR;
-    if (next_q0 >= span.q) next_q0 = from, ++next_head;
-    if (turn + 1 < end) request(next_head, next_q0, slot ^ 1);
+    const int next_head = q0 + QR < span.q ? head : head + 1, next_q0 = q0 + QR < span.q ? q0 + QR : from;
+    if (turn + 1 < end) request(slot ^ 1);
     if constexpr (BIAS)
       if (other_head) {
         expand_bias(s, bounds, kv * group + head, band);
@@ -89,20 +127,25 @@ __global__ __launch_bounds__(kBlock, 1) void k_attn_dkv(BwdArgs a, Bounds bounds
       for (int u = 0; u < SUB; ++u) {
         f32x16 p[KW], ds[KW];
         zero(p);
-        mul_rows<T, DP, KW>(qt, 32 * u, kf, p, lane);
+        if constexpr (VL) reader.rows_by_four(qt, 32 * u, kf[0], short_reader, rest + wave * 32 / Tile<T, 32>::G * Tile<T, 32>::GROUP, p[0]);
+        else reader.rows(qt, 32 * u, kf, p);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {   // (the product starts from -delta)
+          const sgh_v4f x = *reinterpret_cast<const sgh_v4f *>(st + kStats + 32 * u + 8 * g + 4 * hi);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < KW; ++t) ds[t][4 * g + i] = x[i];
+        }
+        if constexpr (VL) reader.rows(dt, 32 * u, values, wave * 32, ds[0]);
+        else reader.rows(dt, 32 * u, vf, ds);
         float row_lse[16];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const sgh_v4f x = *reinterpret_cast<const sgh_v4f *>(st + 32 * u + 8 * g + 4 * hi);
-          const sgh_v4f y = *reinterpret_cast<const sgh_v4f *>(st + kStats + 32 * u + 8 * g + 4 * hi);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            row_lse[4 * g + i] = x[i];
-#pragma unroll
-            for (int t = 0; t < KW; ++t) ds[t][4 * g + i] = y[i];   // (the product starts from -delta)
-          }
+          for (int i = 0; i < 4; ++i) row_lse[4 * g + i] = x[i];
         }
-        mul_rows<T, DP, KW>(dt, 32 * u, vf, ds, lane);
         const int q1 = q0 + 32 * u;
 #pragma unroll
         for (int t = 0; t < KW; ++t) {
@@ -136,13 +179,15 @@ __global__ __launch_bounds__(kBlock, 1) void k_attn_dkv(BwdArgs a, Bounds bounds
         Terms<T> terms[KW];
 #pragma unroll
         for (int t = 0; t < KW; ++t) terms[t].set(p[t]);
-        mul_transposed<T, DP, KW>(dt, 32 * u, terms, dv, lane);
+        if constexpr (VL) reader.transposed_by_four(dt, 32 * u, terms[0], dv[0]);
+        else reader.transposed(dt, 32 * u, terms, dv);
 #pragma unroll
         for (int t = 0; t < KW; ++t) {
           range[t].fit(ds[t], dk[t]);
           terms[t].set(ds[t]);
         }
-        mul_transposed<T, DP, KW>(qt, 32 * u, terms, dk, lane);
+        if constexpr (VL) reader.transposed_by_four(qt, 32 * u, terms[0], dk[0]);
+        else reader.transposed(qt, 32 * u, terms, dk);
       }
     }
     head = next_head, q0 = next_q0;
@@ -185,8 +230,7 @@ __global__ __launch_bounds__(kBlock) void k_attn_dkv_join(BwdArgs a) {
 
 template <class T, int DP, int KW, bool BIAS>
 int launch(const BwdArgs &a, const Bounds &bounds, hipStream_t s) {
-  constexpr int QR = T::half ? 64 : 32;
-  const size_t lds = 4 * QR * Tile<T, DP>::BYTES_OF_ROW + 4 * kStats * 4 + (BIAS ? (2 * a.s.reach + 1) * sizeof(float) : 0);
+  const size_t lds = Form<T, DP>::lds(a.s.reach, BIAS);
   static std::atomic<unsigned long long> asked{0};
   SGH_HIP_TRY(allow_lds(reinterpret_cast<const void *>(k_attn_dkv<T, DP, KW, BIAS>), asked));
   hipLaunchKernelGGL((k_attn_dkv<T, DP, KW, BIAS>), dim3(a.k_tiles * a.k_units * a.k_splits), dim3(kBlock), lds, s, a, bounds);

@@ -12,7 +12,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_dq(BwdArgs a, Bounds bounds)
   typedef typename T::elem elem;
   typedef Tile<T, DP> L;
   constexpr int KT = T::half ? 64 : 32, SUB = KT / 32, ND = DP / 32, WAVE_ROWS = 32 * QT, ROWS = 4 * WAVE_ROWS;
-  constexpr int TILE = KT * L::BYTES_OF_ROW;
+  constexpr int TILE = L::bytes(KT);
   extern __shared__ __align__(16) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
   const Shape &s = a.s;
@@ -90,10 +90,12 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_dq(BwdArgs a, Bounds bounds)
 #pragma unroll
   for (int t = 0; t < QT; ++t) zero(acc[t]);
   const float c = s.scale * kLog2e;
+  const Reader<T, DP> reader(lane);
   auto request = [&](int k0, int slot) {
     stage(lds + slot * 2 * TILE, kp + k0 * stride, span.k - k0);
     stage(lds + slot * 2 * TILE + TILE, vp + k0 * stride, span.k - k0);
   };
+  registers_arrive();
   if (begin < end) request(begin, 0);
   int slot = 0;
   for (int k0 = begin; k0 < end; k0 += KT, slot ^= 1) {
@@ -105,13 +107,13 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_dq(BwdArgs a, Bounds bounds)
     for (int u = 0; u < SUB; ++u) {
       f32x16 p[QT], ds[QT];
       zero(p);
-      mul_rows<T, DP, QT>(kt, 32 * u, qf, p, lane);
+      reader.rows(kt, 32 * u, qf, p);
       // (the product starts from -delta)
 #pragma unroll
       for (int t = 0; t < QT; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) ds[t][i] = -delta[t];
-      mul_rows<T, DP, QT>(vt, 32 * u, df, ds, lane);
+      reader.rows(vt, 32 * u, df, ds);
       const int k1 = k0 + 32 * u;
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
@@ -175,7 +177,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_dq(BwdArgs a, Bounds bounds)
       Terms<T> terms[QT];
 #pragma unroll
       for (int t = 0; t < QT; ++t) terms[t].set(ds[t]);
-      mul_transposed<T, DP, QT>(kt, 32 * u, terms, acc, lane);
+      reader.transposed(kt, 32 * u, terms, acc);
     }
   }
 
@@ -255,7 +257,7 @@ __global__ __launch_bounds__(kBlock) void k_attn_dtable(BwdArgs a, float *dtable
 template <class T, int DP, int QT, bool BIAS>
 int launch(const BwdArgs &a, const Bounds &bounds, float *dtable, hipStream_t s) {
   constexpr int KT = T::half ? 64 : 32;
-  const size_t lds = 4 * KT * Tile<T, DP>::BYTES_OF_ROW + (BIAS ? 5 * (2 * a.s.reach + 1) * sizeof(float) : 0);
+  const size_t lds = 4 * Tile<T, DP>::bytes(KT) + (BIAS ? 5 * (2 * a.s.reach + 1) * sizeof(float) : 0);
   static std::atomic<unsigned long long> asked{0};
   SGH_HIP_TRY(allow_lds(reinterpret_cast<const void *>(k_attn_dq<T, DP, QT, BIAS>), asked));
   hipLaunchKernelGGL((k_attn_dq<T, DP, QT, BIAS>), dim3(a.q_tiles * a.q_units * a.q_splits), dim3(kBlock), lds, s, a, bounds);

@@ -29,7 +29,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
   typedef typename T::elem elem;
   typedef Tile<T, DP> L;
   constexpr int KT = T::half ? 64 : 32, SUB = KT / 32, ND = DP / 32, WAVE_ROWS = 32 * QT, ROWS = 4 * WAVE_ROWS;
-  constexpr int TILE = KT * L::BYTES_OF_ROW;
+  constexpr int TILE = L::bytes(KT);
   // binary16: terms from 2^-14 to 2^14 with all their bits
   constexpr float kShift = std::is_same<T, F16>::value ? 6.f : 0.f;
   extern __shared__ __align__(16) char lds[];
@@ -88,10 +88,12 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
     m[t] = -3e38f, l[t] = 0.f;
   }
   const float c = s.scale * kLog2e;
+  const Reader<T, DP> reader(lane);
   auto request = [&](int k0, int slot) {
     stage(lds + slot * 2 * TILE, kp + k0 * stride, span.k - k0);
     stage(lds + slot * 2 * TILE + TILE, vp + k0 * stride, span.k - k0);
   };
+  registers_arrive();
   if (begin < end) request(begin, 0);
   int slot = 0;
   for (int k0 = begin; k0 < end; k0 += KT, slot ^= 1) {
@@ -103,7 +105,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
       zero(p[u]);
-      mul_rows<T, DP, QT>(kt, 32 * u, qf, p[u], lane);
+      reader.rows(kt, 32 * u, qf, p[u]);
     }
     // scores in units of log2, -inf where the mask is
 #pragma unroll
@@ -171,7 +173,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
       Terms<T> terms[QT];
 #pragma unroll
       for (int t = 0; t < QT; ++t) terms[t].set(p[u][t]);
-      mul_transposed<T, DP, QT>(vt, 32 * u, terms, acc, lane);
+      reader.transposed(vt, 32 * u, terms, acc);
     }
   }
 
@@ -273,7 +275,7 @@ Plan plan_of(const sgh_attn_geom *g) {
 template <class T, int DP>
 int run_dim(const FwdArgs &a, const Bounds &bounds, hipStream_t s) {
   constexpr int KT = T::half ? 64 : 32;
-  const size_t tiles = 4 * KT * Tile<T, DP>::BYTES_OF_ROW;
+  const size_t tiles = 4 * Tile<T, DP>::bytes(KT);
   if (a.s.buckets) return launch<T, DP, 1, true>(a, bounds, tiles + a.pack * (2 * a.s.reach + 1) * sizeof(float), s);
   return launch<T, DP, 1, false>(a, bounds, tiles, s);
 }
