@@ -488,6 +488,26 @@ __device__ __forceinline__ void expand_bias(const Shape &s, const Bounds &bounds
     band[i] = s.table[size_t(bucket_of(s, bounds, i - s.reach)) * s.heads + h] * kLog2e;
 }
 
+// Rows of `dim` values anywhere as rows of `wide` (whole 16-byte chunks) at multiples of 16 bytes, zeros behind them.  What the kernels read many
+// times is copied so first: loads of 16 bytes then write LDS without a register.
+struct PadArgs {
+  const void *from[4];
+  void *to[4];
+  size_t rows[4];
+  int dim, wide;
+};
+template <class T>
+__global__ __launch_bounds__(kBlock) void k_attn_pad(PadArgs a) {
+  const int chunks = a.wide / T::VEC, which = blockIdx.y;
+  const size_t n = a.rows[which] * chunks, step = size_t(gridDim.x) * kBlock;
+  for (size_t i = size_t(blockIdx.x) * kBlock + threadIdx.x; i < n; i += step) {
+    const size_t row = i / unsigned(chunks);
+    const int c = int(i - row * chunks);
+    const u32x4 v = Stage<T, 32, 64>::chunk(static_cast<const typename T::elem *>(a.from[which]) + row * a.dim, c * T::VEC, a.dim);
+    reinterpret_cast<u32x4 *>(a.to[which])[i] = v;
+  }
+}
+
 // Where a call's blocks lie: block w runs on the XCD w % 8, so the blocks of one head of keys, which read the same rows, go to one XCD where
 // their number allows it
 __device__ __forceinline__ void block_at(unsigned w, unsigned tiles, unsigned units, unsigned *tile, unsigned *unit) {

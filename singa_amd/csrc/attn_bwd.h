@@ -20,7 +20,9 @@ struct BwdArgs {
   size_t bias_blocks;
   unsigned q_tiles, q_units, q_splits, k_tiles, k_units, k_splits;
   int pack, keys_each, turns_each;
-  bool direct;
+  bool direct;     // of q, k, v and do, rows of s.dim
+  int io_dim;      // o and the results have rows of io_dim
+  bool io_direct;
 };
 constexpr int kRows = 128;   // queries (keys) of a block of the first (second) half
 

@@ -200,9 +200,9 @@ __global__ __launch_bounds__(kBlock, (Form<T, DP>::PER_SIMD)) void k_attn_dkv(Bw
     constexpr float down = std::is_same<T, F16>::value ? 0x1p-14f : 1.f;
     const float f = key[t] < span.k ? s.scale * range[t].inverse() * down : 0.f;
     if (a.k_splits == 1) {
-      const size_t at = ((size_t(b) * s.k_len + key[t]) * s.kv_heads + kv) * s.dim;
-      store_column<T, DP>(static_cast<elem *>(a.dk) + at, dk[t], f, s.dim, hi, a.direct);
-      store_column<T, DP>(static_cast<elem *>(a.dv) + at, dv[t], down, s.dim, hi, a.direct);
+      const size_t at = ((size_t(b) * s.k_len + key[t]) * s.kv_heads + kv) * a.io_dim;
+      store_column<T, DP>(static_cast<elem *>(a.dk) + at, dk[t], f, a.io_dim, hi, a.io_direct);
+      store_column<T, DP>(static_cast<elem *>(a.dv) + at, dv[t], down, a.io_dim, hi, a.io_direct);
     } else {
       const size_t n = size_t(a.k_units) * s.k_len, at = 2 * split * n + size_t(unit) * s.k_len + key[t];
       store_partial<DP>(a.k_part + at * DP, dk[t], f, hi);
@@ -222,10 +222,10 @@ __global__ __launch_bounds__(kBlock) void k_attn_dkv_join(BwdArgs a) {
   sgh_v4f x = {0.f, 0.f, 0.f, 0.f};
   for (unsigned i = 0; i < a.k_splits; ++i) x += *reinterpret_cast<const sgh_v4f *>(a.k_part + (2 * i * n + at) * DP + d);
   const size_t row = at % n, unit = row / s.k_len, key = row % s.k_len, b = unit / s.kv_heads, kv = unit % s.kv_heads;
-  typename T::elem *out = static_cast<typename T::elem *>(at < n ? a.dk : a.dv) + ((b * s.k_len + key) * s.kv_heads + kv) * s.dim;
+  typename T::elem *out = static_cast<typename T::elem *>(at < n ? a.dk : a.dv) + ((b * s.k_len + key) * s.kv_heads + kv) * a.io_dim;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (d + i < s.dim) T::St::st(out + d + i, x[i]);
+    if (d + i < a.io_dim) T::St::st(out + d + i, x[i]);
 }
 
 template <class T, int DP, int KW, bool BIAS>
@@ -261,8 +261,8 @@ int run_dkv(const BwdArgs &a, const Bounds &bounds, hipStream_t s) {
 // How a backward pass is cut
 struct Plan {
   BwdArgs a;
-  size_t stats, q_part, bias_part, k_part;   // bytes
-  size_t bytes() const { return stats + q_part + bias_part + k_part; }
+  size_t stats, q_part, bias_part, k_part, wide;   // bytes
+  size_t bytes() const { return stats + q_part + bias_part + k_part + wide; }
 };
 size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 Plan plan_of(const sgh_attn_geom *g) {
@@ -293,6 +293,9 @@ Plan plan_of(const sgh_attn_geom *g) {
   p.stats = up16(2 * sizeof(float) * g->batch * g->heads * size_t(g->q_len));
   p.q_part = a.q_splits > 1 ? a.q_splits * a.q_units * size_t(g->q_len) * a.pack * dp * sizeof(float) : 0;
   p.bias_part = g->buckets ? up16(a.bias_blocks * g->heads * g->buckets * sizeof(float)) : 0;
+  // rows that are not whole chunks are copied first, unless each is read once
+  const size_t q_rows = size_t(g->batch) * g->q_len * g->heads, k_rows = size_t(g->batch) * g->k_len * g->kv_heads;
+  p.wide = a.q_tiles * (group / a.pack) >= 2 || a.k_tiles >= 2 ? 2 * wide_bytes(g->dim, q_rows) + 2 * wide_bytes(g->dim, k_rows) : 0;
   p.k_part = a.k_splits > 1 ? 2 * a.k_splits * a.k_units * size_t(g->k_len) * dp * sizeof(float) : 0;
   return p;
 }
@@ -327,16 +330,26 @@ int backward(const sgh_attn_geom *g, const void *dout, const void *q, const void
   a.stats = reinterpret_cast<float *>(at), at += p.stats;
   a.q_part = reinterpret_cast<float *>(at), at += p.q_part;
   a.bias_part = reinterpret_cast<float *>(at), at += p.bias_part;
-  a.k_part = reinterpret_cast<float *>(at);
-  a.direct = g->dim % T::VEC == 0;
-  for (const void *x : {dout, q, k, v, o}) a.direct = a.direct && sgh_aligned16(x);
-  for (const void *x : {dq, dk, dv}) a.direct = a.direct && sgh_aligned16(x);
+  a.k_part = reinterpret_cast<float *>(at), at += p.k_part;
+  a.io_dim = g->dim;
+  a.direct = a.io_direct = g->dim % T::VEC == 0;
+  for (const void *x : {dout, q, k, v}) a.direct = a.direct && sgh_aligned16(x);
+  for (const void *x : {o, (const void *)dq, (const void *)dk, (const void *)dv}) a.io_direct = a.io_direct && sgh_aligned16(x);
   Bounds bounds;
   bounds_of(g, &bounds);
   hipStream_t s = sgh_stream_of(stream);
   sgh_note_write(dq, qn), sgh_note_write(dk, kn), sgh_note_write(dv, kn), sgh_note_write(dtable, tn);
   sgh_prof_kernel_scope prof("attn_bwd/k_attn_dq+k_attn_dkv", 10.0 * g->batch * g->heads * g->q_len * double(g->k_len) * g->dim, s);
   prof.span();
+  const int wide = p.wide ? wide_of(g->dim, e) : 0;
+  if (wide) {
+    const size_t q_rows = bq, k_rows = size_t(g->batch) * g->k_len * g->kv_heads, row = size_t(wide) * e;
+    const PadArgs pad = {{q, dout, k, v}, {at, at + q_rows * row, at + 2 * q_rows * row, at + (2 * q_rows + k_rows) * row}, {q_rows, q_rows, k_rows, k_rows},
+                         g->dim, wide};
+    const int r = pad_rows<T>(pad, 4, s);
+    if (r != SGH_OK) return r;
+    a.q = pad.to[0], a.dout = pad.to[1], a.k = pad.to[2], a.v = pad.to[3], a.s.dim = wide, a.direct = true;
+  }
   if (g->q_len != 0) {
     const int r = run_dq<T>(a, bounds, dtable, s);
     if (r != SGH_OK) return r;

@@ -46,7 +46,8 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_dq(BwdArgs a, Bounds bounds)
     if (!BIAS) lse[t] = lse2;
     float x = 0.f;
     cols_t<T, DP> of;
-    load_columns<T, DP>(of, static_cast<const elem *>(a.o) + at, n, hi, a.direct);
+    load_columns<T, DP>(of, static_cast<const elem *>(a.o) + ((size_t(b) * s.q_len + query[t]) * s.heads + head[t]) * a.io_dim, n ? a.io_dim : 0, hi,
+                        a.io_direct);
 #pragma unroll
     for (int k = 0; k < kSteps<T, DP>; ++k) {
       float o[T::VEC], d[T::VEC];
@@ -188,8 +189,8 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_dq(BwdArgs a, Bounds bounds)
     if (!limit[t]) zero(acc[t]);
     const float f = s.scale * range[t].inverse();
     if (a.q_splits == 1) {
-      store_column<T, DP>(static_cast<elem *>(a.dq) + ((size_t(b) * s.q_len + query[t]) * s.heads + head[t]) * s.dim, acc[t], f, s.dim, hi,
-                          a.direct);
+      store_column<T, DP>(static_cast<elem *>(a.dq) + ((size_t(b) * s.q_len + query[t]) * s.heads + head[t]) * a.io_dim, acc[t], f, a.io_dim, hi,
+                          a.io_direct);
     } else {
       const size_t n = size_t(a.q_units) * rows;
       store_partial<DP>(a.q_part + (split * n + size_t(unit) * rows + r) * DP, acc[t], f, hi);
@@ -233,10 +234,10 @@ __global__ __launch_bounds__(kBlock) void k_attn_dq_join(BwdArgs a) {
   const size_t unit = at / rows;
   const int r = int(at % rows), per_batch = s.heads / a.pack, b = int(unit / per_batch);
   const int query = r / a.pack, head = int(unit % per_batch) * a.pack + r % a.pack;
-  typename T::elem *out = static_cast<typename T::elem *>(a.dq) + ((size_t(b) * s.q_len + query) * s.heads + head) * s.dim;
+  typename T::elem *out = static_cast<typename T::elem *>(a.dq) + ((size_t(b) * s.q_len + query) * s.heads + head) * a.io_dim;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (d + i < s.dim) T::St::st(out + d + i, x[i]);
+    if (d + i < a.io_dim) T::St::st(out + d + i, x[i]);
 }
 
 // dtable[e][h]: the sum over all blocks of head h, each thread's in order, then the threads' by halves

@@ -18,7 +18,9 @@ struct FwdArgs {
   unsigned tiles, units, splits;
   int pack;           // heads of a group that share a tile: row r is query r / pack, head r % pack of the group
   int keys_each;      // keys of a split, a multiple of 64
-  bool direct;
+  bool direct;        // of keys and values, rows of s.dim
+  int io_dim;         // q and o have rows of io_dim
+  bool io_direct;
 };
 
 // m moves only when a row's maximum has grown by more than 2^8: the terms then stay within 2^8 of one, and o is rescaled seldom
@@ -54,8 +56,8 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
     head[t] = a.pack == 1 ? head0 : head0 + r % a.pack;
     limit[t] = r < rows && query[t] < span.q ? (s.causal ? min(span.k, max(span.start + query[t] + 1, 0)) : span.k) : 0;
     most = max(most, limit[t]), least = min(least, limit[t]);
-    load_columns<T, DP>(qf[t], static_cast<const elem *>(a.q) + ((size_t(b) * s.q_len + query[t]) * s.heads + head[t]) * s.dim,
-                        limit[t] ? s.dim : 0, hi, a.direct);
+    load_columns<T, DP>(qf[t], static_cast<const elem *>(a.q) + ((size_t(b) * s.q_len + query[t]) * s.heads + head[t]) * a.io_dim,
+                        limit[t] ? a.io_dim : 0, hi, a.io_direct);
   }
   for (int m = 1; m < 32; m *= 2) most = max(most, __shfl_xor(most, m)), least = min(least, __shfl_xor(least, m));
   most = __builtin_amdgcn_readfirstlane(most), least = __builtin_amdgcn_readfirstlane(least);
@@ -187,8 +189,8 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
     if (sum == 0.f) zero(acc[t]);
     const float lse = sum == 0.f ? kNegInf : (m[t] - kShift + __builtin_amdgcn_logf(sum)) * kLn2;
     if (a.splits == 1) {
-      store_column<T, DP>(static_cast<elem *>(a.o) + ((size_t(b) * s.q_len + query[t]) * s.heads + head[t]) * s.dim, acc[t], inv, s.dim, hi,
-                          a.direct);
+      store_column<T, DP>(static_cast<elem *>(a.o) + ((size_t(b) * s.q_len + query[t]) * s.heads + head[t]) * a.io_dim, acc[t], inv, a.io_dim, hi,
+                          a.io_direct);
       if (hi == 0) a.lse[(size_t(b) * s.heads + head[t]) * s.q_len + query[t]] = lse;
     } else {
       const size_t n = size_t(a.units) * rows, at = split * n + size_t(unit) * rows + r;
@@ -198,34 +200,51 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
   }
 }
 
-// Joins the parts of the keys, DP / 4 lanes to a row: o = sum e^(lse_s - lse) o_s
+// Joins the parts of the keys, a block to a row: o = sum e^(lse_s - lse) o_s.  DP / 4 lanes have four values each, the groups of so many lanes
+// share the parts (16 rows of 128 values in 235 parts: one group to a row 100 us).
 template <class T, int DP>
 __global__ __launch_bounds__(kBlock) void k_attn_join(FwdArgs a) {
   typedef typename T::elem elem;
-  constexpr int TEAM = DP / 4, PER = kBlock / TEAM;
+  constexpr int TEAM = DP / 4, GROUPS = kBlock / TEAM;
+  __shared__ float least[4], total[GROUPS];
+  __shared__ sgh_v4f sums[GROUPS][TEAM];
   const Shape &s = a.s;
-  const size_t rows = size_t(s.q_len) * a.pack, n = a.units * rows, at = size_t(blockIdx.x) * PER + threadIdx.x / TEAM;
-  const int d = int(threadIdx.x % TEAM) * 4;
-  if (threadIdx.x >= PER * TEAM || at >= n) return;
+  const size_t rows = size_t(s.q_len) * a.pack, n = a.units * rows, at = blockIdx.x;
   const float *lses = a.part + a.splits * n * DP + at;
-  float top = kNegInf, sum = 0.f;
-  for (unsigned i = 0; i < a.splits; ++i) top = fmaxf(top, lses[i * n]);
-  sgh_v4f o = {0.f, 0.f, 0.f, 0.f};
-  for (unsigned i = 0; i < a.splits; ++i) {
-    const float lse = lses[i * n];
-    const float f = lse == kNegInf ? 0.f : __builtin_amdgcn_exp2f((lse - top) * kLog2e);
-    const sgh_v4f x = *reinterpret_cast<const sgh_v4f *>(a.part + (i * n + at) * DP + d);
-    sum += f;
-    o += x * f;
+  float top = kNegInf;
+  for (unsigned i = threadIdx.x; i < a.splits; i += kBlock) top = fmaxf(top, lses[i * n]);
+#pragma unroll
+  for (int m = 1; m < SGH_WAVE; m *= 2) top = fmaxf(top, __shfl_xor(top, m));
+  if (threadIdx.x % SGH_WAVE == 0) least[threadIdx.x / SGH_WAVE] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(least[0], least[1]), fmaxf(least[2], least[3]));
+  const int g = threadIdx.x / TEAM, d = int(threadIdx.x % TEAM) * 4;
+  if (g < GROUPS) {
+    float sum = 0.f;
+    sgh_v4f o = {0.f, 0.f, 0.f, 0.f};
+    for (unsigned i = g; i < a.splits; i += GROUPS) {
+      const float lse = lses[i * n];
+      const float f = lse == kNegInf ? 0.f : __builtin_amdgcn_exp2f((lse - top) * kLog2e);   // (a NaN stays one)
+      sum += f;
+      o += *reinterpret_cast<const sgh_v4f *>(a.part + (i * n + at) * DP + d) * f;
+    }
+    sums[g][threadIdx.x % TEAM] = o;
+    if (d == 0) total[g] = sum;
   }
+  __syncthreads();
+  if (threadIdx.x >= TEAM) return;
+  sgh_v4f o = sums[0][threadIdx.x];
+  float sum = total[0];
+#pragma unroll
+  for (int k = 1; k < GROUPS; ++k) o += sums[k][threadIdx.x], sum += total[k];
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const size_t unit = at / rows;
   const int r = int(at % rows), per_batch = s.heads / a.pack, b = int(unit / per_batch);
   const int query = r / a.pack, head = int(unit % per_batch) * a.pack + r % a.pack;
-  elem *out = static_cast<elem *>(a.o) + ((size_t(b) * s.q_len + query) * s.heads + head) * s.dim;
+  elem *out = static_cast<elem *>(a.o) + ((size_t(b) * s.q_len + query) * s.heads + head) * a.io_dim;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (d + i < s.dim) T::St::st(out + d + i, o[i] * inv);
+    if (d + i < a.io_dim) T::St::st(out + d + i, o[i] * inv);
   if (d == 0) a.lse[(size_t(b) * s.heads + head) * s.q_len + query] = sum == 0.f ? kNegInf : top + __builtin_amdgcn_logf(sum) * kLn2;
 }
 
@@ -236,8 +255,7 @@ int launch(const FwdArgs &a, const Bounds &bounds, size_t lds, hipStream_t s) {
   SGH_LAUNCH_TIMED((k_attn_fwd<T, DP, QT, BIAS>), dim3(a.tiles * a.units * a.splits), dim3(kBlock), lds, s, a, bounds);
   SGH_LAUNCH_CHECK();
   if (a.splits > 1) {
-    const size_t n = size_t(a.units) * a.s.q_len * a.pack, per = kBlock / (DP / 4);
-    hipLaunchKernelGGL((k_attn_join<T, DP>), dim3(unsigned((n + per - 1) / per)), dim3(kBlock), 0, s, a);
+    hipLaunchKernelGGL((k_attn_join<T, DP>), dim3(unsigned(size_t(a.units) * a.s.q_len * a.pack)), dim3(kBlock), 0, s, a);
     SGH_LAUNCH_CHECK();
   }
   return SGH_OK;
@@ -248,7 +266,8 @@ struct Plan {
   int dp, pack;
   unsigned tiles, units, splits;
   int keys_each;
-  size_t ws;
+  bool pad;     // keys and values of rows that are not whole chunks are copied first
+  size_t part, ws;
 };
 constexpr int kRows = 128;   // of a block
 Plan plan_of(const sgh_attn_geom *g) {
@@ -268,7 +287,10 @@ Plan plan_of(const sgh_attn_geom *g) {
     p.keys_each = int(((size_t(g->k_len) + n - 1) / n + 63) / 64 * 64);
     p.splits = unsigned((g->k_len + p.keys_each - 1) / p.keys_each);
   }
-  p.ws = p.splits > 1 ? size_t(p.splits) * p.units * g->q_len * p.pack * (p.dp + 1) * sizeof(float) : 0;
+  p.part = p.splits > 1 ? (size_t(p.splits) * p.units * g->q_len * p.pack * (p.dp + 1) * sizeof(float) + 15) / 16 * 16 : 0;
+  // where several blocks read them (4 x 16 heads of 61, 2048 tokens: XXX us, read as they are 228)
+  p.pad = p.tiles * (group / p.pack) >= 2;
+  p.ws = p.part + (p.pad ? 2 * wide_bytes(g->dim, size_t(g->batch) * g->k_len * g->kv_heads) : 0);
   return p;
 }
 
@@ -301,13 +323,24 @@ int forward(const sgh_attn_geom *g, const void *q, const void *k, const void *v,
   a.s = shape_of(g, table, q_lengths, k_lengths, q_starts);
   a.q = q, a.k = k, a.v = v, a.o = o, a.lse = lse, a.part = static_cast<float *>(workspace);
   a.tiles = p.tiles, a.units = p.units, a.splits = p.splits, a.pack = p.pack, a.keys_each = p.keys_each;
-  a.direct = g->dim % T::VEC == 0 && sgh_aligned16(q) && sgh_aligned16(k) && sgh_aligned16(v) && sgh_aligned16(o);
+  a.io_dim = g->dim;
+  a.io_direct = g->dim % T::VEC == 0 && sgh_aligned16(q) && sgh_aligned16(o);
+  a.direct = g->dim % T::VEC == 0 && sgh_aligned16(k) && sgh_aligned16(v);
   Bounds bounds;
   bounds_of(g, &bounds);
   hipStream_t s = sgh_stream_of(stream);
   sgh_note_write(o, qn);
   sgh_prof_kernel_scope prof("attn_fwd/k_attn_fwd", 4.0 * g->batch * g->heads * g->q_len * double(g->k_len) * g->dim, s);
-  if (p.splits > 1) prof.span();
+  const int wide = p.pad ? wide_of(g->dim, e) : 0;
+  if (p.splits > 1 || wide) prof.span();
+  if (wide) {
+    const size_t rows = size_t(g->batch) * g->k_len * g->kv_heads;
+    char *at = static_cast<char *>(workspace) + p.part;
+    const PadArgs pad = {{k, v}, {at, at + rows * wide * e}, {rows, rows}, g->dim, wide};
+    const int r = pad_rows<T>(pad, 2, s);
+    if (r != SGH_OK) return r;
+    a.k = pad.to[0], a.v = pad.to[1], a.s.dim = wide, a.direct = true;
+  }
   switch (p.dp) {
     case 32: return run_dim<T, 32>(a, bounds, s);
     case 64: return run_dim<T, 64>(a, bounds, s);
