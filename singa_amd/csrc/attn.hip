@@ -53,18 +53,18 @@ void bounds_of(const sgh_attn_geom *g, Bounds *bounds) {
   for (int i = 0; i < bounds->n; ++i) bounds->at[i] = g->bound[i];
 }
 
-hipError_t allow_lds(const void *kernel, std::atomic<unsigned long long> &asked) {
+}  // namespace attn
+
+hipError_t sgh_allow_lds(const void *kernel, std::atomic<unsigned long long> &asked) {
   int device;
   const hipError_t e = hipGetDevice(&device);
   if (e != hipSuccess) return e;
   const unsigned long long bit = 1ull << (device & 63);
   if (asked.load(std::memory_order_relaxed) & bit) return hipSuccess;
-  const hipError_t f = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+  const hipError_t f = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 156 * 1024);
   if (f == hipSuccess) asked.fetch_or(bit, std::memory_order_relaxed);
   return f;
 }
-
-}  // namespace attn
 
 extern "C" int sgh_attn_geom_init(sgh_attn_geom *g, int batch, int q_len, int k_len, int heads, int kv_heads, int dim, int causal, float scale,
                                   int buckets, int max_distance, int bidirectional) {

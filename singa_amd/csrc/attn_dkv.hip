@@ -232,7 +232,7 @@ template <class T, int DP, int KW, bool BIAS>
 int launch(const BwdArgs &a, const Bounds &bounds, hipStream_t s) {
   const size_t lds = Form<T, DP>::lds(a.s.reach, BIAS);
   static std::atomic<unsigned long long> asked{0};
-  SGH_HIP_TRY(allow_lds(reinterpret_cast<const void *>(k_attn_dkv<T, DP, KW, BIAS>), asked));
+  SGH_HIP_TRY(sgh_allow_lds(reinterpret_cast<const void *>(k_attn_dkv<T, DP, KW, BIAS>), asked));
   hipLaunchKernelGGL((k_attn_dkv<T, DP, KW, BIAS>), dim3(a.k_tiles * a.k_units * a.k_splits), dim3(kBlock), lds, s, a, bounds);
   SGH_LAUNCH_CHECK();
   if (a.k_splits > 1) {

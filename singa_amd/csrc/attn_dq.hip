@@ -8,7 +8,7 @@ namespace {
 using namespace attn;
 
 template <class T, int DP, int QT, bool BIAS>
-__global__ __launch_bounds__(kBlock, 2) void k_attn_dq(BwdArgs a, Bounds bounds) {
+__global__ __launch_bounds__(kBlock, (T::half || DP <= 64 ? 2 : 1)) void k_attn_dq(BwdArgs a, Bounds bounds) {
   typedef typename T::elem elem;
   typedef Tile<T, DP> L;
   constexpr int KT = T::half ? 64 : 32, SUB = KT / 32, ND = DP / 32, WAVE_ROWS = 32 * QT, ROWS = 4 * WAVE_ROWS;
@@ -260,7 +260,7 @@ int launch(const BwdArgs &a, const Bounds &bounds, float *dtable, hipStream_t s)
   constexpr int KT = T::half ? 64 : 32;
   const size_t lds = 4 * Tile<T, DP>::bytes(KT) + (BIAS ? 5 * (2 * a.s.reach + 1) * sizeof(float) : 0);
   static std::atomic<unsigned long long> asked{0};
-  SGH_HIP_TRY(allow_lds(reinterpret_cast<const void *>(k_attn_dq<T, DP, QT, BIAS>), asked));
+  SGH_HIP_TRY(sgh_allow_lds(reinterpret_cast<const void *>(k_attn_dq<T, DP, QT, BIAS>), asked));
   hipLaunchKernelGGL((k_attn_dq<T, DP, QT, BIAS>), dim3(a.q_tiles * a.q_units * a.q_splits), dim3(kBlock), lds, s, a, bounds);
   SGH_LAUNCH_CHECK();
   if (a.q_splits > 1) {

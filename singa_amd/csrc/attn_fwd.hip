@@ -251,7 +251,7 @@ __global__ __launch_bounds__(kBlock) void k_attn_join(FwdArgs a) {
 template <class T, int DP, int QT, bool BIAS>
 int launch(const FwdArgs &a, const Bounds &bounds, size_t lds, hipStream_t s) {
   static std::atomic<unsigned long long> asked{0};
-  SGH_HIP_TRY(allow_lds(reinterpret_cast<const void *>(k_attn_fwd<T, DP, QT, BIAS>), asked));
+  SGH_HIP_TRY(sgh_allow_lds(reinterpret_cast<const void *>(k_attn_fwd<T, DP, QT, BIAS>), asked));
   SGH_LAUNCH_TIMED((k_attn_fwd<T, DP, QT, BIAS>), dim3(a.tiles * a.units * a.splits), dim3(kBlock), lds, s, a, bounds);
   SGH_LAUNCH_CHECK();
   if (a.splits > 1) {

@@ -2,8 +2,6 @@
 #ifndef SINGA_AMD_CSRC_ATTN_RUN_H_
 #define SINGA_AMD_CSRC_ATTN_RUN_H_
 
-#include <atomic>
-
 #include "attn.h"
 
 namespace attn {
@@ -13,8 +11,6 @@ constexpr size_t kMostBand = 24 << 10;
 
 int check_geom(const sgh_attn_geom *g);                   // (attn.hip)
 void bounds_of(const sgh_attn_geom *g, Bounds *bounds);   // (attn.hip)
-// (attn.hip) more than 64 KB of LDS have to be asked for, once for each kernel and device; `asked` is the kernel's own
-hipError_t allow_lds(const void *kernel, std::atomic<unsigned long long> &asked);
 
 static inline size_t band_bytes(const sgh_attn_geom *g) { return g->buckets ? (2 * size_t(g->max_distance) + 1) * sizeof(float) : 0; }
 

@@ -22,7 +22,7 @@ struct Args {
   float *gate_part;
   size_t dim;
   unsigned rows, gates, per_gate;   // rows of a gate, 0: no gate
-  unsigned each, chunks;            // rows of a team of the grid; workgroups to a gate (backwards)
+  unsigned each, chunks;            // rows of a team of the grid; workgroups to a gate (backwards; 0: a team has whole gates)
   float scale, eps;
 };
 
@@ -64,13 +64,13 @@ struct Place {
 template <class S, int EPL, int NV>
 struct Raw {
   typename S::elem e[NV][EPL];
-  // STREAM: past the caches
+  // STREAM: past the caches; not `there`: zeros
   template <bool STREAM = false, class P>
-  __device__ __forceinline__ void load(const void *t, size_t row, size_t dim, const P &p) {
+  __device__ __forceinline__ void load(const void *t, size_t row, size_t dim, const P &p, bool there = true) {
     const typename S::elem *r = static_cast<const typename S::elem *>(t) + row * dim;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-      if (p.has(j)) {
+      if (p.has(j) && there) {
         if constexpr (STREAM) {
           typedef sgh_v4u anywhere __attribute__((aligned(2)));
           const sgh_v4u v = __builtin_nontemporal_load(reinterpret_cast<const anywhere *>(r + p.at[j]));
@@ -215,82 +215,84 @@ __global__ __launch_bounds__(kThreads<TEAM>) void k_norm_fwd(Args a) {
 template <class S, int TEAM>
 constexpr int kPerSimd = S::VEC == 8 || TEAM == 1024 ? 4 : 2;
 
-template <class S, int EPL, int TEAM, int NV, bool HOLD, bool STREAM>
+template <class S, int EPL, int TEAM, int NV, bool STREAM>
 __global__ __launch_bounds__(kThreads<TEAM>, (kPerSimd<S, TEAM>)) void k_norm_bwd(Args a) {
   constexpr int PER = kThreads<TEAM> / TEAM;
   __shared__ float lds[2][16];
   extern __shared__ __align__(16) float kept[];   // the weights, and in the end the teams' sums
-  if (HOLD) keep_weights<kThreads<TEAM>>(a, kept);
-  const float *const post_at = HOLD ? kept : a.post, *const pre_at = HOLD ? kept + a.dim : a.pre;
+  keep_weights<kThreads<TEAM>>(a, kept);
+  const float *const post_at = kept, *const pre_at = kept + a.dim;
   const size_t dim = a.dim;
   const Place<EPL, TEAM, NV> p{unsigned(dim)};
   const bool block = a.h != nullptr, token_gate = a.per_gate == 1, shared_gate = a.per_gate > 1;
-  // A team's rows: `each` of them one behind the other, or a part of one gate's
-  const size_t team = size_t(blockIdx.x) * PER + threadIdx.x / TEAM;
-  size_t row = team * a.each, end = row + a.each, slot = 0;
-  if (shared_gate && a.chunks > 1) {
-    const size_t g = team / a.chunks, c = team % a.chunks;
-    row = g * a.per_gate + c * a.each, end = row + a.each;
-    const size_t stop = (g + 1) * a.per_gate;
+  // A team's rows: `each` of them one behind the other; of one gate's, where workgroups share it
+  const unsigned mine_of = threadIdx.x / TEAM;
+  size_t row = (size_t(blockIdx.x) * PER + mine_of) * a.each, end = row + a.each;
+  if (a.chunks) {
+    const size_t g = blockIdx.x / a.chunks, stop = (g + 1) * a.per_gate;
+    row = g * a.per_gate + (size_t(blockIdx.x % a.chunks) * PER + mine_of) * a.each, end = row + a.each;
     if (end > stop) end = stop;
-    slot = team;
   }
   if (end > a.rows) end = a.rows;
   const unsigned count = row < end ? unsigned(end - row) : 0;
-  const size_t last = a.rows - 1;
-  float gate[NV][EPL], sum_pre[NV][EPL], sum_post[NV][EPL], sum_gate[NV][EPL];
+  // Sums over the rows: of dn y r, and of scale t unit, times the gate unless rows share it (a shared gate's sums go into sum_post when its rows are
+  // done)
+  float gate[NV][EPL], sum_pre[NV][EPL], sum_unit[NV][EPL], sum_post[NV][EPL];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) sum_pre[j][e] = sum_post[j][e] = sum_gate[j][e] = 0.f;
-  Raw<S, EPL, NV> rt, rn, ry, rh, rg;
-  auto request = [&](size_t r) {
-    r = r < last ? r : last;
-    if (a.dy) rt.load(a.dy, r, dim, p);
-    if (a.pre) rn.load(a.dn, r, dim, p), ry.load(a.y, r, dim, p);
-    if (block) rh.load(a.h, r, dim, p);
-    if (token_gate) rg.load(a.gate, r, dim, p);
+    for (int e = 0; e < EPL; ++e) gate[j][e] = 1.f, sum_pre[j][e] = sum_unit[j][e] = sum_post[j][e] = 0.f;
+  auto load_gate = [&](size_t g) {
+    Raw<S, EPL, NV> r;
+    r.load(a.gate, g, dim, p);
+    r.get(gate);
   };
-  // the gate's sums are complete (or those of this team's part): sum_gate holds the sum of scale t unit
-  auto leave_gate = [&](size_t g) {
-    float d[NV][EPL];
+  // (rows that a team does not have are zeros, and add nothing)
+  Raw<S, EPL, NV> rt, rn, ry, rh, rg;
+  auto request = [&](size_t r, bool there) {
+    rt.load(a.dy, r, dim, p, there && a.dy);
+    if (a.pre) rn.load(a.dn, r, dim, p, there), ry.load(a.y, r, dim, p, there);
+    if (block) rh.load(a.h, r, dim, p, there);
+    if (token_gate) rg.load(a.gate, r, dim, p, there);
+  };
+  size_t group = ~size_t(0), group_end = 0;
+  // a shared gate's sums are complete, or those of this team's part: d gets its gradient
+  auto leave_gate = [&](float (&d)[NV][EPL]) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) d[j][e] = 1.f;
     if (a.post) load_floats(post_at, p, d);
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int e = 0; e < EPL; ++e) {
-        d[j][e] = a.post ? sum_gate[j][e] * d[j][e] : sum_gate[j][e];
-        sum_post[j][e] = __builtin_fmaf(gate[j][e], sum_gate[j][e], sum_post[j][e]);
-        sum_gate[j][e] = 0.f;
+        d[j][e] *= sum_unit[j][e];
+        sum_post[j][e] = __builtin_fmaf(gate[j][e], sum_unit[j][e], sum_post[j][e]);
+        sum_unit[j][e] = 0.f;
       }
-    if (a.chunks > 1) store_floats(a.gate_part + slot * dim, p, d);
-    else store_row<S>(a.dgate, g, dim, p, d);
   };
-  request(row);
-  size_t group = ~size_t(0);
+  request(row, count != 0);
   const float inv_dim = 1.f / float(dim);
   for (unsigned i = 0; i < a.each; ++i, ++row) {
     const bool mine = i < count;
-    const size_t at = row < last ? row : last;
-    if (!HOLD && i) request(row);
     // (as stored until they are used: 16-bit rows then take half of the registers)
     const Raw<S, EPL, NV> ct = rt, cn = rn, cy = ry, ch = rh;
     if (token_gate) rg.get(gate);
-    const float rh_root = a.stats[2 * at], ry_root = a.stats[2 * at + 1];
-    if (HOLD && i + 1 < a.each) request(row + 1);
-    if (shared_gate && mine) {
-      const size_t g = row / a.per_gate;
-      if (g != group) {
-        if (group != ~size_t(0)) leave_gate(group);
-        Raw<S, EPL, NV> r;
-        r.load(a.gate, g, dim, p);
-        r.get(gate);
-        group = g;
+    const float rh_root = mine && a.post ? a.stats[2 * row] : 1.f, ry_root = mine ? a.stats[2 * row + 1] : 0.f;
+    if (i + 1 < a.each) request(row + 1, i + 1 < count);
+    if (shared_gate && mine && row >= group_end) {
+      if (group != ~size_t(0)) {
+        float d[NV][EPL];
+        leave_gate(d);
+        store_row<S>(a.dgate, group, dim, p, d);
       }
+      group = row / a.per_gate, group_end = (group + 1) * a.per_gate;
+      load_gate(group);
     }
-    float t[NV][EPL];
+    float t[NV][EPL], w[NV][EPL];
     if (a.pre) {
-      float w[NV][EPL], c = 0.f;
+      float c = 0.f;
       load_floats(pre_at, p, w);
 #pragma unroll
       for (int j = 0; j < NV; ++j)
@@ -304,62 +306,230 @@ __global__ __launch_bounds__(kThreads<TEAM>, (kPerSimd<S, TEAM>)) void k_norm_bw
       for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int e = 0; e < EPL; ++e) {
-          t[j][e] = __builtin_fmaf(ry_root, __builtin_fmaf(-c, cy(j, e), w[j][e]), a.dy ? ct(j, e) : 0.f);
-          if (mine) sum_pre[j][e] = __builtin_fmaf(cn(j, e), cy(j, e) * ry_root, sum_pre[j][e]);
+          t[j][e] = __builtin_fmaf(ry_root, __builtin_fmaf(-c, cy(j, e), w[j][e]), ct(j, e));
+          sum_pre[j][e] = __builtin_fmaf(cn(j, e), cy(j, e) * ry_root, sum_pre[j][e]);
         }
     } else {
       ct.get(t);
     }
     if (mine) store_row<S, STREAM>(a.dx, row, dim, p, t);
     if (block) {
-      const float root = a.post ? rh_root : 1.f;
-      float w[NV][EPL], c = 0.f;
+      float c = 0.f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) w[j][e] = 1.f;
       if (a.post) load_floats(post_at, p, w);
-      // (w, then the gradient by the normalised result; t, then the gate's gradient)
+      // (w becomes the gradient by the normalised result, t the gate's)
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int e = 0; e < EPL; ++e) {
-          const float st = a.scale * t[j][e], each = st * (ch(j, e) * root), weight = a.post ? w[j][e] : 1.f;
-          t[j][e] = each * weight;
-          w[j][e] = (a.per_gate ? st * gate[j][e] : st) * weight;
-          if (mine) {
-            if (shared_gate) sum_gate[j][e] += each;
-            else sum_post[j][e] += a.per_gate ? each * gate[j][e] : each;
-          }
-          if (a.post) c += e < p.dup[j] ? 0.f : w[j][e] * ch(j, e);
+          const float st = a.scale * t[j][e], each = st * (ch(j, e) * rh_root);
+          t[j][e] = each * w[j][e];
+          sum_unit[j][e] += shared_gate ? each : each * gate[j][e];
+          w[j][e] *= st * gate[j][e];
+          c += e < p.dup[j] ? 0.f : w[j][e] * ch(j, e);
         }
       if (token_gate && mine) store_row<S, STREAM>(a.dgate, row, dim, p, t);
       if (a.post) {
-        c = team_sum<TEAM>(c, lds[1]) * inv_dim * root * root;
+        c = team_sum<TEAM>(c, lds[1]) * inv_dim * rh_root * rh_root;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-          for (int e = 0; e < EPL; ++e) w[j][e] = root * __builtin_fmaf(-c, ch(j, e), w[j][e]);
+          for (int e = 0; e < EPL; ++e) w[j][e] = rh_root * __builtin_fmaf(-c, ch(j, e), w[j][e]);
       }
       if (mine) store_row<S, STREAM>(a.dh, row, dim, p, w);
     }
     if (TEAM > SGH_WAVE && !(a.pre && a.post && block)) __syncthreads();
   }
-  if (shared_gate && group != ~size_t(0)) leave_gate(group);
   // the teams of a workgroup, joined in their order
-  float *out = a.part + size_t(blockIdx.x) * 2 * dim;
-  if constexpr (PER == 1) {
-    if (a.pre) store_floats(out, p, sum_pre);
-    if (a.post) store_floats(out + dim, p, sum_post);
-  } else {
-    float *const sums = kept;   // [PER][dim]
-    for (int which = 0; which < 2; ++which) {
-      if (!(which ? a.post : a.pre)) continue;
-      __syncthreads();
-      store_floats(sums + threadIdx.x / TEAM * dim, p, which ? sum_post : sum_pre);
-      __syncthreads();
-      for (size_t c = threadIdx.x; c < dim; c += kThreads<TEAM>) {
-        float x = 0.f;
-        for (int k = 0; k < PER; ++k) x += sums[k * dim + c];
-        out[which * dim + c] = x;
+  float *const sums = kept, *const out = a.part + size_t(blockIdx.x) * 2 * dim;   // sums: [PER][dim]
+  auto join = [&](const float (&f)[NV][EPL], auto put) {
+    __syncthreads();
+    store_floats(sums + mine_of * dim, p, f);
+    __syncthreads();
+    for (size_t c = threadIdx.x; c < dim; c += kThreads<TEAM>) {
+      float x = 0.f;
+      for (int k = 0; k < PER; ++k) x += sums[k * dim + c];
+      put(c, x);
+    }
+  };
+  float d[NV][EPL];
+  if (shared_gate) {
+    __builtin_memset(d, 0, sizeof(d));
+    if (group != ~size_t(0)) leave_gate(d);
+    float *const part = a.gate_part + size_t(blockIdx.x) * dim;
+    if (!a.chunks) {
+      if (group != ~size_t(0)) store_row<S>(a.dgate, group, dim, p, d);
+    } else if constexpr (PER == 1) {
+      if (a.chunks > 1) store_floats(part, p, d);
+      else store_row<S>(a.dgate, blockIdx.x, dim, p, d);
+    } else {
+      typename S::elem *whole = static_cast<typename S::elem *>(a.dgate) + size_t(blockIdx.x) * dim;
+      join(d, [&](size_t c, float x) {
+        if (a.chunks > 1) part[c] = x;
+        else S::st(whole + c, x);
+      });
+    }
+  }
+  if (a.pre) {
+    if constexpr (PER == 1) store_floats(out, p, sum_pre);
+    else join(sum_pre, [&](size_t c, float x) { out[c] = x; });
+  }
+  if (a.post) {
+    if (!shared_gate)
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) sum_post[j][e] = sum_unit[j][e];
+    if constexpr (PER == 1) store_floats(out + dim, p, sum_post);
+    else join(sum_post, [&](size_t c, float x) { out[dim + c] = x; });
+  }
+}
+
+// Rows of more than 8192 values: a workgroup of 1024 threads has no registers for 16 values of each of four tensors and the sums (kept in scratch
+// memory, every load was waited for before the next: 4000 rows of 16384 bfloat16 values 490 us).  It goes over a row three times, the second and
+// third time out of the caches, and has the sums in LDS, at places of each thread's own.
+constexpr int kWide = 1024;
+template <class S, int NV>
+__global__ __launch_bounds__(kWide, 4) void k_norm_bwd_wide(Args a) {
+  constexpr int EPL = S::VEC;
+  typedef typename S::elem elem;
+  __shared__ float lds[2][16];
+  extern __shared__ __align__(16) float kept[];   // [2][NV][EPL][kWide]
+  const size_t dim = a.dim;
+  const Place<EPL, kWide, NV> p{unsigned(dim)};
+  const bool block = a.h != nullptr, token_gate = a.per_gate == 1, shared_gate = a.per_gate > 1;
+  size_t row = size_t(blockIdx.x) * a.each, end = row + a.each;
+  if (a.chunks) {
+    const size_t g = blockIdx.x / a.chunks, stop = (g + 1) * a.per_gate;
+    row = g * a.per_gate + size_t(blockIdx.x % a.chunks) * a.each, end = row + a.each;
+    if (end > stop) end = stop;
+  }
+  if (end > a.rows) end = a.rows;
+  float *const out = a.part + size_t(blockIdx.x) * 2 * dim;
+  auto sum_pre = [&](int j, int e) -> float & { return kept[(j * EPL + e) * kWide + threadIdx.x]; };
+  auto sum_unit = [&](int j, int e) -> float & { return kept[((NV + j) * EPL + e) * kWide + threadIdx.x]; };
+  auto vec = [&](const void *t, size_t r, int j, float *f) { sgh_load_any<S, EPL>(static_cast<const elem *>(t) + r * dim + p.at[j], f); };
+  auto put = [&](void *t, size_t r, int j, const float *f) { sgh_store_any<S, EPL>(static_cast<elem *>(t) + r * dim + p.at[j], f); };
+  auto weight = [&](const float *t, int j, float *f) { __builtin_memcpy(f, t + p.at[j], EPL * sizeof(float)); };
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) sum_pre(j, e) = sum_unit(j, e) = 0.f;
+  bool left = false;
+  // the part of the gradient of post: an element that two vectors have is the first one's, which the sum so far is read by alone
+  auto keep = [&](int j, const float *f) {
+    if (p.dup[j] == 0) __builtin_memcpy(out + dim + p.at[j], f, EPL * sizeof(float));
+    else
+#pragma unroll
+      for (int e = 0; e < EPL; ++e)
+        if (e >= p.dup[j]) out[dim + p.at[j] + e] = f[e];
+  };
+  // a shared gate's sums are complete, or this workgroup's part of them
+  auto leave_gate = [&](size_t g) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (!p.has(j)) continue;
+      float d[EPL], gate[EPL], sum[EPL];
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) d[e] = 1.f, sum[e] = 0.f;
+      if (a.post) weight(a.post, j, d);
+      vec(a.gate, g, j, gate);
+      if (a.post && left) weight(out + dim, j, sum);
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        const float x = sum_unit(j, e);
+        sum_unit(j, e) = 0.f;
+        d[e] *= x;
+        sum[e] = __builtin_fmaf(gate[e], x, sum[e]);
+      }
+      if (a.post) keep(j, sum);
+      if (a.chunks > 1) __builtin_memcpy(a.gate_part + size_t(blockIdx.x) * dim + p.at[j], d, sizeof(d));
+      else put(a.dgate, g, j, d);
+    }
+    left = true;
+  };
+  size_t group = ~size_t(0), group_end = 0;
+  const float inv_dim = 1.f / float(dim);
+  for (; row < end; ++row) {
+    const float rh_root = a.post ? a.stats[2 * row] : 1.f, ry_root = a.stats[2 * row + 1];
+    if (shared_gate && row >= group_end) {
+      if (group != ~size_t(0)) leave_gate(group);
+      group = row / a.per_gate, group_end = (group + 1) * a.per_gate;
+    }
+    float t[NV][EPL], c = 0.f;
+    if (a.pre) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if (!p.has(j)) continue;
+        float dn[EPL], y[EPL], w[EPL];
+        vec(a.dn, row, j, dn), vec(a.y, row, j, y), weight(a.pre, j, w);
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) c += e < p.dup[j] ? 0.f : w[e] * dn[e] * y[e];
+      }
+      c = team_sum<kWide>(c, lds[0]) * inv_dim * ry_root * ry_root;
+    }
+    float d = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (!p.has(j)) continue;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) t[j][e] = 0.f;
+      if (a.dy) vec(a.dy, row, j, t[j]);
+      if (a.pre) {
+        float dn[EPL], y[EPL], w[EPL];
+        vec(a.dn, row, j, dn), vec(a.y, row, j, y), weight(a.pre, j, w);
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+          t[j][e] = __builtin_fmaf(ry_root, __builtin_fmaf(-c, y[e], w[e] * dn[e]), t[j][e]);
+          sum_pre(j, e) += dn[e] * (y[e] * ry_root);
+        }
+      }
+      put(a.dx, row, j, t[j]);
+      if (!block) continue;
+      float h[EPL], w[EPL], gate[EPL];
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) w[e] = gate[e] = 1.f;
+      vec(a.h, row, j, h);
+      if (a.post) weight(a.post, j, w);
+      if (a.per_gate) vec(a.gate, token_gate ? row : group, j, gate);
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        const float st = a.scale * t[j][e], each = st * (h[e] * rh_root);
+        sum_unit(j, e) += shared_gate ? each : each * gate[e];
+        t[j][e] = w[e] * (st * gate[e]);
+        d += e < p.dup[j] ? 0.f : t[j][e] * h[e];
+        w[e] *= each;
+      }
+      if (token_gate) put(a.dgate, row, j, w);
+      __builtin_amdgcn_sched_barrier(0);   // (one vector of each tensor at a time: more would not leave the registers)
+    }
+    if (block) {
+      if (a.post) d = team_sum<kWide>(d, lds[1]) * inv_dim * rh_root * rh_root;
+      else d = 0.f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if (!p.has(j)) continue;
+        float h[EPL];
+        vec(a.h, row, j, h);
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) h[e] = rh_root * __builtin_fmaf(-d, h[e], t[j][e]);
+        put(a.dh, row, j, h);
       }
     }
+    if (!(a.pre && a.post && block)) __syncthreads();
+  }
+  if (group != ~size_t(0)) leave_gate(group);
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if (!p.has(j)) continue;
+    float f[EPL], g[EPL];
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) f[e] = sum_pre(j, e), g[e] = sum_unit(j, e);
+    if (a.pre) __builtin_memcpy(out + p.at[j], f, sizeof(f));
+    if (a.post && (!shared_gate || !left)) keep(j, g);   // (a workgroup without a row: zeros)
   }
 }
 
@@ -423,23 +593,20 @@ struct Plan {
 Plan plan_of(size_t rows, size_t dim, size_t gates) {
   Plan p{form_of(dim), 1, 1, 1, 0, 0};
   const size_t teams = size_t(sgh_num_cus()) * (p.form.team <= 256 ? 1024 / kThreads<256> : p.form.team == 512 ? 2 : 1) * p.form.per;
-  const size_t per_gate = gates ? rows / gates : 0;
+  const size_t per_gate = gates ? rows / gates : 0, per = p.form.per;
   size_t each = (rows + teams - 1) / teams, n;
   if (each < 2) each = 2;   // (a workgroup's sums are as much to write and read as a row of fp32 values)
-  if (per_gate > 1) {
-    if (per_gate > each) {
-      p.chunks = unsigned((per_gate + each - 1) / each);
-      each = (per_gate + p.chunks - 1) / p.chunks;
-      n = gates * p.chunks;
-    } else {
-      each = each / per_gate * per_gate;
-      n = (rows + each - 1) / each;
-    }
+  p.chunks = 0;
+  if (per_gate > each && per_gate * 2 >= per) {   // (a gate has work for half of a workgroup's teams)
+    p.chunks = unsigned((per_gate + each * per - 1) / (each * per));
+    each = (per_gate + p.chunks * per - 1) / (p.chunks * per);
+    n = gates * p.chunks * per;
   } else {
+    if (per_gate > 1) each = each > per_gate ? each / per_gate * per_gate : per_gate;
     n = (rows + each - 1) / each;
   }
   p.each = unsigned(each);
-  p.blocks = unsigned((n + p.form.per - 1) / p.form.per);
+  p.blocks = unsigned((n + per - 1) / per);
   p.part = size_t(p.blocks) * 2 * dim;
   p.gate_part = p.chunks > 1 ? gates * p.chunks * dim : 0;
   return p;
@@ -478,9 +645,17 @@ template <class S>
 int run_bwd(const Args &a, const Plan &p, float *dpre, float *dpost, hipStream_t s) {
   const Form &f = p.form;
   const bool stream = streams<S>(a);
-#define RUN(S, EPL, TEAM, NV, HOLD, STREAM) \
-  hipLaunchKernelGGL((k_norm_bwd<S, EPL, TEAM, NV, HOLD, STREAM>), dim3(p.blocks), dim3(kThreads<TEAM>), HOLD ? (f.per > 2 ? f.per : 2) * a.dim * 4 : 0, s, a)
+#define LAUNCH(kern, threads, bytes)                                                                     \
+  do {                                                                                                   \
+    static std::atomic<unsigned long long> asked{0};                                                     \
+    SGH_HIP_TRY(sgh_allow_lds(reinterpret_cast<const void *>(kern), asked));                             \
+    hipLaunchKernelGGL(kern, dim3(p.blocks), dim3(threads), bytes, s, a);                                \
+  } while (0)
+#define RUN(S, EPL, TEAM, NV, HOLD, STREAM)                                                              \
+  if constexpr (HOLD) LAUNCH((k_norm_bwd<S, EPL, TEAM, NV, STREAM>), kThreads<TEAM>, (f.per > 2 ? f.per : 2) * a.dim * sizeof(float)); \
+  else LAUNCH((k_norm_bwd_wide<S, NV>), kWide, 2 * sizeof(float) * kWide * NV * EPL)
   SGH_NORM_FORMS(RUN, S)
+#undef LAUNCH
 #undef RUN
   SGH_LAUNCH_CHECK();
   const unsigned gates = p.chunks > 1 ? a.gates : 0, y = 2 + (gates < 32768 ? gates : 32768), z = gates ? (gates + 32767) / 32768 : 1;

@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 #include <hip/hip_ext.h>
+#include <atomic>
 #include <stddef.h>
 #include <stdint.h>
 
@@ -59,6 +60,9 @@ void sgh_bn_mark_exchange_ran();
 // Reads a counter in device memory that kernels on any stream add to, and takes off what was read, both on `s` behind its work: what another
 // stream adds meanwhile is left for the next call (runtime.hip).  Waits for `s`.
 int sgh_take_count(int *counter, hipStream_t s, int *count);
+
+// More than 64 KB of LDS have to be asked for, once for each kernel and device; `asked` is the kernel's own (attn.hip)
+hipError_t sgh_allow_lds(const void *kernel, std::atomic<unsigned long long> &asked);
 
 // Weight epoch: a host-side counter that every entry point which may change a weight tensor advances
 // (optimizer updates, Axpy, fills, casts, copies to the device, sgh_conv_weights_changed).  The note that
