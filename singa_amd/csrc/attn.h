@@ -56,12 +56,8 @@ __device__ __forceinline__ Span span_of(const Shape &s, int b) {
 // the bucket of a key `distance` behind its query
 __device__ __forceinline__ int bucket_of(const Shape &s, const Bounds &bounds, int distance) {
   const int n = s.bidirectional ? abs(distance) : max(-distance, 0);
-  int lo = 0, hi = bounds.n;   // bounds at or below n
-  while (lo < hi) {
-    const int m = (lo + hi) >> 1;
-    if (bounds.at[m] <= n) lo = m + 1;
-    else hi = m;
-  }
+  int lo = 0;
+  for (int m = 0; m < bounds.n; ++m) lo += bounds.at[m] <= n;   // (the same for all lanes: scalar loads, and none waits for another)
   return s.bidirectional && distance > 0 ? lo + s.buckets / 2 : lo;
 }
 
@@ -509,14 +505,25 @@ __global__ __launch_bounds__(kBlock) void k_attn_pad(PadArgs a) {
 }
 
 // Where a call's blocks lie: block w runs on the XCD w % 8, so the blocks of one head of keys, which read the same rows, go to one XCD where
-// their number allows it
-__device__ __forceinline__ void block_at(unsigned w, unsigned tiles, unsigned units, unsigned *tile, unsigned *unit) {
+// their number allows it.  Splits lie one behind the other.  Under a causal mask the tiles are of different lengths: long ones come first
+// (`down`: the last ones), but where all blocks run at once every other 256 of them go the other way, so that a CU gets a short one with
+// each long one (8 x 8 heads, 512 tokens, fp32 backward: XXX -> XXX us).
+struct Where {
+  unsigned tile, unit, split;
+};
+__device__ __forceinline__ Where block_at(unsigned tiles, unsigned units, unsigned splits, bool down) {
+  const unsigned n = tiles * units, split = blockIdx.x / n, w = blockIdx.x % n;
+  Where r = {0, 0, split};
+  unsigned round;
   if (units % 8 == 0) {
-    const unsigned l = w / 8;
-    *unit = (l / tiles) * 8 + w % 8, *tile = l % tiles;
+    const unsigned l = w / 8, group = l / tiles;
+    r.unit = group * 8 + w % 8, r.tile = l % tiles, round = group * tiles * 8;
   } else {
-    *unit = w / tiles, *tile = w % tiles;
+    r.unit = w / tiles, r.tile = w % tiles, round = r.unit * tiles;
   }
+  const bool other = n * splits <= 512 && ((split * n + round) / 256) % 2 != 0;
+  if (down != other) r.tile = tiles - 1 - r.tile;
+  return r;
 }
 
 }  // namespace attn

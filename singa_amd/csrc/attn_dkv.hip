@@ -33,9 +33,8 @@ __global__ __launch_bounds__(kBlock, (Form<T, DP>::PER_SIMD)) void k_attn_dkv(Bw
   extern __shared__ __align__(16) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
   const Shape &s = a.s;
-  const unsigned w = blockIdx.x / a.k_splits, split = blockIdx.x % a.k_splits;
-  unsigned tile, unit;
-  block_at(w, a.k_tiles, a.k_units, &tile, &unit);
+  const Where place = block_at(a.k_tiles, a.k_units, a.k_splits, false);
+  const unsigned tile = place.tile, unit = place.unit, split = place.split;
   const int b = unit / s.kv_heads, kv = unit % s.kv_heads, group = s.heads / s.kv_heads;
   const Span span = span_of(s, b);
   const int key0 = int(tile) * KEYS + wave * WAVE_KEYS;
@@ -278,15 +277,15 @@ Plan plan_of(const sgh_attn_geom *g) {
   // few blocks: several to the keys of a block of queries, and to the queries of a block of keys
   a.q_splits = a.k_splits = 1, a.keys_each = 1 << 30;
   const size_t q_blocks = size_t(a.q_tiles) * a.q_units, k_blocks = size_t(a.k_tiles) * a.k_units;
-  if (q_blocks * 2 <= 2 * cus && g->k_len > 256) {
-    size_t n = 2 * cus / q_blocks, most = (size_t(g->k_len) + 255) / 256;
+  if (q_blocks * 2 <= 2 * cus && g->k_len > 512) {
+    size_t n = 2 * cus / q_blocks, most = size_t(g->k_len) / 512;
     if (n > most) n = most;
     a.keys_each = int(((size_t(g->k_len) + n - 1) / n + 63) / 64 * 64);
     a.q_splits = unsigned((g->k_len + a.keys_each - 1) / a.keys_each);
   }
   const size_t turns = size_t(group) * ((size_t(g->q_len) + 63) / 64);
-  if (k_blocks && k_blocks * 2 <= 2 * cus && turns > 2) {
-    size_t n = 2 * cus / k_blocks, most = turns / 2;
+  if (k_blocks && k_blocks * 2 <= 2 * cus && turns >= 8) {
+    size_t n = 2 * cus / k_blocks, most = turns / 4;
     a.k_splits = unsigned(n < most ? n : most);
   }
   a.bias_blocks = size_t(g->batch) * a.q_tiles * a.q_splits;

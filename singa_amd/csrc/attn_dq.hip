@@ -16,10 +16,8 @@ __global__ __launch_bounds__(kBlock, (T::half || DP <= 64 ? 2 : 1)) void k_attn_
   extern __shared__ __align__(16) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
   const Shape &s = a.s;
-  const unsigned w = blockIdx.x / a.q_splits, split = blockIdx.x % a.q_splits;
-  unsigned tile, unit;
-  block_at(w, a.q_tiles, a.q_units, &tile, &unit);
-  tile = a.q_tiles - 1 - tile;
+  const Where place = block_at(a.q_tiles, a.q_units, a.q_splits, true);
+  const unsigned tile = place.tile, unit = place.unit, split = place.split;
   const int per_batch = s.heads / a.pack, b = unit / per_batch, head0 = int(unit % per_batch) * a.pack;
   const int kv = head0 / (s.heads / s.kv_heads);
   const Span span = span_of(s, b);
@@ -203,19 +201,17 @@ __global__ __launch_bounds__(kBlock, (T::half || DP <= 64 ? 2 : 1)) void k_attn_
     if (lane == 0) sums[0] += far_back, sums[2 * s.reach] += far_on;
     __syncthreads();
     float *out = a.bias_part + (size_t(head0) * a.bias_blocks + (size_t(b) * a.q_tiles + tile) * a.q_splits + split) * s.buckets;
-    const float *all = band + band_len;
+    float *all = band + band_len;
+    for (int d = tid; d < band_len; d += kBlock) all[d] = (all[d] + all[band_len + d]) + (all[2 * band_len + d] + all[3 * band_len + d]);
+    __syncthreads();
+    all += s.reach;
     for (int e = tid; e < s.buckets; e += kBlock) {
-      const int half = s.bidirectional ? s.buckets / 2 : s.buckets, n = e % half, side = e / half;
-      const int from = n == 0 ? 0 : bounds.at[n - 1], to = n == half - 1 ? s.reach : bounds.at[n] - 1;
+      const int half = s.bidirectional ? s.buckets / 2 : s.buckets, n = e % half, sign = e < half ? -1 : 1;
+      const int from = n == 0 ? 0 : bounds.at[n - 1], to = n == half - 1 ? s.reach : min(bounds.at[n] - 1, s.reach);
       float x = 0.f;
-      for (int m = from; m <= to && m <= s.reach; ++m) {
-        const int d = side ? m : -m;
-        if (!side || m > 0)
-          for (int v = 0; v < 4; ++v) x += all[v * band_len + d + s.reach];
-      }
+      for (int m = max(from, sign > 0); m <= to; ++m) x += all[sign * m];
       if (!s.bidirectional && n == 0)   // (one direction: all keys in front have the bucket of distance 0)
-        for (int d = 1; d <= s.reach; ++d)
-          for (int v = 0; v < 4; ++v) x += all[v * band_len + d + s.reach];
+        for (int d = 1; d <= s.reach; ++d) x += all[d];
       out[e] = x;
     }
   }

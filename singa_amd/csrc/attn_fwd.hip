@@ -37,10 +37,8 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
   extern __shared__ __align__(16) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
   const Shape &s = a.s;
-  const unsigned w = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
-  unsigned tile, unit;
-  block_at(w, a.tiles, a.units, &tile, &unit);
-  tile = a.tiles - 1 - tile;   // (with a causal mask the last tiles are the longest)
+  const Where at = block_at(a.tiles, a.units, a.splits, true);
+  const unsigned tile = at.tile, unit = at.unit, split = at.split;
   const int per_batch = s.heads / a.pack, b = unit / per_batch, head0 = int(unit % per_batch) * a.pack;
   const int kv = head0 / (s.heads / s.kv_heads);
   const Span span = span_of(s, b);
@@ -89,7 +87,9 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
     zero(acc[t]);
     m[t] = -3e38f, l[t] = 0.f;
   }
-  const float c = s.scale * kLog2e;
+  // (maxima are taken before the scale, which is therefore made positive: the products are multiplied by -1 or 0 first if it is not)
+  const float factor = s.scale * kLog2e;
+  const float turned = BIAS || factor > 0.f ? 1.f : factor < 0.f ? -1.f : 0.f, c = BIAS || factor != 0.f ? (BIAS ? factor : __builtin_fabsf(factor)) : 1.f;
   const Reader<T, DP> reader(lane);
   auto request = [&](int k0, int slot) {
     stage(lds + slot * 2 * TILE, kp + k0 * stride, span.k - k0);
@@ -109,7 +109,15 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
       zero(p[u]);
       reader.rows(kt, 32 * u, qf, p[u]);
     }
-    // scores in units of log2, -inf where the mask is
+    // Scores: in units of log2 with a bias; else as the products are, and the maximum is multiplied.  -inf where the mask is.
+    if (!BIAS && turned != 1.f) {
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) p[u][t][i] *= turned;
+    }
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       float top = kNegInf;
@@ -132,11 +140,6 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
               p[u][t][i] = __builtin_fmaf(p[u][t][i], c, mine[min(max(d, -s.reach), s.reach)]);
             }
         }
-      } else {
-#pragma unroll
-        for (int u = 0; u < SUB; ++u)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) p[u][t][i] *= c;
       }
       if (k0 + KT > least) {
         const int left = limit[t] - k0 - 4 * hi;
@@ -151,6 +154,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, p[u][t][i]);
       top = max_of_pair(top);
+      if (!BIAS) top *= c;
       if (__ballot(top > m[t] + kGrowth)) {
         const float now = fmaxf(m[t], top), f = __builtin_amdgcn_exp2f(m[t] - now);
         m[t] = now, l[t] *= f;
@@ -165,7 +169,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
       for (int u = 0; u < SUB; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          p[u][t][i] = __builtin_amdgcn_exp2f(p[u][t][i] - from);
+          p[u][t][i] = __builtin_amdgcn_exp2f(BIAS ? p[u][t][i] - from : __builtin_fmaf(p[u][t][i], c, -from));
           sum += p[u][t][i];
         }
       l[t] += sum;
@@ -278,11 +282,11 @@ Plan plan_of(const sgh_attn_geom *g) {
   p.pack = size_t(g->q_len) * group <= kRows && band_bytes(g) * group <= kMostBand ? group : 1;
   p.tiles = unsigned((size_t(g->q_len) * p.pack + kRows - 1) / kRows);
   p.units = unsigned(size_t(g->batch) * (g->heads / p.pack));
-  // few rows: several blocks to the keys of each, of 256 keys at the least
+  // Few rows: several blocks to the keys of each, of 512 keys at the least (the launch that joins them takes 4 us and more, 64 keys of a block 1.2)
   p.splits = 1, p.keys_each = 1 << 30;
   const size_t blocks = size_t(p.tiles) * p.units, want = 4 * size_t(sgh_num_cus());
-  if (blocks * 2 <= want && g->k_len > 256) {
-    size_t n = want / blocks, most = (size_t(g->k_len) + 255) / 256;
+  if (blocks * 2 <= want && g->k_len > 512) {
+    size_t n = want / blocks, most = size_t(g->k_len) / 512;
     if (n > most) n = most;
     p.keys_each = int(((size_t(g->k_len) + n - 1) / n + 63) / 64 * 64);
     p.splits = unsigned((g->k_len + p.keys_each - 1) / p.keys_each);
