@@ -278,7 +278,7 @@ Plan plan_of(const sgh_attn_geom *g) {
   a.q_splits = a.k_splits = 1, a.keys_each = 1 << 30;
   const size_t q_blocks = size_t(a.q_tiles) * a.q_units, k_blocks = size_t(a.k_tiles) * a.k_units;
   if (q_blocks * 2 <= 2 * cus && g->k_len > 512) {
-    size_t n = 2 * cus / q_blocks, most = size_t(g->k_len) / 512;
+    size_t n = 2 * cus / q_blocks, most = (size_t(g->k_len) + 511) / 512;
     if (n > most) n = most;
     a.keys_each = int(((size_t(g->k_len) + n - 1) / n + 63) / 64 * 64);
     a.q_splits = unsigned((g->k_len + a.keys_each - 1) / a.keys_each);
