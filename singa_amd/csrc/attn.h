@@ -147,14 +147,14 @@ struct Stage {
   static constexpr bool kPart = N * NT != ROWS * L::RS;    // (the last wavefronts have one less)
   int voff[N];
   size_t stride;   // elements from row to row
-  int dim;
+  int dim, self;   // self: which of the NT threads that copy together
   bool direct;
   // (`direct`: rows of whole 16-byte chunks at multiples of 16 bytes; loads then write LDS without a register)
-  __device__ __forceinline__ void init(size_t stride_, int dim_, bool direct_) {
-    stride = stride_, dim = dim_, direct = direct_;
+  __device__ __forceinline__ void init(size_t stride_, int dim_, bool direct_, int self_ = int(threadIdx.x)) {
+    stride = stride_, dim = dim_, direct = direct_, self = self_;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int p = j * NT + int(threadIdx.x), r = p / L::RS, c = (p % L::RS) ^ L::turn(r);
+      const int p = j * NT + self, r = p / L::RS, c = (p % L::RS) ^ L::turn(r);
       voff[j] = c * T::VEC < dim ? int((r * stride + size_t(c) * T::VEC) * sizeof(elem)) : kOOB;
     }
   }
@@ -169,16 +169,18 @@ struct Stage {
     rows = min(rows, ROWS);
     if (direct) {
       const int bytes = rows > 0 ? ((rows - 1) * int(stride) + dim) * int(sizeof(elem)) : 0;   // (heads * dim is at most 2^20)
-      const rsrc4_t buffer = buffer_of(p, bytes);
+      rsrc4_t buffer = buffer_of(p, bytes);
+      if constexpr (NT == SGH_WAVE)   // (one wavefront's: the compiler cannot tell that its lanes agree)
+        for (int i = 0; i < 3; ++i) buffer[i] = unsigned(__builtin_amdgcn_readfirstlane(int(buffer[i])));
       const unsigned to = lds_offset(lds);
-      const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+      const int wave = __builtin_amdgcn_readfirstlane(self >> 6);
 #pragma unroll
       for (int j = 0; j < N; ++j)
         if (!kPart || j * NT + wave * SGH_WAVE < ROWS * L::RS) load_lds16(buffer, to + (wave + j * NT / SGH_WAVE) * L::GROUP, voff[j]);
     } else {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const int q = j * NT + int(threadIdx.x), r = q / L::RS, c = (q % L::RS) ^ L::turn(r);
+        const int q = j * NT + self, r = q / L::RS, c = (q % L::RS) ^ L::turn(r);
         if (!kPart || q < ROWS * L::RS) *reinterpret_cast<u32x4 *>(lds + q / SGH_WAVE * L::GROUP + q % SGH_WAVE * 16) = chunk(p + r * stride, c * T::VEC, r < rows ? dim : 0);
       }
     }
@@ -202,17 +204,14 @@ struct Stage {
 // and with that for every tile on its way.
 __device__ __forceinline__ void registers_arrive() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
-// The same where up to `behind` later loads of this wavefront may be under way (0 to 15)
-__device__ __forceinline__ void tiles_arrive(int behind) {
+// A wavefront's own tiles are there, but for up to `behind` later loads (0 to 63 of them)
+__device__ __forceinline__ void own_tiles_arrive(int behind) {
 #define SGH_WAIT(N) case N: asm volatile("s_waitcnt vmcnt(" #N ") lgkmcnt(0)" ::: "memory"); break;
-  switch (behind) {
-    SGH_WAIT(1) SGH_WAIT(2) SGH_WAIT(3) SGH_WAIT(4) SGH_WAIT(5) SGH_WAIT(6) SGH_WAIT(7) SGH_WAIT(8) SGH_WAIT(9) SGH_WAIT(10) SGH_WAIT(11) SGH_WAIT(12)
-    SGH_WAIT(13) SGH_WAIT(14) SGH_WAIT(15)
+  switch (behind) {   // (every multiple of 2 that a kernel here asks for; others wait for all)
+    SGH_WAIT(2) SGH_WAIT(4) SGH_WAIT(6) SGH_WAIT(8) SGH_WAIT(12) SGH_WAIT(16) SGH_WAIT(24) SGH_WAIT(32) SGH_WAIT(48)
     default: asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   }
 #undef SGH_WAIT
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
 }
 // tiles that the block's threads have requested are there, and everybody is done with what was read before
 __device__ __forceinline__ void tiles_arrive() {

@@ -204,6 +204,155 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
   }
 }
 
+// Few queries (32 with the heads of a group): the wavefronts of a block share the keys, 32 at a time, each with tiles of its own in LDS that
+// nobody else waits for, and join what they have in the end.  Bound by the keys' and values' way from memory, of which three quarters would wait for one
+// wavefront's products in the kernel above.  (16 sequences of up to 16384 places, 4 heads of keys of 64, binary16: 75 -> 56 us.)
+template <class T, int DP>
+struct Few {
+  static constexpr int KT = 32, TILE = Tile<T, DP>::bytes(KT), WAVE = 2 * TILE;   // a wavefront's keys and values
+  static constexpr int SLOTS = 4 * 4 * WAVE <= (144 << 10) ? 4 : 4 * 3 * WAVE <= (144 << 10) ? 3 : 2, AHEAD = SLOTS - 1;
+  static constexpr int ROW = DP + 4;                                             // floats of a row of results in LDS
+  static constexpr size_t kTiles = 4 * SLOTS * WAVE, kResults = (4 * 32 * ROW + 8 * 32) * sizeof(float);
+  static constexpr size_t kBytes = kTiles > kResults ? kTiles : kResults;
+  // (two tiles of keys and of values for each wavefront have to fit: rows of up to 256 bytes)
+  static constexpr bool kFits = kBytes + kMostBand <= (156 << 10);
+};
+template <class T, int DP, bool BIAS>
+__global__ __launch_bounds__(kBlock, 1) void k_attn_few(FwdArgs a, Bounds bounds) {
+  typedef typename T::elem elem;
+  typedef Few<T, DP> F;
+  static_assert(F::kFits && F::SLOTS >= 2 && F::kResults <= F::kTiles, "tiles");
+  constexpr int ND = DP / 32;
+  constexpr float kShift = std::is_same<T, F16>::value ? 6.f : 0.f;
+  extern __shared__ __align__(16) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
+  const Shape &s = a.s;
+  const Where at = block_at(1, a.units, a.splits, true);
+  const int unit = int(at.unit), per_batch = s.heads / a.pack, b = unit / per_batch, head0 = unit % per_batch * a.pack;
+  const int kv = head0 / (s.heads / s.kv_heads);
+  const Span span = span_of(s, b);
+  const int rows = s.q_len * a.pack, r = lane & 31, query = r / a.pack, head = head0 + r % a.pack;
+  const int limit = r < rows && query < span.q ? (s.causal ? min(span.k, max(span.start + query + 1, 0)) : span.k) : 0;
+  cols_t<T, DP> qf[1];
+  load_columns<T, DP>(qf[0], static_cast<const elem *>(a.q) + ((size_t(b) * s.q_len + query) * s.heads + head) * a.io_dim, limit ? a.io_dim : 0, hi,
+                      a.io_direct);
+  int most = limit, least = r < rows ? limit : 1 << 30;
+  for (int m = 1; m < 32; m *= 2) most = max(most, __shfl_xor(most, m)), least = min(least, __shfl_xor(least, m));
+  most = __builtin_amdgcn_readfirstlane(most), least = __builtin_amdgcn_readfirstlane(least);
+  // the split's part of the keys that are seen, in whole rounds of the block
+  const int each = ((most + int(a.splits) - 1) / int(a.splits) + 4 * F::KT - 1) / (4 * F::KT) * (4 * F::KT);
+  const int begin = min(most, int(at.split) * each), end = min(most, begin + each);
+
+  float *band = reinterpret_cast<float *>(lds + F::kBytes);
+  const int band_len = 2 * s.reach + 1;
+  if constexpr (BIAS)
+    for (int g = 0; g < a.pack; ++g) expand_bias(s, bounds, head0 + g, band + g * band_len);
+
+  const size_t stride = size_t(s.kv_heads) * s.dim;
+  Stage<T, DP, F::KT, SGH_WAVE> stage;
+  stage.init(stride, s.dim, a.direct, lane);
+  const elem *kp = static_cast<const elem *>(a.k) + (size_t(b) * s.k_len * s.kv_heads + kv) * s.dim;
+  const elem *vp = static_cast<const elem *>(a.v) + (size_t(b) * s.k_len * s.kv_heads + kv) * s.dim;
+  char *const mine = lds + wave * F::SLOTS * F::WAVE;
+  f32x16 acc[1][ND];
+  zero(acc[0]);
+  float m = -3e38f, l = 0.f;
+  const float c = s.scale * kLog2e;
+  const Reader<T, DP> reader(lane);
+  auto request = [&](int k0, int slot) {
+    stage(mine + slot * F::WAVE, kp + k0 * stride, span.k - k0);
+    stage(mine + slot * F::WAVE + F::TILE, vp + k0 * stride, span.k - k0);
+  };
+  registers_arrive();
+  __syncthreads();   // (the bias)
+  const int first_key = begin + wave * F::KT, turns = first_key < end ? (end - first_key + 4 * F::KT - 1) / (4 * F::KT) : 0;
+  const int loads = a.direct ? 2 * stage.loads(0) : 0;
+  for (int i = 0; i < F::AHEAD && i < turns; ++i) request(first_key + i * 4 * F::KT, i);
+  int slot = 0, ahead_slot = F::AHEAD;
+  for (int turn = 0; turn < turns; ++turn) {
+    own_tiles_arrive(loads * min(F::AHEAD - 1, turns - 1 - turn));
+    const int k0 = first_key + turn * 4 * F::KT;
+    if (turn + F::AHEAD < turns) {
+      request(k0 + F::AHEAD * 4 * F::KT, ahead_slot);
+      ahead_slot = ahead_slot == F::SLOTS - 1 ? 0 : ahead_slot + 1;
+    }
+    const char *kt = mine + slot * F::WAVE, *vt = kt + F::TILE;
+    slot = slot == F::SLOTS - 1 ? 0 : slot + 1;
+    f32x16 p[1];
+    zero(p);
+    reader.rows(kt, 0, qf, p);
+    float top = kNegInf;
+    if constexpr (BIAS) {
+      const float *centre = band + (r < rows ? head - head0 : 0) * band_len + s.reach;
+      const int first = k0 - (span.start + query) + 4 * hi;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) p[0][i] = __builtin_fmaf(p[0][i], c, centre[min(max(first + row_of(i), -s.reach), s.reach)]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) p[0][i] *= c;
+    }
+    if (k0 + F::KT > least) {
+      const int left = limit - k0 - 4 * hi;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (row_of(i) >= left) p[0][i] = kNegInf;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, p[0][i]);
+    top = max_of_pair(top);
+    if (__ballot(top > m + kGrowth)) {
+      const float now = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - now);
+      m = now, l *= f;
+#pragma unroll
+      for (int n = 0; n < ND; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[0][n][i] *= f;
+    }
+    const float from = m - kShift;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      p[0][i] = __builtin_amdgcn_exp2f(p[0][i] - from);
+      l += p[0][i];
+    }
+    Terms<T> terms[1];
+    terms[0].set(p[0]);
+    reader.transposed(vt, 0, terms, acc);
+  }
+
+  // what the four have: sums relative to their own maxima
+  float *const results = reinterpret_cast<float *>(lds), *const tops = results + 4 * 32 * F::ROW, *const totals = tops + 4 * 32;
+  l = sum_of_pair(l);
+  __syncthreads();
+  store_partial<DP>(results + (wave * 32 + r) * F::ROW, acc[0], 1.f, hi);
+  if (hi == 0) tops[wave * 32 + r] = m, totals[wave * 32 + r] = l;
+  __syncthreads();
+  for (int i = tid; i < rows * (DP / 4); i += kBlock) {
+    const int row = i / (DP / 4), d = i % (DP / 4) * 4, q = row / a.pack, h = head0 + row % a.pack;
+    float top = tops[row], sum = 0.f;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, tops[w * 32 + row]);
+    sgh_v4f o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float total = totals[w * 32 + row], f = total == 0.f ? 0.f : __builtin_amdgcn_exp2f(tops[w * 32 + row] - top);
+      sum += total * f;
+      if (total != 0.f) o += *reinterpret_cast<const sgh_v4f *>(results + (w * 32 + row) * F::ROW + d) * f;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum, lse = sum == 0.f ? kNegInf : (top - kShift + __builtin_amdgcn_logf(sum)) * kLn2;
+    if (a.splits == 1) {
+      elem *out = static_cast<elem *>(a.o) + ((size_t(b) * s.q_len + q) * s.heads + h) * a.io_dim;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (d + e < a.io_dim) T::St::st(out + d + e, o[e] * inv);
+      if (d == 0) a.lse[(size_t(b) * s.heads + h) * s.q_len + q] = lse;
+    } else {
+      const size_t n = size_t(a.units) * rows, to = at.split * n + size_t(unit) * rows + row;
+      *reinterpret_cast<sgh_v4f *>(a.part + to * DP + d) = o * inv;
+      if (d == 0) a.part[a.splits * n * DP + to] = lse;
+    }
+  }
+}
+
 // Joins the parts of the keys, a block to a row: o = sum e^(lse_s - lse) o_s.  DP / 4 lanes have four values each, the groups of so many lanes
 // share the parts (16 rows of 128 values in 235 parts: one group to a row 100 us).
 template <class T, int DP>
@@ -252,17 +401,30 @@ __global__ __launch_bounds__(kBlock) void k_attn_join(FwdArgs a) {
   if (d == 0) a.lse[(size_t(b) * s.heads + head) * s.q_len + query] = sum == 0.f ? kNegInf : top + __builtin_amdgcn_logf(sum) * kLn2;
 }
 
-template <class T, int DP, int QT, bool BIAS>
-int launch(const FwdArgs &a, const Bounds &bounds, size_t lds, hipStream_t s) {
-  static std::atomic<unsigned long long> asked{0};
-  SGH_HIP_TRY(sgh_allow_lds(reinterpret_cast<const void *>(k_attn_fwd<T, DP, QT, BIAS>), asked));
-  SGH_LAUNCH_TIMED((k_attn_fwd<T, DP, QT, BIAS>), dim3(a.tiles * a.units * a.splits), dim3(kBlock), lds, s, a, bounds);
-  SGH_LAUNCH_CHECK();
+template <class T, int DP>
+int join(const FwdArgs &a, hipStream_t s) {
   if (a.splits > 1) {
     hipLaunchKernelGGL((k_attn_join<T, DP>), dim3(unsigned(size_t(a.units) * a.s.q_len * a.pack)), dim3(kBlock), 0, s, a);
     SGH_LAUNCH_CHECK();
   }
   return SGH_OK;
+}
+template <class T, int DP, int QT, bool BIAS>
+int launch(const FwdArgs &a, const Bounds &bounds, size_t band, hipStream_t s) {
+  static std::atomic<unsigned long long> asked{0};
+  constexpr int KT = T::half ? 64 : 32;
+  SGH_HIP_TRY(sgh_allow_lds(reinterpret_cast<const void *>(k_attn_fwd<T, DP, QT, BIAS>), asked));
+  SGH_LAUNCH_TIMED((k_attn_fwd<T, DP, QT, BIAS>), dim3(a.tiles * a.units * a.splits), dim3(kBlock), (4 * Tile<T, DP>::bytes(KT)) + band, s, a, bounds);
+  SGH_LAUNCH_CHECK();
+  return join<T, DP>(a, s);
+}
+template <class T, int DP, bool BIAS>
+int launch_few(const FwdArgs &a, const Bounds &bounds, size_t band, hipStream_t s) {
+  static std::atomic<unsigned long long> asked{0};
+  SGH_HIP_TRY(sgh_allow_lds(reinterpret_cast<const void *>(k_attn_few<T, DP, BIAS>), asked));
+  SGH_LAUNCH_TIMED((k_attn_few<T, DP, BIAS>), dim3(a.units * a.splits), dim3(kBlock), (Few<T, DP>::kBytes) + band, s, a, bounds);
+  SGH_LAUNCH_CHECK();
+  return join<T, DP>(a, s);
 }
 
 // How a forward pass is cut
@@ -270,11 +432,12 @@ struct Plan {
   int dp, pack;
   unsigned tiles, units, splits;
   int keys_each;
+  bool few;     // queries: k_attn_few
   bool pad;     // keys and values of rows that are not whole chunks are copied first
   size_t part, ws;
 };
-constexpr int kRows = 128;   // of a block
-Plan plan_of(const sgh_attn_geom *g) {
+constexpr int kRows = 128, kFewRows = 32;   // of a block
+Plan plan_of(const sgh_attn_geom *g, size_t e) {
   Plan p;
   p.dp = (g->dim + 31) / 32 * 32;
   const int group = g->heads / g->kv_heads;
@@ -282,9 +445,16 @@ Plan plan_of(const sgh_attn_geom *g) {
   p.pack = size_t(g->q_len) * group <= kRows && band_bytes(g) * group <= kMostBand ? group : 1;
   p.tiles = unsigned((size_t(g->q_len) * p.pack + kRows - 1) / kRows);
   p.units = unsigned(size_t(g->batch) * (g->heads / p.pack));
-  // Few rows: several blocks to the keys of each, of 257 to 512 keys or more (the launch that joins them takes 4 us and more, 64 keys of a block 1.2)
+  // Few queries: wavefronts that share the keys, whose tiles take most of a CU's LDS (binary16, 45 units of 27 rows, heads of 128: 260 keys
+  // 11.8 -> 9.9 us, 100 keys 7.9 -> 7.8, 64 keys 6.6 -> 7.6; more units than CUs, 400 with a bias: 250 keys 17 -> 22, 512 without one, 2000
+  // keys: 100 -> 96).
+  const size_t cus = size_t(sgh_num_cus());
+  p.few = size_t(g->q_len) * p.pack <= size_t(kFewRows) && size_t(p.dp) * e <= 256 && g->k_len > (p.units <= cus ? 64 : 512);
+  // Few rows: several blocks to the keys of each, of 257 to 512 keys or more (the launch that joins them takes 4 us and more, 64 keys of a block
+  // 1.2).  Wavefronts that share keys keep the way to memory full with one block to a CU (16 x 4 heads over 16384 keys: 56 us, two 68, four 92),
+  // others with four (fp32, 16 x 8 heads of 128, 2000 keys: 82 us, one 152).
   p.splits = 1, p.keys_each = 1 << 30;
-  const size_t blocks = size_t(p.tiles) * p.units, want = 4 * size_t(sgh_num_cus());
+  const size_t blocks = size_t(p.tiles) * p.units, want = (p.few ? 1 : 4) * cus;
   if (blocks * 2 <= want && g->k_len > 512) {
     size_t n = want / blocks, most = (size_t(g->k_len) + 511) / 512;
     if (n > most) n = most;
@@ -299,11 +469,15 @@ Plan plan_of(const sgh_attn_geom *g) {
 }
 
 template <class T, int DP>
-int run_dim(const FwdArgs &a, const Bounds &bounds, hipStream_t s) {
-  constexpr int KT = T::half ? 64 : 32;
-  const size_t tiles = 4 * Tile<T, DP>::bytes(KT);
-  if (a.s.buckets) return launch<T, DP, 1, true>(a, bounds, tiles + a.pack * (2 * a.s.reach + 1) * sizeof(float), s);
-  return launch<T, DP, 1, false>(a, bounds, tiles, s);
+int run_dim(const FwdArgs &a, const Bounds &bounds, bool few, hipStream_t s) {
+  const size_t band = a.s.buckets ? a.pack * (2 * a.s.reach + 1) * sizeof(float) : 0;
+  if constexpr (Few<T, DP>::kFits)
+    if (few) {
+      if (a.s.buckets) return launch_few<T, DP, true>(a, bounds, band, s);
+      return launch_few<T, DP, false>(a, bounds, band, s);
+    }
+  if (a.s.buckets) return launch<T, DP, 1, true>(a, bounds, band, s);
+  return launch<T, DP, 1, false>(a, bounds, band, s);
 }
 
 template <class T>
@@ -315,7 +489,7 @@ int forward(const sgh_attn_geom *g, const void *q, const void *k, const void *v,
   const size_t e = sizeof(typename T::elem), bq = size_t(g->batch) * g->q_len * g->heads, qn = bq * g->dim * e;
   const size_t kn = size_t(g->batch) * g->k_len * g->kv_heads * g->dim * e;
   if (!q || !o || !lse || (g->k_len != 0 && (!k || !v)) || (g->buckets != 0 && !table)) return SGH_EINVAL;
-  const Plan p = plan_of(g);
+  const Plan p = plan_of(g, e);
   if (p.ws && (!workspace || ws_bytes < p.ws)) return SGH_EWORKSPACE;
   if (p.ws && !sgh_aligned16(workspace)) return SGH_EINVAL;
   const Extent results[] = {{o, qn}, {lse, bq * 4}, {workspace, p.ws}};
@@ -346,10 +520,10 @@ int forward(const sgh_attn_geom *g, const void *q, const void *k, const void *v,
     a.k = pad.to[0], a.v = pad.to[1], a.s.dim = wide, a.direct = true;
   }
   switch (p.dp) {
-    case 32: return run_dim<T, 32>(a, bounds, s);
-    case 64: return run_dim<T, 64>(a, bounds, s);
-    case 96: return run_dim<T, 96>(a, bounds, s);
-    default: return run_dim<T, 128>(a, bounds, s);
+    case 32: return run_dim<T, 32>(a, bounds, p.few, s);
+    case 64: return run_dim<T, 64>(a, bounds, p.few, s);
+    case 96: return run_dim<T, 96>(a, bounds, p.few, s);
+    default: return run_dim<T, 128>(a, bounds, p.few, s);
   }
 }
 
@@ -358,7 +532,8 @@ int forward(const sgh_attn_geom *g, const void *q, const void *k, const void *v,
 extern "C" {
 
 size_t sgh_attn_fwd_workspace_bytes(const sgh_attn_geom *g) {
-  return check_geom(g) == SGH_OK && g->batch != 0 && g->q_len != 0 ? plan_of(g).ws : 0;
+  if (check_geom(g) != SGH_OK || g->batch == 0 || g->q_len == 0) return 0;
+  return std::max(plan_of(g, 2).ws, plan_of(g, 4).ws);   // (of either size of values)
 }
 
 #define SGH_ATTN_FWD(SFX, S, E)                                                                                                        \

@@ -157,6 +157,18 @@ def test_one_new_token_over_caches_of_different_lengths(dev, t):
         check(singa, dev, t, O.Attn(True, buckets=buckets, bidirectional=False), 5, 1, 3000, h, g, 48, lengths=(None, keys, starts))
 
 
+# one row to 32 and one more, the rounds of four wavefronts (128 keys) full, not full and one more, parts of the keys that do not come out even
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("d", [20, 64, 70, 128])
+@pytest.mark.parametrize("sq,sk,h,g", [(1, 65, 1, 1), (1, 128, 32, 1), (3, 129, 10, 2), (8, 511, 4, 1), (16, 513, 4, 2), (7, 1070, 2, 2), (11, 1300, 3, 1), (1, 9001, 6, 2)])
+def test_few_queries(dev, t, d, sq, sk, h, g):
+    from singa_amd import singa_wrap as singa
+    for causal, buckets, scale in ((True, 0, None), (False, 32, -0.3), (True, 16, 0.0)):
+        a = O.Attn(causal, scale, buckets=buckets, max_distance=200)
+        check(singa, dev, t, a, 3, sq, sk, h, g, d, lengths=((sq, max(0, sq - 2), 0), (sk, sk - 33, sk // 2), (sk - sq, sk - 50, -1)), grads=False)
+        check(singa, dev, t, a, 1, sq, sk, h, g, d, shift=1, grads=False)
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("d", [1, 7, 8, 64, 70])
 def test_tensors_at_any_element(dev, t, d):
