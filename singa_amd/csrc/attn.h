@@ -50,6 +50,7 @@ __device__ __forceinline__ Span span_of(const Shape &s, int b) {
   if (s.q_lengths) r.q = min(max(s.q_lengths[b], 0), s.q_len);
   if (s.k_lengths) r.k = min(max(s.k_lengths[b], 0), s.k_len);
   if (s.q_starts) r.start = min(max(s.q_starts[b], -(1 << 30)), 1 << 30);
+  if (s.causal) r.k = min(r.k, max(r.start + r.q, 0));   // (keys behind the last query are seen by none: not looked at)
   return r;
 }
 

@@ -149,6 +149,37 @@ def test_padded_batches(dev, t, causal, buckets, lengths):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("sq,buckets", [(1, 0), (1, 16), (9, 0), (50, 0), (200, 16)])
+def test_the_unused_part_of_a_cache(dev, t, sq, buckets):
+    """Keys behind the last query of a causal sequence hold NaN and infinities, and no lengths of the keys are given."""
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(8)
+    b, sk, h, g, d, starts = 3, 700, 4, 2, 40, (0, 290, 61)
+    q, do, k, v = (stored(t, r.standard_normal(s)) for s in ((b, sq, h, d), (b, sq, h, d), (b, sk, g, d), (b, sk, g, d)))
+    table = stored("f32", r.standard_normal((buckets, h))) if buckets else None
+    for x in (k, v):
+        for i in range(b):
+            rest = x[i, starts[i] + sq:]
+            rest[...] = np.resize([np.nan, np.inf, -np.inf], rest.shape)
+    seen = tuple(s + sq for s in starts)
+    a = O.Attn(True, buckets=buckets, max_distance=40)
+    H = handle(singa, upload(singa, dev, t, q), upload(singa, dev, t, k), a)
+    results = []
+    for k_lengths in (None, seen):
+        args = [upload(singa, dev, t, x) for x in (q, k, v)]
+        dt = upload(singa, dev, "f32", table) if buckets else None
+        how = dict(k_lengths=None if k_lengths is None else ints(singa, dev, k_lengths), q_starts=ints(singa, dev, starts))
+        o, lse = singa.AttentionForward(H, *args, dt, **how)
+        grads = singa.AttentionBackward(H, upload(singa, dev, t, do), *args, o, lse, dt, **how)
+        results.append([x.to_numpy() for x in (o, lse) + tuple(grads) if x is not None])
+    for x, y in zip(*results):
+        assert np.isfinite(x).all() and np.array_equal(x, y)
+    for i in range(b):
+        assert not results[0][3][i, seen[i]:].any() and not results[0][4][i, seen[i]:].any()
+    check(singa, dev, t, a, b, sq, sk, h, g, d, lengths=(None, seen, starts), case=[q, k, v, do, table])
+
+
+@pytest.mark.parametrize("t", TYPES)
 def test_one_new_token_over_caches_of_different_lengths(dev, t):
     from singa_amd import singa_wrap as singa
     keys = (1, 3000, 64, 1999, 0)
