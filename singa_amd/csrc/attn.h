@@ -214,6 +214,8 @@ __device__ __forceinline__ void own_tiles_arrive(int behind) {
   }
 #undef SGH_WAIT
 }
+// The wavefront's reads of LDS are done (what they read may be written over)
+__device__ __forceinline__ void own_reads_end() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 // tiles that the block's threads have requested are there, and everybody is done with what was read before
 __device__ __forceinline__ void tiles_arrive() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");

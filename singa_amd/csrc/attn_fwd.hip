@@ -206,22 +206,23 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
 
 // Few queries (32 with the heads of a group): the wavefronts of a block share the keys, 32 at a time, each with tiles of its own in LDS that
 // nobody else waits for, and join what they have in the end.  Bound by the keys' and values' way from memory, of which three quarters would wait for one
-// wavefront's products in the kernel above.  (16 sequences of up to 16384 places, 4 heads of keys of 64, binary16: 75 -> 56 us.)
+// wavefront's products in the kernel above.  (16 sequences of up to 16384 places, 4 heads of keys of 64, binary16: 75 -> 56 us; fp32, 5 x 8 heads of keys of 128,
+// 16180 places: 216 -> 126, 5.2 TB/s.)
 template <class T, int DP>
 struct Few {
   static constexpr int KT = 32, TILE = Tile<T, DP>::bytes(KT), WAVE = 2 * TILE;   // a wavefront's keys and values
-  static constexpr int SLOTS = 4 * 4 * WAVE <= (144 << 10) ? 4 : 4 * 3 * WAVE <= (144 << 10) ? 3 : 2, AHEAD = SLOTS - 1;
+  static constexpr int SLOTS = 4 * 4 * WAVE <= (132 << 10) ? 4 : 4 * 2 * WAVE <= (132 << 10) ? 2 : 1;
+  static constexpr bool ONE = SLOTS == 1;   // rows of over 256 bytes: the next keys are requested over those just used, then the values alike
+  static constexpr int AHEAD = ONE ? 1 : SLOTS - 1;
   static constexpr int ROW = DP + 4;                                             // floats of a row of results in LDS
   static constexpr size_t kTiles = 4 * SLOTS * WAVE, kResults = (4 * 32 * ROW + 8 * 32) * sizeof(float);
   static constexpr size_t kBytes = kTiles > kResults ? kTiles : kResults;
-  // (two tiles of keys and of values for each wavefront have to fit: rows of up to 256 bytes)
-  static constexpr bool kFits = kBytes + kMostBand <= (156 << 10);
 };
 template <class T, int DP, bool BIAS>
 __global__ __launch_bounds__(kBlock, 1) void k_attn_few(FwdArgs a, Bounds bounds) {
   typedef typename T::elem elem;
   typedef Few<T, DP> F;
-  static_assert(F::kFits && F::SLOTS >= 2 && F::kResults <= F::kTiles, "tiles");
+  static_assert(F::kBytes + kMostBand <= (156 << 10), "LDS");
   constexpr int ND = DP / 32;
   constexpr float kShift = std::is_same<T, F16>::value ? 6.f : 0.f;
   extern __shared__ __align__(16) char lds[];
@@ -259,21 +260,20 @@ __global__ __launch_bounds__(kBlock, 1) void k_attn_few(FwdArgs a, Bounds bounds
   float m = -3e38f, l = 0.f;
   const float c = s.scale * kLog2e;
   const Reader<T, DP> reader(lane);
-  auto request = [&](int k0, int slot) {
-    stage(mine + slot * F::WAVE, kp + k0 * stride, span.k - k0);
-    stage(mine + slot * F::WAVE + F::TILE, vp + k0 * stride, span.k - k0);
-  };
+  auto request_keys = [&](int k0, int slot) { stage(mine + slot * F::WAVE, kp + k0 * stride, span.k - k0); };
+  auto request_values = [&](int k0, int slot) { stage(mine + slot * F::WAVE + F::TILE, vp + k0 * stride, span.k - k0); };
   registers_arrive();
   __syncthreads();   // (the bias)
   const int first_key = begin + wave * F::KT, turns = first_key < end ? (end - first_key + 4 * F::KT - 1) / (4 * F::KT) : 0;
-  const int loads = a.direct ? 2 * stage.loads(0) : 0;
-  for (int i = 0; i < F::AHEAD && i < turns; ++i) request(first_key + i * 4 * F::KT, i);
+  const int loads = a.direct ? stage.loads(0) : 0;   // of a tile
+  for (int i = 0; i < F::AHEAD && i < turns; ++i) request_keys(first_key + i * 4 * F::KT, i), request_values(first_key + i * 4 * F::KT, i);
   int slot = 0, ahead_slot = F::AHEAD;
   for (int turn = 0; turn < turns; ++turn) {
-    own_tiles_arrive(loads * min(F::AHEAD - 1, turns - 1 - turn));
-    const int k0 = first_key + turn * 4 * F::KT;
-    if (turn + F::AHEAD < turns) {
-      request(k0 + F::AHEAD * 4 * F::KT, ahead_slot);
+    own_tiles_arrive(F::ONE ? loads : 2 * loads * min(F::AHEAD - 1, turns - 1 - turn));
+    const int k0 = first_key + turn * 4 * F::KT, ahead = k0 + F::AHEAD * 4 * F::KT;
+    const bool more = turn + F::AHEAD < turns;
+    if (!F::ONE && more) {
+      request_keys(ahead, ahead_slot), request_values(ahead, ahead_slot);
       ahead_slot = ahead_slot == F::SLOTS - 1 ? 0 : ahead_slot + 1;
     }
     const char *kt = mine + slot * F::WAVE, *vt = kt + F::TILE;
@@ -281,6 +281,10 @@ __global__ __launch_bounds__(kBlock, 1) void k_attn_few(FwdArgs a, Bounds bounds
     f32x16 p[1];
     zero(p);
     reader.rows(kt, 0, qf, p);
+    if constexpr (F::ONE) {
+      own_reads_end();
+      if (more) request_keys(ahead, 0);
+    }
     float top = kNegInf;
     if constexpr (BIAS) {
       const float *centre = band + (r < rows ? head - head0 : 0) * band_len + s.reach;
@@ -316,7 +320,12 @@ __global__ __launch_bounds__(kBlock, 1) void k_attn_few(FwdArgs a, Bounds bounds
     }
     Terms<T> terms[1];
     terms[0].set(p[0]);
+    if constexpr (F::ONE) own_tiles_arrive(more ? loads : 0);
     reader.transposed(vt, 0, terms, acc);
+    if constexpr (F::ONE) {
+      own_reads_end();
+      if (more) request_values(ahead, 0);
+    }
   }
 
   // what the four have: sums relative to their own maxima
@@ -437,7 +446,7 @@ struct Plan {
   size_t part, ws;
 };
 constexpr int kRows = 128, kFewRows = 32;   // of a block
-Plan plan_of(const sgh_attn_geom *g, size_t e) {
+Plan plan_of(const sgh_attn_geom *g) {
   Plan p;
   p.dp = (g->dim + 31) / 32 * 32;
   const int group = g->heads / g->kv_heads;
@@ -449,10 +458,10 @@ Plan plan_of(const sgh_attn_geom *g, size_t e) {
   // 11.8 -> 9.9 us, 100 keys 7.9 -> 7.8, 64 keys 6.6 -> 7.6; more units than CUs, 400 with a bias: 250 keys 17 -> 22, 512 without one, 2000
   // keys: 100 -> 96).
   const size_t cus = size_t(sgh_num_cus());
-  p.few = size_t(g->q_len) * p.pack <= size_t(kFewRows) && size_t(p.dp) * e <= 256 && g->k_len > (p.units <= cus ? 64 : 512);
+  p.few = size_t(g->q_len) * p.pack <= size_t(kFewRows) && g->k_len > (p.units <= cus ? 64 : 512);
   // Few rows: several blocks to the keys of each, of 257 to 512 keys or more (the launch that joins them takes 4 us and more, 64 keys of a block
   // 1.2).  Wavefronts that share keys keep the way to memory full with one block to a CU (16 x 4 heads over 16384 keys: 56 us, two 68, four 92),
-  // others with four (fp32, 16 x 8 heads of 128, 2000 keys: 82 us, one 152).
+  // others with four (the kernel above on fp32, 16 x 8 heads of 128, 2000 keys: 82 us, one 152).
   p.splits = 1, p.keys_each = 1 << 30;
   const size_t blocks = size_t(p.tiles) * p.units, want = (p.few ? 1 : 4) * cus;
   if (blocks * 2 <= want && g->k_len > 512) {
@@ -471,11 +480,10 @@ Plan plan_of(const sgh_attn_geom *g, size_t e) {
 template <class T, int DP>
 int run_dim(const FwdArgs &a, const Bounds &bounds, bool few, hipStream_t s) {
   const size_t band = a.s.buckets ? a.pack * (2 * a.s.reach + 1) * sizeof(float) : 0;
-  if constexpr (Few<T, DP>::kFits)
-    if (few) {
-      if (a.s.buckets) return launch_few<T, DP, true>(a, bounds, band, s);
-      return launch_few<T, DP, false>(a, bounds, band, s);
-    }
+  if (few) {
+    if (a.s.buckets) return launch_few<T, DP, true>(a, bounds, band, s);
+    return launch_few<T, DP, false>(a, bounds, band, s);
+  }
   if (a.s.buckets) return launch<T, DP, 1, true>(a, bounds, band, s);
   return launch<T, DP, 1, false>(a, bounds, band, s);
 }
@@ -489,7 +497,7 @@ int forward(const sgh_attn_geom *g, const void *q, const void *k, const void *v,
   const size_t e = sizeof(typename T::elem), bq = size_t(g->batch) * g->q_len * g->heads, qn = bq * g->dim * e;
   const size_t kn = size_t(g->batch) * g->k_len * g->kv_heads * g->dim * e;
   if (!q || !o || !lse || (g->k_len != 0 && (!k || !v)) || (g->buckets != 0 && !table)) return SGH_EINVAL;
-  const Plan p = plan_of(g, e);
+  const Plan p = plan_of(g);
   if (p.ws && (!workspace || ws_bytes < p.ws)) return SGH_EWORKSPACE;
   if (p.ws && !sgh_aligned16(workspace)) return SGH_EINVAL;
   const Extent results[] = {{o, qn}, {lse, bq * 4}, {workspace, p.ws}};
@@ -532,8 +540,7 @@ int forward(const sgh_attn_geom *g, const void *q, const void *k, const void *v,
 extern "C" {
 
 size_t sgh_attn_fwd_workspace_bytes(const sgh_attn_geom *g) {
-  if (check_geom(g) != SGH_OK || g->batch == 0 || g->q_len == 0) return 0;
-  return std::max(plan_of(g, 2).ws, plan_of(g, 4).ws);   // (of either size of values)
+  return check_geom(g) == SGH_OK && g->batch != 0 && g->q_len != 0 ? plan_of(g).ws : 0;
 }
 
 #define SGH_ATTN_FWD(SFX, S, E)                                                                                                        \
