@@ -269,7 +269,8 @@ struct Plan {
   size_t bytes() const { return stats + q_part + bias_part + k_part + wide; }
 };
 size_t up16(size_t n) { return (n + 15) / 16 * 16; }
-Plan plan_of(const sgh_attn_geom *g) {
+// (elem_bytes: fp32 never needs less of the workspace than the others)
+Plan plan_of(const sgh_attn_geom *g, size_t elem_bytes) {
   Plan p;
   BwdArgs &a = p.a;
   const size_t dp = size_t(g->dim + 31) / 32 * 32, cus = size_t(sgh_num_cus());
@@ -279,18 +280,23 @@ Plan plan_of(const sgh_attn_geom *g) {
   a.q_units = unsigned(size_t(g->batch) * (g->heads / a.pack));
   a.k_tiles = unsigned((size_t(g->k_len) + kRows - 1) / kRows);
   a.k_units = unsigned(size_t(g->batch) * g->kv_heads);
-  // few blocks: several to the keys of a block of queries, and to the queries of a block of keys
+  // Few blocks: several to the keys of a block of queries, and to the queries of a block of keys.  The parts are the smaller the fewer blocks
+  // there are (fp32, 2 x 8 heads of 64, 400 places: parts of up to 512 keys 111 us, of 256 99; 8 x 8 heads, 512 places, a block to a CU: one part
+  // 148, two 156; bfloat16 heads of 128 there: 65 and 75).
   a.q_splits = a.k_splits = 1, a.keys_each = 1 << 30;
   const size_t q_blocks = size_t(a.q_tiles) * a.q_units, k_blocks = size_t(a.k_tiles) * a.k_units;
-  if (q_blocks * 2 <= 2 * cus && g->k_len > 512) {
-    size_t n = 2 * cus / q_blocks, most = (size_t(g->k_len) + 511) / 512;
+  const size_t part = q_blocks * 2 <= cus ? 256 : 512;
+  if (q_blocks <= cus && size_t(g->k_len) > part) {
+    size_t n = 2 * cus / q_blocks, most = (size_t(g->k_len) + part - 1) / part;
     if (n > most) n = most;
     a.keys_each = int(((size_t(g->k_len) + n - 1) / n + 63) / 64 * 64);
     a.q_splits = unsigned((g->k_len + a.keys_each - 1) / a.keys_each);
   }
-  const size_t turns = size_t(group) * ((size_t(g->q_len) + 63) / 64);
-  if (k_blocks && k_blocks * 2 <= 2 * cus && turns >= 8) {
-    size_t n = 2 * cus / k_blocks, most = turns / 4;
+  // (64 queries of fp32 cost four times those of 16 bits, the join the same: parts of two turns and more, fp32, 2 x 8 heads of 64, 400 places 99 ->
+  // 72 us, of 128, 300 places 148 -> 115; bfloat16, 2 x 8 heads, 400 places 28 -> 31)
+  const size_t turns = size_t(group) * ((size_t(g->q_len) + 63) / 64), least = elem_bytes == 4 && k_blocks * 2 <= cus ? 2 : 4;
+  if (k_blocks && k_blocks <= cus && turns >= 2 * least) {
+    size_t n = 2 * cus / k_blocks, most = turns / least;
     a.k_splits = unsigned(n < most ? n : most);
   }
   a.bias_blocks = size_t(g->batch) * a.q_tiles * a.q_splits;
@@ -319,7 +325,7 @@ int backward(const sgh_attn_geom *g, const void *dout, const void *q, const void
   if (qn != 0 && (!dout || !q || !o || !lse || !dq)) return SGH_EINVAL;
   if (kn != 0 && (!k || !v || !dk || !dv)) return SGH_EINVAL;
   if (g->buckets != 0 && (!table || !dtable)) return SGH_EINVAL;
-  Plan p = plan_of(g);
+  Plan p = plan_of(g, e);
   if (p.bytes() && (!workspace || ws_bytes < p.bytes())) return SGH_EWORKSPACE;
   if (p.bytes() && !sgh_aligned16(workspace)) return SGH_EINVAL;
   const Extent results[] = {{dq, qn}, {dk, kn}, {dv, kn}, {dtable, tn}, {workspace, p.bytes()}};
@@ -368,7 +374,9 @@ int backward(const sgh_attn_geom *g, const void *dout, const void *q, const void
 
 extern "C" {
 
-size_t sgh_attn_bwd_workspace_bytes(const sgh_attn_geom *g) { return attn::check_geom(g) == SGH_OK && g->batch != 0 ? plan_of(g).bytes() : 0; }
+size_t sgh_attn_bwd_workspace_bytes(const sgh_attn_geom *g) {
+  return attn::check_geom(g) == SGH_OK && g->batch != 0 ? plan_of(g, sizeof(float)).bytes() : 0;
+}
 
 #define SGH_ATTN_BWD(SFX, S, E)                                                                                                        \
   int sgh_attn_bwd_##SFX(const sgh_attn_geom *g, const E *dout, const E *q, const E *k, const E *v, const E *o, const float *lse,      \
