@@ -452,7 +452,8 @@ struct Plan {
   size_t part, ws;
 };
 constexpr int kRows = 128, kFewRows = 32;   // of a block
-Plan plan_of(const sgh_attn_geom *g) {
+// (elem_bytes: fp32 never needs less of the workspace than the others)
+Plan plan_of(const sgh_attn_geom *g, size_t elem_bytes) {
   Plan p;
   p.dp = (g->dim + 31) / 32 * 32;
   const int group = g->heads / g->kv_heads;
@@ -465,13 +466,17 @@ Plan plan_of(const sgh_attn_geom *g) {
   // keys: 100 -> 96).
   const size_t cus = size_t(sgh_num_cus());
   p.few = size_t(g->q_len) * p.pack <= size_t(kFewRows) && g->k_len > (p.units <= cus ? 64 : 512);
-  // Few rows: several blocks to the keys of each, of 257 to 512 keys or more (the launch that joins them takes 4 us and more, 64 keys of a block
-  // 1.2).  Wavefronts that share keys keep the way to memory full with one block to a CU (16 x 4 heads over 16384 keys: 56 us, two 68, four 92),
-  // others with four (the kernel above on fp32, 16 x 8 heads of 128, 2000 keys: 82 us, one 152).
+  // Few rows: several blocks to the keys of each (the launch that joins them takes 4 us and more, 64 keys of a block 1.2, of fp32 four times that).
+  // Wavefronts that share keys keep the way to memory full with one block to a CU (16 x 4 heads over 16384 keys: 56 us, two 68, four 92),
+  // others with four (the kernel above on fp32, 16 x 8 heads of 128, 2000 keys: 82 us, one 152).  More than 512 keys (fp32: 256) are shared, in
+  // parts of up to 512, or 256 where blocks are few (bfloat16, 100 queries of 8 heads over 900 keys: 20 -> 14 us, 2 x 8 heads, 400 places 12 -> 20;
+  // fp32, 2 x 4 heads of 128, 512 places 74 -> 48).
   p.splits = 1, p.keys_each = 1 << 30;
   const size_t blocks = size_t(p.tiles) * p.units, want = (p.few ? 1 : 4) * cus;
-  if (blocks * 2 <= want && g->k_len > 512) {
-    size_t n = want / blocks, most = (size_t(g->k_len) + 511) / 512;
+  const bool rare = !p.few && blocks * 2 <= cus;
+  if (blocks * 2 <= want && g->k_len > (rare && elem_bytes == 4 ? 256 : 512)) {
+    const size_t part = rare ? 256 : 512;
+    size_t n = want / blocks, most = (size_t(g->k_len) + part - 1) / part;
     if (n > most) n = most;
     p.keys_each = int(((size_t(g->k_len) + n - 1) / n + 63) / 64 * 64);
     p.splits = unsigned((g->k_len + p.keys_each - 1) / p.keys_each);
@@ -503,7 +508,7 @@ int forward(const sgh_attn_geom *g, const void *q, const void *k, const void *v,
   const size_t e = sizeof(typename T::elem), bq = size_t(g->batch) * g->q_len * g->heads, qn = bq * g->dim * e;
   const size_t kn = size_t(g->batch) * g->k_len * g->kv_heads * g->dim * e;
   if (!q || !o || !lse || (g->k_len != 0 && (!k || !v)) || (g->buckets != 0 && !table)) return SGH_EINVAL;
-  const Plan p = plan_of(g);
+  const Plan p = plan_of(g, e);
   if (p.ws && (!workspace || ws_bytes < p.ws)) return SGH_EWORKSPACE;
   if (p.ws && !sgh_aligned16(workspace)) return SGH_EINVAL;
   const Extent results[] = {{o, qn}, {lse, bq * 4}, {workspace, p.ws}};
@@ -546,7 +551,7 @@ int forward(const sgh_attn_geom *g, const void *q, const void *k, const void *v,
 extern "C" {
 
 size_t sgh_attn_fwd_workspace_bytes(const sgh_attn_geom *g) {
-  return check_geom(g) == SGH_OK && g->batch != 0 && g->q_len != 0 ? plan_of(g).ws : 0;
+  return check_geom(g) == SGH_OK && g->batch != 0 && g->q_len != 0 ? plan_of(g, sizeof(float)).ws : 0;
 }
 
 #define SGH_ATTN_FWD(SFX, S, E)                                                                                                        \
