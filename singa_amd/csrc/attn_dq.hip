@@ -28,6 +28,11 @@ __global__ __launch_bounds__(kBlock, (T::half || DP <= 64 ? 2 : 1)) void k_attn_
   const Span span = span_of(s, b);
   const int rows = s.q_len * a.pack, row0 = int(tile) * ROWS + wave * WAVE_ROWS;
 
+  // The 16-bit matrix products' sums are rounded a little downwards (by a thirtieth of a place on the average), which 10^8 terms of a bucket add
+  // up to: odd queries have the gradient of their result negated, so that it goes both ways (13 x 8 heads, 2833 places, table's gradient: 4.4e-6 off,
+  // so 5.0e-7; fp32 products show none of it).
+  constexpr bool kFlip = BIAS && T::half;
+  const float flip = kFlip && (lane & 1) ? -1.f : 1.f;
   int query[QT], head[QT], limit[QT], most = 0, least = 1 << 30;
   float lse[QT], delta[QT];   // (with a bias, natural logarithms: the product with log2 e is rounded with the sum, which the bias's gradient is told by)
   cols_t<T, DP> qf[QT], df[QT];
@@ -63,6 +68,14 @@ __global__ __launch_bounds__(kBlock, (T::half || DP <= 64 ? 2 : 1)) void k_attn_
     if (r < rows && hi == 0 && split == 0) {
       a.stats[stat] = lse2 - term_bits<T>();
       a.stats[size_t(a.q_units) * rows + stat] = -delta[t];
+    }
+    if constexpr (kFlip) {   // (rows are queries here: with a bias no heads share a tile)
+      delta[t] *= flip;
+      if (lane & 1)
+#pragma unroll
+        for (int k = 0; k < kSteps<T, DP>; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) df[t][k][i] ^= 0x80008000u;
     }
   }
   for (int m = 1; m < 32; m *= 2) most = max(most, __shfl_xor(most, m)), least = min(least, __shfl_xor(least, m));
@@ -153,6 +166,7 @@ __global__ __launch_bounds__(kBlock, (T::half || DP <= 64 ? 2 : 1)) void k_attn_
             float x = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) x += ds[t][i];
+            x *= flip;
             if (up <= -s.reach) far_back += x;
             else far_on += x;
           } else {
@@ -164,10 +178,11 @@ __global__ __launch_bounds__(kBlock, (T::half || DP <= 64 ? 2 : 1)) void k_attn_
             for (int i = 0; i < 16; ++i) {
               const int r = row_of(i) + 4 * hi;
               const float x = __shfl(ds[t][i], ((r - j) & 31) + 32 * hi);
-              if (r >= j) on += x;
-              else back += x;
+              const float y = kFlip && row_of(i) & 1 ? -x : x;   // (column r - j: its sign is the row's times this lane's)
+              if (r >= j) on += y;
+              else back += y;
             }
-            on = sum_of_pair(on), back = sum_of_pair(back);
+            on = sum_of_pair(on) * flip, back = sum_of_pair(back) * flip;
             const int d = lo + 31 + (hi ? j - 32 : j);
             const float x = hi ? back : on;
             if (d < -s.reach) far_back += x;
@@ -190,7 +205,7 @@ __global__ __launch_bounds__(kBlock, (T::half || DP <= 64 ? 2 : 1)) void k_attn_
     const int r = row0 + 32 * t + (lane & 31);
     if (r >= rows) continue;
     if (!limit[t]) zero(acc[t]);
-    const float f = s.scale * range[t].inverse();
+    const float f = s.scale * range[t].inverse() * flip;
     if (a.q_splits == 1) {
       store_column<T, DP>(static_cast<elem *>(a.dq) + ((size_t(b) * s.q_len + query[t]) * s.heads + head[t]) * a.io_dim, acc[t], f, a.io_dim, hi,
                           a.io_direct);
