@@ -177,6 +177,12 @@ __global__ __launch_bounds__(kBlock, (Form<T, DP>::PER_SIMD)) void k_attn_dkv(Bw
             for (int i = 0; i < 16; ++i)
               if (row_of(i) < seen_from) p[t][i] = 0.f;
           }
+          if (BIAS && q1 + 32 > span.q) {   // (rows behind the last query are zeros, but e^bias may leave the type, and 0 times infinity is NaN)
+            const int left = span.q - q1 - 4 * hi;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (row_of(i) >= left) p[t][i] = 0.f;
+          }
 #pragma unroll
           for (int i = 0; i < 16; ++i) ds[t][i] *= p[t][i];
         }

@@ -424,3 +424,28 @@ def test_a_long_cache_with_offsets_beyond_32_bits(dev):
     size = np.einsum("hr,rhd->hd", e, np.abs(tail)) / total[:, None]
     assert (np.abs(got[1, 0] - want) <= 3 * 2.0 ** -8 * size).all()
     np.testing.assert_allclose(lse.to_numpy()[:, :, 0], np.stack([np.full(g, np.log(sk)), np.log(total)]), rtol=0, atol=2.0 ** -10)
+
+
+# queries on both sides of a tile of 32 or 64, shared and own heads of keys, every form of the kernels' rows
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("bias", [12.0, 30.0, 100.0])
+@pytest.mark.parametrize("causal,sq,sk,h,g,d", [(False, 37, 37, 2, 2, 16), (True, 31, 31, 4, 2, 40), (False, 65, 50, 2, 1, 64), (True, 63, 63, 2, 2, 100), (False, 33, 129, 3, 3, 128),
+                                                (True, 64, 64, 1, 1, 24), (False, 300, 200, 4, 1, 64)])
+def test_a_large_position_bias(dev, monkeypatch, t, bias, causal, sq, sk, h, g, d):
+    """What softmax cannot see, a number added to the whole table, and large values of some buckets: the rows behind the last query, which a tile of
+    queries holds as zeros, have no probabilities.
+
+    Beside the usual bounds stands that of numbers below fp32's least normal one, 2^-126, which are zeros on the device (e^-100 is 2^-144): a
+    result has fewer than 3 * 300 * 200 < 2^18 terms, each a probability times |do (v - o)| |scale k| < 2^8 or less: 2^-100."""
+    from singa_amd import singa_wrap as singa
+    usual = close
+    monkeypatch.setitem(globals(), "close", lambda got, want, bound, what: usual(got, want, bound + 2.0 ** -100, what))
+    r = np.random.default_rng(17)
+    a = O.Attn(causal, buckets=8, max_distance=20)
+    for some in (False, True):
+        q, do, k, v = (stored(t, r.standard_normal((3, n, c, d))) for n, c in ((sq, h), (sq, h), (sk, g), (sk, g)))
+        table = r.standard_normal((8, h))
+        table[[1, 2, 6] if some else slice(None)] += bias
+        case = (q, k, v, do, stored("f32", table))
+        check(singa, dev, t, a, 3, sq, sk, h, g, d, case=case)
+        check(singa, dev, t, a, 3, sq, sk, h, g, d, case=case, lengths=((sq - 2, sq, 1), (sk, sk - 5, sk), None))
