@@ -292,7 +292,7 @@ Plan plan_of(const sgh_attn_geom *g, size_t elem_bytes) {
   a.q_splits = a.k_splits = 1, a.keys_each = 1 << 30;
   const size_t q_blocks = size_t(a.q_tiles) * a.q_units, k_blocks = size_t(a.k_tiles) * a.k_units;
   const size_t part = q_blocks * 2 <= cus ? 256 : 512;
-  if (q_blocks <= cus && size_t(g->k_len) > part) {
+  if (q_blocks && q_blocks <= cus && size_t(g->k_len) > part) {
     size_t n = 2 * cus / q_blocks, most = (size_t(g->k_len) + part - 1) / part;
     if (n > most) n = most;
     a.keys_each = int(((size_t(g->k_len) + n - 1) / n + 63) / 64 * 64);

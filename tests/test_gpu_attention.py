@@ -449,3 +449,20 @@ def test_a_large_position_bias(dev, monkeypatch, t, bias, causal, sq, sk, h, g, 
         case = (q, k, v, do, stored("f32", table))
         check(singa, dev, t, a, 3, sq, sk, h, g, d, case=case)
         check(singa, dev, t, a, 3, sq, sk, h, g, d, case=case, lengths=((sq - 2, sq, 1), (sk, sk - 5, sk), None))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("buckets", [0, 8])
+def test_no_queries_over_a_cache(dev, t, buckets):
+    """More keys than the backward pass has in one part: their gradients and the table's are zeros."""
+    from singa_amd import singa_wrap as singa
+    a = O.Attn(True, buckets=buckets, max_distance=20)
+    kind = upload(singa, dev, t, [0.0]).data_type()
+    q, k = singa.Tensor((2, 0, 4, 24), dev, kind), upload(singa, dev, t, np.ones((2, 700, 2, 24)))
+    table = upload(singa, dev, "f32", np.ones((buckets, 4))) if buckets else None
+    H = handle(singa, q, k, a)
+    o, lse = singa.AttentionForward(H, q, k, k, table)
+    dq, dk, dv, dtable = singa.AttentionBackward(H, q, q, k, k, o, lse, table)
+    assert o.shape() == dq.shape() == [2, 0, 4, 24] and lse.shape() == [2, 4, 0]
+    for x in (dk, dv) + ((dtable,) if buckets else ()):
+        assert not x.to_numpy().any()

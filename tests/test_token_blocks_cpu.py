@@ -246,3 +246,24 @@ answer([recorder.recorder_built().decode().split(), sorted(out), largest])
     assert len(ours) > 100 and not {n for n in run if "k_attn" in n or "k_norm" in n} - ours
     left = sorted(ours - set(run))
     assert not left, "\n" + "\n".join(left)
+
+
+@pytest.mark.parametrize("q_len,k_len", [(0, 256), (0, 257), (0, 5000), (0, 1 << 24), (5000, 0), (1 << 20, 0), (0, 0), (1, 1 << 24)])
+def test_geometries_without_queries_or_keys(q_len, k_len):
+    """What a handle asks for of an empty batch of queries over a cache, and of queries over an empty one; in a process of its own."""
+    asked, runs = recorded("""
+S, runs, asked = 1 << 50, [], []
+for buckets in (0, 8):
+    g = _lib.AttnGeom()
+    assert lib.sgh_attn_geom_init(C.byref(g), 2, %d, %d, 4, 2, 24, 0, 0.2, buckets, 20, 1) == 0
+    f, b = lib.sgh_attn_fwd_workspace_bytes(C.byref(g)), lib.sgh_attn_bwd_workspace_bytes(C.byref(g))
+    asked.append([f, b])
+    t, d = (4 * S, 12 * S) if buckets else (None, None)
+    for sfx in ("f32", "f16", "bf16"):
+        runs.append(getattr(lib, "sgh_attn_fwd_" + sfx)(C.byref(g), S, 2 * S, 3 * S, t, None, None, None, 5 * S, 6 * S, 7 * S, f, None))
+        runs.append(getattr(lib, "sgh_attn_bwd_" + sfx)(C.byref(g), 8 * S, S, 2 * S, 3 * S, 5 * S, 6 * S, t, None, None, None, 9 * S, 10 * S, 11 * S, d, 7 * S, b, None))
+answer([asked, runs])
+""" % (q_len, k_len))
+    assert runs == [0] * len(runs)
+    if q_len == 0:
+        assert all(f == 0 for f, _ in asked)
