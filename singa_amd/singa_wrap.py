@@ -916,6 +916,11 @@ def DistillationFwdBwd(x, top, teacher, labels=None, weights=None, temperature=1
     return loss, dx
 
 
+# A handle's geometry goes to the library by address.  The address is asked for at every call: a copied or unpickled handle,
+# and one whose `geom` was replaced, has a structure of its own.
+_address = C.addressof
+
+
 class AttentionHandle(object):
     """Sizes of an attention between the queries `q` [batch, q_len, heads, dim] and the keys `k` [batch, k_len, kv_heads, dim] (of the values
     as well), head h reading the keys of head ``h // (heads // kv_heads)``, with its mask, the scale of its products (None:
@@ -941,7 +946,6 @@ class AttentionHandle(object):
         check(_L().sgh_attn_geom_init(C.byref(self.geom), self.batch, self.q_len, self.k_len, self.heads, self.kv_heads, self.dim,
                                       int(self.causal), self.scale, self.buckets, int(max_distance), int(bidirectional)),
               "sgh_attn_geom_init")
-        self._at = C.addressof(self.geom)
         self._forward_bytes = _L().sgh_attn_fwd_workspace_bytes(C.byref(self.geom))
         self._backward_bytes = _L().sgh_attn_bwd_workspace_bytes(C.byref(self.geom))
 
@@ -983,7 +987,7 @@ def AttentionForward(h, q, k, v, table=None, q_lengths=None, k_lengths=None, q_s
     dev = q._dev
     o, lse = _like(q), _empty(Tensor, (h.batch, h.heads, h.q_len), dev, kFloat32)
     ws, at = _workspace(h._forward_bytes, dev)
-    check(fn(h._at, q.ptr, k.ptr, v.ptr, *args, o.ptr, lse.ptr, at, h._forward_bytes, dev.stream), name)
+    check(fn(_address(h.geom), q.ptr, k.ptr, v.ptr, *args, o.ptr, lse.ptr, at, h._forward_bytes, dev.stream), name)
     return o, lse
 
 
@@ -999,7 +1003,7 @@ def AttentionBackward(h, do, q, k, v, o, lse, table=None, q_lengths=None, k_leng
     dq, dk, dv = _like(q), _like(k), _like(v)
     dtable = None if table is None else _like(table)
     ws, at = _workspace(h._backward_bytes, dev)
-    check(fn(h._at, do.ptr, q.ptr, k.ptr, v.ptr, o.ptr, lse.ptr, *args, dq.ptr, dk.ptr, dv.ptr, None if dtable is None else dtable.ptr,
+    check(fn(_address(h.geom), do.ptr, q.ptr, k.ptr, v.ptr, o.ptr, lse.ptr, *args, dq.ptr, dk.ptr, dv.ptr, None if dtable is None else dtable.ptr,
              at, h._backward_bytes, dev.stream), name)
     return dq, dk, dv, dtable
 
@@ -1074,11 +1078,6 @@ def ResidualNormBackward(dy, dn, y, stats, h=None, post=None, gate=None, scale=1
 
 
 # ------------------------------------------------------------------------------------ operations
-
-# A handle's geometry goes to the library by address.  The address is asked for at every call: a copied or unpickled handle,
-# and one whose `geom` was replaced, has a structure of its own.
-_address = C.addressof
-
 
 class CudnnConvHandle(object):
     """Geometry + workspace of a convolution on the GPU device.  Same constructor arguments and

@@ -267,3 +267,32 @@ answer([asked, runs])
     assert runs == [0] * len(runs)
     if q_len == 0:
         assert all(f == 0 for f, _ in asked)
+
+
+def test_copied_attention_handles_pass_their_own_geometry(monkeypatch):
+    """Both passes of a handle that was copied, unpickled or given another geometry call with the structure that it holds."""
+    import copy
+    import pickle
+
+    from singa_amd import singa_wrap as singa
+
+    class Device(object):
+        stream = None
+
+    passed, dev = [], Device()
+    make = lambda shape: singa.from_device_pointer(4096, shape, dev, singa.kFloat32)
+    q, k, lse = make((2, 5, 4, 8)), make((2, 7, 2, 8)), make((2, 4, 5))
+    monkeypatch.setattr(singa, "_fn", lambda name, t: (lambda geom, *rest: passed.append(geom) or 0, name))
+    monkeypatch.setattr(singa, "_empty", lambda *a: q)
+    monkeypatch.setattr(singa, "_like", lambda t: t)
+    h = singa.AttentionHandle(q, k)
+    other, loaded = copy.deepcopy(h), pickle.loads(pickle.dumps(h))
+    for handle in (h, other, loaded):
+        singa.AttentionForward(handle, q, k, k)
+        singa.AttentionBackward(handle, q, q, k, k, q, lse)
+    assert passed == [C.addressof(x.geom) for x in (h, other, loaded) for _ in range(2)] and len(set(passed)) == 3
+    for x in (other, loaded):
+        assert bytes(x.geom) == bytes(h.geom) and vars(x).keys() == vars(h).keys()
+    h.geom = other.geom
+    singa.AttentionForward(h, q, k, k)
+    assert passed[-1] == C.addressof(other.geom)
