@@ -259,7 +259,7 @@ __global__ __launch_bounds__(kBlock) void k_attn_dq_join(BwdArgs a) {
 // dtable[e][h]: the sum over all blocks of head h, each thread's in order, then the threads' by halves
 __global__ __launch_bounds__(kBlock) void k_attn_dtable(BwdArgs a, float *dtable) {
   __shared__ float part[kBlock];
-  const int h = blockIdx.x % a.s.heads, e = blockIdx.x / a.s.heads;
+  const int h = blockIdx.x, e = blockIdx.y;
   const float *p = a.bias_part + size_t(h) * a.bias_blocks * a.s.buckets + e;
   float x = 0.f;
   for (size_t i = threadIdx.x; i < a.bias_blocks; i += kBlock) x += p[i * a.s.buckets];
@@ -285,7 +285,7 @@ int launch(const BwdArgs &a, const Bounds &bounds, float *dtable, hipStream_t s)
     SGH_LAUNCH_CHECK();
   }
   if (BIAS) {
-    hipLaunchKernelGGL(k_attn_dtable, dim3(unsigned(a.s.heads * a.s.buckets)), dim3(kBlock), 0, s, a, dtable);
+    hipLaunchKernelGGL(k_attn_dtable, dim3(unsigned(a.s.heads), unsigned(a.s.buckets)), dim3(kBlock), 0, s, a, dtable);
     SGH_LAUNCH_CHECK();
   }
   return SGH_OK;

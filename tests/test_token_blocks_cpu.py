@@ -296,3 +296,22 @@ def test_copied_attention_handles_pass_their_own_geometry(monkeypatch):
     h.geom = other.geom
     singa.AttentionForward(h, q, k, k)
     assert passed[-1] == C.addressof(other.geom)
+
+
+def test_most_heads_with_a_position_bias():
+    """Every head has a sum for every bucket: heads of one value, as many as a row may have, stay within a launch."""
+    runs, seen = recorded("""
+S, runs, seen = 1 << 50, [], []
+for heads, buckets, both in ((1 << 20, 128, 1), (1 << 20, 2, 0), (1 << 19, 64, 0)):
+    g = _lib.AttnGeom()
+    assert lib.sgh_attn_geom_init(C.byref(g), 1, 5, 5, heads, 1, 1, 0, 1.0, buckets, 128, both) == 0
+    f, b = lib.sgh_attn_fwd_workspace_bytes(C.byref(g)), lib.sgh_attn_bwd_workspace_bytes(C.byref(g))
+    for sfx in ("f32", "f16", "bf16"):
+        runs.append(getattr(lib, "sgh_attn_fwd_" + sfx)(C.byref(g), S, 2 * S, 3 * S, 4 * S, None, None, None, 5 * S, 6 * S, 7 * S, f, None))
+        launched()
+        runs.append(getattr(lib, "sgh_attn_bwd_" + sfx)(C.byref(g), 8 * S, S, 2 * S, 3 * S, 5 * S, 6 * S, 4 * S, None, None, None, 9 * S, 10 * S, 11 * S, 12 * S, 7 * S, b, None))
+        seen += [[heads * buckets, x * y * z, t] for n, (x, y, z), t in launched() if "k_attn_dtable" in n]
+answer([runs, seen])
+""")
+    assert runs == [0] * 18
+    assert len(seen) == 9 and all(want == blocks and threads == 256 for want, blocks, threads in seen), seen
