@@ -38,8 +38,9 @@ int check_geom(const sgh_attn_geom *g) {
     return SGH_EINVAL;
   if (!(g->scale > -__builtin_inff() && g->scale < __builtin_inff())) return SGH_EINVAL;
   if (g->dim > SGH_ATTN_MAX_DIM || g->q_len > kMostLength || g->k_len > kMostLength || (long long)g->heads * g->dim > kMostRow) return SGH_ELIMIT;
-  const unsigned long long b = g->batch;
-  if (b * g->heads * (g->q_len / 32 + 1) > kMostBlocks || b * g->kv_heads * (g->k_len / 32 + 1) > kMostBlocks) return SGH_ELIMIT;
+  // (the product of all three sizes may pass 64 bits)
+  const unsigned long long most = g->batch ? kMostBlocks / unsigned(g->batch) : ~0ull, tiles = g->q_len / 32 + 1, kv_tiles = g->k_len / 32 + 1;
+  if (g->heads * tiles > most || g->kv_heads * kv_tiles > most) return SGH_ELIMIT;
   if (g->buckets == 0) return SGH_OK;
   const int n = g->bidirectional ? g->buckets / 2 : g->buckets;
   if (g->buckets < 0 || (g->bidirectional && g->buckets % 2 != 0) || n < 2 || g->max_distance <= n / 2) return SGH_EINVAL;

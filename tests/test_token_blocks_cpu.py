@@ -315,3 +315,12 @@ answer([runs, seen])
 """)
     assert runs == [0] * 18
     assert len(seen) == 9 and all(want == blocks and threads == 256 for want, blocks, threads in seen), seen
+
+
+@pytest.mark.parametrize("how", [dict(batch=1 << 21, q_len=(1 << 28) - 32, heads=1 << 20), dict(batch=1 << 30, q_len=(1 << 28) - 32, heads=1 << 11),
+                                 dict(batch=1 << 21, k_len=(1 << 28) - 32, heads=1 << 20, kv_heads=1 << 20), dict(batch=(1 << 31) - 1, q_len=1 << 28, heads=1 << 20)])
+def test_counts_of_blocks_beyond_64_bits_are_refused(how):
+    """Products of sizes that are 0 modulo 2^64 (2^21 * 2^20 * 2^23) are as large as they are."""
+    g = _lib.AttnGeom()
+    sizes = dict(dict(batch=1, q_len=5, k_len=5, heads=1, kv_heads=1), **how)
+    assert _lib.lib().sgh_attn_geom_init(C.byref(g), *sizes.values(), 1, 0, 1.0, 0, 0, 0) == ELIMIT
