@@ -685,8 +685,14 @@ bool any_overlap(const Extent (&results)[R], const Extent (&arguments)[A]) {
   return false;
 }
 int check_sizes(size_t rows, size_t dim, size_t gates) {
-  if (rows > kMostRows || (gates != 0 && (gates > rows || rows % gates != 0))) return SGH_EINVAL;
+  if (rows > kMostRows || (gates != 0 && rows % gates != 0)) return SGH_EINVAL;   // (no rows are divided by any number)
   return dim > kMostDim ? SGH_ELIMIT : SGH_OK;
+}
+
+template <class S>
+int clear(void *p, size_t n, void *stream) {   // (the bits of 0 are the same in both 16-bit types)
+  if constexpr (sizeof(typename S::elem) == 4) return sgh_memset_f32(static_cast<float *>(p), 0.f, n, stream);
+  else return sgh_memset_f16(static_cast<uint16_t *>(p), 0.f, n, stream);
 }
 
 template <class S>
@@ -724,13 +730,14 @@ int backward(const void *dy, const void *dn, const void *y, const float *stats, 
   if (rc != SGH_OK) return rc;
   if ((!h && (post || gate)) || (!h && !pre) || (gate && gates == 0 && rows != 0)) return SGH_EINVAL;
   if (dim == 0) return SGH_OK;
-  if ((post && !dpost) || (pre && !dpre)) return SGH_EINVAL;
+  if ((post && !dpost) || (pre && !dpre) || (gate && gates != 0 && !dgate)) return SGH_EINVAL;
   if (rows == 0) {   // (sums over no rows)
     int r = pre ? sgh_memset_f32(dpre, 0.f, dim, stream) : SGH_OK;
     if (r == SGH_OK && post) r = sgh_memset_f32(dpost, 0.f, dim, stream);
+    if (r == SGH_OK && gate) r = clear<S>(dgate, gates * dim, stream);
     return r;
   }
-  if ((!dy && !dn) || !stats || !dx || (pre && (!dn || !y)) || (h && !dh) || (gate && !dgate)) return SGH_EINVAL;
+  if ((!dy && !dn) || !stats || !dx || (pre && (!dn || !y)) || (h && !dh)) return SGH_EINVAL;
   const Plan p = plan_of(rows, dim, gate ? gates : 0);
   if (!workspace || ws_bytes < p.bytes()) return SGH_EWORKSPACE;
   if (!sgh_aligned16(workspace)) return SGH_EINVAL;

@@ -207,3 +207,17 @@ def test_recorded_calls_replay(dev, t):
                 assert np.isfinite(y).all() and np.array_equal(x, y), turn
     finally:
         dev.ResetGraph()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("gates", [0, 1, 5])
+def test_no_rows_and_a_gate(dev, t, gates):
+    from singa_amd import singa_wrap as singa
+    w = upload(singa, dev, "f32", np.ones(12))
+    kind = upload(singa, dev, t, [0.0]).data_type()
+    x, gate = singa.Tensor((0, 12), dev, kind), singa.Tensor((0, 12), dev, kind) if gates == 0 else upload(singa, dev, t, np.ones((gates, 12)))
+    y, n, stats = singa.ResidualNormForward(x, x, w, gate, 0.5, w)
+    dx, dh, dpost, dgate, dpre = singa.ResidualNormBackward(x, x, y, stats, x, w, gate, 0.5, w)
+    assert y.shape() == n.shape() == dx.shape() == dh.shape() == [0, 12] and stats.shape() == [0, 2] and dgate.shape() == [gates, 12]
+    for g in (dpost, dgate, dpre):
+        assert not g.to_numpy().any()

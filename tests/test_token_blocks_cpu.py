@@ -324,3 +324,20 @@ def test_counts_of_blocks_beyond_64_bits_are_refused(how):
     g = _lib.AttnGeom()
     sizes = dict(dict(batch=1, q_len=5, k_len=5, heads=1, kv_heads=1), **how)
     assert _lib.lib().sgh_attn_geom_init(C.byref(g), *sizes.values(), 1, 0, 1.0, 0, 0, 0) == ELIMIT
+
+
+def test_norms_of_no_rows_with_a_gate():
+    """Any number of gates divides no rows: the forward pass has nothing to do, the backward pass leaves zeros for the weights and the gate."""
+    runs, refused = recorded("""
+S, runs, refused = 1 << 50, [], []
+for sfx in ("f32", "f16", "bf16"):
+    for g in (0, 1, 4):
+        n = lib.sgh_residual_norm_bwd_workspace_bytes(0, 24, g, 4 if sfx == "f32" else 2)
+        fwd = getattr(lib, "sgh_residual_norm_fwd_" + sfx)(None, None, 3 * S, 4 * S, 5 * S, 0, 24, g, 0.5, 1e-5, None, None, None, None), kernels()
+        bwd = getattr(lib, "sgh_residual_norm_bwd_" + sfx)(9 * S, 10 * S, 6 * S, 8 * S, 2 * S, 3 * S, 4 * S, 5 * S, 0, 24, g, 0.5, 11 * S, 12 * S, 13 * S, 14 * S, 15 * S, None, n, None), launched()
+        runs.append([g, n, fwd[0], len(fwd[1]), bwd[0], len(bwd[1])])
+    refused.append(getattr(lib, "sgh_residual_norm_bwd_" + sfx)(9 * S, 10 * S, 6 * S, 8 * S, 2 * S, 3 * S, 4 * S, 5 * S, 0, 24, 2, 0.5, 11 * S, 12 * S, 13 * S, None, 15 * S, None, 0, None))
+answer([runs, refused])
+""")
+    assert runs == [[g, 0, 0, 0, 0, 3 if g else 2] for _ in range(3) for g in (0, 1, 4)], runs
+    assert refused == [EINVAL] * 3
