@@ -127,15 +127,14 @@ __device__ __forceinline__ unsigned lds_offset(const void *lds) {
   typedef __attribute__((address_space(3))) const void lds_void;
   return unsigned(size_t((lds_void *)lds));
 }
-// (m0 is the compiler's to set wherever it needs it, as here: it keeps nothing there.)
 // 16 (4) bytes for each lane, one behind the other from `lds` on, the same for the whole wavefront; offsets behind the buffer give zeros
 __device__ __forceinline__ void load_lds16(rsrc4_t buffer, unsigned lds, int offset) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(int(lds))), "v"(offset), "s"(buffer)
-               : "memory");
+               : "memory", "m0");
 }
 __device__ __forceinline__ void load_lds4(rsrc4_t buffer, unsigned lds, int offset) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(int(lds))), "v"(offset), "s"(buffer)
-               : "memory");
+               : "memory", "m0");
 }
 
 // Copies rows of a matrix into a tile.  Rows from `rows` on and values from `dim` on become zeros, whatever lies there.

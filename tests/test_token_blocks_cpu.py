@@ -341,3 +341,19 @@ answer([runs, refused])
 """)
     assert runs == [[g, 0, 0, 0, 0, 3 if g else 2] for _ in range(3) for g in (0, 1, 4)], runs
     assert refused == [EINVAL] * 3
+
+
+def test_assembly_names_the_register_that_it_writes():
+    """What the compiler is not told of it may keep a value in."""
+    import os
+    import re
+
+    where = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "singa_amd", "csrc")
+    found = 0
+    for name in sorted(os.listdir(where)):
+        with open(os.path.join(where, name)) as f:
+            for statement in re.findall(r"\basm\b[^;]*;", f.read()):
+                if re.search(r"\bs_mov_b32 m0\b", statement):
+                    found += 1
+                    assert '"m0"' in statement.rsplit(":", 1)[1], (name, statement)
+    assert found
