@@ -128,6 +128,9 @@ __device__ __forceinline__ unsigned lds_offset(const void *lds) {
   return unsigned(size_t((lds_void *)lds));
 }
 // 16 (4) bytes for each lane, one behind the other from `lds` on, the same for the whole wavefront; offsets behind the buffer give zeros
+// (m0 is reserved: the compiler sets it in front of what needs it and, told that it is written here, again behind.  It warns of every such register.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_lds16(rsrc4_t buffer, unsigned lds, int offset) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(int(lds))), "v"(offset), "s"(buffer)
                : "memory", "m0");
@@ -136,6 +139,7 @@ __device__ __forceinline__ void load_lds4(rsrc4_t buffer, unsigned lds, int offs
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(int(lds))), "v"(offset), "s"(buffer)
                : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // Copies rows of a matrix into a tile.  Rows from `rows` on and values from `dim` on become zeros, whatever lies there.
 template <class T, int DP, int ROWS, int NT = kBlock>
