@@ -343,31 +343,25 @@ struct Reader {
 #pragma unroll
       for (int n = 0; n < DP / 32; ++n) col_chunk(tile, row0, s, n, &a.v[s][n]);
   }
-  // c[q] += rows x columns f[q]
-  template <int Q>
-  static __device__ __forceinline__ void mul(const Rows &a, const cols_t<T, DP> (&f)[Q], f32x16 (&c)[Q]) {
+  // c += rows x columns f
+  static __device__ __forceinline__ void mul(const Rows &a, const cols_t<T, DP> &f, f32x16 &c) {
 #pragma unroll
-    for (int k = 0; k < kSteps<T, DP>; ++k)
-#pragma unroll
-      for (int q = 0; q < Q; ++q) c[q] = mul_step<T>(a.v[k], f[q][k], c[q]);
+    for (int k = 0; k < kSteps<T, DP>; ++k) c = mul_step<T>(a.v[k], f[k], c);
   }
-  // c[q][n] += (rows, transposed: values 32 n ..) x t[q]
-  template <int Q>
-  static __device__ __forceinline__ void mul(const Cols &a, const Terms<T> (&t)[Q], f32x16 (&c)[Q][DP / 32]) {
+  // c[n] += (rows, transposed: values 32 n ..) x t
+  static __device__ __forceinline__ void mul(const Cols &a, const Terms<T> &t, f32x16 (&c)[DP / 32]) {
 #pragma unroll
     for (int s = 0; s < (T::half ? 2 : 16); ++s)
 #pragma unroll
-      for (int n = 0; n < DP / 32; ++n)
-#pragma unroll
-        for (int q = 0; q < Q; ++q) {
-          if constexpr (T::half) c[q][n] = T::mfma(a.v[s][n], t[q].v[s], c[q][n]);
-          else c[q][n] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[s][n], t[q].v[s], c[q][n], 0, 0, 0);
-        }
+      for (int n = 0; n < DP / 32; ++n) {
+        if constexpr (T::half) c[n] = T::mfma(a.v[s][n], t.v[s], c[n]);
+        else c[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[s][n], t.v[s], c[n], 0, 0, 0);
+      }
   }
-  template <int Q>
-  __device__ __forceinline__ void rows(const char *tile, int row0, const cols_t<T, DP> (&f)[Q], f32x16 (&c)[Q]) const {
+  __device__ __forceinline__ void rows(const char *tile, int row0, const cols_t<T, DP> &f, f32x16 &c) const {
     Rows a;
     load(tile, row0, a);
+    if constexpr (T::half && DP <= 64) pin();   // (bfloat16 heads of 64, 8 x 12 of 1024 places, bias, backward: 163 -> 159 us; of 128 1750 -> 1920)
     mul(a, f, c);
   }
   // The same with few registers: four chunk pairs at a time, the columns' last ones (from HELD on) from another tile, of 32 values
@@ -421,8 +415,7 @@ struct Reader {
       pin();
     }
   }
-  template <int Q>
-  __device__ __forceinline__ void transposed(const char *tile, int row0, const Terms<T> (&t)[Q], f32x16 (&c)[Q][DP / 32]) const {
+  __device__ __forceinline__ void transposed(const char *tile, int row0, const Terms<T> &t, f32x16 (&c)[DP / 32]) const {
     Cols a;
     load(tile, row0, a);
     mul(a, t, c);
@@ -438,12 +431,14 @@ __device__ __forceinline__ float sum_of_pair(float x) {
   return __builtin_bit_cast(float, unsigned(r[0])) + __builtin_bit_cast(float, unsigned(r[1]));
 }
 
+__device__ __forceinline__ void zero(f32x16 &c) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) c[i] = 0.f;
+}
 template <int N>
 __device__ __forceinline__ void zero(f32x16 (&c)[N]) {
 #pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) c[n][i] = 0.f;
+  for (int n = 0; n < N; ++n) zero(c[n]);
 }
 
 // Stores a lane's column (values 32 n + row of c[n]) times f as a row of `dim` values

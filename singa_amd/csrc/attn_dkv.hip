@@ -29,11 +29,11 @@ struct Form {
   static constexpr size_t lds(int reach, bool bias) { return 2 * SLOT + VALUES + REST + (bias ? (2 * reach + 1) * sizeof(float) : 0); }
 };
 
-template <class T, int DP, int KW, bool BIAS>
+template <class T, int DP, bool BIAS>
 __global__ __launch_bounds__(kBlock, (Form<T, DP>::PER_SIMD)) void k_attn_dkv(BwdArgs a, Bounds bounds) {
   typedef typename T::elem elem;
   typedef Form<T, DP> F;
-  constexpr int QR = F::QR, SUB = QR / 32, ND = DP / 32, WAVE_KEYS = 32 * KW, KEYS = 4 * WAVE_KEYS, TILE = F::TILE, SLOT = F::SLOT;
+  constexpr int QR = F::QR, SUB = QR / 32, ND = DP / 32, KEYS = kRows, TILE = F::TILE, SLOT = F::SLOT;
   constexpr bool VL = F::VL;
   extern __shared__ __align__(16) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
@@ -42,22 +42,17 @@ __global__ __launch_bounds__(kBlock, (Form<T, DP>::PER_SIMD)) void k_attn_dkv(Bw
   const unsigned tile = place.tile, unit = place.unit, split = place.split;
   const int b = unit / s.kv_heads, kv = unit % s.kv_heads, group = s.heads / s.kv_heads;
   const Span span = span_of(s, b);
-  const int key0 = int(tile) * KEYS + wave * WAVE_KEYS;
+  const int key0 = int(tile) * KEYS + wave * 32, key = key0 + (lane & 31);
 
-  int key[KW];
-  frag_t kf[KW][F::HELD];
-  cols_t<T, DP> vf[VL ? 1 : KW];
-#pragma unroll
-  for (int t = 0; t < KW; ++t) {
-    key[t] = key0 + 32 * t + (lane & 31);
-    const size_t at = ((size_t(b) * s.k_len + key[t]) * s.kv_heads + kv) * s.dim;
-    const int n = key[t] < span.k ? s.dim : 0;
-    load_columns<T, F::HELD * 2 * T::VEC>(kf[t], static_cast<const elem *>(a.k) + at, n, hi, a.direct);
-    if (!VL) load_columns<T, DP>(vf[t], static_cast<const elem *>(a.v) + at, n, hi, a.direct);
-  }
+  frag_t kf[F::HELD];
+  cols_t<T, DP> vf;
+  const size_t first_value = ((size_t(b) * s.k_len + key) * s.kv_heads + kv) * s.dim;
+  const int values_of_key = key < span.k ? s.dim : 0;
+  load_columns<T, F::HELD * 2 * T::VEC>(kf, static_cast<const elem *>(a.k) + first_value, values_of_key, hi, a.direct);
+  if (!VL) load_columns<T, DP>(vf, static_cast<const elem *>(a.v) + first_value, values_of_key, hi, a.direct);
   // queries [from, span.q) see a key of the block, [mine, span.q) one of the wavefront
   const int from = s.causal ? max(int(tile) * KEYS - span.start, 0) / QR * QR : 0;
-  const int mine = s.causal ? key0 - span.start : 0, all_see = s.causal ? key0 + WAVE_KEYS - 1 - span.start : 0;
+  const int mine = s.causal ? key0 - span.start : 0, all_see = s.causal ? key0 + 31 - span.start : 0;
   const int turns_of_head = int(tile) * KEYS < span.k && from < span.q ? (span.q - from + QR - 1) / QR : 0;
   const int turns = turns_of_head * group, each = (turns + int(a.k_splits) - 1) / int(a.k_splits);
   const int begin = min(turns, int(split) * each), end = min(turns, begin + each);
@@ -73,10 +68,9 @@ __global__ __launch_bounds__(kBlock, (Form<T, DP>::PER_SIMD)) void k_attn_dkv(Bw
   const float *lse = a.stats + (size_t(b) * s.heads + size_t(kv) * group) * s.q_len;
   const float *delta = lse + size_t(s.q_len) * s.heads * (a.k_units / s.kv_heads);
 
-  f32x16 dk[KW][ND], dv[KW][ND];
-  Range<T> range[KW];
-#pragma unroll
-  for (int t = 0; t < KW; ++t) zero(dk[t]), zero(dv[t]);
+  f32x16 dk[ND], dv[ND];
+  Range<T> range;
+  zero(dk), zero(dv);
   const float c = s.scale * kLog2e;
   const Reader<T, DP> reader(lane);
   const Reader<T, 32> short_reader(lane);
@@ -129,19 +123,17 @@ __global__ __launch_bounds__(kBlock, (Form<T, DP>::PER_SIMD)) void k_attn_dkv(Bw
     if (q0 + QR > mine) {
 #pragma unroll
       for (int u = 0; u < SUB; ++u) {
-        f32x16 p[KW], ds[KW];
+        f32x16 p, ds;
         zero(p);
-        if constexpr (VL) reader.rows_by_four(qt, 32 * u, kf[0], short_reader, rest + wave * 32 / Tile<T, 32>::G * Tile<T, 32>::GROUP, p[0]);
+        if constexpr (VL) reader.rows_by_four(qt, 32 * u, kf, short_reader, rest + wave * 32 / Tile<T, 32>::G * Tile<T, 32>::GROUP, p);
         else reader.rows(qt, 32 * u, kf, p);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {   // (the product starts from -delta)
           const sgh_v4f x = *reinterpret_cast<const sgh_v4f *>(st + kStats + 32 * u + 8 * g + 4 * hi);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int t = 0; t < KW; ++t) ds[t][4 * g + i] = x[i];
+          for (int i = 0; i < 4; ++i) ds[4 * g + i] = x[i];
         }
-        if constexpr (VL) reader.rows(dt, 32 * u, values, wave * 32, ds[0]);
+        if constexpr (VL) reader.rows(dt, 32 * u, values, wave * 32, ds);
         else reader.rows(dt, 32 * u, vf, ds);
         float row_lse[16];
 #pragma unroll
@@ -151,73 +143,63 @@ __global__ __launch_bounds__(kBlock, (Form<T, DP>::PER_SIMD)) void k_attn_dkv(Bw
           for (int i = 0; i < 4; ++i) row_lse[4 * g + i] = x[i];
         }
         const int q1 = q0 + 32 * u;
+        if constexpr (BIAS) {
+          const int first = key - (span.start + q1) - 4 * hi;   // distance in row 0
+          const int lo = key0 - (span.start + q1 + 31), up = key0 + 31 - (span.start + q1);
+          const float *centre = band + s.reach;
+          if (up <= -s.reach || lo >= s.reach) {
+            const float far = centre[up <= -s.reach ? -s.reach : s.reach];
 #pragma unroll
-        for (int t = 0; t < KW; ++t) {
-          if constexpr (BIAS) {
-            const int first = key[t] - (span.start + q1) - 4 * hi;   // distance in row 0
-            const int lo = key0 + 32 * t - (span.start + q1 + 31), up = key0 + 32 * t + 31 - (span.start + q1);
-            const float *centre = band + s.reach;
-            if (up <= -s.reach || lo >= s.reach) {
-              const float far = centre[up <= -s.reach ? -s.reach : s.reach];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[t][i], c, far) - row_lse[i]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                p[t][i] = __builtin_amdgcn_exp2f(
-                    __builtin_fmaf(p[t][i], c, centre[min(max(first - row_of(i), -s.reach), s.reach)]) - row_lse[i]);
-            }
+            for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i], c, far) - row_lse[i]);
           } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[t][i], c, -row_lse[i]));
-          }
-          if (s.causal && q1 < all_see) {
-            const int seen_from = key[t] - span.start - q1 - 4 * hi;   // first row that sees the lane's key
-#pragma unroll
             for (int i = 0; i < 16; ++i)
-              if (row_of(i) < seen_from) p[t][i] = 0.f;
+              p[i] = __builtin_amdgcn_exp2f(
+                  __builtin_fmaf(p[i], c, centre[min(max(first - row_of(i), -s.reach), s.reach)]) - row_lse[i]);
           }
-          if (BIAS && q1 + 32 > span.q) {   // (rows behind the last query are zeros, but e^bias may leave the type, and 0 times infinity is NaN)
-            const int left = span.q - q1 - 4 * hi;
+        } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (row_of(i) >= left) p[t][i] = 0.f;
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) ds[t][i] *= p[t][i];
+          for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i], c, -row_lse[i]));
         }
-        Terms<T> terms[KW];
+        if (s.causal && q1 < all_see) {
+          const int seen_from = key - span.start - q1 - 4 * hi;   // first row that sees the lane's key
 #pragma unroll
-        for (int t = 0; t < KW; ++t) terms[t].set(p[t]);
-        if constexpr (VL) reader.transposed_by_four(dt, 32 * u, terms[0], dv[0]);
+          for (int i = 0; i < 16; ++i)
+            if (row_of(i) < seen_from) p[i] = 0.f;
+        }
+        if (BIAS && q1 + 32 > span.q) {   // (rows behind the last query are zeros, but e^bias may leave the type, and 0 times infinity is NaN)
+          const int left = span.q - q1 - 4 * hi;
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (row_of(i) >= left) p[i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ds[i] *= p[i];
+        Terms<T> terms;
+        terms.set(p);
+        if constexpr (VL) reader.transposed_by_four(dt, 32 * u, terms, dv);
         else reader.transposed(dt, 32 * u, terms, dv);
-#pragma unroll
-        for (int t = 0; t < KW; ++t) {
-          range[t].fit(ds[t], dk[t]);
-          terms[t].set(ds[t]);
-        }
-        if constexpr (VL) reader.transposed_by_four(qt, 32 * u, terms[0], dk[0]);
+        range.fit(ds, dk);
+        terms.set(ds);
+        if constexpr (VL) reader.transposed_by_four(qt, 32 * u, terms, dk);
         else reader.transposed(qt, 32 * u, terms, dk);
       }
     }
     head = next_head, q0 = next_q0;
   }
 
-#pragma unroll
-  for (int t = 0; t < KW; ++t) {
-    if (key[t] >= s.k_len) continue;
-    if (key[t] >= span.k) zero(dk[t]), zero(dv[t]);   // (what lies behind a sequence gets zeros)
-    constexpr float down = std::is_same<T, F16>::value ? 0x1p-14f : 1.f;
-    const float f = key[t] < span.k ? s.scale * range[t].inverse() * down : 0.f;
-    if (a.k_splits == 1) {
-      const size_t at = ((size_t(b) * s.k_len + key[t]) * s.kv_heads + kv) * a.io_dim;
-      store_column<T, DP>(static_cast<elem *>(a.dk) + at, dk[t], f, a.io_dim, hi, a.io_direct);
-      store_column<T, DP>(static_cast<elem *>(a.dv) + at, dv[t], down, a.io_dim, hi, a.io_direct);
-    } else {
-      const size_t n = size_t(a.k_units) * s.k_len, at = 2 * split * n + size_t(unit) * s.k_len + key[t];
-      store_partial<DP>(a.k_part + at * DP, dk[t], f, hi);
-      store_partial<DP>(a.k_part + (at + n) * DP, dv[t], down, hi);
-    }
+  if (key >= s.k_len) return;
+  if (key >= span.k) zero(dk), zero(dv);   // (what lies behind a sequence gets zeros)
+  constexpr float down = std::is_same<T, F16>::value ? 0x1p-14f : 1.f;
+  const float f = key < span.k ? s.scale * range.inverse() * down : 0.f;
+  if (a.k_splits == 1) {
+    const size_t at = ((size_t(b) * s.k_len + key) * s.kv_heads + kv) * a.io_dim;
+    store_column<T, DP>(static_cast<elem *>(a.dk) + at, dk, f, a.io_dim, hi, a.io_direct);
+    store_column<T, DP>(static_cast<elem *>(a.dv) + at, dv, down, a.io_dim, hi, a.io_direct);
+  } else {
+    const size_t n = size_t(a.k_units) * s.k_len, at = 2 * split * n + size_t(unit) * s.k_len + key;
+    store_partial<DP>(a.k_part + at * DP, dk, f, hi);
+    store_partial<DP>(a.k_part + (at + n) * DP, dv, down, hi);
   }
 }
 
@@ -238,12 +220,12 @@ __global__ __launch_bounds__(kBlock) void k_attn_dkv_join(BwdArgs a) {
     if (d + i < a.io_dim) T::St::st(out + d + i, x[i]);
 }
 
-template <class T, int DP, int KW, bool BIAS>
+template <class T, int DP, bool BIAS>
 int launch(const BwdArgs &a, const Bounds &bounds, hipStream_t s) {
   const size_t lds = Form<T, DP>::lds(a.s.reach, BIAS);
   static std::atomic<unsigned long long> asked{0};
-  SGH_HIP_TRY(sgh_allow_lds(reinterpret_cast<const void *>(k_attn_dkv<T, DP, KW, BIAS>), asked));
-  hipLaunchKernelGGL((k_attn_dkv<T, DP, KW, BIAS>), dim3(a.k_tiles * a.k_units * a.k_splits), dim3(kBlock), lds, s, a, bounds);
+  SGH_HIP_TRY(sgh_allow_lds(reinterpret_cast<const void *>(k_attn_dkv<T, DP, BIAS>), asked));
+  hipLaunchKernelGGL((k_attn_dkv<T, DP, BIAS>), dim3(a.k_tiles * a.k_units * a.k_splits), dim3(kBlock), lds, s, a, bounds);
   SGH_LAUNCH_CHECK();
   if (a.k_splits > 1) {
     const size_t n = 2 * size_t(a.k_units) * a.s.k_len, per = kBlock / (DP / 4);
@@ -254,8 +236,8 @@ int launch(const BwdArgs &a, const Bounds &bounds, hipStream_t s) {
 }
 template <class T, int DP>
 int run_dim(const BwdArgs &a, const Bounds &bounds, hipStream_t s) {
-  if (a.s.buckets) return launch<T, DP, 1, true>(a, bounds, s);
-  return launch<T, DP, 1, false>(a, bounds, s);
+  if (a.s.buckets) return launch<T, DP, true>(a, bounds, s);
+  return launch<T, DP, false>(a, bounds, s);
 }
 
 template <class T>

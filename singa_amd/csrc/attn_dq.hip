@@ -12,11 +12,11 @@ namespace {
 
 using namespace attn;
 
-template <class T, int DP, int QT, bool BIAS>
+template <class T, int DP, bool BIAS>
 __global__ __launch_bounds__(kBlock, (T::half || DP <= 64 ? 2 : 1)) void k_attn_dq(BwdArgs a, Bounds bounds) {
   typedef typename T::elem elem;
   typedef Tile<T, DP> L;
-  constexpr int KT = T::half ? 64 : 32, SUB = KT / 32, ND = DP / 32, WAVE_ROWS = 32 * QT, ROWS = 4 * WAVE_ROWS;
+  constexpr int KT = T::half ? 64 : 32, SUB = KT / 32, ND = DP / 32, ROWS = kRows;
   constexpr int TILE = L::bytes(KT);
   extern __shared__ __align__(16) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
@@ -26,57 +26,51 @@ __global__ __launch_bounds__(kBlock, (T::half || DP <= 64 ? 2 : 1)) void k_attn_
   const int per_batch = s.heads / a.pack, b = unit / per_batch, head0 = int(unit % per_batch) * a.pack;
   const int kv = head0 / (s.heads / s.kv_heads);
   const Span span = span_of(s, b);
-  const int rows = s.q_len * a.pack, row0 = int(tile) * ROWS + wave * WAVE_ROWS;
+  const int rows = s.q_len * a.pack, row0 = int(tile) * ROWS + wave * 32;
 
   // The 16-bit matrix products' sums are rounded a little downwards (by a thirtieth of a place on the average), which 10^8 terms of a bucket add
   // up to: odd queries have the gradient of their result negated, so that it goes both ways (13 x 8 heads, 2833 places, table's gradient: 4.4e-6 off,
   // so 5.0e-7; fp32 products show none of it).
   constexpr bool kFlip = BIAS && T::half;
   const float flip = kFlip && (lane & 1) ? -1.f : 1.f;
-  int query[QT], head[QT], limit[QT], most = 0, least = 1 << 30;
-  float lse[QT], delta[QT];   // (with a bias, natural logarithms: the product with log2 e is rounded with the sum, which the bias's gradient is told by)
-  cols_t<T, DP> qf[QT], df[QT];
+  const int r = row0 + (lane & 31), query = a.pack == 1 ? r : r / a.pack, head = a.pack == 1 ? head0 : head0 + r % a.pack;
+  const int limit = r < rows && query < span.q ? (s.causal ? min(span.k, max(span.start + query + 1, 0)) : span.k) : 0;
+  int most = limit, least = limit;
+  const size_t at = ((size_t(b) * s.q_len + query) * s.heads + head) * s.dim;
+  const size_t stat = (size_t(b) * s.heads + head) * s.q_len + query;
+  const int n = limit ? s.dim : 0;
+  cols_t<T, DP> qf, df;
+  load_columns<T, DP>(qf, static_cast<const elem *>(a.q) + at, n, hi, a.direct);
+  load_columns<T, DP>(df, static_cast<const elem *>(a.dout) + at, n, hi, a.direct);
+  // (with a bias a natural logarithm: the product with log2 e is rounded with the sum, which the bias's gradient is told by)
+  float lse = limit ? a.lse[stat] : kNegInf;
+  if (lse == kNegInf) lse = -kNegInf;
+  const float lse2 = lse * kLog2e;
+  if (!BIAS) lse = lse2;
+  float x = 0.f;
+  cols_t<T, DP> of;
+  load_columns<T, DP>(of, static_cast<const elem *>(a.o) + ((size_t(b) * s.q_len + query) * s.heads + head) * a.io_dim, n ? a.io_dim : 0, hi,
+                      a.io_direct);
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int r = row0 + 32 * t + (lane & 31);
-    query[t] = a.pack == 1 ? r : r / a.pack;
-    head[t] = a.pack == 1 ? head0 : head0 + r % a.pack;
-    limit[t] = r < rows && query[t] < span.q ? (s.causal ? min(span.k, max(span.start + query[t] + 1, 0)) : span.k) : 0;
-    most = max(most, limit[t]), least = min(least, limit[t]);
-    const size_t at = ((size_t(b) * s.q_len + query[t]) * s.heads + head[t]) * s.dim;
-    const size_t stat = (size_t(b) * s.heads + head[t]) * s.q_len + query[t];
-    const int n = limit[t] ? s.dim : 0;
-    load_columns<T, DP>(qf[t], static_cast<const elem *>(a.q) + at, n, hi, a.direct);
-    load_columns<T, DP>(df[t], static_cast<const elem *>(a.dout) + at, n, hi, a.direct);
-    lse[t] = limit[t] ? a.lse[stat] : kNegInf;
-    if (lse[t] == kNegInf) lse[t] = -kNegInf;
-    const float lse2 = lse[t] * kLog2e;
-    if (!BIAS) lse[t] = lse2;
-    float x = 0.f;
-    cols_t<T, DP> of;
-    load_columns<T, DP>(of, static_cast<const elem *>(a.o) + ((size_t(b) * s.q_len + query[t]) * s.heads + head[t]) * a.io_dim, n ? a.io_dim : 0, hi,
-                        a.io_direct);
+  for (int k = 0; k < kSteps<T, DP>; ++k) {
+    float o[T::VEC], d[T::VEC];
+    T::St::template load16<false>(reinterpret_cast<const elem *>(&of[k]), o);
+    T::St::template load16<false>(reinterpret_cast<const elem *>(&df[k]), d);
 #pragma unroll
-    for (int k = 0; k < kSteps<T, DP>; ++k) {
-      float o[T::VEC], d[T::VEC];
-      T::St::template load16<false>(reinterpret_cast<const elem *>(&of[k]), o);
-      T::St::template load16<false>(reinterpret_cast<const elem *>(&df[t][k]), d);
+    for (int i = 0; i < T::VEC; ++i) x = __builtin_fmaf(o[i], d[i], x);
+  }
+  float delta = sum_of_pair(x);
+  if (r < rows && hi == 0 && split == 0) {
+    a.stats[stat] = lse2 - term_bits<T>();
+    a.stats[size_t(a.q_units) * rows + stat] = -delta;
+  }
+  if constexpr (kFlip) {   // (rows are queries here: with a bias no heads share a tile)
+    delta *= flip;
+    if (lane & 1)
 #pragma unroll
-      for (int i = 0; i < T::VEC; ++i) x = __builtin_fmaf(o[i], d[i], x);
-    }
-    delta[t] = sum_of_pair(x);
-    if (r < rows && hi == 0 && split == 0) {
-      a.stats[stat] = lse2 - term_bits<T>();
-      a.stats[size_t(a.q_units) * rows + stat] = -delta[t];
-    }
-    if constexpr (kFlip) {   // (rows are queries here: with a bias no heads share a tile)
-      delta[t] *= flip;
-      if (lane & 1)
+      for (int k = 0; k < kSteps<T, DP>; ++k)
 #pragma unroll
-        for (int k = 0; k < kSteps<T, DP>; ++k)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) df[t][k][i] ^= 0x80008000u;
-    }
+        for (int i = 0; i < 4; ++i) df[k][i] ^= 0x80008000u;
   }
   for (int m = 1; m < 32; m *= 2) most = max(most, __shfl_xor(most, m)), least = min(least, __shfl_xor(least, m));
   most = __builtin_amdgcn_readfirstlane(most), least = __builtin_amdgcn_readfirstlane(least);
@@ -102,10 +96,9 @@ __global__ __launch_bounds__(kBlock, (T::half || DP <= 64 ? 2 : 1)) void k_attn_
   stage.init(stride, s.dim, a.direct);
   const elem *kp = static_cast<const elem *>(a.k) + (size_t(b) * s.k_len * s.kv_heads + kv) * s.dim;
   const elem *vp = static_cast<const elem *>(a.v) + (size_t(b) * s.k_len * s.kv_heads + kv) * s.dim;
-  f32x16 acc[QT][ND];
-  Range<T> range[QT];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) zero(acc[t]);
+  f32x16 acc[ND];
+  Range<T> range;
+  zero(acc);
   const float c = s.scale * kLog2e;
   const Reader<T, DP> reader(lane);
   auto request = [&](int k0, int slot) {
@@ -122,96 +115,88 @@ __global__ __launch_bounds__(kBlock, (T::half || DP <= 64 ? 2 : 1)) void k_attn_
     if (k0 >= most) continue;
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
-      f32x16 p[QT], ds[QT];
+      f32x16 p, ds;
       zero(p);
       reader.rows(kt, 32 * u, qf, p);
+      if constexpr (T::half) pin();   // (one product's loads under way at a time: 2 x 16 heads of 128, 8192 places, 1870 -> 1720 us, fp32 heads of 64 125 -> 128)
       // (the product starts from -delta)
 #pragma unroll
-      for (int t = 0; t < QT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) ds[t][i] = -delta[t];
+      for (int i = 0; i < 16; ++i) ds[i] = -delta;
       reader.rows(vt, 32 * u, df, ds);
       const int k1 = k0 + 32 * u;
+      const int first = k1 - (span.start + query) + 4 * hi;
+      if constexpr (BIAS) {
+        const int lo = k1 - (span.start + row0 + 31), up = k1 + 31 - (span.start + row0);
+        const float *mine = band + s.reach;
+        if (up <= -s.reach || lo >= s.reach) {
+          const float far = __builtin_fmaf(-lse, kLog2e, mine[up <= -s.reach ? -s.reach : s.reach]);
 #pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        const int first = k1 - (span.start + query[t]) + 4 * hi;
-        if constexpr (BIAS) {
-          const int lo = k1 - (span.start + row0 + 32 * t + 31), up = k1 + 31 - (span.start + row0 + 32 * t);
-          const float *mine = band + s.reach;
-          if (up <= -s.reach || lo >= s.reach) {
-            const float far = __builtin_fmaf(-lse[t], kLog2e, mine[up <= -s.reach ? -s.reach : s.reach]);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[t][i], c, far));
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              p[t][i] = __builtin_amdgcn_exp2f(
-                  __builtin_fmaf(p[t][i], c, __builtin_fmaf(-lse[t], kLog2e, mine[min(max(first + row_of(i), -s.reach), s.reach)])));
-          }
+          for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i], c, far));
         } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[t][i], c, -lse[t]));
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) ds[t][i] *= p[t][i];
-        if (k1 + 32 > least) {
-          const int left = limit[t] - k1 - 4 * hi;
-#pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (row_of(i) >= left) ds[t][i] = 0.f;
+            p[i] = __builtin_amdgcn_exp2f(
+                __builtin_fmaf(p[i], c, __builtin_fmaf(-lse, kLog2e, mine[min(max(first + row_of(i), -s.reach), s.reach)])));
         }
-        if constexpr (BIAS) {
-          const int lo = k1 - (span.start + row0 + 32 * t + 31), up = k1 + 31 - (span.start + row0 + 32 * t);
-          if (up <= -s.reach || lo >= s.reach) {
-            float x = 0.f;
+      } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x += ds[t][i];
-            x *= flip;
-            if (up <= -s.reach) far_back += x;
-            else far_on += x;
-          } else {
-            // Sums of the diagonals.  Lane j gets from row r the column (r - j) mod 32, whose distance is j or j - 32 on from the block's
-            // corner: two sums for each lane, in the order of the rows.
-            float on = 0.f, back = 0.f;
-            const int j = lane & 31;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int r = row_of(i) + 4 * hi;
-              const float x = __shfl(ds[t][i], ((r - j) & 31) + 32 * hi);
-              const float y = kFlip && row_of(i) & 1 ? -x : x;   // (column r - j: its sign is the row's times this lane's)
-              if (r >= j) on += y;
-              else back += y;
-            }
-            on = sum_of_pair(on) * flip, back = sum_of_pair(back) * flip;
-            const int d = lo + 31 + (hi ? j - 32 : j);
-            const float x = hi ? back : on;
-            if (d < -s.reach) far_back += x;
-            else if (d > s.reach) far_on += x;
-            else sums[d + s.reach] += x;
-            __builtin_amdgcn_wave_barrier();
-          }
-        }
-        range[t].fit(ds[t], acc[t]);
+        for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i], c, -lse));
       }
-      Terms<T> terms[QT];
 #pragma unroll
-      for (int t = 0; t < QT; ++t) terms[t].set(ds[t]);
+      for (int i = 0; i < 16; ++i) ds[i] *= p[i];
+      if (k1 + 32 > least) {
+        const int left = limit - k1 - 4 * hi;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (row_of(i) >= left) ds[i] = 0.f;
+      }
+      if constexpr (BIAS) {
+        const int lo = k1 - (span.start + row0 + 31), up = k1 + 31 - (span.start + row0);
+        if (up <= -s.reach || lo >= s.reach) {
+          float x = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x += ds[i];
+          x *= flip;
+          if (up <= -s.reach) far_back += x;
+          else far_on += x;
+        } else {
+          // Sums of the diagonals.  Lane j gets from row r the column (r - j) mod 32, whose distance is j or j - 32 on from the block's
+          // corner: two sums for each lane, in the order of the rows.
+          float on = 0.f, back = 0.f;
+          const int j = lane & 31;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int r = row_of(i) + 4 * hi;
+            const float x = __shfl(ds[i], ((r - j) & 31) + 32 * hi);
+            const float y = kFlip && row_of(i) & 1 ? -x : x;   // (column r - j: its sign is the row's times this lane's)
+            if (r >= j) on += y;
+            else back += y;
+          }
+          on = sum_of_pair(on) * flip, back = sum_of_pair(back) * flip;
+          const int d = lo + 31 + (hi ? j - 32 : j);
+          const float x = hi ? back : on;
+          if (d < -s.reach) far_back += x;
+          else if (d > s.reach) far_on += x;
+          else sums[d + s.reach] += x;
+          __builtin_amdgcn_wave_barrier();
+        }
+      }
+      range.fit(ds, acc);
+      Terms<T> terms;
+      terms.set(ds);
       reader.transposed(kt, 32 * u, terms, acc);
     }
   }
 
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int r = row0 + 32 * t + (lane & 31);
-    if (r >= rows) continue;
-    if (!limit[t]) zero(acc[t]);
-    const float f = s.scale * range[t].inverse() * flip;
+  if (r < rows) {
+    if (!limit) zero(acc);
+    const float f = s.scale * range.inverse() * flip;
     if (a.q_splits == 1) {
-      store_column<T, DP>(static_cast<elem *>(a.dq) + ((size_t(b) * s.q_len + query[t]) * s.heads + head[t]) * a.io_dim, acc[t], f, a.io_dim, hi,
+      store_column<T, DP>(static_cast<elem *>(a.dq) + ((size_t(b) * s.q_len + query) * s.heads + head) * a.io_dim, acc, f, a.io_dim, hi,
                           a.io_direct);
     } else {
       const size_t n = size_t(a.q_units) * rows;
-      store_partial<DP>(a.q_part + (split * n + size_t(unit) * rows + r) * DP, acc[t], f, hi);
+      store_partial<DP>(a.q_part + (split * n + size_t(unit) * rows + r) * DP, acc, f, hi);
     }
   }
   if constexpr (BIAS) {
@@ -271,13 +256,13 @@ __global__ __launch_bounds__(kBlock) void k_attn_dtable(BwdArgs a, float *dtable
   if (threadIdx.x == 0) dtable[size_t(e) * a.s.heads + h] = part[0];
 }
 
-template <class T, int DP, int QT, bool BIAS>
+template <class T, int DP, bool BIAS>
 int launch(const BwdArgs &a, const Bounds &bounds, float *dtable, hipStream_t s) {
   constexpr int KT = T::half ? 64 : 32;
   const size_t lds = 4 * Tile<T, DP>::bytes(KT) + (BIAS ? 5 * (2 * a.s.reach + 1) * sizeof(float) : 0);
   static std::atomic<unsigned long long> asked{0};
-  SGH_HIP_TRY(sgh_allow_lds(reinterpret_cast<const void *>(k_attn_dq<T, DP, QT, BIAS>), asked));
-  hipLaunchKernelGGL((k_attn_dq<T, DP, QT, BIAS>), dim3(a.q_tiles * a.q_units * a.q_splits), dim3(kBlock), lds, s, a, bounds);
+  SGH_HIP_TRY(sgh_allow_lds(reinterpret_cast<const void *>(k_attn_dq<T, DP, BIAS>), asked));
+  hipLaunchKernelGGL((k_attn_dq<T, DP, BIAS>), dim3(a.q_tiles * a.q_units * a.q_splits), dim3(kBlock), lds, s, a, bounds);
   SGH_LAUNCH_CHECK();
   if (a.q_splits > 1) {
     const size_t n = size_t(a.q_units) * a.s.q_len * a.pack, per = kBlock / (DP / 4);
@@ -292,8 +277,8 @@ int launch(const BwdArgs &a, const Bounds &bounds, float *dtable, hipStream_t s)
 }
 template <class T, int DP>
 int run_dim(const BwdArgs &a, const Bounds &bounds, float *dtable, hipStream_t s) {
-  if (a.s.buckets) return launch<T, DP, 1, true>(a, bounds, dtable, s);
-  return launch<T, DP, 1, false>(a, bounds, dtable, s);
+  if (a.s.buckets) return launch<T, DP, true>(a, bounds, dtable, s);
+  return launch<T, DP, false>(a, bounds, dtable, s);
 }
 
 }  // namespace

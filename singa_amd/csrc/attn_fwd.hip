@@ -31,12 +31,13 @@ struct FwdArgs {
 
 // m moves only when a row's maximum has grown by more than 2^8: the terms then stay within 2^8 of one, and o is rescaled seldom
 constexpr float kGrowth = 8.f;
+constexpr int kRows = 128, kFewRows = 32;   // queries of a block
 
-template <class T, int DP, int QT, bool BIAS>
+template <class T, int DP, bool BIAS>
 __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds) {
   typedef typename T::elem elem;
   typedef Tile<T, DP> L;
-  constexpr int KT = T::half ? 64 : 32, SUB = KT / 32, ND = DP / 32, WAVE_ROWS = 32 * QT, ROWS = 4 * WAVE_ROWS;
+  constexpr int KT = T::half ? 64 : 32, SUB = KT / 32, ND = DP / 32, ROWS = kRows;
   constexpr int TILE = L::bytes(KT);
   // binary16: terms from 2^-14 to 2^14 with all their bits
   constexpr float kShift = std::is_same<T, F16>::value ? 6.f : 0.f;
@@ -48,21 +49,15 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
   const int per_batch = s.heads / a.pack, b = unit / per_batch, head0 = int(unit % per_batch) * a.pack;
   const int kv = head0 / (s.heads / s.kv_heads);
   const Span span = span_of(s, b);
-  const int rows = s.q_len * a.pack, row0 = int(tile) * ROWS + wave * WAVE_ROWS;
+  const int rows = s.q_len * a.pack, row0 = int(tile) * ROWS + wave * 32;
 
-  // the lane's queries: keys [0, limit) are seen
-  int query[QT], head[QT], limit[QT], most = 0, least = 1 << 30;
-  cols_t<T, DP> qf[QT];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int r = row0 + 32 * t + (lane & 31);
-    query[t] = a.pack == 1 ? r : r / a.pack;
-    head[t] = a.pack == 1 ? head0 : head0 + r % a.pack;
-    limit[t] = r < rows && query[t] < span.q ? (s.causal ? min(span.k, max(span.start + query[t] + 1, 0)) : span.k) : 0;
-    most = max(most, limit[t]), least = min(least, limit[t]);
-    load_columns<T, DP>(qf[t], static_cast<const elem *>(a.q) + ((size_t(b) * s.q_len + query[t]) * s.heads + head[t]) * a.io_dim,
-                        limit[t] ? a.io_dim : 0, hi, a.io_direct);
-  }
+  // the lane's query: keys [0, limit) are seen
+  const int r = row0 + (lane & 31), query = a.pack == 1 ? r : r / a.pack, head = a.pack == 1 ? head0 : head0 + r % a.pack;
+  const int limit = r < rows && query < span.q ? (s.causal ? min(span.k, max(span.start + query + 1, 0)) : span.k) : 0;
+  int most = limit, least = limit;
+  cols_t<T, DP> qf;
+  load_columns<T, DP>(qf, static_cast<const elem *>(a.q) + ((size_t(b) * s.q_len + query) * s.heads + head) * a.io_dim,
+                      limit ? a.io_dim : 0, hi, a.io_direct);
   for (int m = 1; m < 32; m *= 2) most = max(most, __shfl_xor(most, m)), least = min(least, __shfl_xor(least, m));
   most = __builtin_amdgcn_readfirstlane(most), least = __builtin_amdgcn_readfirstlane(least);
   // of the whole block: the last row's
@@ -86,13 +81,9 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
   const elem *kp = static_cast<const elem *>(a.k) + (size_t(b) * s.k_len * s.kv_heads + kv) * s.dim;
   const elem *vp = static_cast<const elem *>(a.v) + (size_t(b) * s.k_len * s.kv_heads + kv) * s.dim;
 
-  f32x16 acc[QT][ND];
-  float m[QT], l[QT];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    zero(acc[t]);
-    m[t] = -3e38f, l[t] = 0.f;
-  }
+  f32x16 acc[ND];
+  zero(acc);
+  float m = -3e38f, l = 0.f;
   // (maxima are taken before the scale, which is therefore made positive: the products are multiplied by -1 or 0 first if it is not)
   const float factor = s.scale * kLog2e;
   const float turned = BIAS || factor > 0.f ? 1.f : factor < 0.f ? -1.f : 0.f, c = BIAS || factor != 0.f ? (BIAS ? factor : __builtin_fabsf(factor)) : 1.f;
@@ -109,7 +100,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
     if (k0 + KT < end) request(k0 + KT, slot ^ 1);
     const char *kt = lds + slot * 2 * TILE, *vt = kt + TILE;
     if (k0 >= most) continue;   // (no row of this wavefront sees any of them)
-    f32x16 p[SUB][QT];
+    f32x16 p[SUB];
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
       zero(p[u]);
@@ -120,93 +111,83 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
 #pragma unroll
       for (int u = 0; u < SUB; ++u)
 #pragma unroll
-        for (int t = 0; t < QT; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) p[u][t][i] *= turned;
+        for (int i = 0; i < 16; ++i) p[u][i] *= turned;
     }
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      float top = kNegInf;
-      if constexpr (BIAS) {
-        const int first = k0 - (span.start + query[t]);   // the distance of key k0
-        const int lo = k0 - (span.start + (row0 + 32 * t + 31) / a.pack), up = k0 + KT - 1 - (span.start + (row0 + 32 * t) / a.pack);
-        const float *mine = band + (head[t] - head0) * band_len + s.reach;
-        if (up <= -s.reach || lo >= s.reach) {   // far away the bias is one number
-          const float far = mine[up <= -s.reach ? -s.reach : s.reach];
-#pragma unroll
-          for (int u = 0; u < SUB; ++u)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) p[u][t][i] = __builtin_fmaf(p[u][t][i], c, far);
-        } else {
-#pragma unroll
-          for (int u = 0; u < SUB; ++u)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int d = first + 32 * u + row_of(i) + 4 * hi;
-              p[u][t][i] = __builtin_fmaf(p[u][t][i], c, mine[min(max(d, -s.reach), s.reach)]);
-            }
-        }
-      }
-      if (k0 + KT > least) {
-        const int left = limit[t] - k0 - 4 * hi;
+    float top = kNegInf;
+    if constexpr (BIAS) {
+      const int first = k0 - (span.start + query);   // the distance of key k0
+      const int lo = k0 - (span.start + (row0 + 31) / a.pack), up = k0 + KT - 1 - (span.start + row0 / a.pack);
+      const float *mine = band + (head - head0) * band_len + s.reach;
+      if (up <= -s.reach || lo >= s.reach) {   // far away the bias is one number
+        const float far = mine[up <= -s.reach ? -s.reach : s.reach];
 #pragma unroll
         for (int u = 0; u < SUB; ++u)
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (32 * u + row_of(i) >= left) p[u][t][i] = kNegInf;
+          for (int i = 0; i < 16; ++i) p[u][i] = __builtin_fmaf(p[u][i], c, far);
+      } else {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int d = first + 32 * u + row_of(i) + 4 * hi;
+            p[u][i] = __builtin_fmaf(p[u][i], c, mine[min(max(d, -s.reach), s.reach)]);
+          }
       }
+    }
+    if (k0 + KT > least) {
+      const int left = limit - k0 - 4 * hi;
 #pragma unroll
       for (int u = 0; u < SUB; ++u)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, p[u][t][i]);
-      top = max_of_pair(top);
-      if (!BIAS) top *= c;
-      if (__ballot(top > m[t] + kGrowth)) {
-        const float now = fmaxf(m[t], top), f = __builtin_amdgcn_exp2f(m[t] - now);
-        m[t] = now, l[t] *= f;
-#pragma unroll
-        for (int n = 0; n < ND; ++n)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[t][n][i] *= f;
-      }
-      const float from = m[t] - kShift;
-      float sum = 0.f;
-#pragma unroll
-      for (int u = 0; u < SUB; ++u)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          p[u][t][i] = __builtin_amdgcn_exp2f(BIAS ? p[u][t][i] - from : __builtin_fmaf(p[u][t][i], c, -from));
-          sum += p[u][t][i];
-        }
-      l[t] += sum;
+        for (int i = 0; i < 16; ++i)
+          if (32 * u + row_of(i) >= left) p[u][i] = kNegInf;
     }
 #pragma unroll
-    for (int u = 0; u < SUB; ++u) {
-      Terms<T> terms[QT];
+    for (int u = 0; u < SUB; ++u)
 #pragma unroll
-      for (int t = 0; t < QT; ++t) terms[t].set(p[u][t]);
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, p[u][i]);
+    top = max_of_pair(top);
+    if (!BIAS) top *= c;
+    if (__ballot(top > m + kGrowth)) {
+      const float now = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - now);
+      m = now, l *= f;
+#pragma unroll
+      for (int n = 0; n < ND; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[n][i] *= f;
+    }
+    const float from = m - kShift;
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        p[u][i] = __builtin_amdgcn_exp2f(BIAS ? p[u][i] - from : __builtin_fmaf(p[u][i], c, -from));
+        sum += p[u][i];
+      }
+    l += sum;
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+      Terms<T> terms;
+      terms.set(p[u]);
       reader.transposed(vt, 32 * u, terms, acc);
     }
   }
 
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int r = row0 + 32 * t + (lane & 31);
-    if (r >= rows) continue;
-    const float sum = sum_of_pair(l[t]);
-    // (a row that sees nothing has o = 0 and the logarithm of 0)
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    if (sum == 0.f) zero(acc[t]);
-    const float lse = sum == 0.f ? kNegInf : (m[t] - kShift + __builtin_amdgcn_logf(sum)) * kLn2;
-    if (a.splits == 1) {
-      store_column<T, DP>(static_cast<elem *>(a.o) + ((size_t(b) * s.q_len + query[t]) * s.heads + head[t]) * a.io_dim, acc[t], inv, a.io_dim, hi,
-                          a.io_direct);
-      if (hi == 0) a.lse[(size_t(b) * s.heads + head[t]) * s.q_len + query[t]] = lse;
-    } else {
-      const size_t n = size_t(a.units) * rows, at = split * n + size_t(unit) * rows + r;
-      store_partial<DP>(a.part + at * DP, acc[t], inv, hi);
-      if (hi == 0) a.part[a.splits * n * DP + at] = lse;
-    }
+  if (r >= rows) return;
+  const float sum = sum_of_pair(l);
+  // (a row that sees nothing has o = 0 and the logarithm of 0)
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  if (sum == 0.f) zero(acc);
+  const float lse = sum == 0.f ? kNegInf : (m - kShift + __builtin_amdgcn_logf(sum)) * kLn2;
+  if (a.splits == 1) {
+    store_column<T, DP>(static_cast<elem *>(a.o) + ((size_t(b) * s.q_len + query) * s.heads + head) * a.io_dim, acc, inv, a.io_dim, hi,
+                        a.io_direct);
+    if (hi == 0) a.lse[(size_t(b) * s.heads + head) * s.q_len + query] = lse;
+  } else {
+    const size_t n = size_t(a.units) * rows, at = split * n + size_t(unit) * rows + r;
+    store_partial<DP>(a.part + at * DP, acc, inv, hi);
+    if (hi == 0) a.part[a.splits * n * DP + at] = lse;
   }
 }
 
@@ -240,8 +221,8 @@ __global__ __launch_bounds__(kBlock, 1) void k_attn_few(FwdArgs a, Bounds bounds
   const Span span = span_of(s, b);
   const int rows = s.q_len * a.pack, r = lane & 31, query = r / a.pack, head = head0 + r % a.pack;
   const int limit = r < rows && query < span.q ? (s.causal ? min(span.k, max(span.start + query + 1, 0)) : span.k) : 0;
-  cols_t<T, DP> qf[1];
-  load_columns<T, DP>(qf[0], static_cast<const elem *>(a.q) + ((size_t(b) * s.q_len + query) * s.heads + head) * a.io_dim, limit ? a.io_dim : 0, hi,
+  cols_t<T, DP> qf;
+  load_columns<T, DP>(qf, static_cast<const elem *>(a.q) + ((size_t(b) * s.q_len + query) * s.heads + head) * a.io_dim, limit ? a.io_dim : 0, hi,
                       a.io_direct);
   int most = limit, least = r < rows ? limit : 1 << 30;
   for (int m = 1; m < 32; m *= 2) most = max(most, __shfl_xor(most, m)), least = min(least, __shfl_xor(least, m));
@@ -261,8 +242,8 @@ __global__ __launch_bounds__(kBlock, 1) void k_attn_few(FwdArgs a, Bounds bounds
   const elem *kp = static_cast<const elem *>(a.k) + (size_t(b) * s.k_len * s.kv_heads + kv) * s.dim;
   const elem *vp = static_cast<const elem *>(a.v) + (size_t(b) * s.k_len * s.kv_heads + kv) * s.dim;
   char *const mine = lds + wave * F::SLOTS * F::WAVE;
-  f32x16 acc[1][ND];
-  zero(acc[0]);
+  f32x16 acc[ND];
+  zero(acc);
   float m = -3e38f, l = 0.f;
   const float c = s.scale * kLog2e;
   const Reader<T, DP> reader(lane);
@@ -284,7 +265,7 @@ __global__ __launch_bounds__(kBlock, 1) void k_attn_few(FwdArgs a, Bounds bounds
     }
     const char *kt = mine + slot * F::WAVE, *vt = kt + F::TILE;
     slot = slot == F::SLOTS - 1 ? 0 : slot + 1;
-    f32x16 p[1];
+    f32x16 p;
     zero(p);
     reader.rows(kt, 0, qf, p);
     if constexpr (F::ONE) {
@@ -296,19 +277,19 @@ __global__ __launch_bounds__(kBlock, 1) void k_attn_few(FwdArgs a, Bounds bounds
       const float *centre = band + (r < rows ? head - head0 : 0) * band_len + s.reach;
       const int first = k0 - (span.start + query) + 4 * hi;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) p[0][i] = __builtin_fmaf(p[0][i], c, centre[min(max(first + row_of(i), -s.reach), s.reach)]);
+      for (int i = 0; i < 16; ++i) p[i] = __builtin_fmaf(p[i], c, centre[min(max(first + row_of(i), -s.reach), s.reach)]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) p[0][i] *= c;
+      for (int i = 0; i < 16; ++i) p[i] *= c;
     }
     if (k0 + F::KT > least) {
       const int left = limit - k0 - 4 * hi;
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (row_of(i) >= left) p[0][i] = kNegInf;
+        if (row_of(i) >= left) p[i] = kNegInf;
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) top = fmaxf(top, p[0][i]);
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, p[i]);
     top = max_of_pair(top);
     if (__ballot(top > m + kGrowth)) {
       const float now = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - now);
@@ -316,16 +297,16 @@ __global__ __launch_bounds__(kBlock, 1) void k_attn_few(FwdArgs a, Bounds bounds
 #pragma unroll
       for (int n = 0; n < ND; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[0][n][i] *= f;
+        for (int i = 0; i < 16; ++i) acc[n][i] *= f;
     }
     const float from = m - kShift;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      p[0][i] = __builtin_amdgcn_exp2f(p[0][i] - from);
-      l += p[0][i];
+      p[i] = __builtin_amdgcn_exp2f(p[i] - from);
+      l += p[i];
     }
-    Terms<T> terms[1];
-    terms[0].set(p[0]);
+    Terms<T> terms;
+    terms.set(p);
     if constexpr (F::ONE) own_tiles_arrive(more ? loads : 0);
     reader.transposed(vt, 0, terms, acc);
     if constexpr (F::ONE) {
@@ -338,7 +319,7 @@ __global__ __launch_bounds__(kBlock, 1) void k_attn_few(FwdArgs a, Bounds bounds
   float *const results = reinterpret_cast<float *>(lds), *const tops = results + 4 * 32 * F::ROW, *const totals = tops + 4 * 32;
   l = sum_of_pair(l);
   __syncthreads();
-  store_partial<DP>(results + (wave * 32 + r) * F::ROW, acc[0], 1.f, hi);
+  store_partial<DP>(results + (wave * 32 + r) * F::ROW, acc, 1.f, hi);
   if (hi == 0) tops[wave * 32 + r] = m, totals[wave * 32 + r] = l;
   __syncthreads();
   for (int i = tid; i < rows * (DP / 4); i += kBlock) {
@@ -424,12 +405,12 @@ int join(const FwdArgs &a, hipStream_t s) {
   }
   return SGH_OK;
 }
-template <class T, int DP, int QT, bool BIAS>
+template <class T, int DP, bool BIAS>
 int launch(const FwdArgs &a, const Bounds &bounds, size_t band, hipStream_t s) {
   static std::atomic<unsigned long long> asked{0};
   constexpr int KT = T::half ? 64 : 32;
-  SGH_HIP_TRY(sgh_allow_lds(reinterpret_cast<const void *>(k_attn_fwd<T, DP, QT, BIAS>), asked));
-  SGH_LAUNCH_TIMED((k_attn_fwd<T, DP, QT, BIAS>), dim3(a.tiles * a.units * a.splits), dim3(kBlock), (4 * Tile<T, DP>::bytes(KT)) + band, s, a, bounds);
+  SGH_HIP_TRY(sgh_allow_lds(reinterpret_cast<const void *>(k_attn_fwd<T, DP, BIAS>), asked));
+  SGH_LAUNCH_TIMED((k_attn_fwd<T, DP, BIAS>), dim3(a.tiles * a.units * a.splits), dim3(kBlock), (4 * Tile<T, DP>::bytes(KT)) + band, s, a, bounds);
   SGH_LAUNCH_CHECK();
   return join<T, DP>(a, s);
 }
@@ -451,7 +432,6 @@ struct Plan {
   bool pad;     // keys and values of rows that are not whole chunks are copied first
   size_t part, ws;
 };
-constexpr int kRows = 128, kFewRows = 32;   // of a block
 // (elem_bytes: fp32 never needs less of the workspace than the others)
 Plan plan_of(const sgh_attn_geom *g, size_t elem_bytes) {
   Plan p;
@@ -495,8 +475,8 @@ int run_dim(const FwdArgs &a, const Bounds &bounds, bool few, hipStream_t s) {
     if (a.s.buckets) return launch_few<T, DP, true>(a, bounds, band, s);
     return launch_few<T, DP, false>(a, bounds, band, s);
   }
-  if (a.s.buckets) return launch<T, DP, 1, true>(a, bounds, band, s);
-  return launch<T, DP, 1, false>(a, bounds, band, s);
+  if (a.s.buckets) return launch<T, DP, true>(a, bounds, band, s);
+  return launch<T, DP, false>(a, bounds, band, s);
 }
 
 template <class T>
