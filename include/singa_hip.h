@@ -872,7 +872,8 @@ SGH_API int sgh_attn_geom_init(sgh_attn_geom *g, int batch, int q_len, int k_len
  * backward pass needs.  q_lengths, k_lengths (int32, [batch], taken into [0, q_len] and [0, k_len]): how many rows of each sequence count, NULL: all.
  * Rows behind them are not looked at; their results, and those of a query that sees no key, are 0 (lse: -inf).  q_starts (int32, [batch], within
  * +-2^30): see above.  What lies behind the lengths, or under a causal mask behind the position of the last query, reaches nothing, whatever it
- * is.  Among the keys that some query of a sequence sees, an infinite or NaN value may reach that sequence's other queries.
+ * is.  Among the keys that some query of a sequence sees, and backwards among its queries, an infinite or NaN value may reach that sequence's other
+ * results.  A bias of -inf, or below -2.1e38, hides its keys from those queries.
  * _bwd: the gradients of q, k, v and of the table (dtable, with a table only) from dout, the gradient of o, and the o and lse of the same
  * arguments.  The probabilities are computed anew.  Every sum has one order: the same bits every time.  The terms p and ds of the products
  * over the keys and queries are rounded to the tensors' type (binary16: scaled into its range); statistics, sums and the table's

@@ -466,3 +466,55 @@ def test_no_queries_over_a_cache(dev, t, buckets):
     assert o.shape() == dq.shape() == [2, 0, 4, 24] and lse.shape() == [2, 4, 0]
     for x in (dk, dv) + ((dtable,) if buckets else ()):
         assert not x.to_numpy().any()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("low", [-np.inf, np.finfo(np.float32).min, -2.5e38, -2.2e38])
+def test_a_bias_that_hides_keys(dev, t, low):
+    """Buckets of -inf, and of values from fp32's lowest on up to -2.1e38 (-3e38 in units of log2), which hide keys alike: both passes, with queries
+    that see nothing else.  Their results and gradients are 0."""
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(1)
+    for causal, (sq, sk, h, g, d) in ((False, (90, 90, 2, 2, 16)), (True, (70, 70, 4, 2, 64)), (True, (33, 33, 2, 1, 128))):
+        a = O.Attn(causal, buckets=8, max_distance=16)
+        q, do, k, v = (stored(t, r.standard_normal((2, n, c, d))) for n, c in ((sq, h), (sq, h), (sk, g), (sk, g)))
+        table = stored("f32", r.standard_normal((8, h)))
+        table[0, 0] = table[3, 1] = table[6, 1] = -np.inf   # (a causal first query sees the first key only, of bucket 0)
+        lengths = ((sq, sq - 3), (sk, 1), None)
+        device = np.where(np.isinf(table), np.float32(low), table.astype(np.float32))
+        dq_, dk_, dv_, ddo, dt = (upload(singa, dev, kind, x) for kind, x in ((t, q), (t, k), (t, v), (t, do), ("f32", device)))
+        dl = dict(q_lengths=ints(singa, dev, lengths[0]), k_lengths=ints(singa, dev, lengths[1]))
+        H = handle(singa, dq_, dk_, a)
+        o, lse = singa.AttentionForward(H, dq_, dk_, dv_, dt, **dl)
+        grads = [x.to_numpy() for x in singa.AttentionBackward(H, ddo, dq_, dk_, dv_, o, lse, dt, **dl)]
+        assert all(np.isfinite(x).all() for x in grads)
+        if causal:   # the first query of head 0 has no key left
+            assert (lse.to_numpy()[:, 0, 0] == -np.inf).all() and not o.to_numpy()[:, 0, 0].any() and not grads[0][:, 0, 0].any()
+        assert not grads[3][np.isinf(table)].any()
+        check(singa, dev, t, a, 2, sq, sk, h, g, d, case=(q, k, v, do, table), lengths=lengths)
+        hidden = upload(singa, dev, "f32", table)   # the same bits as of -inf
+        again = singa.AttentionForward(H, dq_, dk_, dv_, hidden, **dl)
+        for x, y in zip((o, lse), again):
+            assert np.array_equal(x.to_numpy(), y.to_numpy())
+        for x, y in zip(grads, singa.AttentionBackward(H, ddo, dq_, dk_, dv_, *again, hidden, **dl)):
+            assert np.array_equal(x, y.to_numpy())
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_few_queries_and_hidden_keys(dev, t):
+    """The form for few queries, its keys in parts: a bias of fp32's lowest value for all keys but those of one bucket, and for all."""
+    from singa_amd import singa_wrap as singa
+    r = np.random.default_rng(2)
+    a = O.Attn(True, buckets=8, max_distance=16, bidirectional=False)
+    q, k, v = (stored(t, r.standard_normal(s)) for s in ((2, 1, 4, 64), (2, 1500, 2, 64), (2, 1500, 2, 64)))
+    for some in (True, False):
+        table = np.full((8, 4), np.finfo(np.float32).min, np.float32)
+        if some:
+            table[2] = 0.5   # the key two places back
+        dq_, dk_, dv_, dt = upload(singa, dev, t, q), upload(singa, dev, t, k), upload(singa, dev, t, v), upload(singa, dev, "f32", table)
+        o, lse = singa.AttentionForward(handle(singa, dq_, dk_, a), dq_, dk_, dv_, dt)
+        if some:
+            want = np.repeat(v[:, 1497:1498], 2, 2)
+            close(o.to_numpy(), want, (HALF[t] * 2 + 4 * U) * np.abs(want) + TINY[t], "o")   # (p is 1, o and p v are rounded)
+        else:
+            assert not o.to_numpy().any() and (lse.to_numpy() == -np.inf).all()
