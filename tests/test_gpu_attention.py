@@ -518,3 +518,92 @@ def test_few_queries_and_hidden_keys(dev, t):
             close(o.to_numpy(), want, (HALF[t] * 2 + 4 * U) * np.abs(want) + TINY[t], "o")   # (p is 1, o and p v are rounded)
         else:
             assert not o.to_numpy().any() and (lse.to_numpy() == -np.inf).all()
+
+
+def _part(singa, dev, t, at, shape):
+    """`shape` elements of a bfloat16 tensor from the element `at` on, as a view over its memory."""
+    return singa.from_device_pointer(t.ptr + at * 2, shape, dev, singa.kBFloat16, keepalive=t)
+
+
+def _zeros(singa, dev, shape):
+    t = singa.Tensor(shape, dev, singa.kBFloat16)
+    t.SetFloatValue(0.0)
+    return t
+
+
+def test_gradients_of_a_long_cache_with_offsets_beyond_32_bits(dev):
+    """Keys of 2^32 bytes for a sequence: the last sequence's last rows are not zeros, nor are the gradients there."""
+    from singa_amd import singa_wrap as singa
+    b, sk, g, d, rows, scale = 2, 1 << 20, 16, 128, 300, 128 ** -0.5
+    r = np.random.default_rng(9)
+    k = _zeros(singa, dev, (b, sk, g, d))
+    tail = stored("bf16", r.standard_normal((rows, g, d)))
+    _part(singa, dev, k, k.Size() - tail.size, tail.shape).CopyHalfDataFromHostPtr(singa.float_to_bf16_bits(tail))
+    q, do = (stored("bf16", r.standard_normal((b, 1, g, d))) for _ in range(2))
+    dq_, ddo = upload(singa, dev, "bf16", q), upload(singa, dev, "bf16", do)
+    H = singa.AttentionHandle(dq_, k)
+    o, lse = singa.AttentionForward(H, dq_, k, k)
+    dq, dk, dv, _ = singa.AttentionBackward(H, ddo, dq_, k, k, o, lse)
+    o, lse = o.to_numpy().astype(np.float64), lse.to_numpy().astype(np.float64)[:, :, 0]
+    read = lambda t, at, shape: _part(singa, dev, t, at, shape).to_numpy().astype(np.float64)
+    row, half = g * d, HALF["bf16"]
+    # a probability is off by the product's (d + 4) u, 4 u of the logarithm (14) and of the score (below 30): E; then as in the module's description
+    E = (d + 4 + 4 * 44 + 8) * U
+    gap_size = (np.abs(do[1, 0]) * np.abs(o[1, 0])).sum(1)
+    s = np.einsum("hd,rhd->rh", q[1, 0], tail) * scale
+    size = np.einsum("hd,rhd->rh", np.abs(q[1, 0]), np.abs(tail)) * scale
+    p = np.exp(s - lse[1])
+    gap = np.einsum("hd,rhd->rh", do[1, 0], tail) - (do[1, 0] * o[1, 0]).sum(1)
+    off = p * (np.abs(gap) * E * (1 + size) + (d + 4) * U * (np.einsum("hd,rhd->rh", np.abs(do[1, 0]), np.abs(tail)) + gap_size))
+    want = p[:, :, None] * do[1, 0]
+    close(read(dv, dv.Size() - tail.size, tail.shape), want, (2 * half + E * (1 + size[:, :, None])) * np.abs(want) * 1.01, "dv")
+    want = scale * (p * gap)[:, :, None] * q[1, 0]
+    close(read(dk, dk.Size() - tail.size, tail.shape), want, (2 * half * np.abs(want) + scale * off[:, :, None] * np.abs(q[1, 0])) * 1.01, "dk")
+    want = scale * np.einsum("rh,rhd->hd", p * gap, tail)
+    room = scale * np.einsum("rh,rhd->hd", off + (half + 400 * U) * np.abs(p * gap), np.abs(tail)) + half * np.abs(want)
+    close(dq.to_numpy()[1, 0], want, room * 1.01, "dq")
+    # keys of zeros on both sides of where a sequence ends: a probability of e^-lse, do . v of 0
+    for i, at in ((0, 0), (0, (sk - 5) * row), (1, sk * row), (1, (2 * sk - rows - 5) * row)):
+        each = np.exp(-lse[i])[:, None]
+        want = np.broadcast_to(each * do[i, 0], (5, g, d))
+        close(read(dv, at, (5, g, d)), want, (2 * half + E) * np.abs(want) * 1.01, "dv of zeros")
+        want = np.broadcast_to(-scale * each * (do[i, 0] * o[i, 0]).sum(1)[:, None] * q[i, 0], (5, g, d))
+        room = 2 * half * np.abs(want) + scale * each * (E + (d + 4) * U) * (np.abs(do[i, 0]) * np.abs(o[i, 0])).sum(1)[:, None] * np.abs(q[i, 0])
+        close(read(dk, at, (5, g, d)), want, room * 1.01, "dk of zeros")
+    assert not dq.to_numpy()[0].any()
+
+
+def test_gradients_of_long_sequences_with_offsets_beyond_32_bits(dev):
+    """Queries of 2^32 bytes for a sequence: only the last sequence's last rows are not zeros."""
+    from singa_amd import singa_wrap as singa
+    b, sq, sk, h, d, rows = 2, 1 << 20, 40, 16, 128, 300
+    r = np.random.default_rng(10)
+    q, do = (stored("bf16", r.standard_normal((1, rows, h, d))) for _ in range(2))
+    k, v = (stored("bf16", r.standard_normal((b, sk, h, d))) for _ in range(2))
+    dq_, ddo = _zeros(singa, dev, (b, sq, h, d)), _zeros(singa, dev, (b, sq, h, d))
+    for t, x in ((dq_, q), (ddo, do)):
+        _part(singa, dev, t, t.Size() - x.size, x.shape).CopyHalfDataFromHostPtr(singa.float_to_bf16_bits(x))
+    dk_, dv_ = upload(singa, dev, "bf16", k), upload(singa, dev, "bf16", v)
+    H = singa.AttentionHandle(dq_, dk_)
+    o, lse = singa.AttentionForward(H, dq_, dk_, dv_)
+    dq, dk, dv, _ = singa.AttentionBackward(H, ddo, dq_, dk_, dv_, o, lse)
+    read = lambda t, at, shape: _part(singa, dev, t, at, shape).to_numpy().astype(np.float64)
+    tail_o = read(o, o.Size() - q.size, q.shape)
+    a, K, V = O.Attn(), k[1:], v[1:]
+    wo, wl = O.attention(a, q, K, V)
+    eo, el, eq, ek, ev, _ = bounds("bf16", a, do, q, K, V, tail_o, None, None, None, None)
+    rounded = lambda bound, want: bound * 1.01 + HALF["bf16"] * np.abs(want) * 1.01
+    close(tail_o, wo, rounded(eo, wo), "o")
+    tail_lse = lse.to_numpy()[1:, :, sq - rows:]
+    close(tail_lse, wl, el * 1.01, "lse")
+    want = O.attention_bwd(a, do, q, K, V, tail_o, tail_lse.astype(np.float64))
+    close(read(dq, dq.Size() - q.size, q.shape), want[0], rounded(eq, want[0]), "dq")
+    for name, x, w, e in (("dk", dk, want[1], ek), ("dv", dv, want[2], ev)):   # (rows without a gradient add zeros)
+        x = x.to_numpy()
+        close(x[1:], w, rounded(e, w), name)
+        assert not x[0].any(), name
+    for at in (0, (sq - 3) * h * d, sq * h * d, (2 * sq - rows - 3) * h * d):
+        assert not read(dq, at, (3, h, d)).any()
+        i = at // (sq * h * d)
+        mean = np.broadcast_to(v[i].mean(0), (3, h, d))   # a query of zeros sees all keys alike
+        close(read(o, at, (3, h, d)), mean, (2 * HALF["bf16"] + 200 * U) * np.abs(v[i]).mean(0) * 1.01, "o of zeros")
