@@ -221,3 +221,41 @@ def test_no_rows_and_a_gate(dev, t, gates):
     assert y.shape() == n.shape() == dx.shape() == dh.shape() == [0, 12] and stats.shape() == [0, 2] and dgate.shape() == [gates, 12]
     for g in (dpost, dgate, dpre):
         assert not g.to_numpy().any()
+
+
+@pytest.mark.parametrize("dim,gates", [(16384, 1), (4096, 2), (1000, 0)])
+def test_tensors_of_more_than_32_bits(dev, dim, gates):
+    """More than 2^32 values, zeros but for the last row: the same bits as of that row alone, zeros where a shorter offset would have put them."""
+    from singa_amd import singa_wrap as singa
+    rows = ((1 << 32) // dim + 300) // 4 * 4
+    r = np.random.default_rng(dim)
+    f = lambda t, row, n=1: singa.from_device_pointer(t.ptr + row * dim * 2, (n, dim), dev, singa.kBFloat16, keepalive=t)
+    kept = [stored("bf16", r.standard_normal((1, dim))) for _ in range(4)]
+    large = []
+    for x in kept:
+        t = singa.Tensor((rows, dim), dev, singa.kBFloat16)
+        t.SetFloatValue(0.0)
+        f(t, rows - 1).CopyHalfDataFromHostPtr(singa.float_to_bf16_bits(x))
+        large.append(t)
+    post, pre = (upload(singa, dev, "f32", 1 + 0.2 * r.standard_normal(dim)) for _ in range(2))
+    gate = stored("bf16", r.standard_normal((max(gates, 1), dim)))
+
+    def run(tensors, gate):
+        x, h, dy, dn = tensors
+        given = dict(post=post, gate=None if gate is None else upload(singa, dev, "bf16", gate), scale=0.5, pre=pre)
+        y, n, stats = singa.ResidualNormForward(x, h, **given)
+        return [y, n, stats, *singa.ResidualNormBackward(dy, dn, y, stats, h, **given)]
+
+    got = run(large, gate if gates else None)
+    want = run([upload(singa, dev, "bf16", x) for x in kept], gate[-1:] if gates else None)
+    for name, x, w in zip(("y", "n", "stats", "dx", "dh", "dpost", "dgate", "dpre"), got, want):
+        if name in ("y", "n", "dx", "dh"):
+            assert np.array_equal(f(x, rows - 1).to_numpy(), w.to_numpy()), name
+            for row in (0, rows - 2, rows - 1 - (1 << 31) // dim, rows - 2 - (1 << 31) // dim, rows - 1 - (1 << 32) // dim, rows - 2 - (1 << 32) // dim):
+                assert not f(x, row).to_numpy().any(), (name, row)
+        elif name == "stats":
+            x = x.to_numpy()
+            assert np.array_equal(x[-1], w.to_numpy()[0]) and (x[:-1] == x[0]).all()
+        elif w is not None:   # (a sum of one row's and zeros)
+            assert np.array_equal(x.to_numpy()[-1:] if name == "dgate" else x.to_numpy(), w.to_numpy()), name
+            assert name != "dgate" or not x.to_numpy()[:-1].any()
