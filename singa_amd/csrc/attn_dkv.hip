@@ -3,10 +3,10 @@
 //   dv = sum p do,  dk = scale sum ds q.
 // Each sum is one wavefront's, in the order of the heads and queries: the same bits every time, and nothing is added in memory.
 //
-// Four products of a tile (the scores and do . v once more, then dv and dk), so that the matrix units bound it: busy 56 % with bfloat16 heads
-// of 128 (2 x 16 heads, 8192 places, causal: 1000 to 1070 us), 60 % with fp32 heads of 64 (8 x 8 heads, 512 places: 57 us).  Scores and do . v
-// once for both halves would need dq added up in memory, in an order that changes, or a dq for each block of keys.  Two wavefronts to a
-// group of keys, each with half the queries, were slower.
+// Four products of a tile: the scores and do . v once more, then dv and dk.  Bound by their chain with the exponentials between them, in two
+// wavefronts to a SIMD: matrix units 56 % busy with bfloat16 heads of 128 (2 x 16 heads, 8192 places, causal: 1000 to 1070 us), 59 % with fp32 heads of
+// 64 (8 x 8 heads, 512 places: 58 us).  Scores and do . v once for both halves would need dq added up in memory, in an order that changes, or a dq for
+// each block of keys.  Two wavefronts to a group of keys, each with half the queries, were slower.
 #include "attn_bwd.h"
 
 namespace {
@@ -316,11 +316,11 @@ int backward(const sgh_attn_geom *g, const void *dout, const void *q, const void
   Plan p = plan_of(g, e);
   if (p.bytes() && (!workspace || ws_bytes < p.bytes())) return SGH_EWORKSPACE;
   if (p.bytes() && !sgh_aligned16(workspace)) return SGH_EINVAL;
-  const Extent results[] = {{dq, qn}, {dk, kn}, {dv, kn}, {dtable, tn}, {workspace, p.bytes()}};
-  const Extent arguments[] = {{dout, qn}, {q, qn}, {k, kn}, {v, kn}, {o, qn}, {lse, bq * 4}, {table, tn},
+  const sgh_extent results[] = {{dq, qn}, {dk, kn}, {dv, kn}, {dtable, tn}, {workspace, p.bytes()}};
+  const sgh_extent arguments[] = {{dout, qn}, {q, qn}, {k, kn}, {v, kn}, {o, qn}, {lse, bq * 4}, {table, tn},
                               {q_lengths, q_lengths ? size_t(g->batch) * 4 : 0}, {k_lengths, k_lengths ? size_t(g->batch) * 4 : 0},
                               {q_starts, q_starts ? size_t(g->batch) * 4 : 0}};
-  if (any_overlap(results, arguments)) return SGH_EINVAL;
+  if (sgh_any_overlap(results, arguments)) return SGH_EINVAL;
   BwdArgs &a = p.a;
   a.s = shape_of(g, table, q_lengths, k_lengths, q_starts);
   a.q = q, a.k = k, a.v = v, a.o = o, a.dout = dout, a.lse = lse, a.dq = dq, a.dk = dk, a.dv = dv;

@@ -3,9 +3,9 @@
 // sums:  p = e^(s - lse),  ds = p (do . v - delta),  dq = scale sum ds k.
 //
 // As the forward pass, with three products for its two: a tile of values is read by rows only, a tile of keys by rows and by columns.  Bound by
-// the matrix units and what stands between their products (busy 46 % with bfloat16 heads of 128, 54 % with fp32 heads of 64): bfloat16, 2 x 16
-// heads of 128, 8192 places, causal: 760 to 890 us as the clock is; fp32, 8 x 8 heads of 64, 512 places: 63 us.  A bias adds a look-up for each
-// pair near the diagonal and the buckets' sums: bfloat16, 8 x 12 heads of 64, 1024 places: 92 us.
+// the chain of products and exponentials in each wavefront, two to a SIMD (matrix units 61 % busy with bfloat16 heads of 128, 53 % with fp32 heads of
+// 64): bfloat16, 2 x 16 heads of 128, 8192 places, causal: 727 us; fp32, 8 x 8 heads of 64, 512 places: 64 us.  A bias adds a look-up for each
+// pair near the diagonal and the buckets' sums: bfloat16, 8 x 12 heads of 64, 1024 places: 91 us.
 #include "attn_bwd.h"
 
 namespace {

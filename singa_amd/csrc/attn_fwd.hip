@@ -5,9 +5,10 @@
 //
 // A block is four wavefronts of 32 queries; tiles of 64 keys and values (fp32: 32) lie twice in LDS, one pair being filled while the other is
 // used.  With one query to a lane a row's maximum and sum cost one exchange of two lanes, and the probabilities are where the product with the
-// values wants them; 64 queries to a wavefront left no registers for a second one on its SIMD.  Bound by the matrix units (43 % busy) and, in
-// the same wavefronts, the exponentials and conversions between their products: bfloat16, 4 x 32 heads of 128 over 4096 places, groups of 4,
-// causal, ragged: 387 to 409 us, 830 to 880 TFLOP/s of the pairs that are seen.
+// values wants them; 64 queries to a wavefront left no registers for a second one on its SIMD.  Bound by the chain in each wavefront,
+// product, exponentials and conversions, product: with two of them on a SIMD the matrix units are 43 % busy.  bfloat16, 4 x 32 heads of 128 over 4096
+// places, groups of 4, causal, ragged: 387 to 409 us, 830 to 880 TFLOP/s of the pairs that are seen; fp32, 4 x 16 heads of 128 over 2048 places, causal:
+// 875 us, 78 TFLOP/s.
 #include "attn.h"
 #include "attn_run.h"
 
@@ -193,8 +194,8 @@ __global__ __launch_bounds__(kBlock, 2) void k_attn_fwd(FwdArgs a, Bounds bounds
 
 // Few queries (32 with the heads of a group): the wavefronts of a block share the keys, 32 at a time, each with tiles of its own in LDS that
 // nobody else waits for, and join what they have in the end.  Bound by the way of keys and values from memory; in the kernel above one wavefront
-// would have all the products, and three wait.  (16 sequences of up to 16384 places, 4 heads of keys of 64, binary16, bias: 75 -> 56 us, and
-// its join 4; fp32, 5 x 8 heads of keys of 128, 16180 places: 216 -> 126, 5.2 TB/s.)
+// would have all the products, and three wait.  (16 sequences of up to 16384 places, 4 heads of keys of 64, binary16, bias: 52 us, and
+// its join 5; fp32, 5 x 8 heads of keys of 128, 16180 places: 216 -> 126, 5.2 TB/s.)
 template <class T, int DP>
 struct Few {
   static constexpr int KT = 32, TILE = Tile<T, DP>::bytes(KT), WAVE = 2 * TILE;   // a wavefront's keys and values
@@ -491,11 +492,11 @@ int forward(const sgh_attn_geom *g, const void *q, const void *k, const void *v,
   const Plan p = plan_of(g, e);
   if (p.ws && (!workspace || ws_bytes < p.ws)) return SGH_EWORKSPACE;
   if (p.ws && !sgh_aligned16(workspace)) return SGH_EINVAL;
-  const Extent results[] = {{o, qn}, {lse, bq * 4}, {workspace, p.ws}};
-  const Extent arguments[] = {{q, qn}, {k, kn}, {v, kn}, {table, g->buckets ? size_t(g->buckets) * g->heads * 4 : 0},
+  const sgh_extent results[] = {{o, qn}, {lse, bq * 4}, {workspace, p.ws}};
+  const sgh_extent arguments[] = {{q, qn}, {k, kn}, {v, kn}, {table, g->buckets ? size_t(g->buckets) * g->heads * 4 : 0},
                               {q_lengths, q_lengths ? size_t(g->batch) * 4 : 0}, {k_lengths, k_lengths ? size_t(g->batch) * 4 : 0},
                               {q_starts, q_starts ? size_t(g->batch) * 4 : 0}};
-  if (any_overlap(results, arguments)) return SGH_EINVAL;
+  if (sgh_any_overlap(results, arguments)) return SGH_EINVAL;
   FwdArgs a;
   a.s = shape_of(g, table, q_lengths, k_lengths, q_starts);
   a.q = q, a.k = k, a.v = v, a.o = o, a.lse = lse, a.part = static_cast<float *>(workspace);

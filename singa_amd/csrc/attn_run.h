@@ -1,4 +1,4 @@
-// Host side that the attention's entry points share: checks of a geometry and of what may overlap, arguments of the kernels.
+// Host side that the attention's entry points share: checks of a geometry, arguments of the kernels.
 #ifndef SINGA_AMD_CSRC_ATTN_RUN_H_
 #define SINGA_AMD_CSRC_ATTN_RUN_H_
 
@@ -39,22 +39,6 @@ static inline int pad_rows(const PadArgs &a, int tensors, hipStream_t s) {
   hipLaunchKernelGGL((k_attn_pad<T>), dim3(unsigned(blocks < limit ? blocks : limit), unsigned(tensors)), dim3(kBlock), 0, s, a);
   SGH_LAUNCH_CHECK();
   return SGH_OK;
-}
-
-struct Extent {
-  const void *p;
-  size_t bytes;
-};
-// a result meets an argument or another result
-template <int R, int A>
-static inline bool any_overlap(const Extent (&results)[R], const Extent (&arguments)[A]) {
-  for (int i = 0; i < R; ++i) {
-    for (int j = i + 1; j < R; ++j)
-      if (sgh_ranges_meet(results[i].p, results[i].bytes, results[j].p, results[j].bytes)) return true;
-    for (int j = 0; j < A; ++j)
-      if (sgh_ranges_meet(results[i].p, results[i].bytes, arguments[j].p, arguments[j].bytes)) return true;
-  }
-  return false;
 }
 
 }  // namespace attn

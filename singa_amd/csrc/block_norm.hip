@@ -670,20 +670,6 @@ int run_bwd(const Args &a, const Plan &p, float *dpre, float *dpost, hipStream_t
   return SGH_OK;
 }
 
-struct Extent {
-  const void *p;
-  size_t bytes;
-};
-template <int R, int A>
-bool any_overlap(const Extent (&results)[R], const Extent (&arguments)[A]) {
-  for (int i = 0; i < R; ++i) {
-    for (int j = i + 1; j < R; ++j)
-      if (sgh_ranges_meet(results[i].p, results[i].bytes, results[j].p, results[j].bytes)) return true;
-    for (int j = 0; j < A; ++j)
-      if (sgh_ranges_meet(results[i].p, results[i].bytes, arguments[j].p, arguments[j].bytes)) return true;
-  }
-  return false;
-}
 int check_sizes(size_t rows, size_t dim, size_t gates) {
   if (rows > kMostRows || (gates != 0 && rows % gates != 0)) return SGH_EINVAL;   // (no rows are divided by any number)
   return dim > kMostDim ? SGH_ELIMIT : SGH_OK;
@@ -704,10 +690,10 @@ int forward(const void *x, const void *h, const float *post, const void *gate, c
   if (!x || !stats || (h && !y) || (pre && !n) || (!h && (post || gate)) || (!h && !pre) || (gate && gates == 0)) return SGH_EINVAL;
   if (!(eps >= 0.f) || !__builtin_isfinite(eps)) return SGH_EINVAL;
   const size_t bytes = rows * dim * sizeof(typename S::elem), weights = dim * sizeof(float);
-  const Extent results[] = {{y, h ? bytes : 0}, {n, pre ? bytes : 0}, {stats, rows * 8}};
-  const Extent arguments[] = {{x, bytes}, {h, h ? bytes : 0}, {post, post ? weights : 0}, {pre, pre ? weights : 0},
+  const sgh_extent results[] = {{y, h ? bytes : 0}, {n, pre ? bytes : 0}, {stats, rows * 8}};
+  const sgh_extent arguments[] = {{x, bytes}, {h, h ? bytes : 0}, {post, post ? weights : 0}, {pre, pre ? weights : 0},
                               {gate, gate ? gates * dim * sizeof(typename S::elem) : 0}};
-  if (any_overlap(results, arguments)) return SGH_EINVAL;
+  if (sgh_any_overlap(results, arguments)) return SGH_EINVAL;
   Args a = {};
   a.x = x, a.h = h, a.gate = gate, a.post = post, a.pre = pre, a.stats = stats, a.out_y = y, a.out_n = n;
   a.dim = dim, a.rows = unsigned(rows), a.gates = unsigned(gates), a.per_gate = gate ? unsigned(rows / gates) : 0, a.scale = scale, a.eps = eps;
@@ -743,11 +729,11 @@ int backward(const void *dy, const void *dn, const void *y, const float *stats, 
   if (!sgh_aligned16(workspace)) return SGH_EINVAL;
   const size_t bytes = rows * dim * sizeof(typename S::elem), weights = dim * sizeof(float);
   const size_t gate_bytes = gate ? gates * dim * sizeof(typename S::elem) : 0;
-  const Extent results[] = {{dx, bytes}, {dh, h ? bytes : 0}, {dpost, post ? weights : 0}, {dgate, gate_bytes}, {dpre, pre ? weights : 0},
+  const sgh_extent results[] = {{dx, bytes}, {dh, h ? bytes : 0}, {dpost, post ? weights : 0}, {dgate, gate_bytes}, {dpre, pre ? weights : 0},
                             {workspace, p.bytes()}};
-  const Extent arguments[] = {{dy, dy ? bytes : 0}, {dn, pre ? bytes : 0}, {y, pre ? bytes : 0}, {stats, rows * 8}, {h, h ? bytes : 0},
+  const sgh_extent arguments[] = {{dy, dy ? bytes : 0}, {dn, pre ? bytes : 0}, {y, pre ? bytes : 0}, {stats, rows * 8}, {h, h ? bytes : 0},
                               {post, post ? weights : 0}, {gate, gate_bytes}, {pre, pre ? weights : 0}};
-  if (any_overlap(results, arguments)) return SGH_EINVAL;
+  if (sgh_any_overlap(results, arguments)) return SGH_EINVAL;
   Args a = {};
   a.dy = dy, a.dn = dn, a.y = y, a.stats = const_cast<float *>(stats), a.h = h, a.post = post, a.gate = gate, a.pre = pre;
   a.dx = dx, a.dh = dh, a.dgate = dgate, a.part = static_cast<float *>(workspace), a.gate_part = a.part + p.part;

@@ -65,4 +65,20 @@ static inline bool sgh_ranges_meet(const void *a, size_t a_bytes, const void *b,
   return a_bytes != 0 && b_bytes != 0 && x < y + b_bytes && y < x + a_bytes;
 }
 
+struct sgh_extent {
+  const void *p;
+  size_t bytes;
+};
+// a result meets an argument or another result
+template <int R, int A>
+static inline bool sgh_any_overlap(const sgh_extent (&results)[R], const sgh_extent (&arguments)[A]) {
+  for (int i = 0; i < R; ++i) {
+    for (int j = i + 1; j < R; ++j)
+      if (sgh_ranges_meet(results[i].p, results[i].bytes, results[j].p, results[j].bytes)) return true;
+    for (int j = 0; j < A; ++j)
+      if (sgh_ranges_meet(results[i].p, results[i].bytes, arguments[j].p, arguments[j].bytes)) return true;
+  }
+  return false;
+}
+
 #endif  // SINGA_AMD_CSRC_ROWS_H_
