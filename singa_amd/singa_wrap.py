@@ -946,8 +946,20 @@ class AttentionHandle(object):
         check(_L().sgh_attn_geom_init(C.byref(self.geom), self.batch, self.q_len, self.k_len, self.heads, self.kv_heads, self.dim,
                                       int(self.causal), self.scale, self.buckets, int(max_distance), int(bidirectional)),
               "sgh_attn_geom_init")
-        self._forward_bytes = _L().sgh_attn_fwd_workspace_bytes(C.byref(self.geom))
-        self._backward_bytes = _L().sgh_attn_bwd_workspace_bytes(C.byref(self.geom))
+        self._looked_at = None
+        self._geometry()
+
+    def _geometry(self):
+        """The geometry's address; one that has taken the place of another has to have the handle's sizes, which the tensors are held to."""
+        g = self.geom
+        if g is not self._looked_at:
+            for name in ("batch", "q_len", "k_len", "heads", "kv_heads", "dim", "buckets"):
+                if getattr(g, name) != getattr(self, name):
+                    raise SingaHipError("AttentionHandle: a geometry of other sizes than the handle's: %s" % name)
+            self._forward_bytes = _L().sgh_attn_fwd_workspace_bytes(C.byref(g))
+            self._backward_bytes = _L().sgh_attn_bwd_workspace_bytes(C.byref(g))
+            self._looked_at = g
+        return _address(g)
 
 
 def _attn_args(what, h, q_like, k_like, table, lengths):
@@ -984,10 +996,10 @@ def AttentionForward(h, q, k, v, table=None, q_lengths=None, k_lengths=None, q_s
     first query among its keys, as of a new token behind a cache of `k_len` places."""
     args = _attn_args("AttentionForward", h, (q,), (k, v), table, (q_lengths, k_lengths, q_starts))
     fn, name = _fn("attn_fwd", q)
-    dev = q._dev
+    dev, geom = q._dev, h._geometry()
     o, lse = _like(q), _empty(Tensor, (h.batch, h.heads, h.q_len), dev, kFloat32)
     ws, at = _workspace(h._forward_bytes, dev)
-    check(fn(_address(h.geom), q.ptr, k.ptr, v.ptr, *args, o.ptr, lse.ptr, at, h._forward_bytes, dev.stream), name)
+    check(fn(geom, q.ptr, k.ptr, v.ptr, *args, o.ptr, lse.ptr, at, h._forward_bytes, dev.stream), name)
     return o, lse
 
 
@@ -999,11 +1011,11 @@ def AttentionBackward(h, do, q, k, v, o, lse, table=None, q_lengths=None, k_leng
     if lse._dtype != kFloat32 or lse._shape != (h.batch, h.heads, h.q_len):
         raise SingaHipError("AttentionBackward: the row sums do not match: %s" % lse.shape())
     fn, name = _fn("attn_bwd", q)
-    dev = q._dev
+    dev, geom = q._dev, h._geometry()
     dq, dk, dv = _like(q), _like(k), _like(v)
     dtable = None if table is None else _like(table)
     ws, at = _workspace(h._backward_bytes, dev)
-    check(fn(_address(h.geom), do.ptr, q.ptr, k.ptr, v.ptr, o.ptr, lse.ptr, *args, dq.ptr, dk.ptr, dv.ptr, None if dtable is None else dtable.ptr,
+    check(fn(geom, do.ptr, q.ptr, k.ptr, v.ptr, o.ptr, lse.ptr, *args, dq.ptr, dk.ptr, dv.ptr, None if dtable is None else dtable.ptr,
              at, h._backward_bytes, dev.stream), name)
     return dq, dk, dv, dtable
 

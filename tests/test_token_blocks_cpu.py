@@ -357,3 +357,34 @@ def test_assembly_names_the_register_that_it_writes():
                     found += 1
                     assert '"m0"' in statement.rsplit(":", 1)[1], (name, statement)
     assert found
+
+
+def test_a_geometry_of_other_sizes_is_refused(monkeypatch):
+    """A handle's tensors are held to its sizes; a structure put in place of its own that has others would read beyond them."""
+    from singa_amd import singa_wrap as singa
+
+    class Device(object):
+        stream = None
+
+    passed, dev = [], Device()
+    make = lambda shape: singa.from_device_pointer(4096, shape, dev, singa.kFloat32)
+    q, k, lse = make((2, 5, 4, 8)), make((2, 7, 2, 8)), make((2, 4, 5))
+    monkeypatch.setattr(singa, "_fn", lambda name, t: (lambda geom, *rest: passed.append(geom) or 0, name))
+    monkeypatch.setattr(singa, "_empty", lambda *a: q)
+    monkeypatch.setattr(singa, "_like", lambda t: t)
+    h = singa.AttentionHandle(q, k)
+    own = h.geom
+    for shape in ((2, 6, 4, 8), (2, 5, 2, 8)):
+        h.geom = singa.AttentionHandle(make(shape), k).geom
+        for call in (lambda: singa.AttentionForward(h, q, k, k), lambda: singa.AttentionBackward(h, q, q, k, k, q, lse)):
+            with pytest.raises(singa.SingaHipError):
+                call()
+    h.geom = singa.AttentionHandle(q, make((2, 9, 2, 8))).geom
+    with pytest.raises(singa.SingaHipError):
+        singa.AttentionForward(h, q, k, k)
+    assert not passed
+    h.geom = own
+    singa.AttentionForward(h, q, k, k)
+    h.geom = singa.AttentionHandle(q, k, causal=True).geom
+    singa.AttentionForward(h, q, k, k)
+    assert passed == [C.addressof(own), C.addressof(h.geom)]
